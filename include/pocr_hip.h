@@ -275,6 +275,155 @@ int pocr_time_attention(pocr_ctx *ctx, int heads, int kv_heads, int head_dim, in
  * in the reference (a measurement aid); allocates and frees its buffers. */
 int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters, float *avg_us);
 
+/* ---------------- cache operators (device buffers, caller's stream) ---------------- */
+/* No counterpart in the reference: operators on K/V caches that the caller
+ * owns, fp32 rows [row][kv_heads][head_dim], for decoders and serving loops
+ * that draft tokens, pack prompts or let cache rows go.
+ *
+ * Conventions of this section:
+ *  - Every pointer is a device address on the context's device.  Buffers of
+ *    floats are 16-byte aligned and their strides, counted in floats, are
+ *    multiples of 4 (POCR_ERR_ARG otherwise); index buffers are 4-byte aligned.
+ *  - `stream` is the hipStream_t the work is queued on, null HIP's default
+ *    stream; a stream of another device is POCR_ERR_ARG.  A call returns once
+ *    its kernels are queued, allocates nothing, keeps nothing, waits for
+ *    nothing and leaves the calling thread's current device as it was: it may
+ *    be captured into a HIP graph.
+ *  - A workspace belongs to one call in flight: calls (or graphs) that may run
+ *    at the same time each take their own.  It needs no initialization.
+ *  - Shapes are checked before any device work; numbers that live on the
+ *    device (lengths, counts, parents, spans, row lists) are read by the
+ *    kernels and forced into their ranges there, as stated at each field.
+ *  - head_dim is 64 or 128 (POCR_ERR_UNSUPPORTED otherwise); heads is a
+ *    multiple of kv_heads, query head h reads KV head h / (heads / kv_heads).
+ *  - Sums and softmax statistics are fp32; products keep 22 bits of each
+ *    operand.  A row whose query is NaN, or that sees a NaN or an infinite
+ *    value, comes out not finite; what an infinite query or key gives its rows
+ *    is unspecified (sizes of 2^110 and more count as infinite).  Rows that do
+ *    not see such a key or value do not change.
+ *
+ * Scores of query row i and cache row j:
+ *   s = scale * q·k, then cap * tanh(s / cap) where cap > 0, then
+ *   s - slopes[h] * |position(i) - position(j)| where slopes is given. */
+
+/* softmax attention of n rows over a cache whose last n rows are their own
+ * (rows [0, rows_before + n)): a prompt's rows, or one token (n = 1).  Row i
+ * sees cache rows [row_begin[i], row_end[i]): documents packed into one
+ * prompt, prefixes whose rows see each other, windows, and padding that sees
+ * nothing (begin >= end: its out row is zeros, its lse -inf).  position(j) = j. */
+typedef struct {
+    const float *q;           /* row i, head h: q + i*q_stride + h*head_dim */
+    const float *k, *v;       /* row j, KV head g: k + j*k_stride + g*head_dim */
+    float *out;               /* row i, head h: out + i*out_stride + h*head_dim */
+    float *lse;               /* [n][heads] log-sum-exp of the scores, or null */
+    const int32_t *row_begin; /* [n] first visible row and */
+    const int32_t *row_end;   /* [n] end, both forced into [0, rows_before + n]; null: [0, rows_before + i + 1) */
+    const float *slopes;      /* [heads], or null */
+    void *workspace;          /* pocr_prompt_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    int32_t n;                /* 1 .. 2^22 rows */
+    int32_t rows_before;      /* rows_before + n <= 2^30 */
+    int32_t heads, kv_heads, head_dim;
+    float scale;              /* > 0; 0: 1 / sqrt(head_dim) */
+    float cap;                /* > 0; 0: scores as they are */
+} pocr_prompt_args;
+int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *args, void *stream);
+/* workspace bytes of such a call (pointers and strides are not looked at), or an error status */
+int64_t pocr_prompt_attention_workspace(const pocr_prompt_args *args);
+
+/* softmax attention of drafted tokens: sequence s has lens[s] rows in its
+ * cache and behind them the K/V rows of its counts[s] drafted tokens.  Token t
+ * follows parents[s][t] (an earlier token, or -1: the cache's last row) and
+ * sees the cache, its ancestors and itself.  Rows of out and lse behind a
+ * sequence's last token are left as they were.
+ * positions, where given, holds the position of every cache row per KV head
+ * (rows that moved, pocr_cache_keep); otherwise a cached row's is its index
+ * and a drafted token's lens[s] + its depth in the tree. */
+typedef struct {
+    const float *q;           /* sequence s, token t, head h: q + s*q_seq_stride + t*q_stride + h*head_dim */
+    const float *k, *v;       /* sequence s, row j, KV head g: k + s*k_seq_stride + j*k_stride + g*head_dim */
+    const int32_t *lens;      /* [seqs], forced into [0, max_rows - count] */
+    const int32_t *counts;    /* [seqs] tokens of each sequence, forced into [0, n]; null: n */
+    const int32_t *parents;   /* [seqs][n], outside [-1, t): -1; null: chains (t - 1) */
+    const float *slopes;      /* [heads], or null */
+    const int32_t *positions; /* [seqs][kv_heads][side_stride], or null */
+    float *out;               /* as q, by out_seq_stride and out_stride */
+    float *lse;               /* [seqs][n][heads]: written where not null; read by pocr_cache_weights */
+    float *weights;           /* pocr_cache_weights: [seqs][kv_heads][side_stride] */
+    const uint64_t *take;     /* pocr_cache_weights: [seqs] bit t: token t counts; null: all */
+    void *workspace;          /* pocr_tree_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t q_seq_stride, q_stride, k_seq_stride, k_stride, v_seq_stride, v_stride, out_seq_stride, out_stride;
+    int64_t side_stride;      /* >= max_rows; 0: max_rows */
+    int32_t seqs;             /* 1 .. 65535 */
+    int32_t n;                /* 1 .. 64 tokens */
+    int32_t max_rows;         /* no sequence has more rows, drafted ones included; n .. 2^30 */
+    int32_t heads, kv_heads, head_dim;
+    float scale, cap;         /* as above */
+} pocr_tree_args;
+int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *args, void *stream);
+int64_t pocr_tree_attention_workspace(const pocr_tree_args *args);
+/* accumulates what each cache row weighs: for every KV head g and visible row j
+ *   weights[s][g][j] += sum over taken tokens t and heads h of g: exp(s - lse[s][t][h])
+ * with the scores and the visibility of pocr_tree_attention and the lse it
+ * wrote (v, out and workspace are not used).  A row whose lse is -inf adds nothing.
+ * The order of each sum is fixed. */
+int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *args, void *stream);
+
+/* which rows of each cache and KV head stay when a cache falls to `budget`
+ * rows: the first `sinks`, the last `recent`, and of those between the
+ * heaviest (equal weights: the lower row; a NaN weighs least).  A cache of at
+ * most `budget` rows keeps all.  kept lists the rows in ascending order,
+ * counts[c] of them: min(lens[c], budget) for every KV head; entries behind
+ * them are left as they were. */
+typedef struct {
+    const float *weights;     /* [caches][kv_heads][side_stride] */
+    const int32_t *lens;      /* [caches], forced into [0, max_rows] */
+    int32_t *kept;            /* [caches][kv_heads][budget] */
+    int32_t *counts;          /* [caches]; not lens itself */
+    int64_t side_stride;      /* >= max_rows; 0: max_rows */
+    int32_t caches;           /* 1 .. 65535 */
+    int32_t kv_heads;         /* 1 .. 65535 */
+    int32_t max_rows;         /* 1 .. 2^30 */
+    int32_t budget;           /* 1 .. 2^30, sinks + recent <= budget */
+    int32_t sinks, recent;    /* >= 0 */
+} pocr_select_args;
+int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *args, void *stream);
+
+/* moves listed cache rows together: row first[c] + i of the destination
+ * becomes row rows[c][g][i] of the source, i < counts[c], for K, V and, where
+ * given, the rows' weights and positions.  weights_out rows behind the moved
+ * ones, up to max_rows_out, become 0 (a row written there later starts
+ * there); no other destination row changes.
+ * In place (k_out = k, v_out = v, and so on for the side buffers, with equal
+ * strides) each list must ascend with rows[i] >= first + i, as
+ * pocr_cache_select's lists and the path of accepted tokens behind first =
+ * lens do; a list that does not leaves unspecified rows.  Otherwise a
+ * destination may not overlap its source (POCR_ERR_ARG). */
+typedef struct {
+    const float *k, *v;       /* cache c, row j, KV head g: k + c*k_cache_stride + j*k_stride + g*head_dim */
+    const float *weights;     /* [caches][kv_heads][side_stride], or null */
+    const int32_t *positions; /* likewise */
+    float *k_out, *v_out;
+    float *weights_out;       /* [caches][kv_heads][side_out_stride], null with weights */
+    int32_t *positions_out;   /* likewise */
+    const int32_t *rows;      /* [caches][kv_heads][max_keep], or [caches][max_keep] without per_head;
+                                 forced into [0, max_rows) (in place: [first + i, max_rows)) */
+    const int32_t *counts;    /* [caches], forced into [0, min(max_keep, max_rows_out - first)] */
+    const int32_t *first;     /* [caches], forced into [0, max_rows_out]; null: 0 */
+    int64_t k_cache_stride, k_stride, v_cache_stride, v_stride;
+    int64_t k_out_cache_stride, k_out_stride, v_out_cache_stride, v_out_stride;
+    int64_t side_stride;      /* >= max_rows; 0: max_rows */
+    int64_t side_out_stride;  /* >= max_rows_out; 0: max_rows_out */
+    int32_t caches, kv_heads; /* 1 .. 65535 */
+    int32_t head_dim;         /* 64 or 128 */
+    int32_t max_keep;         /* 1 .. 2^30 */
+    int32_t per_head;         /* each KV head has its own list */
+    int32_t max_rows, max_rows_out; /* rows of a source and of a destination cache, 1 .. 2^30 */
+} pocr_keep_args;
+int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *args, void *stream);
+
 /* ---------------- model / step level (device-resident) ---------------- */
 int pocr_model_create(pocr_ctx *ctx, const pocr_config *cfg, pocr_model **out);
 void pocr_model_destroy(pocr_model *m);

@@ -1,0 +1,370 @@
+// cache_ops.hip — the cache operators' entry points (cache_ops.hpp): argument
+// checks, launch shapes, and the device and stream they run on.
+#include <cmath>
+
+#include "cache_ops.hpp"
+#include "internal.hpp"
+
+using namespace pocr;
+
+namespace {
+
+constexpr int kMaxGridYZ = 65535;
+constexpr int kMaxCacheRows = 1 << 30;
+constexpr int kMaxPromptRows = 1 << 22;
+constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
+constexpr int kMaxQueryHeads = 1024;
+
+// The calling thread's device becomes the context's for one call.
+struct DeviceScope {
+    int was = -1;
+    int enter(int device) {
+        int now = 0;
+        HIP_TRY(hipGetDevice(&now));
+        if (now == device) return POCR_OK;
+        HIP_TRY(hipSetDevice(device));
+        was = now;
+        return POCR_OK;
+    }
+    ~DeviceScope() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+};
+
+int check_stream(const pocr_ctx *ctx, hipStream_t s, const char *op) {
+    if (!s) return POCR_OK;
+    hipDevice_t dev = 0;
+    if (hipStreamGetDevice(s, &dev) != hipSuccess) return fail(POCR_ERR_ARG, "%s: not a stream", op);
+    if (dev != ctx->device) return fail(POCR_ERR_ARG, "%s: a stream of device %d, the context is on %d", op, dev, ctx->device);
+    return POCR_OK;
+}
+
+#define CACHE_OP_ENTER(ctx, stream, op)                        \
+    if (!(ctx)) return fail(POCR_ERR_ARG, "%s: null context", op); \
+    CHECK_INJECT((op) + 5); /* the name without pocr_ */       \
+    DeviceScope scope_;                                        \
+    RC(scope_.enter((ctx)->device));                           \
+    RC(check_stream(ctx, (hipStream_t)(stream), op))
+
+bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+int check_heads(int heads, int kv_heads, int head_dim, const char *op) {
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > kMaxQueryHeads)
+        return fail(POCR_ERR_ARG, "%s: %d heads over %d KV heads", op, heads, kv_heads);
+    if (head_dim != 64 && head_dim != 128) return fail(POCR_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", op, head_dim);
+    return POCR_OK;
+}
+
+int check_scores(float scale, float cap, const char *op) {
+    if (!(scale >= 0.0f) || std::isinf(scale)) return fail(POCR_ERR_ARG, "%s: scale must be finite and >= 0", op);
+    if (!(cap >= 0.0f) || std::isinf(cap)) return fail(POCR_ERR_ARG, "%s: cap must be finite and >= 0", op);
+    return POCR_OK;
+}
+
+// rows of `width` floats, `stride` apart
+int check_rows(const void *p, int64_t stride, int64_t width, const char *what, const char *op) {
+    if (!p) return fail(POCR_ERR_ARG, "%s: null %s", op, what);
+    if (!aligned(p, 16)) return fail(POCR_ERR_ARG, "%s: %s is not 16-byte aligned", op, what);
+    if (stride < width || stride % 4) return fail(POCR_ERR_ARG, "%s: %s rows %lld floats apart: at least %lld, a multiple of 4", op, what, (long long)stride, (long long)width);
+    return POCR_OK;
+}
+
+// `count` blocks of rows, `stride` apart (any multiple of 4 where there is one)
+int check_outer(int64_t stride, int count, const char *what, const char *op) {
+    if (count > 1 && (stride < 1 || stride % 4)) return fail(POCR_ERR_ARG, "%s: %s blocks %lld floats apart", op, what, (long long)stride);
+    return POCR_OK;
+}
+
+int check_index(const void *p, const char *what, const char *op, size_t a = 4) {
+    return aligned(p, a) ? POCR_OK : fail(POCR_ERR_ARG, "%s: %s is not %zu-byte aligned", op, what, a);
+}
+
+int check_workspace(const void *p, int64_t have, int64_t need, const char *op) {
+    if (need && (!p || !aligned(p, 16) || have < need))
+        return fail(POCR_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes, has %lld", op, (long long)need, (long long)(p ? have : 0));
+    return POCR_OK;
+}
+
+int prompt_shape(const pocr_prompt_args *a, const char *op) {
+    if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
+    RC(check_heads(a->heads, a->kv_heads, a->head_dim, op));
+    RC(check_scores(a->scale, a->cap, op));
+    if (a->n < 1 || a->n > kMaxPromptRows) return fail(POCR_ERR_ARG, "%s: %d rows", op, a->n);
+    if (a->rows_before < 0 || a->rows_before > kMaxCacheRows - a->n) return fail(POCR_ERR_ARG, "%s: %d rows before", op, a->rows_before);
+    return POCR_OK;
+}
+
+int tree_shape(const pocr_tree_args *a, const char *op) {
+    if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
+    RC(check_heads(a->heads, a->kv_heads, a->head_dim, op));
+    RC(check_scores(a->scale, a->cap, op));
+    if (a->seqs < 1 || a->seqs > kMaxGridYZ) return fail(POCR_ERR_ARG, "%s: %d sequences", op, a->seqs);
+    if (a->n < 1 || a->n > kMaxTreeTokens) return fail(POCR_ERR_ARG, "%s: %d tokens (1 to %d)", op, a->n, kMaxTreeTokens);
+    if (a->max_rows < a->n || a->max_rows > kMaxCacheRows) return fail(POCR_ERR_ARG, "%s: max_rows %d", op, a->max_rows);
+    return POCR_OK;
+}
+
+int check_side(int64_t stride, int rows, const char *what, const char *op) {
+    if (stride && stride < rows) return fail(POCR_ERR_ARG, "%s: %s %lld for %d rows", op, what, (long long)stride, rows);
+    return POCR_OK;
+}
+
+float default_scale(float scale, int head_dim) { return scale > 0.0f ? scale : (float)(1.0 / std::sqrt((double)head_dim)); }
+
+// what pocr_tree_attention and pocr_cache_weights share
+int tree_params(const pocr_tree_args *a, const char *op, CacheAttn *p) {
+    RC(tree_shape(a, op));
+    const int64_t kvd = (int64_t)a->kv_heads * a->head_dim, qd = (int64_t)a->heads * a->head_dim;
+    RC(check_rows(a->q, a->q_stride, qd, "q", op));
+    RC(check_rows(a->k, a->k_stride, kvd, "k", op));
+    RC(check_outer(a->q_seq_stride, a->seqs, "q", op));
+    RC(check_outer(a->k_seq_stride, a->seqs, "k", op));
+    if (!a->lens) return fail(POCR_ERR_ARG, "%s: null lens", op);
+    RC(check_side(a->side_stride, a->max_rows, "side_stride", op));
+    for (const void *x : {(const void *)a->lens, (const void *)a->counts, (const void *)a->parents, (const void *)a->slopes,
+                          (const void *)a->positions, (const void *)a->lse})
+        RC(check_index(x, "an index or side buffer", op));
+    p->q = a->q;
+    p->k = a->k;
+    p->lens = a->lens;
+    p->counts = a->counts;
+    p->parents = a->parents;
+    p->slopes = a->slopes;
+    p->pos = a->positions;
+    p->lse = a->lse;
+    p->q_ss = a->q_seq_stride;
+    p->q_st = a->q_stride;
+    p->k_ss = a->k_seq_stride;
+    p->k_st = a->k_stride;
+    p->side = a->side_stride ? a->side_stride : a->max_rows;
+    p->n = a->n;
+    p->rows = a->max_rows;
+    p->heads = a->heads;
+    p->kvh = a->kv_heads;
+    p->group = a->heads / a->kv_heads;
+    p->scale = default_scale(a->scale, a->head_dim);
+    p->cap = a->cap;
+    return POCR_OK;
+}
+
+template <bool TREE>
+int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs) {
+    const dim3 grid(p.n, p.heads, seqs);
+    if (head_dim == 128) hipLaunchKernelGGL((k_cache_attn_rows<128, TREE>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((k_cache_attn_rows<64, TREE>), grid, dim3(256), 0, s, p);
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}
+
+int64_t prompt_workspace(const pocr_prompt_args *a) { return 0; }
+int64_t tree_workspace(const pocr_tree_args *a) { return 0; }
+
+// the addresses of `caches` blocks of `rows` rows overlap
+bool overlap(const void *a, int64_t acs, int64_t ast, int arows, const void *b, int64_t bcs, int64_t bst, int brows,
+             int caches, int64_t width) {
+    const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
+    const char *a1 = a0 + 4 * ((caches - 1) * acs + (arows - 1) * ast + width);
+    const char *b1 = b0 + 4 * ((caches - 1) * bcs + (brows - 1) * bst + width);
+    return a0 < b1 && b0 < a1;
+}
+
+}  // namespace
+
+extern "C" int64_t pocr_prompt_attention_workspace(const pocr_prompt_args *a) {
+    RC(prompt_shape(a, "pocr_prompt_attention_workspace"));
+    return prompt_workspace(a);
+}
+
+extern "C" int64_t pocr_tree_attention_workspace(const pocr_tree_args *a) {
+    RC(tree_shape(a, "pocr_tree_attention_workspace"));
+    return tree_workspace(a);
+}
+
+extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, void *stream) {
+    const char *op = "pocr_prompt_attention";
+    RC(prompt_shape(a, op));
+    const int64_t kvd = (int64_t)a->kv_heads * a->head_dim, qd = (int64_t)a->heads * a->head_dim;
+    RC(check_rows(a->q, a->q_stride, qd, "q", op));
+    RC(check_rows(a->k, a->k_stride, kvd, "k", op));
+    RC(check_rows(a->v, a->v_stride, kvd, "v", op));
+    RC(check_rows(a->out, a->out_stride, qd, "out", op));
+    if (!a->row_begin != !a->row_end) return fail(POCR_ERR_ARG, "%s: row_begin and row_end come together", op);
+    for (const void *x : {(const void *)a->row_begin, (const void *)a->row_end, (const void *)a->slopes, (const void *)a->lse})
+        RC(check_index(x, "an index or side buffer", op));
+    RC(check_workspace(a->workspace, a->workspace_bytes, prompt_workspace(a), op));
+    CACHE_OP_ENTER(ctx, stream, op);
+    CacheAttn p{};
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.out = a->out;
+    p.lse = a->lse;
+    p.begin = a->row_begin;
+    p.end = a->row_end;
+    p.slopes = a->slopes;
+    p.q_st = a->q_stride;
+    p.k_st = a->k_stride;
+    p.v_st = a->v_stride;
+    p.o_st = a->out_stride;
+    p.n = a->n;
+    p.rows0 = a->rows_before;
+    p.rows = a->rows_before + a->n;
+    p.heads = a->heads;
+    p.kvh = a->kv_heads;
+    p.group = a->heads / a->kv_heads;
+    p.scale = default_scale(a->scale, a->head_dim);
+    p.cap = a->cap;
+    return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1);
+}
+
+extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {
+    const char *op = "pocr_tree_attention";
+    CacheAttn p{};
+    RC(tree_params(a, op, &p));
+    RC(check_rows(a->v, a->v_stride, (int64_t)a->kv_heads * a->head_dim, "v", op));
+    RC(check_rows(a->out, a->out_stride, (int64_t)a->heads * a->head_dim, "out", op));
+    RC(check_outer(a->v_seq_stride, a->seqs, "v", op));
+    RC(check_outer(a->out_seq_stride, a->seqs, "out", op));
+    RC(check_workspace(a->workspace, a->workspace_bytes, tree_workspace(a), op));
+    CACHE_OP_ENTER(ctx, stream, op);
+    p.v = a->v;
+    p.out = a->out;
+    p.v_ss = a->v_seq_stride;
+    p.v_st = a->v_stride;
+    p.o_ss = a->out_seq_stride;
+    p.o_st = a->out_stride;
+    return launch_attn<true>((hipStream_t)stream, p, a->head_dim, a->seqs);
+}
+
+extern "C" int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {
+    const char *op = "pocr_cache_weights";
+    CacheAttn p{};
+    RC(tree_params(a, op, &p));
+    if (!a->lse || !a->weights) return fail(POCR_ERR_ARG, "%s: null lse or weights", op);
+    RC(check_index(a->weights, "weights", op));
+    RC(check_index(a->take, "take", op, 8));
+    CACHE_OP_ENTER(ctx, stream, op);
+    p.weights = a->weights;
+    p.take = a->take;
+    const dim3 grid(p.rows, p.kvh, a->seqs);
+    if (a->head_dim == 128) hipLaunchKernelGGL(k_cache_weights_rows<128>, grid, dim3(64), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL(k_cache_weights_rows<64>, grid, dim3(64), 0, (hipStream_t)stream, p);
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}
+
+extern "C" int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *a, void *stream) {
+    const char *op = "pocr_cache_select";
+    if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
+    if (a->caches < 1 || a->caches > kMaxGridYZ || a->kv_heads < 1 || a->kv_heads > kMaxGridYZ)
+        return fail(POCR_ERR_ARG, "%s: %d caches of %d KV heads", op, a->caches, a->kv_heads);
+    if (a->max_rows < 1 || a->max_rows > kMaxCacheRows) return fail(POCR_ERR_ARG, "%s: max_rows %d", op, a->max_rows);
+    if (a->budget < 1 || a->budget > kMaxCacheRows) return fail(POCR_ERR_ARG, "%s: budget %d", op, a->budget);
+    if (a->sinks < 0 || a->recent < 0 || (int64_t)a->sinks + a->recent > a->budget)
+        return fail(POCR_ERR_ARG, "%s: %d first and %d last rows in a budget of %d", op, a->sinks, a->recent, a->budget);
+    RC(check_side(a->side_stride, a->max_rows, "side_stride", op));
+    if (!a->weights || !a->lens || !a->kept || !a->counts) return fail(POCR_ERR_ARG, "%s: null buffer", op);
+    if (a->counts == a->lens) return fail(POCR_ERR_ARG, "%s: counts is lens", op);
+    for (const void *x : {(const void *)a->weights, (const void *)a->lens, (const void *)a->kept, (const void *)a->counts})
+        RC(check_index(x, "a buffer", op));
+    CACHE_OP_ENTER(ctx, stream, op);
+    CacheSelect p{};
+    p.weights = a->weights;
+    p.lens = a->lens;
+    p.kept = a->kept;
+    p.counts = a->counts;
+    p.side = a->side_stride ? a->side_stride : a->max_rows;
+    p.kvh = a->kv_heads;
+    p.max_rows = a->max_rows;
+    p.budget = a->budget;
+    p.sinks = a->sinks;
+    p.recent = a->recent;
+    hipLaunchKernelGGL(k_cache_select<8>, dim3(a->kv_heads, a->caches), dim3(kSelThreads), 0, (hipStream_t)stream, p);
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}
+
+extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *stream) {
+    const char *op = "pocr_cache_keep";
+    if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
+    if (a->caches < 1 || a->caches > kMaxGridYZ || a->kv_heads < 1 || a->kv_heads > kMaxGridYZ)
+        return fail(POCR_ERR_ARG, "%s: %d caches of %d KV heads", op, a->caches, a->kv_heads);
+    if (a->head_dim != 64 && a->head_dim != 128) return fail(POCR_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", op, a->head_dim);
+    for (const int32_t n : {a->max_keep, a->max_rows, a->max_rows_out})
+        if (n < 1 || n > kMaxCacheRows) return fail(POCR_ERR_ARG, "%s: max_keep, max_rows and max_rows_out are 1 to 2^30", op);
+    const int64_t kvd = (int64_t)a->kv_heads * a->head_dim;
+    RC(check_rows(a->k, a->k_stride, kvd, "k", op));
+    RC(check_rows(a->v, a->v_stride, kvd, "v", op));
+    RC(check_rows(a->k_out, a->k_out_stride, kvd, "k_out", op));
+    RC(check_rows(a->v_out, a->v_out_stride, kvd, "v_out", op));
+    RC(check_outer(a->k_cache_stride, a->caches, "k", op));
+    RC(check_outer(a->v_cache_stride, a->caches, "v", op));
+    RC(check_outer(a->k_out_cache_stride, a->caches, "k_out", op));
+    RC(check_outer(a->v_out_cache_stride, a->caches, "v_out", op));
+    if (!a->rows || !a->counts) return fail(POCR_ERR_ARG, "%s: null rows or counts", op);
+    if (!a->weights != !a->weights_out || !a->positions != !a->positions_out)
+        return fail(POCR_ERR_ARG, "%s: weights and positions come with their destinations", op);
+    for (const void *x : {(const void *)a->weights, (const void *)a->weights_out, (const void *)a->positions,
+                          (const void *)a->positions_out, (const void *)a->rows, (const void *)a->counts, (const void *)a->first})
+        RC(check_index(x, "an index or side buffer", op));
+    RC(check_side(a->side_stride, a->max_rows, "side_stride", op));
+    RC(check_side(a->side_out_stride, a->max_rows_out, "side_out_stride", op));
+    CacheKeep p{};
+    p.side = a->side_stride ? a->side_stride : a->max_rows;
+    p.side_out = a->side_out_stride ? a->side_out_stride : a->max_rows_out;
+    const bool inplace = a->k_out == a->k;
+    if (inplace != (a->v_out == a->v) || (a->weights && inplace != (a->weights_out == a->weights)) ||
+        (a->positions && inplace != (a->positions_out == a->positions)))
+        return fail(POCR_ERR_ARG, "%s: K, V, weights and positions move in place together or not at all", op);
+    if (inplace) {
+        if (a->k_stride != a->k_out_stride || a->v_stride != a->v_out_stride ||
+            (a->caches > 1 && (a->k_cache_stride != a->k_out_cache_stride || a->v_cache_stride != a->v_out_cache_stride)) ||
+            a->max_rows != a->max_rows_out || ((a->weights || a->positions) && p.side != p.side_out))
+            return fail(POCR_ERR_ARG, "%s: in place, the strides and row counts of source and destination are equal", op);
+    } else {
+        const int64_t heads = (int64_t)a->kv_heads;
+        if (overlap(a->k, a->k_cache_stride, a->k_stride, a->max_rows, a->k_out, a->k_out_cache_stride, a->k_out_stride, a->max_rows_out, a->caches, kvd) ||
+            overlap(a->v, a->v_cache_stride, a->v_stride, a->max_rows, a->v_out, a->v_out_cache_stride, a->v_out_stride, a->max_rows_out, a->caches, kvd) ||
+            (a->weights && overlap(a->weights, heads * p.side, 1, 1, a->weights_out, heads * p.side_out, 1, 1, a->caches, (heads - 1) * p.side + a->max_rows)) ||
+            (a->positions && overlap(a->positions, heads * p.side, 1, 1, a->positions_out, heads * p.side_out, 1, 1, a->caches, (heads - 1) * p.side + a->max_rows)))
+            return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
+    }
+    CACHE_OP_ENTER(ctx, stream, op);
+    p.src[0] = a->k;
+    p.src[1] = a->v;
+    p.dst[0] = a->k_out;
+    p.dst[1] = a->v_out;
+    p.weights = a->weights;
+    p.weights_out = a->weights_out;
+    p.pos = a->positions;
+    p.pos_out = a->positions_out;
+    p.rows = a->rows;
+    p.counts = a->counts;
+    p.first = a->first;
+    p.src_cs[0] = a->k_cache_stride;
+    p.src_cs[1] = a->v_cache_stride;
+    p.src_st[0] = a->k_stride;
+    p.src_st[1] = a->v_stride;
+    p.dst_cs[0] = a->k_out_cache_stride;
+    p.dst_cs[1] = a->v_out_cache_stride;
+    p.dst_st[0] = a->k_out_stride;
+    p.dst_st[1] = a->v_out_stride;
+    p.kvh = a->kv_heads;
+    p.max_keep = a->max_keep;
+    p.per_head = a->per_head != 0;
+    p.max_rows = a->max_rows;
+    p.max_rows_out = a->max_rows_out;
+    const int slots = 2 * a->head_dim / kKeepSlab + 1;
+    const int chunks = inplace ? 1 : std::min(64, (a->max_keep + 255) / 256);
+    const dim3 grid(slots * chunks, a->kv_heads, a->caches);
+    hipStream_t s = (hipStream_t)stream;
+    if (a->head_dim == 128) {
+        if (inplace) hipLaunchKernelGGL((k_cache_keep<128, true>), grid, dim3(kKeepThreads), 0, s, p);
+        else hipLaunchKernelGGL((k_cache_keep<128, false>), grid, dim3(kKeepThreads), 0, s, p);
+    } else {
+        if (inplace) hipLaunchKernelGGL((k_cache_keep<64, true>), grid, dim3(kKeepThreads), 0, s, p);
+        else hipLaunchKernelGGL((k_cache_keep<64, false>), grid, dim3(kKeepThreads), 0, s, p);
+    }
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}

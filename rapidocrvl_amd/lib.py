@@ -50,6 +50,46 @@ class PocrConfig(C.Structure):
     ]
 
 
+class PromptArgs(C.Structure):
+    """pocr_prompt_args: attention of prompt rows.  Pointers are device
+    addresses (ints, None for null); every field left out is zero."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "row_begin", "row_end", "slopes", "workspace")]
+    _fields_ += [(n, C.c_int64) for n in ("workspace_bytes", "q_stride", "k_stride", "v_stride", "out_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("n", "rows_before", "heads", "kv_heads", "head_dim")]
+    _fields_ += [("scale", C.c_float), ("cap", C.c_float)]
+
+
+class TreeArgs(C.Structure):
+    """pocr_tree_args: attention of drafted trees, and the weights of their rows."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "lens", "counts", "parents", "slopes", "positions", "out",
+                                          "lse", "weights", "take", "workspace")]
+    _fields_ += [(n, C.c_int64) for n in ("workspace_bytes", "q_seq_stride", "q_stride", "k_seq_stride", "k_stride",
+                                          "v_seq_stride", "v_stride", "out_seq_stride", "out_stride", "side_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("seqs", "n", "max_rows", "heads", "kv_heads", "head_dim")]
+    _fields_ += [("scale", C.c_float), ("cap", C.c_float)]
+
+
+class SelectArgs(C.Structure):
+    """pocr_select_args: which cache rows stay within a budget."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("weights", "lens", "kept", "counts")] + [("side_stride", C.c_int64)]
+    _fields_ += [(n, C.c_int32) for n in ("caches", "kv_heads", "max_rows", "budget", "sinks", "recent")]
+
+
+class KeepArgs(C.Structure):
+    """pocr_keep_args: listed cache rows moved together."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "weights", "positions", "k_out", "v_out", "weights_out",
+                                          "positions_out", "rows", "counts", "first")]
+    _fields_ += [(n, C.c_int64) for n in ("k_cache_stride", "k_stride", "v_cache_stride", "v_stride",
+                                          "k_out_cache_stride", "k_out_stride", "v_out_cache_stride", "v_out_stride",
+                                          "side_stride", "side_out_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("caches", "kv_heads", "head_dim", "max_keep", "per_head", "max_rows",
+                                          "max_rows_out")]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _SIGS = {
@@ -85,6 +125,13 @@ _SIGS = {
     "pocr_swiglu_down_add_rmsnorm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i, _vp]),
     "pocr_add_rmsnorm": (_i, [_vp, _vp, _vp, _vp, _i, C.c_float, _i, _vp]),
     "pocr_mrope": (_i, [_vp, _vp, _vp, _vp, _i, _i]),
+    "pocr_prompt_attention": (_i, [_vp, C.POINTER(PromptArgs), _vp]),
+    "pocr_prompt_attention_workspace": (C.c_int64, [C.POINTER(PromptArgs)]),
+    "pocr_tree_attention": (_i, [_vp, C.POINTER(TreeArgs), _vp]),
+    "pocr_tree_attention_workspace": (C.c_int64, [C.POINTER(TreeArgs)]),
+    "pocr_cache_weights": (_i, [_vp, C.POINTER(TreeArgs), _vp]),
+    "pocr_cache_select": (_i, [_vp, C.POINTER(SelectArgs), _vp]),
+    "pocr_cache_keep": (_i, [_vp, C.POINTER(KeepArgs), _vp]),
     "pocr_model_create": (_i, [_vp, C.POINTER(PocrConfig), C.POINTER(_vp)]),
     "pocr_model_destroy": (None, [_vp]),
     "pocr_model_set_weight": (_i, [_vp, _i, _i, _vp]),
@@ -299,6 +346,35 @@ class Batch:
         out = np.zeros(max(cap, 1), np.int32)
         n = check(load().pocr_batch_leave(self.h, seq.h, _ptr(out), cap))
         return out[:min(n, cap)]
+
+
+def prompt_attention_workspace(args: PromptArgs) -> int:
+    """Workspace bytes of Context.prompt_attention for these shapes."""
+    return check(load().pocr_prompt_attention_workspace(C.byref(args)))
+
+
+def tree_attention_workspace(args: TreeArgs) -> int:
+    """Workspace bytes of Context.tree_attention for these shapes."""
+    return check(load().pocr_tree_attention_workspace(C.byref(args)))
+
+
+_known_streams = set()
+
+
+def _stream(stream):
+    """A hipStream_t handle for the cache operators (0: HIP's default stream).
+    A handle, and the buffers, have to come from the HIP runtime that the
+    library itself runs on: a process that loads the library and only then
+    another package with a HIP runtime of its own holds two."""
+    if stream and stream not in _known_streams:
+        load()
+        with open("/proc/self/maps") as f:
+            runtimes = {os.path.realpath(ln.split()[-1]) for ln in f if "libamdhip64" in ln}
+        if len(runtimes) > 1:
+            raise RuntimeError("two HIP runtimes are loaded (" + ", ".join(sorted(runtimes)) + "): a stream of one is "
+                               "not known to the other; import the package that made it before this library is loaded")
+        _known_streams.add(stream)
+    return stream
 
 
 def device_count() -> int:
@@ -562,6 +638,28 @@ class Context:
         """pocr_text_attention_noalloc over device addresses (ints) the caller owns."""
         check(load().pocr_text_attention_noalloc(self.h, C.c_void_p(q_dev), C.c_void_p(k_dev), C.c_void_p(v_dev),
                                                  cache_len, heads, kv_heads, head_dim, C.c_void_p(out_dev)))
+
+
+    # -- cache operators: device buffers, queued on the caller's stream --------
+    def prompt_attention(self, args: PromptArgs, stream=0):
+        """Attention of a prompt's rows (masks as spans, capped scores, distance biases)."""
+        check(load().pocr_prompt_attention(self.h, C.byref(args), _stream(stream)))
+
+    def tree_attention(self, args: TreeArgs, stream=0):
+        """Attention of drafted trees over their sequences' caches."""
+        check(load().pocr_tree_attention(self.h, C.byref(args), _stream(stream)))
+
+    def cache_weights(self, args: TreeArgs, stream=0):
+        """Adds what each cache row weighs for the taken tokens to args.weights."""
+        check(load().pocr_cache_weights(self.h, C.byref(args), _stream(stream)))
+
+    def cache_select(self, args: SelectArgs, stream=0):
+        """Lists the rows that stay when each cache falls to args.budget rows."""
+        check(load().pocr_cache_select(self.h, C.byref(args), _stream(stream)))
+
+    def cache_keep(self, args: KeepArgs, stream=0):
+        """Moves the listed rows of each cache together."""
+        check(load().pocr_cache_keep(self.h, C.byref(args), _stream(stream)))
 
 
 class Model:
