@@ -390,9 +390,10 @@ def _plan(case, st):
         a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
         return ctx, a, work
     if case["op"] in ("tree", "weights"):
+        lse = st["lse"].contiguous()  # [seq][token][head], as the attention writes it
         a = lib.TreeArgs(q=_ptr(st["q"]), k=_ptr(st["k"]), v=_ptr(st["v"]), lens=_ptr(st["lens"]),
                          counts=_ptr(st["counts"]), parents=_ptr(st["parents"]), slopes=_ptr(st["slopes"]),
-                         out=_ptr(st.get("out")), lse=_ptr(st["lse"]),
+                         out=_ptr(st.get("out")), lse=_ptr(lse),
                          weights=_ptr(st.get("weights")), seqs=case["seqs"], n=case["n"],
                          max_rows=case["rows"] + case["n"], q_seq_stride=st["q"].stride(0), q_stride=st["q"].stride(1),
                          k_seq_stride=st["k"].stride(0), k_stride=kvd, v_seq_stride=st["v"].stride(0), v_stride=kvd,
@@ -402,7 +403,7 @@ def _plan(case, st):
         if case["op"] == "tree":
             work = _work_buffer(lib.tree_attention_workspace(a))
             a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
-        return ctx, a, work
+        return ctx, a, (work, lse)
     if case["op"] == "evict":
         rows, b = case["rows"], case["budget"]
         s = lib.SelectArgs(weights=_ptr(st["weights"]), lens=_ptr(st["lens"]), kept=_ptr(st["kept"]),
