@@ -297,7 +297,7 @@ int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters
  *  - head_dim is 64 or 128 (POCR_ERR_UNSUPPORTED otherwise); heads is a
  *    multiple of kv_heads, query head h reads KV head h / (heads / kv_heads).
  *  - Sums and softmax statistics are fp32; products keep 22 bits of each
- *    operand.  A row whose query is NaN, or that sees a NaN or an infinite
+ *    operand, or 2^-32 of the largest of its row and head.  A row whose query is NaN, or that sees a NaN or an infinite
  *    value, comes out not finite; what an infinite query or key gives its rows
  *    is unspecified (sizes of 2^110 and more count as infinite).  Rows that do
  *    not see such a key or value do not change.

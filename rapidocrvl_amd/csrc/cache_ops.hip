@@ -147,17 +147,62 @@ int tree_params(const pocr_tree_args *a, const char *op, CacheAttn *p) {
     return POCR_OK;
 }
 
-template <bool TREE>
-int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs) {
-    const dim3 grid(p.n, p.heads, seqs);
-    if (head_dim == 128) hipLaunchKernelGGL((k_cache_attn_rows<128, TREE>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((k_cache_attn_rows<64, TREE>), grid, dim3(256), 0, s, p);
+int round_up_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Row tiles and key shares of one attention call.  `rows` query rows (token,
+// head) per sequence and KV head over at most `keys` keys.
+struct AttnShape {
+    int qt, tiles, splits;
+    int64_t bytes;  // workspace
+};
+AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim) {
+    AttnShape a;
+    a.qt = rows > 64 ? 2 : 1;
+    a.tiles = round_up_div(rows, 64 * a.qt);
+    const int64_t work = a.tiles * groups;
+    const int64_t want = std::max<int64_t>(1, 512 / work);
+    a.splits = (int)std::min<int64_t>({want, 64, std::max<int64_t>(1, keys / (kBlock * kMinSteps))});
+    a.bytes = a.splits == 1 ? 0 : work * a.splits * 64 * a.qt * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
+    return a;
+}
+
+template <int HD, bool TREE, bool SHAPED, int QT>
+int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
+    AttnPlan pl{sh.tiles, sh.splits, nullptr, nullptr};
+    if (sh.splits > 1) {
+        pl.part = static_cast<float *>(work);
+        pl.parts = reinterpret_cast<int32_t *>(static_cast<float *>(work) +
+                                               (size_t)p.kvh * seqs * sh.tiles * sh.splits * 64 * QT * (HD + 2));
+    }
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(kAttnThreads), 0, s, p, pl);
+    if (sh.splits > 1)
+        hipLaunchKernelGGL((k_cache_attn_join<HD, QT>), dim3(sh.tiles * (64 * QT / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl, seqs);
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }
 
-int64_t prompt_workspace(const pocr_prompt_args *a) { return 0; }
-int64_t tree_workspace(const pocr_tree_args *a) { return 0; }
+template <bool TREE>
+int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, void *work) {
+    const AttnShape sh = attn_shape((int64_t)p.n * p.group, p.rows, (int64_t)p.kvh * seqs, head_dim);
+    const int pick = (head_dim == 128 ? 4 : 0) + (p.cap > 0.0f || p.slopes ? 2 : 0) + (sh.qt == 2 ? 1 : 0);
+    switch (pick) {
+    case 0: return launch_attn_t<64, TREE, false, 1>(s, p, sh, work, seqs);
+    case 1: return launch_attn_t<64, TREE, false, 2>(s, p, sh, work, seqs);
+    case 2: return launch_attn_t<64, TREE, true, 1>(s, p, sh, work, seqs);
+    case 3: return launch_attn_t<64, TREE, true, 2>(s, p, sh, work, seqs);
+    case 4: return launch_attn_t<128, TREE, false, 1>(s, p, sh, work, seqs);
+    case 5: return launch_attn_t<128, TREE, false, 2>(s, p, sh, work, seqs);
+    case 6: return launch_attn_t<128, TREE, true, 1>(s, p, sh, work, seqs);
+    default: return launch_attn_t<128, TREE, true, 2>(s, p, sh, work, seqs);
+    }
+}
+
+int64_t prompt_workspace(const pocr_prompt_args *a) {
+    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), (int64_t)a->rows_before + a->n, a->kv_heads, a->head_dim).bytes;
+}
+int64_t tree_workspace(const pocr_tree_args *a) {
+    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), a->max_rows, (int64_t)a->kv_heads * a->seqs, a->head_dim).bytes;
+}
 
 // the addresses of `caches` blocks of `rows` rows overlap
 bool overlap(const void *a, int64_t acs, int64_t ast, int arows, const void *b, int64_t bcs, int64_t bst, int brows,
@@ -214,7 +259,7 @@ extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, v
     p.group = a->heads / a->kv_heads;
     p.scale = default_scale(a->scale, a->head_dim);
     p.cap = a->cap;
-    return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1);
+    return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1, a->workspace);
 }
 
 extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {
@@ -233,7 +278,7 @@ extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void 
     p.v_st = a->v_stride;
     p.o_ss = a->out_seq_stride;
     p.o_st = a->out_stride;
-    return launch_attn<true>((hipStream_t)stream, p, a->head_dim, a->seqs);
+    return launch_attn<true>((hipStream_t)stream, p, a->head_dim, a->seqs, a->workspace);
 }
 
 extern "C" int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {

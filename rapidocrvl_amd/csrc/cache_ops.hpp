@@ -65,79 +65,540 @@ __device__ __forceinline__ float shape_score(float dot, float scale, float cap, 
     return s - slope * fabsf((float)dist);
 }
 
-// One workgroup per (token, head, sequence), one key per wave and step: each
-// lane holds head_dim / 64 dims, an online softmax per wave, joined at the end.
-template <int HD, bool TREE>
-__global__ void __launch_bounds__(256) k_cache_attn_rows(CacheAttn p) {
-    constexpr int D = HD / 64;
-    __shared__ float sm[4], sl[4], sacc[4][HD];
-    __shared__ uint64_t sbits[64];
-    __shared__ int sdepth[64];
-    const int t = blockIdx.x, h = blockIdx.y, s = blockIdx.z, g = h / p.group;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int lo = 0, hi = 0, len = p.rows, count = p.n, own = p.rows0 + t;
+// ---------------------------------------------------------------------------
+// attention on the matrix cores
+// ---------------------------------------------------------------------------
+// Products of fp32 operands as products of their fp16 halves x = hi + lo (11
+// bits each, so 22 of the operand's 24): hi·hi + hi·lo + lo·hi, three
+// v_mfma_f32_16x16x32_f16 where the fp32 matrix instruction takes eight times
+// one's time.  Exponents are taken out first, by a power of two per query row,
+// key row, value row and row of weights, so that no size of an operand leaves
+// fp16's range and none costs another its bits.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void split_h(float a, float b, v2h &hi, v2h &lo) {
+    hi = __builtin_convertvector((v2f){a, b}, v2h);
+    lo = __builtin_convertvector((v2f){a - (float)hi[0], b - (float)hi[1]}, v2h);
+}
+
+constexpr int kTop = 8;         // operand rows are scaled to sizes in [2^(kTop-1), 2^kTop): fp16's last step is 2^-32 of that
+constexpr int kMaxExp = 110;    // rows of larger exponents count as infinite
+constexpr float kLowest = -3.0e38f;
+constexpr int kBlock = 32;      // keys per step
+constexpr int kAttnThreads = 256;
+
+// exponent e of a row from the bits of its largest size: |x| < 2^e
+__device__ __forceinline__ int row_exp(uint32_t bits) { return max((int)(bits >> 23) - 126, -kMaxExp); }
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t umax3(uint32_t a, uint32_t b, uint32_t c) { return max(max(a, b), c); }
+
+// max over the lanes l, l^16, l^32, l^48 (an MFMA column's four lane groups)
+__device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+__device__ __forceinline__ float groups_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// max over 8 consecutive lanes
+__device__ __forceinline__ uint32_t lanes8_umax(uint32_t v) {
+    v = max(v, __float_as_uint(xchg<XQ1>(__uint_as_float(v))));
+    v = max(v, __float_as_uint(xchg<XQ2>(__uint_as_float(v))));
+    return max(v, __float_as_uint(xchg<XM8>(__uint_as_float(v))));
+}
+
+// tanh to about 2^-23 of its value: below 1.75 Lambert's continued fraction
+// x/(1 + x²/(3 + x²/(5 + … x²/13))) as a quotient of polynomials (off by 2^-27
+// at 1.75), above it 1 − 2/(e^2x + 1), where the difference no longer cancels
+__device__ __forceinline__ float tanh_f(float x) {
+    const float a = fabsf(x), z = a * a;
+    const bool low = a < 1.75f;
+    const float e = __builtin_amdgcn_exp2f(fminf(a, 20.0f) * (2.0f * kLog2e));
+    const float num = a * fmaf(z, fmaf(z, z + 378.0f, 17325.0f), 135135.0f);
+    const float den = fmaf(z, fmaf(z, fmaf(z, 28.0f, 3150.0f), 62370.0f), 135135.0f);
+    const float d = low ? den : e + 1.0f, n = low ? num : 2.0f;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    const float t = low ? n * r : fmaf(-n, r, 1.0f);
+    return copysignf(t, x);
+}
+
+// the rows of one tile and its share of the keys
+struct AttnTile {
+    int lo, hi;        // keys some row of the tile sees: [lo, hi)
+    int parts;         // shares they are cut into
+    int from, to;      // this share's steps of kBlock keys, from lo rounded down
+};
+
+// steps of a tile cut into at most `splits` shares of at least kMinSteps
+constexpr int kMinSteps = 2;
+__device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int part) {
+    t.lo &= ~(kBlock - 1);
+    const int steps = max(0, (t.hi - t.lo + kBlock - 1) / kBlock);
+    t.parts = min(splits, max(1, steps / kMinSteps));
+    t.from = (int)((int64_t)steps * part / t.parts);
+    t.to = (int)((int64_t)steps * (part + 1) / t.parts);
+}
+
+// what the launch adds to a call's arguments
+struct AttnPlan {
+    int tiles;        // row tiles per (sequence, KV head)
+    int splits;       // shares a tile's keys may be cut into; 1: no workspace
+    float *part;      // [tile][split][64·QT rows][HD] sums, then [rows][2] maximum and denominator
+    int32_t *parts;   // [tile] shares in use
+};
+
+// Workgroup: 64·QT rows (token, head of the KV head's group) of one sequence
+// and KV head, four waves of 16·QT rows; one share of the keys, 32 a step.  A
+// step's K and V rows are read once, in whole 128-byte lines, split into their
+// halves and laid into LDS in the order the matrix instructions take them:
+//   K  lane l = 16·q + r of a 16-key tile: key r, dims 32c + 8q .. +7
+//   V  lane l = 16·q + j: keys 4q .. 4q+3 and 16+4q .. +3, dim 32d + 2j + t
+// Scores come out transposed (lane l: query row l%16, keys 4·(l/16) + i of each
+// 16), so a row's maximum, denominator and weights stay with its four lanes and
+// the weights are the second product's operand as they are; the sums come out
+// transposed too (lane: the same query row, 8 consecutive dims of each 32).
+// Two LDS buffers: a step's products run on one while the next step's rows
+// arrive and are laid into the other.
+template <int HD, bool TREE, bool SHAPED, int QT>
+__global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
+    constexpr int C = HD / 32;              // 32-dim chunks
+    constexpr int kRows = 64 * QT;
+    constexpr int kVKeys = HD == 128 ? 8 : 4;  // keys a lane lays out of V
+    constexpr int kKBytes = 2 * C * 2 * 1024, kVBytes = C * 2 * 2 * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t sk[2][kKBytes], sv[2][kVBytes];
+    __shared__ __attribute__((aligned(16))) float s_kf[2][kBlock], s_vf[2][kBlock];
+    __shared__ __attribute__((aligned(16))) uint32_t s_vmax[C][kBlock];
+    __shared__ uint64_t s_bits[64];
+    __shared__ int s_depth[64], s_lo, s_hi;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
+    const int g = blockIdx.y, s = blockIdx.z;
+    const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
+    const int first_row = tile * kRows;
+    int len = 0, count = p.n;
     if (TREE) {
-        const SeqRows r = seq_rows(p, s);
-        len = r.len;
-        count = r.count;
-        if (t >= count) return;
+        const SeqRows q = seq_rows(p, s);
+        len = q.len;
+        count = q.count;
+    }
+    const int rows = count * p.group;
+    const size_t slot = ((size_t)s * p.kvh + g) * pl.tiles + tile;
+    if (first_row >= rows) {
+        if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = 0;
+        return;
+    }
+    // the keys of the tile
+    AttnTile t{0, 0, 1, 0, 0};
+    const int tok0 = first_row / p.group, tok1 = (min(first_row + kRows, rows) - 1) / p.group;
+    if (TREE) {
+        t.hi = len + count;
         if (wave == 0) {
             const uint64_t b = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
-            sbits[lane] = b;
-            sdepth[lane] = __popcll(b) - 1;
+            s_bits[lane] = b;
+            s_depth[lane] = __popcll(b) - 1;
         }
         __syncthreads();
-        hi = len + count;
+    } else if (p.begin) {
+        if (tid == 0) {
+            s_lo = p.rows;
+            s_hi = 0;
+        }
+        __syncthreads();
+        const int tok = tok0 + tid;
+        if (tok <= tok1) {  // at most kRows tokens
+            const int b = min(max(p.begin[tok], 0), p.rows), e = min(max(p.end[tok], 0), p.rows);
+            if (b < e) {
+                atomicMin(&s_lo, b);
+                atomicMax(&s_hi, e);
+            }
+        }
+        __syncthreads();
+        t.lo = s_lo;
+        t.hi = s_hi;
     } else {
-        hi = p.end ? min(max(p.end[t], 0), p.rows) : p.rows0 + t + 1;
-        lo = p.begin ? min(max(p.begin[t], 0), p.rows) : 0;
+        t.hi = p.rows0 + tok1 + 1;
     }
-    const int32_t *pos = TREE && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
-    const uint64_t bits = TREE ? sbits[t] : 0;
-    if (TREE) own = pos ? pos[len + t] : len + sdepth[t];
-    const float slope = p.slopes ? p.slopes[h] : 0.0f;
-    float q[D], acc[D];
+    cut_tile(t, pl.splits, part);
+    if (part >= t.parts) return;
+    if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
+
+    // query rows: halves, scale, what they see
+    v8h qh[QT][C], ql[QT][C];
+    float qf[QT], slope[QT];
+    int row_lo[QT], row_hi[QT], row_pos[QT];
+    uint64_t bits[QT];
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-        q[d] = p.q[s * p.q_ss + t * p.q_st + h * HD + 64 * d + lane];
-        acc[d] = 0.0f;
+    for (int u = 0; u < QT; ++u) {
+        const int row = first_row + (wave * QT + u) * 16 + r16;
+        const bool live = row < rows;
+        const int tok = live ? row / p.group : tok0, h = g * p.group + (live ? row % p.group : 0);
+        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 8 * kg;
+        float x[C][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[c][i] = a[i];
+                x[c][4 + i] = b[i];
+                top = umax3(top, abs_bits(a[i]), abs_bits(b[i]));
+            }
+        }
+        const int e = row_exp(groups_umax(top));
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                v2h hi, lo;
+                split_h(__builtin_ldexpf(x[c][i], kTop - e), __builtin_ldexpf(x[c][i + 1], kTop - e), hi, lo);
+                qh[u][c][i] = hi[0];
+                qh[u][c][i + 1] = hi[1];
+                ql[u][c][i] = lo[0];
+                ql[u][c][i + 1] = lo[1];
+            }
+        qf[u] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
+        slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+        row_lo[u] = row_hi[u] = row_pos[u] = 0;
+        bits[u] = 0;
+        if (TREE) {
+            if (live) {
+                row_hi[u] = len;
+                bits[u] = s_bits[tok];
+                if (SHAPED) row_pos[u] = p.pos ? p.pos[((size_t)s * p.kvh + g) * p.side + len + tok] : len + s_depth[tok];
+            }
+        } else if (live) {
+            row_lo[u] = p.begin ? min(max(p.begin[tok], 0), p.rows) : 0;
+            row_hi[u] = p.end ? min(max(p.end[tok], 0), p.rows) : p.rows0 + tok + 1;
+            row_pos[u] = p.rows0 + tok;
+        }
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = lo + wave; j < hi; j += 4) {
-        if (TREE && j >= len && !(bits >> (j - len) & 1)) continue;
-        float dot = 0.0f;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+
+    // a step's rows: K keys 8·wave + lane/8, dims 4·(lane%8) + 32c; V the keys
+    // of the lane's group, two dims of the wave's 32
+    const int k_key = 8 * wave + (lane >> 3), k_part = lane & 7;
+    const int v_q = HD == 128 ? wave : wave & 1, v_half = HD == 128 ? 0 : wave >> 1;
+    const float *kbase = p.k + s * p.k_ss + g * HD + 4 * k_part;
+    const float *vbase = p.v + s * p.v_ss + g * HD + 32 * v_q + 2 * r16;
+    const int last = t.hi - 1;
+    v4f kx[C];
+    v2f vx[kVKeys];
+    auto load = [&](int step) {
+        const int k0 = t.lo + step * kBlock;
+        const float *ks = kbase + min(k0 + k_key, last) * p.k_st;
 #pragma unroll
-        for (int d = 0; d < D; ++d) dot = fmaf(q[d], p.k[s * p.k_ss + j * p.k_st + g * HD + 64 * d + lane], dot);
-        const int at = TREE ? (pos ? pos[j] : (j < len ? j : len + sdepth[j - len])) : j;
-        const float x = shape_score(wave_sum(dot), p.scale, p.cap, slope, own - at);
-        const float mn = fmaxf(m, x);
-        const float old = m == -INFINITY ? 0.0f : expf(m - mn), e = expf(x - mn);
-        l = l * old + e;
+        for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
 #pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] = acc[d] * old + e * p.v[s * p.v_ss + j * p.v_st + g * HD + 64 * d + lane];
-        m = mn;
+        for (int i = 0; i < kVKeys; ++i) {
+            const int key = HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i;
+            vx[i] = *reinterpret_cast<const v2f *>(vbase + min(k0 + key, last) * p.v_st);
+        }
+    };
+    // K into its buffer, and the sizes of V's rows
+    auto lay_k = [&](int b) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
+        const int e = row_exp(lanes8_umax(top));
+        if (k_part == 0) s_kf[b][k_key] = pow2(e - kTop);
+        const int q = k_part >> 1, key = k_key & 15;
+        uint8_t *dst = sk[b] + (k_key >> 4) * C * 2048 + (16 * q + (key ^ (q << 2))) * 16 + (k_part & 1) * 8;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            v2h h0, l0, h1, l1;
+            split_h(__builtin_ldexpf(kx[c][0], kTop - e), __builtin_ldexpf(kx[c][1], kTop - e), h0, l0);
+            split_h(__builtin_ldexpf(kx[c][2], kTop - e), __builtin_ldexpf(kx[c][3], kTop - e), h1, l1);
+            *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+        }
+        uint32_t m[kVKeys];
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) {
+            m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
+            m[i] = max(m[i], __float_as_uint(xchg<XQ1>(__uint_as_float(m[i]))));
+            m[i] = max(m[i], __float_as_uint(xchg<XQ2>(__uint_as_float(m[i]))));
+            m[i] = max(m[i], __float_as_uint(xchg<XM8>(__uint_as_float(m[i]))));
+            m[i] = max(m[i], __float_as_uint(xchg<XM16>(__uint_as_float(m[i]))));
+        }
+        if (r16 == 0)
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i)
+                s_vmax[v_q][HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i] = m[i];
+    };
+    // V into its buffer, once the sizes of all its quarters are there
+    auto lay_v = [&](int b) {
+        float x[kVKeys], y[kVKeys];
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) {
+            const int key = HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i;
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c) top = max(top, s_vmax[c][key]);
+            const int e = row_exp(top);
+            const bool bad = e > kMaxExp;
+            if (v_q == 0 && r16 == 0) s_vf[b][key] = bad ? __uint_as_float(0x7fc00000u) : pow2(e);
+            x[i] = bad ? 0.0f : __builtin_ldexpf(vx[i][0], kTop - e);
+            y[i] = bad ? 0.0f : __builtin_ldexpf(vx[i][1], kTop - e);
+        }
+        uint8_t *dst = sv[b] + v_q * 4096 + lane * 16 + v_half * 8;
+#pragma unroll
+        for (int i = 0; i < kVKeys; i += 4) {
+            v2h h0, l0, h1, l1;
+            split_h(x[i], x[i + 1], h0, l0);
+            split_h(x[i + 2], x[i + 3], h1, l1);
+            *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+            split_h(y[i], y[i + 1], h0, l0);
+            split_h(y[i + 2], y[i + 3], h1, l1);
+            *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+        }
+    };
+
+    v4f o[QT][2 * C];
+    float m[QT], l[QT];
+    int a[QT];  // o holds the weighted sums, relative to 2^m, times 2^(14 + kTop - a)
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        m[u] = kLowest;
+        l[u] = 0.0f;
+        a[u] = -16384;
+#pragma unroll
+        for (int d = 0; d < 2 * C; ++d) o[u][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (lane == 0) {
-        sm[wave] = m;
-        sl[wave] = l;
+    const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
+
+    if (t.from < t.to) {
+        load(t.from);
+        lay_k(0);
+        __syncthreads();
+        lay_v(0);
+        __syncthreads();
     }
+    for (int step = t.from; step < t.to; ++step) {
+        const int b = (step - t.from) & 1, k0 = t.lo + step * kBlock;
+        const bool more = step + 1 < t.to;
+        if (more) load(step + 1);
+        // what each row sees of the step's keys, as bits
+        uint32_t see[QT];
+        bool any = false;
 #pragma unroll
-    for (int d = 0; d < D; ++d) sacc[wave][64 * d + lane] = acc[d];
-    __syncthreads();
-    if (wave) return;
-    float mm = -INFINITY, ll = 0.0f;
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w]);
-    float o[D] = {};
-    for (int w = 0; w < 4; ++w) {
-        const float e = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - mm);
-        ll += sl[w] * e;
+        for (int u = 0; u < QT; ++u) {
+            const int n1 = min(max(row_hi[u] - k0, 0), 32), n0 = min(max(row_lo[u] - k0, 0), 32);
+            see[u] = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
+            if (TREE) {
+                const int off = k0 - len;  // the step's first key among the drafted ones
+                if (off > -32 && off < 64) see[u] |= (uint32_t)(off >= 0 ? bits[u] >> off : bits[u] << -off);
+            }
+            any = any || see[u];
+        }
+        if (__any(any)) {
+            v4f sc[QT][2];
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] += sacc[w][64 * d + lane] * e;
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int u = 0; u < QT; ++u) sc[u][kt] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                const uint8_t *src = sk[b] + kt * C * 2048 + (16 * kg + (r16 ^ (kg << 2))) * 16;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const v8h kh = *reinterpret_cast<const v8h *>(src + c * 2048);
+                    const v8h kl = *reinterpret_cast<const v8h *>(src + c * 2048 + 1024);
+#pragma unroll
+                    for (int u = 0; u < QT; ++u) {
+                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[u][c], sc[u][kt], 0, 0, 0);
+                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[u][c], sc[u][kt], 0, 0, 0);
+                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[u][c], sc[u][kt], 0, 0, 0);
+                    }
+                }
+            }
+            float kf[8], vf[8];
+            int kpos[8];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const v4f fk = *reinterpret_cast<const v4f *>(&s_kf[b][16 * kt + 4 * kg]);
+                const v4f fv = *reinterpret_cast<const v4f *>(&s_vf[b][16 * kt + 4 * kg]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    kf[4 * kt + i] = fk[i];
+                    vf[4 * kt + i] = fv[i];
+                    const int key = k0 + 16 * kt + 4 * kg + i;
+                    kpos[4 * kt + i] = key;
+                    if (TREE && SHAPED) {
+                        if (pos) kpos[4 * kt + i] = pos[min(key, last)];
+                        else if (key >= len) kpos[4 * kt + i] = len + s_depth[min(key - len, 63)];
+                    }
+                }
+            }
+            v8h ph[QT], pL[QT];
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+                const bool whole = __all(see[u] == 0xffffffffu);
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = sc[u][e >> 2][e & 3] * kf[e] * qf[u];
+                    if (SHAPED) {
+                        if (p.cap > 0.0f) x[e] = p.cap * tanh_f(x[e] * inv_cap);
+                        x[e] = fmaf(x[e], kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])));
+                    }
+                }
+                if (!whole) {
+                    const uint32_t mine = see[u] >> (4 * kg);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = groups_max(top);
+                if (__any(top > m[u])) {
+                    const float mn = top > m[u] ? ceilf(top) + 2.0f : m[u];
+                    l[u] *= __builtin_amdgcn_exp2f(m[u] - mn);
+                    a[u] = max(a[u] - (int)fminf(mn - m[u], 16384.0f), -16384);
+                    m[u] = mn;
+                }
+                float w[8], sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(x[e] - m[u]);
+                    sum += w[e];
+                    w[e] *= vf[e];
+                }
+                l[u] += sum;
+                if (!whole) {  // a bad value row is NaN here, for the rows that see it only
+                    const uint32_t mine = see[u] >> (4 * kg);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? w[e] : 0.0f;
+                }
+                float big = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
+                big = groups_max(big);
+                const int need = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -16384;  // big < 2^need
+                if (__any(need > a[u])) {
+                    const int an = need > a[u] ? need + 3 : a[u];
+                    const float f = __builtin_ldexpf(1.0f, max(a[u] - an, -200));
+#pragma unroll
+                    for (int d = 0; d < 2 * C; ++d) o[u][d] *= f;
+                    a[u] = an;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    v2h hi, lo;
+                    split_h(__builtin_ldexpf(w[e], 14 - a[u]), __builtin_ldexpf(w[e + 1], 14 - a[u]), hi, lo);
+                    ph[u][e] = hi[0];
+                    ph[u][e + 1] = hi[1];
+                    pL[u][e] = lo[0];
+                    pL[u][e + 1] = lo[1];
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 2 * C; ++d) {
+                const v8h vh = *reinterpret_cast<const v8h *>(sv[b] + d * 2048 + lane * 16);
+                const v8h vl = *reinterpret_cast<const v8h *>(sv[b] + d * 2048 + 1024 + lane * 16);
+#pragma unroll
+                for (int u = 0; u < QT; ++u) {
+                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[u], o[u][d], 0, 0, 0);
+                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pL[u], o[u][d], 0, 0, 0);
+                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[u], o[u][d], 0, 0, 0);
+                }
+            }
+        }
+        if (more) {
+            lay_k(b ^ 1);
+            __syncthreads();
+            lay_v(b ^ 1);
+            __syncthreads();
+        }
     }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+
 #pragma unroll
-    for (int d = 0; d < D; ++d) p.out[s * p.o_ss + t * p.o_st + h * HD + 64 * d + lane] = o[d] * inv;
-    if (p.lse && lane == 0) p.lse[((size_t)s * p.n + t) * p.heads + h] = mm + logf(ll);
+    for (int u = 0; u < QT; ++u) {
+        const int local = (wave * QT + u) * 16 + r16, row = first_row + local;
+        const float total = groups_sum(l[u]);
+        if (row >= rows) continue;
+        if (t.parts > 1) {
+            float *dst = pl.part + ((slot * pl.splits + part) * kRows + local) * HD + 8 * kg;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v4f x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(o[u][2 * c + (i & 1)][2 * h + (i >> 1)], a[u] - 14 - kTop);
+                    *reinterpret_cast<v4f *>(dst + 32 * c + 4 * h) = x;
+                }
+            if (kg == 0) {
+                float *st = pl.part + (size_t)p.kvh * gridDim.z * pl.tiles * pl.splits * kRows * HD +
+                            ((slot * pl.splits + part) * kRows + local) * 2;
+                st[0] = m[u];
+                st[1] = total;
+            }
+            continue;
+        }
+        const int tok = row / p.group, h = g * p.group + row % p.group;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        float *dst = p.out + s * p.o_ss + tok * p.o_st + h * HD + 8 * kg;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                v4f x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(o[u][2 * c + (i & 1)][2 * y + (i >> 1)] * inv, a[u] - 14 - kTop);
+                *reinterpret_cast<v4f *>(dst + 32 * c + 4 * y) = x;
+            }
+        if (p.lse && kg == 0)
+            p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m[u] + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    }
+}
+
+// Joins the shares of the tiles that were cut: one half wave per row and 32
+// lanes, or HD / 4, of float4; rows of uncut tiles are done already.
+template <int HD, int QT>
+__global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan pl, int seqs) {
+    constexpr int kRows = 64 * QT, kLanes = HD / 4, kPer = 256 / kLanes;
+    const int per_tile = kRows / kPer;
+    const int tile = blockIdx.x / per_tile, local = blockIdx.x % per_tile * kPer + threadIdx.x / kLanes;
+    const int g = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes;
+    const size_t slot = ((size_t)s * p.kvh + g) * pl.tiles + tile;
+    const int parts = pl.parts[slot];
+    const int rows = (p.lens ? seq_rows(p, s).count : p.n) * p.group, row = tile * kRows + local;
+    if (parts < 2 || row >= rows) return;
+    const float *st = pl.part + (size_t)p.kvh * seqs * pl.tiles * pl.splits * kRows * HD + (slot * pl.splits * kRows + local) * 2;
+    const float *src = pl.part + (slot * pl.splits * kRows + local) * HD + 4 * lane;
+    float m = kLowest;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, st[(size_t)i * kRows * 2]);
+    float total = 0.0f;
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < parts; ++i) {
+        const float f = __builtin_amdgcn_exp2f(st[(size_t)i * kRows * 2] - m);
+        total = fmaf(st[(size_t)i * kRows * 2 + 1], f, total);
+        const v4f x = *reinterpret_cast<const v4f *>(src + (size_t)i * kRows * HD);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[c], f, acc[c]);
+    }
+    const int tok = row / p.group, h = g * p.group + row % p.group;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    *reinterpret_cast<v4f *>(p.out + s * p.o_ss + tok * p.o_st + h * HD + 4 * lane) = acc * inv;
+    if (p.lse && lane == 0)
+        p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
 }
 
 // One wave per (row, KV head, sequence): the weights of its tokens and heads, in order.

@@ -29,6 +29,7 @@ def attention(q, k, v, seen, scale, cap=0.0, slope=None, dist=None):
     k = np.where(used[:, None], k, 0.0)
     s = q @ k.T * scale
     err = np.abs(q) @ np.abs(k).T * scale * (17 * U + 2 * 2.0 ** -21) + np.abs(s) * 4 * U
+    err += scale * 2.0 ** -32 * (np.abs(q).max(1)[:, None] * np.abs(k).sum(1) + np.abs(q).sum(1)[:, None] * np.abs(k).max(1))
     if cap:
         s = cap * np.tanh(s / cap)
         err = err + np.abs(s) * 8 * U
@@ -53,6 +54,8 @@ def attention(q, k, v, seen, scale, cap=0.0, slope=None, dist=None):
         return None, lse, p, None, lse_err, p_err
     v = np.where(used[:, None], np.asarray(v, np.float64), 0.0)
     out_err = p_err @ np.abs(v) + (p @ np.abs(v)) * (2 * 2.0 ** -21 + steps[:, None] + 2 * U) + 1e-38
+    top = np.abs(v).max(1)
+    out_err += (p @ top)[:, None] * 2.0 ** -32 + ((p * top).max(1) * seen.sum(1))[:, None] * 2.0 ** -36
     return p @ v, lse, p, out_err, lse_err, p_err
 
 
