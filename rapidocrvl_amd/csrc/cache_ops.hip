@@ -291,9 +291,16 @@ extern "C" int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *a, void *
     CACHE_OP_ENTER(ctx, stream, op);
     p.weights = a->weights;
     p.take = a->take;
-    const dim3 grid(p.rows, p.kvh, a->seqs);
-    if (a->head_dim == 128) hipLaunchKernelGGL(k_cache_weights_rows<128>, grid, dim3(64), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(k_cache_weights_rows<64>, grid, dim3(64), 0, (hipStream_t)stream, p);
+    const dim3 grid((p.rows + kWKeys - 1) / kWKeys, p.kvh, a->seqs);
+    hipStream_t s = (hipStream_t)stream;
+    const bool shaped = p.cap > 0.0f || p.slopes;
+    if (a->head_dim == 128) {
+        if (shaped) hipLaunchKernelGGL((k_cache_weights<128, true>), grid, dim3(kAttnThreads), 0, s, p);
+        else hipLaunchKernelGGL((k_cache_weights<128, false>), grid, dim3(kAttnThreads), 0, s, p);
+    } else {
+        if (shaped) hipLaunchKernelGGL((k_cache_weights<64, true>), grid, dim3(kAttnThreads), 0, s, p);
+        else hipLaunchKernelGGL((k_cache_weights<64, false>), grid, dim3(kAttnThreads), 0, s, p);
+    }
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }

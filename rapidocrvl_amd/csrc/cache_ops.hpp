@@ -58,13 +58,6 @@ __device__ __forceinline__ SeqRows seq_rows(const CacheAttn &p, int s) {
     return {min(max(p.lens[s], 0), p.rows - count), count};
 }
 
-// s = scale·q·k with the cap and the distance bias applied
-__device__ __forceinline__ float shape_score(float dot, float scale, float cap, float slope, int dist) {
-    float s = dot * scale;
-    if (cap > 0.0f) s = cap * tanhf(s / cap);
-    return s - slope * fabsf((float)dist);
-}
-
 // ---------------------------------------------------------------------------
 // attention on the matrix cores
 // ---------------------------------------------------------------------------
@@ -96,6 +89,22 @@ __device__ __forceinline__ int row_exp(uint32_t bits) { return max((int)(bits >>
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ uint32_t umax3(uint32_t a, uint32_t b, uint32_t c) { return max(max(a, b), c); }
+
+// a lane's share of a row, scaled by its exponent, as halves
+template <int C>
+__device__ __forceinline__ void split_row(const float (&x)[C][8], int e, v8h (&hi)[C], v8h (&lo)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            v2h h, l;
+            split_h(__builtin_ldexpf(x[c][i], kTop - e), __builtin_ldexpf(x[c][i + 1], kTop - e), h, l);
+            hi[c][i] = h[0];
+            hi[c][i + 1] = h[1];
+            lo[c][i] = l[0];
+            lo[c][i + 1] = l[1];
+        }
+}
 
 // max over the lanes l, l^16, l^32, l^48 (an MFMA column's four lane groups)
 __device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
@@ -264,17 +273,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
             }
         }
         const int e = row_exp(groups_umax(top));
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                v2h hi, lo;
-                split_h(__builtin_ldexpf(x[c][i], kTop - e), __builtin_ldexpf(x[c][i + 1], kTop - e), hi, lo);
-                qh[u][c][i] = hi[0];
-                qh[u][c][i + 1] = hi[1];
-                ql[u][c][i] = lo[0];
-                ql[u][c][i + 1] = lo[1];
-            }
+        split_row<C>(x, e, qh[u], ql[u]);
         qf[u] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
         slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
         row_lo[u] = row_hi[u] = row_pos[u] = 0;
@@ -601,36 +600,152 @@ __global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan p
         p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
 }
 
-// One wave per (row, KV head, sequence): the weights of its tokens and heads, in order.
-template <int HD>
-__global__ void __launch_bounds__(64) k_cache_weights_rows(CacheAttn p) {
-    constexpr int D = HD / 64;
-    const int j = blockIdx.x, g = blockIdx.y, s = blockIdx.z, lane = threadIdx.x;
-    const SeqRows r = seq_rows(p, s);
-    if (j >= r.len + r.count) return;
-    const uint64_t bits = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
-    const int32_t *pos = p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
-    const int depth_j = j < r.len ? 0 : __popcll(__shfl((unsigned long long)bits, j - r.len)) - 1;
-    const int at = pos ? pos[j] : (j < r.len ? j : r.len + depth_j);
-    float k[D];
+// The weights of cache rows.  Workgroup: 64 rows of one sequence and KV head,
+// 16 a wave, their halves in registers throughout; the query rows (token, head)
+// pass through LDS 64 at a time, laid out as the matrix instructions take them.
+// A lane sums its query row of each 16 for four keys; the sum over a key's 16
+// lanes ends the kernel, so the order of every sum is fixed.
+constexpr int kWKeys = 64, kWRows = 64;
+template <int HD, bool SHAPED>
+__global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) {
+    constexpr int C = HD / 32;
+    __shared__ __attribute__((aligned(16))) uint8_t sq[4 * C * 2 * 1024];
+    __shared__ float s_qf[kWRows], s_lse[kWRows], s_slope[kWRows];
+    __shared__ int s_pos[kWRows];
+    __shared__ uint64_t s_see[kWRows];
+    __shared__ uint64_t s_bits[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
+    const int g = blockIdx.y, s = blockIdx.z, key0 = blockIdx.x * kWKeys;
+    const SeqRows q = seq_rows(p, s);
+    const int end = q.len + q.count;
+    if (key0 >= end || q.count == 0) return;
+    const uint64_t mine = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
+    if (wave == 0) s_bits[lane] = mine;
+    const uint64_t take = p.take ? p.take[s] : ~0ull;
+    const int32_t *pos = SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
+
+    v8h kh[C], kl[C];
+    float kf[4];
+    int kpos[4];
+    {
+        const float *src = p.k + s * p.k_ss + min(key0 + 16 * wave + r16, end - 1) * p.k_st + g * HD + 8 * kg;
+        float x[C][8];
+        uint32_t top = 0;
 #pragma unroll
-    for (int d = 0; d < D; ++d) k[d] = p.k[s * p.k_ss + j * p.k_st + g * HD + 64 * d + lane];
-    float w = 0.0f;
-    for (int t = 0; t < r.count; ++t) {
-        const uint64_t b = __shfl((unsigned long long)bits, t);
-        if (p.take && !(p.take[s] >> t & 1)) continue;
-        if (j >= r.len && !(b >> (j - r.len) & 1)) continue;
-        const int own = pos ? pos[r.len + t] : r.len + __popcll(b) - 1;
-        for (int h = g * p.group; h < (g + 1) * p.group; ++h) {
-            float dot = 0.0f;
+        for (int c = 0; c < C; ++c) {
+            const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
 #pragma unroll
-            for (int d = 0; d < D; ++d) dot = fmaf(p.q[s * p.q_ss + t * p.q_st + h * HD + 64 * d + lane], k[d], dot);
-            const float x = shape_score(wave_sum(dot), p.scale, p.cap, p.slopes ? p.slopes[h] : 0.0f, own - at);
-            const float lse = p.lse[((size_t)s * p.n + t) * p.heads + h];
-            if (lse != -INFINITY) w += expf(x - lse);
+            for (int i = 0; i < 4; ++i) {
+                x[c][i] = a[i];
+                x[c][4 + i] = b[i];
+                top = umax3(top, abs_bits(a[i]), abs_bits(b[i]));
+            }
+        }
+        const int e = row_exp(groups_umax(top));
+        split_row<C>(x, e, kh, kl);
+        const float f = pow2(e - kTop);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * wave + 4 * kg + i;
+            kf[i] = __shfl(f, 4 * kg + i);
+            kpos[i] = key;
+            if (SHAPED) {
+                const int depth = __popcll(__shfl((unsigned long long)mine, min(max(key - q.len, 0), 63))) - 1;
+                if (pos) kpos[i] = pos[min(key, end - 1)];
+                else if (key >= q.len) kpos[i] = q.len + depth;
+            }
         }
     }
-    if (lane == 0) p.weights[((size_t)s * p.kvh + g) * p.side + j] += w;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const int rows = q.count * p.group;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float x[C][8];
+    auto load = [&](int row) {
+        const int tok = min(row, rows - 1) / p.group, h = g * p.group + min(row, rows - 1) % p.group;
+        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 8 * kg;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[c][i] = a[i];
+                x[c][4 + i] = b[i];
+            }
+        }
+    };
+    load(16 * wave + r16);
+    for (int row0 = 0; row0 < rows; row0 += kWRows) {
+        __syncthreads();
+        {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) top = umax3(top, abs_bits(x[c][i]), abs_bits(x[c][i + 1]));
+            const int e = row_exp(groups_umax(top));
+            v8h hi[C], lo[C];
+            split_row<C>(x, e, hi, lo);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                *reinterpret_cast<v8h *>(sq + ((wave * C + c) * 2) * 1024 + lane * 16) = hi[c];
+                *reinterpret_cast<v8h *>(sq + ((wave * C + c) * 2 + 1) * 1024 + lane * 16) = lo[c];
+            }
+            const int local = 16 * wave + r16, row = row0 + local;
+            if (kg == 0) {
+                const int tok = min(row, rows - 1) / p.group, h = g * p.group + min(row, rows - 1) % p.group;
+                const float lse = p.lse[((size_t)s * p.n + tok) * p.heads + h];
+                const bool live = row < rows && (take >> tok & 1) && lse != -INFINITY;
+                s_qf[local] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
+                s_lse[local] = live ? lse : INFINITY;
+                const uint64_t b = s_bits[tok];
+                s_see[local] = b;
+                if (SHAPED) {
+                    s_slope[local] = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+                    s_pos[local] = pos ? pos[q.len + tok] : q.len + __popcll(b) - 1;
+                }
+            }
+        }
+        __syncthreads();
+        if (row0 + kWRows < rows) load(row0 + kWRows + 16 * wave + r16);
+        const int tiles = min(4, (rows - row0 + 15) / 16);
+        for (int t = 0; t < tiles; ++t) {
+            v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const v8h qh = *reinterpret_cast<const v8h *>(sq + ((t * C + c) * 2) * 1024 + lane * 16);
+                const v8h ql = *reinterpret_cast<const v8h *>(sq + ((t * C + c) * 2 + 1) * 1024 + lane * 16);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[c], qh, sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c], ql, sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c], qh, sc, 0, 0, 0);
+            }
+            const int local = 16 * t + r16;
+            const float qf = s_qf[local], lse = s_lse[local];
+            const uint64_t see = s_see[local];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = sc[i] * kf[i] * qf;
+                if (SHAPED) {
+                    if (p.cap > 0.0f) y = p.cap * tanh_f(y * inv_cap);
+                    y = fmaf(y, kLog2e, -s_slope[local] * fabsf((float)(int)((uint32_t)s_pos[local] - (uint32_t)kpos[i])));
+                }
+                const int draft = key0 + 16 * wave + 4 * kg + i - q.len;
+                const bool seen = lse != INFINITY && (draft < 0 || (draft < 64 && (see >> draft & 1)));
+                acc[i] += seen ? __builtin_amdgcn_exp2f(fmaf(lse, -kLog2e, y)) : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        acc[i] += xchg<XQ1>(acc[i]);
+        acc[i] += xchg<XQ2>(acc[i]);
+        acc[i] += xchg<XM8>(acc[i]);
+        acc[i] += xchg<XM16>(acc[i]);
+    }
+    const int key = key0 + 16 * wave + 4 * kg + r16;
+    if (r16 < 4 && key < end) {
+        const float w = r16 == 0 ? acc[0] : (r16 == 1 ? acc[1] : (r16 == 2 ? acc[2] : acc[3]));
+        p.weights[((size_t)s * p.kvh + g) * p.side + key] += w;
+    }
 }
 
 // ---------------------------------------------------------------------------
