@@ -14,6 +14,7 @@ constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kMaxPromptRows = 1 << 22;
 constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
 constexpr int kMaxQueryHeads = 1024;
+constexpr int kImageTiles = 4;
 
 // The calling thread's device becomes the context's for one call.
 struct DeviceScope {
@@ -149,59 +150,72 @@ int tree_params(const pocr_tree_args *a, const char *op, CacheAttn *p) {
 
 int round_up_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Row tiles and key shares of one attention call.  `rows` query rows (token,
+// Row tiles and key shares of one attention call: `rows` query rows (token,
 // head) per sequence and KV head over at most `keys` keys.
 struct AttnShape {
-    int qt, tiles, splits;
-    int64_t bytes;  // workspace
+    int qt, tiles, splits, steps;  // steps: images of a prompt's rows, or 0
+    int64_t part_bytes, bytes;     // of the workspace
 };
-AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim) {
+template <int HD>
+constexpr int64_t image_bytes = StepImage<HD>::kBytes;
+AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, bool images) {
     AttnShape a;
     a.qt = rows > 64 ? 2 : 1;
     a.tiles = round_up_div(rows, 64 * a.qt);
     const int64_t work = a.tiles * groups;
     const int64_t want = std::max<int64_t>(1, 512 / work);
     a.splits = (int)std::min<int64_t>({want, 64, std::max<int64_t>(1, keys / (kBlock * kMinSteps))});
-    a.bytes = a.splits == 1 ? 0 : work * a.splits * 64 * a.qt * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
+    a.steps = images && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
+    a.part_bytes = a.splits == 1 ? 0 : work * a.splits * 64 * a.qt * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
+    a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
     return a;
 }
 
-template <int HD, bool TREE, bool SHAPED, int QT>
+template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
-    AttnPlan pl{sh.tiles, sh.splits, nullptr, nullptr};
+    AttnPlan pl{sh.tiles, sh.splits, nullptr, nullptr, nullptr, sh.steps};
     if (sh.splits > 1) {
         pl.part = static_cast<float *>(work);
         pl.parts = reinterpret_cast<int32_t *>(static_cast<float *>(work) +
                                                (size_t)p.kvh * seqs * sh.tiles * sh.splits * 64 * QT * (HD + 2));
     }
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(kAttnThreads), 0, s, p, pl);
+    if (IMG) {
+        uint8_t *img = static_cast<uint8_t *>(work) + sh.part_bytes;
+        pl.img = img;
+        hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps, p.kvh), dim3(kAttnThreads), 0, s, p, img);
+    }
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT, IMG>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(kAttnThreads), 0, s, p, pl);
     if (sh.splits > 1)
         hipLaunchKernelGGL((k_cache_attn_join<HD, QT>), dim3(sh.tiles * (64 * QT / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl, seqs);
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }
 
-template <bool TREE>
-int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, void *work) {
-    const AttnShape sh = attn_shape((int64_t)p.n * p.group, p.rows, (int64_t)p.kvh * seqs, head_dim);
-    const int pick = (head_dim == 128 ? 4 : 0) + (p.cap > 0.0f || p.slopes ? 2 : 0) + (sh.qt == 2 ? 1 : 0);
-    switch (pick) {
-    case 0: return launch_attn_t<64, TREE, false, 1>(s, p, sh, work, seqs);
-    case 1: return launch_attn_t<64, TREE, false, 2>(s, p, sh, work, seqs);
-    case 2: return launch_attn_t<64, TREE, true, 1>(s, p, sh, work, seqs);
-    case 3: return launch_attn_t<64, TREE, true, 2>(s, p, sh, work, seqs);
-    case 4: return launch_attn_t<128, TREE, false, 1>(s, p, sh, work, seqs);
-    case 5: return launch_attn_t<128, TREE, false, 2>(s, p, sh, work, seqs);
-    case 6: return launch_attn_t<128, TREE, true, 1>(s, p, sh, work, seqs);
-    default: return launch_attn_t<128, TREE, true, 2>(s, p, sh, work, seqs);
-    }
+template <int HD, bool TREE, bool SHAPED>
+int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
+    if constexpr (!TREE)
+        if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, 2, true>(s, p, sh, work, seqs);
+    return sh.qt == 2 ? launch_attn_t<HD, TREE, SHAPED, 2, false>(s, p, sh, work, seqs)
+                      : launch_attn_t<HD, TREE, SHAPED, 1, false>(s, p, sh, work, seqs);
 }
 
-int64_t prompt_workspace(const pocr_prompt_args *a) {
-    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), (int64_t)a->rows_before + a->n, a->kv_heads, a->head_dim).bytes;
+template <bool TREE>
+int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, const AttnShape &sh, void *work) {
+    const bool shaped = p.cap > 0.0f || p.slopes;
+    if (head_dim == 128)
+        return shaped ? launch_attn_s<128, TREE, true>(s, p, sh, work, seqs) : launch_attn_s<128, TREE, false>(s, p, sh, work, seqs);
+    return shaped ? launch_attn_s<64, TREE, true>(s, p, sh, work, seqs) : launch_attn_s<64, TREE, false>(s, p, sh, work, seqs);
 }
-int64_t tree_workspace(const pocr_tree_args *a) {
-    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), a->max_rows, (int64_t)a->kv_heads * a->seqs, a->head_dim).bytes;
+
+AttnShape prompt_attn(const pocr_prompt_args *a) {
+    const int64_t rows = (int64_t)a->rows_before + a->n;
+    // spans may leave out most of a long cache: its images are worth their
+    // making where all rows are seen, or not many more than the prompt's own
+    const bool images = !a->row_begin || a->rows_before <= 4 * (int64_t)a->n;
+    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), rows, a->kv_heads, a->head_dim, images);
+}
+AttnShape tree_attn(const pocr_tree_args *a) {
+    return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), a->max_rows, (int64_t)a->kv_heads * a->seqs, a->head_dim, false);
 }
 
 // the addresses of `caches` blocks of `rows` rows overlap
@@ -217,12 +231,12 @@ bool overlap(const void *a, int64_t acs, int64_t ast, int arows, const void *b, 
 
 extern "C" int64_t pocr_prompt_attention_workspace(const pocr_prompt_args *a) {
     RC(prompt_shape(a, "pocr_prompt_attention_workspace"));
-    return prompt_workspace(a);
+    return prompt_attn(a).bytes;
 }
 
 extern "C" int64_t pocr_tree_attention_workspace(const pocr_tree_args *a) {
     RC(tree_shape(a, "pocr_tree_attention_workspace"));
-    return tree_workspace(a);
+    return tree_attn(a).bytes;
 }
 
 extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, void *stream) {
@@ -236,7 +250,8 @@ extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, v
     if (!a->row_begin != !a->row_end) return fail(POCR_ERR_ARG, "%s: row_begin and row_end come together", op);
     for (const void *x : {(const void *)a->row_begin, (const void *)a->row_end, (const void *)a->slopes, (const void *)a->lse})
         RC(check_index(x, "an index or side buffer", op));
-    RC(check_workspace(a->workspace, a->workspace_bytes, prompt_workspace(a), op));
+    const AttnShape shape = prompt_attn(a);
+    RC(check_workspace(a->workspace, a->workspace_bytes, shape.bytes, op));
     CACHE_OP_ENTER(ctx, stream, op);
     CacheAttn p{};
     p.q = a->q;
@@ -259,7 +274,7 @@ extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, v
     p.group = a->heads / a->kv_heads;
     p.scale = default_scale(a->scale, a->head_dim);
     p.cap = a->cap;
-    return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1, a->workspace);
+    return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1, shape, a->workspace);
 }
 
 extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {
@@ -270,7 +285,8 @@ extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void 
     RC(check_rows(a->out, a->out_stride, (int64_t)a->heads * a->head_dim, "out", op));
     RC(check_outer(a->v_seq_stride, a->seqs, "v", op));
     RC(check_outer(a->out_seq_stride, a->seqs, "out", op));
-    RC(check_workspace(a->workspace, a->workspace_bytes, tree_workspace(a), op));
+    const AttnShape shape = tree_attn(a);
+    RC(check_workspace(a->workspace, a->workspace_bytes, shape.bytes, op));
     CACHE_OP_ENTER(ctx, stream, op);
     p.v = a->v;
     p.out = a->out;
@@ -278,7 +294,7 @@ extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void 
     p.v_st = a->v_stride;
     p.o_ss = a->out_seq_stride;
     p.o_st = a->out_stride;
-    return launch_attn<true>((hipStream_t)stream, p, a->head_dim, a->seqs, a->workspace);
+    return launch_attn<true>((hipStream_t)stream, p, a->head_dim, a->seqs, shape, a->workspace);
 }
 
 extern "C" int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *a, void *stream) {

@@ -75,10 +75,11 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ void split_h(float a, float b, v2h &hi, v2h &lo) {
     hi = __builtin_convertvector((v2f){a, b}, v2h);
-    lo = __builtin_convertvector((v2f){a - (float)hi[0], b - (float)hi[1]}, v2h);
+    lo = __builtin_convertvector((v2f){__builtin_fmaf((float)hi[0], -1.0f, a), __builtin_fmaf((float)hi[1], -1.0f, b)}, v2h);
 }
 
-constexpr int kTop = 8;         // operand rows are scaled to sizes in [2^(kTop-1), 2^kTop): fp16's last step is 2^-32 of that
+constexpr int kTop = 14;        // operand rows are scaled to sizes below 2^kTop
+constexpr int kSpread = 4;      // key (value) rows of one exponent's scale lie within 2^kSpread
 constexpr int kMaxExp = 110;    // rows of larger exponents count as infinite
 constexpr float kLowest = -3.0e38f;
 constexpr int kBlock = 32;      // keys per step
@@ -169,34 +170,206 @@ __device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int part) {
 // what the launch adds to a call's arguments
 struct AttnPlan {
     int tiles;        // row tiles per (sequence, KV head)
-    int splits;       // shares a tile's keys may be cut into; 1: no workspace
+    int splits;       // shares a tile's keys may be cut into; 1: no partial sums
     float *part;      // [tile][split][64·QT rows][HD] sums, then [rows][2] maximum and denominator
     int32_t *parts;   // [tile] shares in use
+    const uint8_t *img;  // [kv head][step] images of all rows, or null: the rows are laid out here
+    int steps;        // images per KV head
 };
 
+// A step's 32 key and value rows as the matrix instructions take them, in LDS
+// and, for prompts of many tiles, in memory:
+//   K  [16-key tile][32-dim chunk][half] lane l = 16·q + r: key r, dims 32c + 8q .. +7,
+//      at place 16·q + (r ^ 4q) of 64 (the writers' 8-byte pieces then spread
+//      over the banks)
+//   V  [32-dim chunk][t][half] lane l = 16·q + j: keys 4q .. +3 and 16+4q .. +3, dim 32c + 2j + t
+//   the keys' factors kf (key row = stored · kf) and vf (value row = stored · 2^-kTop · vf),
+//   and whether one factor holds for all of them.
+template <int HD>
+struct StepImage {
+    static constexpr int C = HD / 32, kK = 2 * C * 2 * 1024, kV = C * 2 * 2 * 1024, kSide = kK + kV, kBytes = kSide + 1024;
+    uint8_t k[kK], v[kV];
+    float kf[kBlock], vf[kBlock];
+    float kf_all;  // where `even`: every key's kf, and the exponent of every vf
+    int ve_all, even;
+    uint8_t pad[1024 - 8 * kBlock - 12];
+};
+static_assert(sizeof(StepImage<128>) == StepImage<128>::kBytes && sizeof(StepImage<64>) == StepImage<64>::kBytes, "whole KB");
+
+// Lays a step's rows into its image: 256 threads, K keys 8·wave + lane/8 by
+// whole 128-byte lines, V the keys of a lane group and two dims of the wave's
+// 32.  Two barriers in between, which the caller places: k(), barrier, v(), barrier.
+// EVEN: the image of one factor where the rows' exponents allow it.
+template <int HD, bool EVEN>
+struct StepLayer {
+    static constexpr int C = HD / 32, kVKeys = HD == 128 ? 8 : 4;
+    v4f kx[C];
+    v2f vx[kVKeys];
+    int wave, lane, ke;
+    __device__ __forceinline__ int v_q() const { return HD == 128 ? wave : wave & 1; }
+    __device__ __forceinline__ int v_half() const { return HD == 128 ? 0 : wave >> 1; }
+    __device__ __forceinline__ int k_key() const { return 8 * wave + (lane >> 3); }
+    __device__ __forceinline__ int v_key(int i) const {
+        const int kg = lane >> 4;
+        return HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half() + 4 * kg + i;
+    }
+    // k, v: row 0 of the KV head; keys k0 .. k0+31, those past `last` as it
+    __device__ __forceinline__ void load(const float *k, int64_t k_st, const float *v, int64_t v_st, int k0, int last) {
+        const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * (lane & 7);
+#pragma unroll
+        for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
+        const float *vs = v + 32 * v_q() + 2 * (lane & 15);
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) vx[i] = *reinterpret_cast<const v2f *>(vs + min(k0 + v_key(i), last) * v_st);
+    }
+    // sizes of the rows: s_k[32] exponents of K, s_v[C][32] bits of V's parts
+    __device__ __forceinline__ void sizes(int *s_k, uint32_t (*s_v)[kBlock]) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
+        ke = row_exp(lanes8_umax(top));
+        if ((lane & 7) == 0) s_k[k_key()] = ke;
+        uint32_t m[kVKeys];
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) {
+            m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
+            m[i] = lanes8_umax(m[i]);
+            m[i] = max(m[i], __float_as_uint(xchg<XM16>(__uint_as_float(m[i]))));
+        }
+        if ((lane & 15) == 0)
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i) s_v[v_q()][v_key(i)] = m[i];
+    }
+    __device__ __forceinline__ void put_k(StepImage<HD> *im, int e) const {
+        const int q = (lane & 7) >> 1, key = k_key() & 15;
+        uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * q + (key ^ (q << 2))) * 16 + (lane & 1) * 8;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            v2h h0, l0, h1, l1;
+            split_h(__builtin_ldexpf(kx[c][0], kTop - e), __builtin_ldexpf(kx[c][1], kTop - e), h0, l0);
+            split_h(__builtin_ldexpf(kx[c][2], kTop - e), __builtin_ldexpf(kx[c][3], kTop - e), h1, l1);
+            *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+        }
+    }
+    __device__ __forceinline__ void put_v(StepImage<HD> *im, const int (&e)[kVKeys]) const {
+        float x[kVKeys], y[kVKeys];
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) {
+            x[i] = e[i] > kMaxExp ? 0.0f : __builtin_ldexpf(vx[i][0], kTop - e[i]);
+            y[i] = e[i] > kMaxExp ? 0.0f : __builtin_ldexpf(vx[i][1], kTop - e[i]);
+        }
+        uint8_t *dst = im->v + v_q() * 4096 + lane * 16 + v_half() * 8;
+#pragma unroll
+        for (int i = 0; i < kVKeys; i += 4) {
+            v2h h0, l0, h1, l1;
+            split_h(x[i], x[i + 1], h0, l0);
+            split_h(x[i + 2], x[i + 3], h1, l1);
+            *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+            split_h(y[i], y[i + 1], h0, l0);
+            split_h(y[i + 2], y[i + 3], h1, l1);
+            *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+        }
+    }
+    __device__ __forceinline__ static float v_factor(int e) { return e > kMaxExp ? __uint_as_float(0x7fc00000u) : pow2(e); }
+    // before the first barrier
+    __device__ __forceinline__ void k(StepImage<HD> *im, int *s_k, uint32_t (*s_v)[kBlock]) {
+        sizes(s_k, s_v);
+        if (!EVEN) {
+            if ((lane & 7) == 0) im->kf[k_key()] = pow2(ke - kTop);
+            put_k(im, ke);
+        }
+    }
+    // after it
+    __device__ __forceinline__ void v(StepImage<HD> *im, const int *s_k, const uint32_t (*s_v)[kBlock]) {
+        int e[kVKeys];
+        if (EVEN) {  // every wave looks at all 32 keys: lane l at key l % 32
+            uint32_t bits = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c) bits = max(bits, s_v[c][lane & 31]);
+            const int k1 = s_k[lane & 31], v1 = row_exp(bits);
+            int k_hi = k1, v_hi = v1;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                k_hi = max(k_hi, __shfl_xor(k_hi, o));
+                v_hi = max(v_hi, __shfl_xor(v_hi, o));
+            }
+            const bool even = __all(k1 >= k_hi - kSpread && v1 >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
+            const int kk = even ? k_hi : ke;
+            put_k(im, kk);
+            if ((lane & 7) == 0) im->kf[k_key()] = pow2(kk - kTop);
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i) e[i] = even ? v_hi : __shfl(v1, v_key(i));
+            if (wave == 0 && lane == 0) {
+                im->kf_all = pow2(min(k_hi, kMaxExp) - kTop);
+                im->ve_all = v_hi;
+                im->even = even;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c) top = max(top, s_v[c][v_key(i)]);
+                e[i] = row_exp(top);
+            }
+        }
+        put_v(im, e);
+        if (v_q() == 0 && (lane & 15) == 0)
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i) im->vf[v_key(i)] = v_factor(e[i]);
+    }
+};
+
+// Images of all of a prompt's rows, for prompts of so many tiles that laying
+// every step out in each of them would cost more.  Workgroup: one step of one KV head.
+template <int HD>
+__global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, uint8_t *img) {
+    using Im = StepImage<HD>;
+    __shared__ __attribute__((aligned(16))) Im im;
+    __shared__ int s_k[kBlock];
+    __shared__ uint32_t s_v[Im::C][kBlock];
+    const int tid = threadIdx.x, g = blockIdx.y;
+    StepLayer<HD, true> st;
+    st.wave = tid >> 6;
+    st.lane = tid & 63;
+    st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, blockIdx.x * kBlock, p.rows - 1);
+    st.k(&im, s_k, s_v);
+    __syncthreads();
+    st.v(&im, s_k, s_v);
+    __syncthreads();
+    const uint4 *src = reinterpret_cast<const uint4 *>(&im);
+    uint4 *dst = reinterpret_cast<uint4 *>(img + ((size_t)g * gridDim.x + blockIdx.x) * Im::kBytes);
+    for (int i = tid; i < Im::kBytes / 16; i += kAttnThreads) dst[i] = src[i];
+}
+
 // Workgroup: 64·QT rows (token, head of the KV head's group) of one sequence
-// and KV head, four waves of 16·QT rows; one share of the keys, 32 a step.  A
-// step's K and V rows are read once, in whole 128-byte lines, split into their
-// halves and laid into LDS in the order the matrix instructions take them:
-//   K  lane l = 16·q + r of a 16-key tile: key r, dims 32c + 8q .. +7
-//   V  lane l = 16·q + j: keys 4q .. 4q+3 and 16+4q .. +3, dim 32d + 2j + t
+// and KV head, four waves of 16·QT rows; one share of the keys, 32 a step.
 // Scores come out transposed (lane l: query row l%16, keys 4·(l/16) + i of each
 // 16), so a row's maximum, denominator and weights stay with its four lanes and
 // the weights are the second product's operand as they are; the sums come out
 // transposed too (lane: the same query row, 8 consecutive dims of each 32).
-// Two LDS buffers: a step's products run on one while the next step's rows
-// arrive and are laid into the other.
-template <int HD, bool TREE, bool SHAPED, int QT>
+// Two LDS buffers: a step's products run on one while the next step's image
+// arrives in the other (IMG: direct loads; else the rows, laid out here).
+//
+// A row's weights are e = 2^(x - m), m an integer above its maximum so far; the
+// products take e·vf·2^(14-a) with 2^a above the row's largest e·vf so far, so
+// the halves hold the products that count whatever the sizes of V's rows.  All
+// rescales are by powers of two.  Steps that every row of the tile sees, with
+// one factor for all keys, need neither masks nor factors per key.
+template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
 __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
+    using Im = StepImage<HD>;
     constexpr int C = HD / 32;              // 32-dim chunks
     constexpr int kRows = 64 * QT;
-    constexpr int kVKeys = HD == 128 ? 8 : 4;  // keys a lane lays out of V
-    constexpr int kKBytes = 2 * C * 2 * 1024, kVBytes = C * 2 * 2 * 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t sk[2][kKBytes], sv[2][kVBytes];
-    __shared__ __attribute__((aligned(16))) float s_kf[2][kBlock], s_vf[2][kBlock];
-    __shared__ __attribute__((aligned(16))) uint32_t s_vmax[C][kBlock];
+    __shared__ __attribute__((aligned(16))) Im ims[2];
+    __shared__ int s_ke[kBlock];
+    __shared__ uint32_t s_ve[C][kBlock];
     __shared__ uint64_t s_bits[64];
-    __shared__ int s_depth[64], s_lo, s_hi;
+    __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
@@ -214,11 +387,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = 0;
         return;
     }
-    // the keys of the tile
+    // the keys of the tile, and those that all its rows see
     AttnTile t{0, 0, 1, 0, 0};
+    int all_lo = 0, all_hi;
     const int tok0 = first_row / p.group, tok1 = (min(first_row + kRows, rows) - 1) / p.group;
     if (TREE) {
         t.hi = len + count;
+        all_hi = len;
         if (wave == 0) {
             const uint64_t b = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
             s_bits[lane] = b;
@@ -227,8 +402,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         __syncthreads();
     } else if (p.begin) {
         if (tid == 0) {
-            s_lo = p.rows;
-            s_hi = 0;
+            s_lo = s_hi_min = p.rows;
+            s_hi = s_lo_max = 0;
         }
         __syncthreads();
         const int tok = tok0 + tid;
@@ -238,16 +413,41 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
                 atomicMin(&s_lo, b);
                 atomicMax(&s_hi, e);
             }
+            atomicMax(&s_lo_max, b);
+            atomicMin(&s_hi_min, e);
         }
         __syncthreads();
         t.lo = s_lo;
         t.hi = s_hi;
+        all_lo = s_lo_max;
+        all_hi = s_hi_min;
     } else {
         t.hi = p.rows0 + tok1 + 1;
+        all_hi = p.rows0 + tok0 + 1;
     }
     cut_tile(t, pl.splits, part);
     if (part >= t.parts) return;
     if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
+
+    // the first step's rows are on their way before the query rows
+    const uint8_t *images = IMG ? pl.img + ((size_t)g * pl.steps + t.lo / kBlock) * Im::kBytes : nullptr;
+    auto fetch = [&](int step, Im *im) {
+        constexpr int kChunks = Im::kBytes / 1024;
+#pragma unroll
+        for (int i = 0; i < (kChunks + 3) / 4; ++i) {
+            const int c = 4 * i + wave;
+            if (c < kChunks) lds_load(images + (size_t)step * Im::kBytes + c * 1024 + 16 * lane, reinterpret_cast<uint8_t *>(im) + c * 1024);
+        }
+    };
+    StepLayer<HD, false> rowsin;
+    rowsin.wave = wave;
+    rowsin.lane = lane;
+    const float *kbase = IMG ? nullptr : p.k + s * p.k_ss + g * HD, *vbase = IMG ? nullptr : p.v + s * p.v_ss + g * HD;
+    const int last = t.hi - 1;
+    if (t.from < t.to) {
+        if (IMG) fetch(t.from, &ims[0]);
+        else rowsin.load(kbase, p.k_st, vbase, p.v_st, t.lo + t.from * kBlock, last);
+    }
 
     // query rows: halves, scale, what they see
     v8h qh[QT][C], ql[QT][C];
@@ -291,88 +491,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         }
     }
     const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
-
-    // a step's rows: K keys 8·wave + lane/8, dims 4·(lane%8) + 32c; V the keys
-    // of the lane's group, two dims of the wave's 32
-    const int k_key = 8 * wave + (lane >> 3), k_part = lane & 7;
-    const int v_q = HD == 128 ? wave : wave & 1, v_half = HD == 128 ? 0 : wave >> 1;
-    const float *kbase = p.k + s * p.k_ss + g * HD + 4 * k_part;
-    const float *vbase = p.v + s * p.v_ss + g * HD + 32 * v_q + 2 * r16;
-    const int last = t.hi - 1;
-    v4f kx[C];
-    v2f vx[kVKeys];
-    auto load = [&](int step) {
-        const int k0 = t.lo + step * kBlock;
-        const float *ks = kbase + min(k0 + k_key, last) * p.k_st;
-#pragma unroll
-        for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
-#pragma unroll
-        for (int i = 0; i < kVKeys; ++i) {
-            const int key = HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i;
-            vx[i] = *reinterpret_cast<const v2f *>(vbase + min(k0 + key, last) * p.v_st);
-        }
-    };
-    // K into its buffer, and the sizes of V's rows
-    auto lay_k = [&](int b) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
-        const int e = row_exp(lanes8_umax(top));
-        if (k_part == 0) s_kf[b][k_key] = pow2(e - kTop);
-        const int q = k_part >> 1, key = k_key & 15;
-        uint8_t *dst = sk[b] + (k_key >> 4) * C * 2048 + (16 * q + (key ^ (q << 2))) * 16 + (k_part & 1) * 8;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            v2h h0, l0, h1, l1;
-            split_h(__builtin_ldexpf(kx[c][0], kTop - e), __builtin_ldexpf(kx[c][1], kTop - e), h0, l0);
-            split_h(__builtin_ldexpf(kx[c][2], kTop - e), __builtin_ldexpf(kx[c][3], kTop - e), h1, l1);
-            *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
-        }
-        uint32_t m[kVKeys];
-#pragma unroll
-        for (int i = 0; i < kVKeys; ++i) {
-            m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
-            m[i] = max(m[i], __float_as_uint(xchg<XQ1>(__uint_as_float(m[i]))));
-            m[i] = max(m[i], __float_as_uint(xchg<XQ2>(__uint_as_float(m[i]))));
-            m[i] = max(m[i], __float_as_uint(xchg<XM8>(__uint_as_float(m[i]))));
-            m[i] = max(m[i], __float_as_uint(xchg<XM16>(__uint_as_float(m[i]))));
-        }
-        if (r16 == 0)
-#pragma unroll
-            for (int i = 0; i < kVKeys; ++i)
-                s_vmax[v_q][HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i] = m[i];
-    };
-    // V into its buffer, once the sizes of all its quarters are there
-    auto lay_v = [&](int b) {
-        float x[kVKeys], y[kVKeys];
-#pragma unroll
-        for (int i = 0; i < kVKeys; ++i) {
-            const int key = HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half + 4 * kg + i;
-            uint32_t top = 0;
-#pragma unroll
-            for (int c = 0; c < C; ++c) top = max(top, s_vmax[c][key]);
-            const int e = row_exp(top);
-            const bool bad = e > kMaxExp;
-            if (v_q == 0 && r16 == 0) s_vf[b][key] = bad ? __uint_as_float(0x7fc00000u) : pow2(e);
-            x[i] = bad ? 0.0f : __builtin_ldexpf(vx[i][0], kTop - e);
-            y[i] = bad ? 0.0f : __builtin_ldexpf(vx[i][1], kTop - e);
-        }
-        uint8_t *dst = sv[b] + v_q * 4096 + lane * 16 + v_half * 8;
-#pragma unroll
-        for (int i = 0; i < kVKeys; i += 4) {
-            v2h h0, l0, h1, l1;
-            split_h(x[i], x[i + 1], h0, l0);
-            split_h(x[i + 2], x[i + 3], h1, l1);
-            *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
-            split_h(y[i], y[i + 1], h0, l0);
-            split_h(y[i + 2], y[i + 3], h1, l1);
-            *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
-        }
-    };
+    const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
 
     v4f o[QT][2 * C];
     float m[QT], l[QT];
@@ -385,39 +504,69 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
 #pragma unroll
         for (int d = 0; d < 2 * C; ++d) o[u][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
+    // a row's maximum (in its four lanes) and the largest exponent of its weighted values
+    auto raise_m = [&](int u, float top) {
+        if (__any(top > m[u])) {
+            const float mn = top > m[u] ? ceilf(top) + 2.0f : m[u];
+            l[u] *= __builtin_amdgcn_exp2f(m[u] - mn);
+            a[u] = max(a[u] - (int)fminf(mn - m[u], 16384.0f), -16384);
+            m[u] = mn;
+        }
+    };
+    auto raise_a = [&](int u, int need) {
+        if (__any(need > a[u])) {
+            const int an = need > a[u] ? need + 3 : a[u];
+            const float f = __builtin_ldexpf(1.0f, max(a[u] - an, -200));
+#pragma unroll
+            for (int d = 0; d < 2 * C; ++d) o[u][d] *= f;
+            a[u] = an;
+        }
+    };
+    auto max8 = [](const float (&x)[8]) {
+        return groups_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+    };
 
-    if (t.from < t.to) {
-        load(t.from);
-        lay_k(0);
+    if (!IMG && t.from < t.to) {
+        rowsin.k(&ims[0], s_ke, s_ve);
         __syncthreads();
-        lay_v(0);
+        rowsin.v(&ims[0], s_ke, s_ve);
         __syncthreads();
     }
     for (int step = t.from; step < t.to; ++step) {
         const int b = (step - t.from) & 1, k0 = t.lo + step * kBlock;
         const bool more = step + 1 < t.to;
-        if (more) load(step + 1);
+        const Im &im = ims[b];
+        if (IMG) {
+            wait_vm<0>();   // this wave's part of the step's image is in LDS,
+            lds_barrier();  // now everybody's is, and nobody reads the other buffer any more
+            if (more) fetch(step + 1, &ims[b ^ 1]);
+        } else if (more) {
+            rowsin.load(kbase, p.k_st, vbase, p.v_st, k0 + kBlock, last);
+        }
+        const bool whole = k0 >= all_lo && k0 + kBlock <= all_hi;
         // what each row sees of the step's keys, as bits
         uint32_t see[QT];
-        bool any = false;
+        bool any = whole;
+        if (!whole) {
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const int n1 = min(max(row_hi[u] - k0, 0), 32), n0 = min(max(row_lo[u] - k0, 0), 32);
-            see[u] = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
-            if (TREE) {
-                const int off = k0 - len;  // the step's first key among the drafted ones
-                if (off > -32 && off < 64) see[u] |= (uint32_t)(off >= 0 ? bits[u] >> off : bits[u] << -off);
+            for (int u = 0; u < QT; ++u) {
+                const int n1 = min(max(row_hi[u] - k0, 0), 32), n0 = min(max(row_lo[u] - k0, 0), 32);
+                see[u] = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
+                if (TREE) {
+                    const int off = k0 - len;  // the step's first key among the drafted ones
+                    if (off > -32 && off < 64) see[u] |= (uint32_t)(off >= 0 ? bits[u] >> off : bits[u] << -off);
+                }
+                any = any || see[u];
             }
-            any = any || see[u];
+            any = __any(any);
         }
-        if (__any(any)) {
+        if (any) {
             v4f sc[QT][2];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
                 for (int u = 0; u < QT; ++u) sc[u][kt] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                const uint8_t *src = sk[b] + kt * C * 2048 + (16 * kg + (r16 ^ (kg << 2))) * 16;
+                const uint8_t *src = im.k + kt * C * 2048 + (16 * kg + (r16 ^ (kg << 2))) * 16;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     const v8h kh = *reinterpret_cast<const v8h *>(src + c * 2048);
@@ -430,87 +579,103 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
                     }
                 }
             }
-            float kf[8], vf[8];
             int kpos[8];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const v4f fk = *reinterpret_cast<const v4f *>(&s_kf[b][16 * kt + 4 * kg]);
-                const v4f fv = *reinterpret_cast<const v4f *>(&s_vf[b][16 * kt + 4 * kg]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    kf[4 * kt + i] = fk[i];
-                    vf[4 * kt + i] = fv[i];
-                    const int key = k0 + 16 * kt + 4 * kg + i;
-                    kpos[4 * kt + i] = key;
-                    if (TREE && SHAPED) {
-                        if (pos) kpos[4 * kt + i] = pos[min(key, last)];
-                        else if (key >= len) kpos[4 * kt + i] = len + s_depth[min(key - len, 63)];
-                    }
+            for (int e = 0; e < 8; ++e) {
+                const int key = k0 + 16 * (e >> 2) + 4 * kg + (e & 3);
+                kpos[e] = key;
+                if (TREE && SHAPED) {
+                    if (pos) kpos[e] = pos[min(key, last)];
+                    else if (key >= len) kpos[e] = len + s_depth[min(key - len, 63)];
                 }
             }
+            // capped and biased scores, to the base 2
+            auto shape = [&](int u, float x, int e) {
+                if (p.cap > 0.0f) x = p.cap * tanh_f(x * inv_cap);
+                return fmaf(x, kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])));
+            };
             v8h ph[QT], pL[QT];
+            if (IMG && whole && im.even) {
+                const float kf = im.kf_all;
+                const int ve = im.ve_all;
 #pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                const bool whole = __all(see[u] == 0xffffffffu);
-                float x[8];
+                for (int u = 0; u < QT; ++u) {
+                    const float f = kf * qf[u];
+                    float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = sc[u][e >> 2][e & 3] * kf[e] * qf[u];
-                    if (SHAPED) {
-                        if (p.cap > 0.0f) x[e] = p.cap * tanh_f(x[e] * inv_cap);
-                        x[e] = fmaf(x[e], kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])));
+                    for (int e = 0; e < 8; ++e) x[e] = SHAPED ? shape(u, sc[u][e >> 2][e & 3] * f, e) : sc[u][e >> 2][e & 3];
+                    const float top = SHAPED ? max8(x) : max8(x) * f;
+                    raise_m(u, top);
+                    raise_a(u, ve + (int)ceilf(fmaxf(top - m[u], -16000.0f)));
+                    // weights below 2^-60 of the largest come out 0 either way
+                    const int sh = max(14 + ve - a[u], -60);
+                    const float mm = m[u] - (float)sh;
+                    float w[8], sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        w[e] = __builtin_amdgcn_exp2f(SHAPED ? x[e] - mm : fmaf(x[e], f, -mm));
+                        sum += w[e];
+                    }
+                    l[u] += __builtin_ldexpf(sum, -sh);
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        v2h hi, lo;
+                        split_h(w[e], w[e + 1], hi, lo);
+                        ph[u][e] = hi[0];
+                        ph[u][e + 1] = hi[1];
+                        pL[u][e] = lo[0];
+                        pL[u][e + 1] = lo[1];
                     }
                 }
-                if (!whole) {
-                    const uint32_t mine = see[u] >> (4 * kg);
+            } else {
+                float kf[8], vf[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
-                }
-                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                top = groups_max(top);
-                if (__any(top > m[u])) {
-                    const float mn = top > m[u] ? ceilf(top) + 2.0f : m[u];
-                    l[u] *= __builtin_amdgcn_exp2f(m[u] - mn);
-                    a[u] = max(a[u] - (int)fminf(mn - m[u], 16384.0f), -16384);
-                    m[u] = mn;
-                }
-                float w[8], sum = 0.0f;
+                for (int kt = 0; kt < 2; ++kt) {
+                    const v4f fk = *reinterpret_cast<const v4f *>(&im.kf[16 * kt + 4 * kg]);
+                    const v4f fv = *reinterpret_cast<const v4f *>(&im.vf[16 * kt + 4 * kg]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(x[e] - m[u]);
-                    sum += w[e];
-                    w[e] *= vf[e];
-                }
-                l[u] += sum;
-                if (!whole) {  // a bad value row is NaN here, for the rows that see it only
-                    const uint32_t mine = see[u] >> (4 * kg);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? w[e] : 0.0f;
-                }
-                float big = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
-                big = groups_max(big);
-                const int need = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -16384;  // big < 2^need
-                if (__any(need > a[u])) {
-                    const int an = need > a[u] ? need + 3 : a[u];
-                    const float f = __builtin_ldexpf(1.0f, max(a[u] - an, -200));
-#pragma unroll
-                    for (int d = 0; d < 2 * C; ++d) o[u][d] *= f;
-                    a[u] = an;
+                    for (int i = 0; i < 4; ++i) {
+                        kf[4 * kt + i] = fk[i];
+                        vf[4 * kt + i] = fv[i];
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    v2h hi, lo;
-                    split_h(__builtin_ldexpf(w[e], 14 - a[u]), __builtin_ldexpf(w[e + 1], 14 - a[u]), hi, lo);
-                    ph[u][e] = hi[0];
-                    ph[u][e + 1] = hi[1];
-                    pL[u][e] = lo[0];
-                    pL[u][e + 1] = lo[1];
+                for (int u = 0; u < QT; ++u) {
+                    const uint32_t mine = whole ? ~0u : see[u] >> (4 * kg);
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = sc[u][e >> 2][e & 3] * (kf[e] * qf[u]);
+                        if (SHAPED) x[e] = shape(u, x[e], e);
+                        x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
+                    }
+                    raise_m(u, max8(x));
+                    float w[8], sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        w[e] = __builtin_amdgcn_exp2f(x[e] - m[u]);
+                        sum += w[e];
+                        // a bad value row is NaN, for the rows that see it only
+                        w[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? w[e] * vf[e] : 0.0f;
+                    }
+                    l[u] += sum;
+                    const float big = max8(w);
+                    raise_a(u, big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -16384);  // big < 2^that
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        v2h hi, lo;
+                        split_h(__builtin_ldexpf(w[e], 14 - a[u]), __builtin_ldexpf(w[e + 1], 14 - a[u]), hi, lo);
+                        ph[u][e] = hi[0];
+                        ph[u][e + 1] = hi[1];
+                        pL[u][e] = lo[0];
+                        pL[u][e + 1] = lo[1];
+                    }
                 }
             }
 #pragma unroll
             for (int d = 0; d < 2 * C; ++d) {
-                const v8h vh = *reinterpret_cast<const v8h *>(sv[b] + d * 2048 + lane * 16);
-                const v8h vl = *reinterpret_cast<const v8h *>(sv[b] + d * 2048 + 1024 + lane * 16);
+                const v8h vh = *reinterpret_cast<const v8h *>(im.v + d * 2048 + lane * 16);
+                const v8h vl = *reinterpret_cast<const v8h *>(im.v + d * 2048 + 1024 + lane * 16);
 #pragma unroll
                 for (int u = 0; u < QT; ++u) {
                     o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[u], o[u][d], 0, 0, 0);
@@ -519,10 +684,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
                 }
             }
         }
-        if (more) {
-            lay_k(b ^ 1);
+        if (!IMG && more) {
+            rowsin.k(&ims[b ^ 1], s_ke, s_ve);
             __syncthreads();
-            lay_v(b ^ 1);
+            rowsin.v(&ims[b ^ 1], s_ke, s_ve);
             __syncthreads();
         }
     }
@@ -532,39 +697,29 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         const int local = (wave * QT + u) * 16 + r16, row = first_row + local;
         const float total = groups_sum(l[u]);
         if (row >= rows) continue;
-        if (t.parts > 1) {
-            float *dst = pl.part + ((slot * pl.splits + part) * kRows + local) * HD + 8 * kg;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    v4f x;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(o[u][2 * c + (i & 1)][2 * h + (i >> 1)], a[u] - 14 - kTop);
-                    *reinterpret_cast<v4f *>(dst + 32 * c + 4 * h) = x;
-                }
-            if (kg == 0) {
-                float *st = pl.part + (size_t)p.kvh * gridDim.z * pl.tiles * pl.splits * kRows * HD +
-                            ((slot * pl.splits + part) * kRows + local) * 2;
-                st[0] = m[u];
-                st[1] = total;
-            }
-            continue;
-        }
+        const bool whole_row = t.parts == 1;
         const int tok = row / p.group, h = g * p.group + row % p.group;
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        float *dst = p.out + s * p.o_ss + tok * p.o_st + h * HD + 8 * kg;
+        const float f = whole_row ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
+        float *dst = whole_row ? p.out + s * p.o_ss + tok * p.o_st + h * HD + 8 * kg
+                               : pl.part + ((slot * pl.splits + part) * kRows + local) * HD + 8 * kg;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 v4f x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(o[u][2 * c + (i & 1)][2 * y + (i >> 1)] * inv, a[u] - 14 - kTop);
+                for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(o[u][2 * c + (i & 1)][2 * y + (i >> 1)] * f, a[u] - 14 - kTop);
                 *reinterpret_cast<v4f *>(dst + 32 * c + 4 * y) = x;
             }
-        if (p.lse && kg == 0)
+        if (kg != 0) continue;
+        if (!whole_row) {
+            float *st = pl.part + (size_t)p.kvh * gridDim.z * pl.tiles * pl.splits * kRows * HD +
+                        ((slot * pl.splits + part) * kRows + local) * 2;
+            st[0] = m[u];
+            st[1] = total;
+        } else if (p.lse) {
             p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m[u] + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+        }
     }
 }
 
@@ -723,7 +878,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) 
             const uint64_t see = s_see[local];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float y = sc[i] * kf[i] * qf;
+                float y = sc[i] * (kf[i] * qf);
                 if (SHAPED) {
                     if (p.cap > 0.0f) y = p.cap * tanh_f(y * inv_cap);
                     y = fmaf(y, kLog2e, -s_slope[local] * fabsf((float)(int)((uint32_t)s_pos[local] - (uint32_t)kpos[i])));

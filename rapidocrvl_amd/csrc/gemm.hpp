@@ -842,32 +842,6 @@ static __global__ void __launch_bounds__(kThreads) k_tile_weight(const uint8_t *
 template <int NPL>
 constexpr int kGemmStage = 2 * NPL * 2 * 64 * 16;
 
-// HBM → LDS load of 16 bytes per lane: lane i's bytes land at lds + 16·i.
-// Written as inline asm so the compiler's wait-count pass does
-// not see an LDS write it cannot place (it would wait for every load in flight
-// before each LDS read); the kernel orders these loads itself with wait_vm and
-// lds_barrier.
-__device__ __forceinline__ void lds_load(const void *g, void *lds) {
-    const uint32_t base = __builtin_amdgcn_readfirstlane(
-        (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(base) : "m0");
-}
-
-// s_waitcnt vmcnt(N): at most N of this wave's vector-memory loads in flight
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// workgroup barrier that keeps LDS reads and loads on their side of it: this
-// wave's LDS reads have returned before it, since other waves' direct loads may
-// overwrite what it read right after.  (The compiler's own wait for a read
-// stands at the read's use, and the MFMAs may sink below a bare s_barrier.)
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 template <int QT, int NMAT, int RB, int NPL = 3>
 static __global__ void __launch_bounds__(kThreads) k_gemm_lds(GemmParams p, int epi) {
     static_assert(NMAT * RB <= 4, "at most four row blocks per wave");

@@ -55,7 +55,7 @@ def attention(q, k, v, seen, scale, cap=0.0, slope=None, dist=None):
     v = np.where(used[:, None], np.asarray(v, np.float64), 0.0)
     out_err = p_err @ np.abs(v) + (p @ np.abs(v)) * (2 * 2.0 ** -21 + steps[:, None] + 2 * U) + 1e-38
     top = np.abs(v).max(1)
-    out_err += (p @ top)[:, None] * 2.0 ** -32 + ((p * top).max(1) * seen.sum(1))[:, None] * 2.0 ** -36
+    out_err += (p @ top)[:, None] * 2.0 ** -32 + ((p * top).max(1) * seen.sum(1))[:, None] * 2.0 ** -30
     return p @ v, lse, p, out_err, lse_err, p_err
 
 
