@@ -107,6 +107,11 @@ __device__ __forceinline__ void split_row(const float (&x)[C][8], int e, v8h (&h
         }
 }
 
+// lds_load from a uniform address and a lane's offset to a uniform LDS address
+__device__ __forceinline__ void lds_load_at(const void *base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0");
+}
+
 // max over the lanes l, l^16, l^32, l^48 (an MFMA column's four lane groups)
 __device__ __forceinline__ uint32_t groups_umax(uint32_t v) {
     const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
@@ -179,9 +184,7 @@ struct AttnPlan {
 
 // A step's 32 key and value rows as the matrix instructions take them, in LDS
 // and, for prompts of many tiles, in memory:
-//   K  [16-key tile][32-dim chunk][half] lane l = 16·q + r: key r, dims 32c + 8q .. +7,
-//      at place 16·q + (r ^ 4q) of 64 (the writers' 8-byte pieces then spread
-//      over the banks)
+//   K  [16-key tile][32-dim chunk][half] lane l = 16·q + r: key r, dims 32c + 8q .. +7
 //   V  [32-dim chunk][t][half] lane l = 16·q + j: keys 4q .. +3 and 16+4q .. +3, dim 32c + 2j + t
 //   the keys' factors kf (key row = stored · kf) and vf (value row = stored · 2^-kTop · vf),
 //   and whether one factor holds for all of them.
@@ -196,8 +199,8 @@ struct StepImage {
 };
 static_assert(sizeof(StepImage<128>) == StepImage<128>::kBytes && sizeof(StepImage<64>) == StepImage<64>::kBytes, "whole KB");
 
-// Lays a step's rows into its image: 256 threads, K keys 8·wave + lane/8 by
-// whole 128-byte lines, V the keys of a lane group and two dims of the wave's
+// Lays a step's rows into its image: 256 threads, K keys 8·wave + lane%8 by
+// whole 128-byte lines (their pieces meet in a bank in pairs), V the keys of a lane group and two dims of the wave's
 // 32.  Two barriers in between, which the caller places: k(), barrier, v(), barrier.
 // EVEN: the image of one factor where the rows' exponents allow it.
 template <int HD, bool EVEN>
@@ -208,14 +211,15 @@ struct StepLayer {
     int wave, lane, ke;
     __device__ __forceinline__ int v_q() const { return HD == 128 ? wave : wave & 1; }
     __device__ __forceinline__ int v_half() const { return HD == 128 ? 0 : wave >> 1; }
-    __device__ __forceinline__ int k_key() const { return 8 * wave + (lane >> 3); }
+    __device__ __forceinline__ int k_key() const { return 8 * wave + (lane & 7); }
+    __device__ __forceinline__ int k_part() const { return lane >> 3; }
     __device__ __forceinline__ int v_key(int i) const {
         const int kg = lane >> 4;
         return HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half() + 4 * kg + i;
     }
     // k, v: row 0 of the KV head; keys k0 .. k0+31, those past `last` as it
     __device__ __forceinline__ void load(const float *k, int64_t k_st, const float *v, int64_t v_st, int k0, int last) {
-        const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * (lane & 7);
+        const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * k_part();
 #pragma unroll
         for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
         const float *vs = v + 32 * v_q() + 2 * (lane & 15);
@@ -228,8 +232,9 @@ struct StepLayer {
 #pragma unroll
         for (int c = 0; c < C; ++c)
             top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
-        ke = row_exp(lanes8_umax(top));
-        if ((lane & 7) == 0) s_k[k_key()] = ke;
+        top = max(top, (uint32_t)__shfl_xor((int)top, 8));
+        ke = row_exp(groups_umax(top));
+        if (k_part() == 0) s_k[k_key()] = ke;
         uint32_t m[kVKeys];
 #pragma unroll
         for (int i = 0; i < kVKeys; ++i) {
@@ -242,8 +247,7 @@ struct StepLayer {
             for (int i = 0; i < kVKeys; ++i) s_v[v_q()][v_key(i)] = m[i];
     }
     __device__ __forceinline__ void put_k(StepImage<HD> *im, int e) const {
-        const int q = (lane & 7) >> 1, key = k_key() & 15;
-        uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * q + (key ^ (q << 2))) * 16 + (lane & 1) * 8;
+        uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * (k_part() >> 1) + (k_key() & 15)) * 16 + (k_part() & 1) * 8;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             v2h h0, l0, h1, l1;
@@ -279,7 +283,7 @@ struct StepLayer {
     __device__ __forceinline__ void k(StepImage<HD> *im, int *s_k, uint32_t (*s_v)[kBlock]) {
         sizes(s_k, s_v);
         if (!EVEN) {
-            if ((lane & 7) == 0) im->kf[k_key()] = pow2(ke - kTop);
+            if (k_part() == 0) im->kf[k_key()] = pow2(ke - kTop);
             put_k(im, ke);
         }
     }
@@ -300,7 +304,7 @@ struct StepLayer {
             const bool even = __all(k1 >= k_hi - kSpread && v1 >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
             const int kk = even ? k_hi : ke;
             put_k(im, kk);
-            if ((lane & 7) == 0) im->kf[k_key()] = pow2(kk - kTop);
+            if (k_part() == 0) im->kf[k_key()] = pow2(kk - kTop);
 #pragma unroll
             for (int i = 0; i < kVKeys; ++i) e[i] = even ? v_hi : __shfl(v1, v_key(i));
             if (wave == 0 && lane == 0) {
@@ -370,6 +374,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     __shared__ uint32_t s_ve[C][kBlock];
     __shared__ uint64_t s_bits[64];
     __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
+    __shared__ int2 s_row[kRows];  // the cache rows that each row sees: [x, y)
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
@@ -431,13 +436,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
 
     // the first step's rows are on their way before the query rows
     const uint8_t *images = IMG ? pl.img + ((size_t)g * pl.steps + t.lo / kBlock) * Im::kBytes : nullptr;
-    auto fetch = [&](int step, Im *im) {
+    const uint32_t ims_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)ims;
+    const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+    auto fetch = [&](int step, int b) {
         constexpr int kChunks = Im::kBytes / 1024;
+        const uint8_t *src = images + (size_t)step * Im::kBytes + wave_u * 1024;
+        const uint32_t dst = ims_at + b * Im::kBytes + wave_u * 1024;
 #pragma unroll
-        for (int i = 0; i < (kChunks + 3) / 4; ++i) {
-            const int c = 4 * i + wave;
-            if (c < kChunks) lds_load(images + (size_t)step * Im::kBytes + c * 1024 + 16 * lane, reinterpret_cast<uint8_t *>(im) + c * 1024);
-        }
+        for (int i = 0; i < (kChunks + 3) / 4; ++i)
+            if (4 * i + wave_u < kChunks) lds_load_at(src + i * 4096, 16 * lane, dst + i * 4096);
     };
     StepLayer<HD, false> rowsin;
     rowsin.wave = wave;
@@ -445,14 +452,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     const float *kbase = IMG ? nullptr : p.k + s * p.k_ss + g * HD, *vbase = IMG ? nullptr : p.v + s * p.v_ss + g * HD;
     const int last = t.hi - 1;
     if (t.from < t.to) {
-        if (IMG) fetch(t.from, &ims[0]);
+        if (IMG) fetch(t.from, 0);
         else rowsin.load(kbase, p.k_st, vbase, p.v_st, t.lo + t.from * kBlock, last);
     }
 
     // query rows: halves, scale, what they see
     v8h qh[QT][C], ql[QT][C];
     float qf[QT], slope[QT];
-    int row_lo[QT], row_hi[QT], row_pos[QT];
+    int row_pos[QT];
     uint64_t bits[QT];
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
@@ -476,19 +483,21 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         split_row<C>(x, e, qh[u], ql[u]);
         qf[u] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
         slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-        row_lo[u] = row_hi[u] = row_pos[u] = 0;
+        row_pos[u] = 0;
         bits[u] = 0;
+        int2 sees = {0, 0};
         if (TREE) {
             if (live) {
-                row_hi[u] = len;
+                sees.y = len;
                 bits[u] = s_bits[tok];
                 if (SHAPED) row_pos[u] = p.pos ? p.pos[((size_t)s * p.kvh + g) * p.side + len + tok] : len + s_depth[tok];
             }
         } else if (live) {
-            row_lo[u] = p.begin ? min(max(p.begin[tok], 0), p.rows) : 0;
-            row_hi[u] = p.end ? min(max(p.end[tok], 0), p.rows) : p.rows0 + tok + 1;
+            sees.x = p.begin ? min(max(p.begin[tok], 0), p.rows) : 0;
+            sees.y = p.end ? min(max(p.end[tok], 0), p.rows) : p.rows0 + tok + 1;
             row_pos[u] = p.rows0 + tok;
         }
+        if (kg == 0) s_row[row - first_row] = sees;  // for this wave alone
     }
     const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
     const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
@@ -539,7 +548,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         if (IMG) {
             wait_vm<0>();   // this wave's part of the step's image is in LDS,
             lds_barrier();  // now everybody's is, and nobody reads the other buffer any more
-            if (more) fetch(step + 1, &ims[b ^ 1]);
+            if (more) fetch(step + 1, b ^ 1);
         } else if (more) {
             rowsin.load(kbase, p.k_st, vbase, p.v_st, k0 + kBlock, last);
         }
@@ -550,7 +559,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < QT; ++u) {
-                const int n1 = min(max(row_hi[u] - k0, 0), 32), n0 = min(max(row_lo[u] - k0, 0), 32);
+                const int2 sees = s_row[(wave * QT + u) * 16 + r16];
+                const int n1 = min(max(sees.y - k0, 0), 32), n0 = min(max(sees.x - k0, 0), 32);
                 see[u] = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
                 if (TREE) {
                     const int off = k0 - len;  // the step's first key among the drafted ones
@@ -563,36 +573,38 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         if (any) {
             v4f sc[QT][2];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
+            for (int u = 0; u < QT; ++u) sc[u][0] = sc[u][1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int u = 0; u < QT; ++u) sc[u][kt] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                const uint8_t *src = im.k + kt * C * 2048 + (16 * kg + (r16 ^ (kg << 2))) * 16;
+            for (int c = 0; c < C; ++c) {  // neighbouring products go to different sums
+                v8h kh[2], kl[2];
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const v8h kh = *reinterpret_cast<const v8h *>(src + c * 2048);
-                    const v8h kl = *reinterpret_cast<const v8h *>(src + c * 2048 + 1024);
-#pragma unroll
-                    for (int u = 0; u < QT; ++u) {
-                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[u][c], sc[u][kt], 0, 0, 0);
-                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[u][c], sc[u][kt], 0, 0, 0);
-                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[u][c], sc[u][kt], 0, 0, 0);
-                    }
+                for (int kt = 0; kt < 2; ++kt) {
+                    kh[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + lane * 16);
+                    kl[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + 1024 + lane * 16);
                 }
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int u = 0; u < QT; ++u)
+                            sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? kl[kt] : kh[kt], x == 1 ? ql[u][c] : qh[u][c],
+                                                                               sc[u][kt], 0, 0, 0);
             }
             int kpos[8];
+            if (TREE && SHAPED) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = k0 + 16 * (e >> 2) + 4 * kg + (e & 3);
-                kpos[e] = key;
-                if (TREE && SHAPED) {
-                    if (pos) kpos[e] = pos[min(key, last)];
-                    else if (key >= len) kpos[e] = len + s_depth[min(key - len, 63)];
+                for (int e = 0; e < 8; ++e) {
+                    const int key = k0 + 16 * (e >> 2) + 4 * kg + (e & 3);
+                    kpos[e] = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
                 }
             }
             // capped and biased scores, to the base 2
             auto shape = [&](int u, float x, int e) {
                 if (p.cap > 0.0f) x = p.cap * tanh_f(x * inv_cap);
-                return fmaf(x, kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])));
+                const float dist = TREE ? (float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])
+                                        : (float)(row_pos[u] - k0 - 4 * kg) - (float)(16 * (e >> 2) + (e & 3));
+                return fmaf(x, kLog2e, -slope[u] * fabsf(dist));
             };
             v8h ph[QT], pL[QT];
             if (IMG && whole && im.even) {
@@ -673,15 +685,21 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
                 }
             }
 #pragma unroll
-            for (int d = 0; d < 2 * C; ++d) {
-                const v8h vh = *reinterpret_cast<const v8h *>(im.v + d * 2048 + lane * 16);
-                const v8h vl = *reinterpret_cast<const v8h *>(im.v + d * 2048 + 1024 + lane * 16);
+            for (int d = 0; d < 2 * C; d += 2) {
+                v8h vh[2], vl[2];
 #pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[u], o[u][d], 0, 0, 0);
-                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pL[u], o[u][d], 0, 0, 0);
-                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[u], o[u][d], 0, 0, 0);
+                for (int y = 0; y < 2; ++y) {
+                    vh[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + lane * 16);
+                    vl[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + 1024 + lane * 16);
                 }
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int u = 0; u < QT; ++u)
+                            o[u][d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? vl[y] : vh[y], x == 1 ? pL[u] : ph[u],
+                                                                                 o[u][d + y], 0, 0, 0);
             }
         }
         if (!IMG && more) {
