@@ -153,7 +153,7 @@ int round_up_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Row tiles and key shares of one attention call: `rows` query rows (token,
 // head) per sequence and KV head over at most `keys` keys.
 struct AttnShape {
-    int qt, tiles, splits, steps;  // steps: images of a prompt's rows, or 0
+    int qt, tiles, splits, least, steps;  // steps: images of a prompt's rows, or 0
     int64_t part_bytes, bytes;     // of the workspace
 };
 template <int HD>
@@ -163,8 +163,11 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
     a.qt = rows > 64 ? 2 : 1;
     a.tiles = round_up_div(rows, 64 * a.qt);
     const int64_t work = a.tiles * groups;
-    const int64_t want = std::max<int64_t>(1, 512 / work);
-    a.splits = (int)std::min<int64_t>({want, 64, std::max<int64_t>(1, keys / (kBlock * kMinSteps))});
+    // two workgroups a CU; prompts of many short rows (documents) leave most
+    // CUs idle behind their longest tile unless that is cut too
+    const int64_t want = std::max<int64_t>(1, (work < 256 ? 512 : 1024) / work);
+    a.least = work < 128 ? 2 : 6;
+    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (kBlock * a.least))});
     a.steps = images && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
     a.part_bytes = a.splits == 1 ? 0 : work * a.splits * 64 * a.qt * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
     a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
@@ -173,7 +176,7 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
 
 template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
-    AttnPlan pl{sh.tiles, sh.splits, nullptr, nullptr, nullptr, sh.steps};
+    AttnPlan pl{sh.tiles, sh.splits, sh.least, nullptr, nullptr, nullptr, sh.steps};
     if (sh.splits > 1) {
         pl.part = static_cast<float *>(work);
         pl.parts = reinterpret_cast<int32_t *>(static_cast<float *>(work) +
@@ -347,7 +350,12 @@ extern "C" int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *a, void 
     p.budget = a->budget;
     p.sinks = a->sinks;
     p.recent = a->recent;
-    hipLaunchKernelGGL(k_cache_select<8>, dim3(a->kv_heads, a->caches), dim3(kSelThreads), 0, (hipStream_t)stream, p);
+    // rows per thread: the fewest that hold the cache in registers (1,609 rows: 2)
+    const dim3 grid(a->kv_heads, a->caches);
+    hipStream_t s = (hipStream_t)stream;
+    if (a->max_rows <= 2 * kSelThreads) hipLaunchKernelGGL(k_cache_select<2>, grid, dim3(kSelThreads), 0, s, p);
+    else if (a->max_rows <= 8 * kSelThreads) hipLaunchKernelGGL(k_cache_select<8>, grid, dim3(kSelThreads), 0, s, p);
+    else hipLaunchKernelGGL(k_cache_select<16>, grid, dim3(kSelThreads), 0, s, p);
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }
@@ -422,16 +430,23 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
     p.per_head = a->per_head != 0;
     p.max_rows = a->max_rows;
     p.max_rows_out = a->max_rows_out;
-    const int slots = 2 * a->head_dim / kKeepSlab + 1;
-    const int chunks = inplace ? 1 : std::min(64, (a->max_keep + 255) / 256);
-    const dim3 grid(slots * chunks, a->kv_heads, a->caches);
     hipStream_t s = (hipStream_t)stream;
-    if (a->head_dim == 128) {
-        if (inplace) hipLaunchKernelGGL((k_cache_keep<128, true>), grid, dim3(kKeepThreads), 0, s, p);
-        else hipLaunchKernelGGL((k_cache_keep<128, false>), grid, dim3(kKeepThreads), 0, s, p);
+    const dim3 threads(kKeepThreads);
+    const int side = a->weights || a->positions ? 1 : 0;
+    if (inplace && a->max_keep > kKeepRows) {
+        const dim3 grid(2 * a->head_dim / kKeepSlab + side, a->kv_heads, a->caches);
+        if (a->head_dim == 128) hipLaunchKernelGGL(k_cache_keep_slabs<128>, grid, threads, 0, s, p);
+        else hipLaunchKernelGGL(k_cache_keep_slabs<64>, grid, threads, 0, s, p);
     } else {
-        if (inplace) hipLaunchKernelGGL((k_cache_keep<64, true>), grid, dim3(kKeepThreads), 0, s, p);
-        else hipLaunchKernelGGL((k_cache_keep<64, false>), grid, dim3(kKeepThreads), 0, s, p);
+        const int chunks = (a->max_keep + kKeepRows - 1) / kKeepRows;
+        const dim3 grid((2 + side) * chunks, a->kv_heads, a->caches);
+        if (a->head_dim == 128) {
+            if (inplace) hipLaunchKernelGGL((k_cache_keep<128, true>), grid, threads, 0, s, p, chunks);
+            else hipLaunchKernelGGL((k_cache_keep<128, false>), grid, threads, 0, s, p, chunks);
+        } else {
+            if (inplace) hipLaunchKernelGGL((k_cache_keep<64, true>), grid, threads, 0, s, p, chunks);
+            else hipLaunchKernelGGL((k_cache_keep<64, false>), grid, threads, 0, s, p, chunks);
+        }
     }
     HIP_TRY(hipGetLastError());
     return POCR_OK;

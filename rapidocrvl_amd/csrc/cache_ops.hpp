@@ -162,12 +162,12 @@ struct AttnTile {
     int from, to;      // this share's steps of kBlock keys, from lo rounded down
 };
 
-// steps of a tile cut into at most `splits` shares of at least kMinSteps
-constexpr int kMinSteps = 2;
-__device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int part) {
+// steps of a tile cut into at most `splits` shares of at least `least` steps
+constexpr int kMaxShares = 64;
+__device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int least, int part) {
     t.lo &= ~(kBlock - 1);
     const int steps = max(0, (t.hi - t.lo + kBlock - 1) / kBlock);
-    t.parts = min(splits, max(1, steps / kMinSteps));
+    t.parts = min(splits, max(1, steps / least));
     t.from = (int)((int64_t)steps * part / t.parts);
     t.to = (int)((int64_t)steps * (part + 1) / t.parts);
 }
@@ -176,6 +176,7 @@ __device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int part) {
 struct AttnPlan {
     int tiles;        // row tiles per (sequence, KV head)
     int splits;       // shares a tile's keys may be cut into; 1: no partial sums
+    int least;        // steps of a share
     float *part;      // [tile][split][64·QT rows][HD] sums, then [rows][2] maximum and denominator
     int32_t *parts;   // [tile] shares in use
     const uint8_t *img;  // [kv head][step] images of all rows, or null: the rows are laid out here
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         t.hi = p.rows0 + tok1 + 1;
         all_hi = p.rows0 + tok0 + 1;
     }
-    cut_tile(t, pl.splits, part);
+    cut_tile(t, pl.splits, pl.least, part);
     if (part >= t.parts) return;
     if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
 
@@ -741,30 +742,58 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     }
 }
 
-// Joins the shares of the tiles that were cut: one half wave per row and 32
-// lanes, or HD / 4, of float4; rows of uncut tiles are done already.
+// Joins the shares of the tiles that were cut: HD / 4 lanes of float4 per row;
+// rows of uncut tiles are done already.  The lanes first take the shares'
+// maxima and denominators, one or a few each, then all walk the shares with
+// the factors that those give, kJoin loads in flight.
+constexpr int kJoin = 8;
 template <int HD, int QT>
 __global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan pl, int seqs) {
-    constexpr int kRows = 64 * QT, kLanes = HD / 4, kPer = 256 / kLanes;
+    constexpr int kRows = 64 * QT, kLanes = HD / 4, kPer = 256 / kLanes, kOwn = kMaxShares / kLanes;
     const int per_tile = kRows / kPer;
     const int tile = blockIdx.x / per_tile, local = blockIdx.x % per_tile * kPer + threadIdx.x / kLanes;
     const int g = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes;
     const size_t slot = ((size_t)s * p.kvh + g) * pl.tiles + tile;
     const int parts = pl.parts[slot];
     const int rows = (p.lens ? seq_rows(p, s).count : p.n) * p.group, row = tile * kRows + local;
-    if (parts < 2 || row >= rows) return;
-    const float *st = pl.part + (size_t)p.kvh * seqs * pl.tiles * pl.splits * kRows * HD + (slot * pl.splits * kRows + local) * 2;
+    if (parts < 2 || row >= rows) return;  // the same for a row's lanes
+    const float2 *st = reinterpret_cast<const float2 *>(pl.part + (size_t)p.kvh * seqs * pl.tiles * pl.splits * kRows * HD) +
+                       slot * pl.splits * kRows + local;
     const float *src = pl.part + (slot * pl.splits * kRows + local) * HD + 4 * lane;
+    float2 mine[kOwn];
     float m = kLowest;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, st[(size_t)i * kRows * 2]);
-    float total = 0.0f;
-    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < parts; ++i) {
-        const float f = __builtin_amdgcn_exp2f(st[(size_t)i * kRows * 2] - m);
-        total = fmaf(st[(size_t)i * kRows * 2 + 1], f, total);
-        const v4f x = *reinterpret_cast<const v4f *>(src + (size_t)i * kRows * HD);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[c], f, acc[c]);
+    for (int i = 0; i < kOwn; ++i) {
+        const int x = i * kLanes + lane;
+        mine[i] = x < parts ? st[(size_t)x * kRows] : make_float2(kLowest, 0.0f);
+        m = fmaxf(m, mine[i].x);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kLanes));
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        mine[i].x = __builtin_amdgcn_exp2f(mine[i].x - m);
+        total = fmaf(mine[i].y, mine[i].x, total);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) total += __shfl_xor(total, o, kLanes);
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < parts; i0 += kJoin) {
+        v4f x[kJoin];
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) x[i] = *reinterpret_cast<const v4f *>(src + (size_t)min(i0 + i, parts - 1) * kRows * HD);
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) {
+            const int at = i0 + i;
+            float f = mine[0].x;
+#pragma unroll
+            for (int y = 1; y < kOwn; ++y) f = at / kLanes == y ? mine[y].x : f;
+            f = __shfl(f, at % kLanes, kLanes);
+            if (at < parts)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[i][c], f, acc[c]);
+        }
     }
     const int tok = row / p.group, h = g * p.group + row % p.group;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -943,15 +972,17 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // One workgroup per (KV head, cache).  The need-th largest key of the rows
-// between sinks and recent by four histogram passes over its bytes (integer
-// counts: the order of the atomics does not matter), then one pass that writes
-// the kept rows in order: a wave owns 64·KPT consecutive rows of a tile, so a
-// row's place is a count of ballots.  KPT rows per thread and tile; where one
-// tile holds the cache its keys are read once and stay in registers.
+// between sinks and recent by three histogram passes over 11, 11 and 10 of its
+// bits (integer counts: the order of the atomics does not matter; eleven bits
+// hold two of the mantissa, which spreads weights of few exponents over the
+// bins), then one pass that writes the kept rows in order: a wave owns 64·KPT
+// consecutive rows of a tile, so a row's place is a count of ballots.  KPT rows
+// per thread and tile; where one tile holds the cache its keys are read once
+// and stay in registers.
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
-    constexpr int kTile = kSelThreads * KPT;
-    __shared__ int hist[256];
+    constexpr int kTile = kSelThreads * KPT, kBins = 2048;
+    __shared__ int hist[kBins];
     __shared__ int s_bin, s_need;
     __shared__ int s_eq[kSelWaves], s_gt[kSelWaves];
     const int g = blockIdx.x, c = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -976,50 +1007,47 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     };
     uint32_t prefix = 0, mask = 0;
     if (need > 0)
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : kBins;
+            hist[tid] = 0;
+            hist[tid + kSelThreads] = 0;
+            if (tiles == 1 && pass == 0) load(0);
             __syncthreads();
             for (int tile = 0; tile < tiles; ++tile) {
-                if (tiles > 1 || shift == 24) load(tile);
+                if (tiles > 1) load(tile);
 #pragma unroll
                 for (int i = 0; i < KPT; ++i) {
                     const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
-                    if (j >= first && j < last && (key[i] & mask) == prefix) atomicAdd(&hist[key[i] >> shift & 255], 1);
+                    if (j >= first && j < last && (key[i] & mask) == prefix) atomicAdd(&hist[key[i] >> shift & (bins - 1)], 1);
                 }
             }
             __syncthreads();
-            if (wave == 0) {  // lane l: bins 255 - 4l .. 252 - 4l, from the top
-                int n[4], sum = 0;
+            // thread t: bins 2047 - 2t and 2046 - 2t, counts above them by a scan
+            const int n0 = hist[kBins - 1 - 2 * tid], n1 = hist[kBins - 2 - 2 * tid];
+            int upto = n0 + n1;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    n[i] = hist[255 - 4 * lane - i];
-                    sum += n[i];
-                }
-                int above = sum;
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int x = __shfl_up(above, o);
-                    if (lane >= o) above += x;
-                }
-                above -= sum;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (above < need && above + n[i] >= need) {
-                        s_bin = 255 - 4 * lane - i;
-                        s_need = need - above;
-                    }
-                    above += n[i];
-                }
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (lane == 63) s_gt[wave] = upto;
+            __syncthreads();
+            int above = upto - n0 - n1;
+            for (int x = 0; x < kSelWaves; ++x) above += x < wave ? s_gt[x] : 0;
+            if (above < need && above + n0 + n1 >= need) {  // one thread
+                const bool lower = above + n0 < need;
+                s_bin = kBins - 1 - 2 * tid - (lower ? 1 : 0);
+                s_need = need - above - (lower ? n0 : 0);
             }
             __syncthreads();
             prefix |= (uint32_t)s_bin << shift;
-            mask |= 255u << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
             need = s_need;  // how many keys equal to prefix are taken, after the last pass
         }
     const bool none = p.budget == p.sinks + p.recent;
     int done = 0, eq_done = 0;  // rows written, equal keys met
     for (int tile = 0; tile < tiles; ++tile) {
-        if (tiles > 1 || none) load(tile);
+        if (tiles > 1) load(tile);
         int gt = 0, eq = 0;
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
@@ -1074,8 +1102,8 @@ struct CacheKeep {
 };
 
 constexpr int kKeepThreads = 256;
-constexpr int kKeepSlab = 16;  // floats of a row that a workgroup moves
-constexpr int kKeepUnroll = 4;
+constexpr int kKeepRows = 64;  // rows that a workgroup of k_cache_keep moves
+constexpr int kKeepSlab = 16;  // floats of a row that a workgroup of k_cache_keep_slabs moves
 
 // every wave's loads have arrived
 __device__ __forceinline__ void loads_done() {
@@ -1083,66 +1111,107 @@ __device__ __forceinline__ void loads_done() {
     __syncthreads();
 }
 
-// Workgroup: one slab of 16 columns of K or V of one KV head and cache, or (the
-// last x) its weights and positions.  Chunks of rows: all loads of a chunk,
-// then its stores.  In place one workgroup walks a slab's chunks in order: a
-// list ascends with rows[i] >= first + i, so what a later chunk reads lies at
-// or behind its own places, past everything written before it, and only the
-// chunk's own loads have to end (the barrier) before its stores.
-template <int HD, bool INPLACE>
-__global__ void __launch_bounds__(kKeepThreads) k_cache_keep(CacheKeep p) {
-    constexpr int kSlabs = HD / kKeepSlab;
-    const int g = blockIdx.y, c = blockIdx.z, tid = threadIdx.x, x = blockIdx.x;
-    const int first = p.first ? min(max(p.first[c], 0), p.max_rows_out) : 0;
-    const int count = min(max(p.counts[c], 0), min(p.max_keep, p.max_rows_out - first));
-    const int32_t *rows = p.rows + (p.per_head ? (size_t)c * p.kvh + g : (size_t)c) * p.max_keep;
-    auto source = [&](int i) {
-        return min(max(rows[i], INPLACE ? min(first + i, p.max_rows - 1) : 0), p.max_rows - 1);
-    };
-    const int part = INPLACE ? x : x % (2 * kSlabs + 1);
-    const int from = INPLACE ? 0 : x / (2 * kSlabs + 1), step = INPLACE ? 1 : gridDim.x / (2 * kSlabs + 1);
-    if (part == 2 * kSlabs) {
-        if (!p.weights && !p.pos) return;
-        const size_t in = ((size_t)c * p.kvh + g) * p.side, out = ((size_t)c * p.kvh + g) * p.side_out + first;
-        constexpr int kChunk = kKeepThreads;
-        for (int b = from; b * kChunk < count; b += step) {
-            const int i = b * kChunk + tid;
-            float w = 0.0f;
-            int32_t at = 0;
-            if (i < count) {
-                const int j = source(i);
-                if (p.weights) w = p.weights[in + j];
-                if (p.pos) at = p.pos[in + j];
-            }
-            if (INPLACE) loads_done();
-            if (i < count) {
-                if (p.weights) p.weights_out[out + i] = w;
-                if (p.pos) p.pos_out[out + i] = at;
-            }
-        }
-        if (INPLACE) __syncthreads();
-        if (p.weights)
-            for (int i = count + from * kChunk + tid; first + i < p.max_rows_out; i += step * kChunk)
-                p.weights_out[out + i] = 0.0f;
-        return;
-    }
-    const int which = part / kSlabs, slab = part % kSlabs;
-    constexpr int kLanes = kKeepSlab / 4, kRows = kKeepThreads / kLanes, kChunk = kRows * kKeepUnroll;
-    const float *src = p.src[which] + c * p.src_cs[which] + g * HD + slab * kKeepSlab + tid % kLanes * 4;
-    float *dst = p.dst[which] + c * p.dst_cs[which] + g * HD + slab * kKeepSlab + tid % kLanes * 4;
-    for (int b = from; b * kChunk < count; b += step) {
-        float4 v[kKeepUnroll];
-#pragma unroll
-        for (int u = 0; u < kKeepUnroll; ++u) {
-            const int i = b * kChunk + u * kRows + tid / kLanes;
-            if (i < count) v[u] = *reinterpret_cast<const float4 *>(src + source(i) * p.src_st[which]);
+struct KeepRange {
+    int first, count;
+    const int32_t *rows;
+};
+__device__ __forceinline__ KeepRange keep_range(const CacheKeep &p, int c, int g) {
+    KeepRange r;
+    r.first = p.first ? min(max(p.first[c], 0), p.max_rows_out) : 0;
+    r.count = min(max(p.counts[c], 0), min(p.max_keep, p.max_rows_out - r.first));
+    r.rows = p.rows + (p.per_head ? (size_t)c * p.kvh + g : (size_t)c) * p.max_keep;
+    return r;
+}
+// the source row of list entry i, read whatever the count is (i < max_keep)
+template <bool INPLACE>
+__device__ __forceinline__ int keep_source(const CacheKeep &p, int listed, int first, int i) {
+    return min(max(listed, INPLACE ? min(first + i, p.max_rows - 1) : 0), p.max_rows - 1);
+}
+
+// weights and positions of list entries from, from + step, ... chunks of 256
+template <bool INPLACE>
+__device__ __forceinline__ void keep_side(const CacheKeep &p, const KeepRange &r, int c, int g, int from, int step) {
+    const size_t in = ((size_t)c * p.kvh + g) * p.side, out = ((size_t)c * p.kvh + g) * p.side_out + r.first;
+    for (int b = from * kKeepThreads; b < r.count; b += step * kKeepThreads) {
+        const int i = b + threadIdx.x;
+        float w = 0.0f;
+        int32_t at = 0;
+        if (i < r.count) {
+            const int j = keep_source<INPLACE>(p, r.rows[i], r.first, i);
+            if (p.weights) w = p.weights[in + j];
+            if (p.pos) at = p.pos[in + j];
         }
         if (INPLACE) loads_done();
-#pragma unroll
-        for (int u = 0; u < kKeepUnroll; ++u) {
-            const int i = b * kChunk + u * kRows + tid / kLanes;
-            if (i < count) *reinterpret_cast<float4 *>(dst + (first + i) * p.dst_st[which]) = v[u];
+        if (i < r.count) {
+            if (p.weights) p.weights_out[out + i] = w;
+            if (p.pos) p.pos_out[out + i] = at;
         }
+    }
+    if (INPLACE) __syncthreads();
+    if (p.weights)
+        for (int i = r.count + from * kKeepThreads + threadIdx.x; r.first + i < p.max_rows_out; i += step * kKeepThreads)
+            p.weights_out[out + i] = 0.0f;
+}
+
+// Workgroup: 64 listed rows of K or V of one KV head and cache (x even, odd),
+// HD / 4 lanes a row, all loads before the first store; or (the last x's) their
+// weights and positions.  In place for lists of at most 64 rows, which one
+// workgroup holds whole.
+template <int HD, bool INPLACE>
+__global__ void __launch_bounds__(kKeepThreads) k_cache_keep(CacheKeep p, int chunks) {
+    constexpr int kLanes = HD / 4, kStep = kKeepThreads / kLanes, kUnroll = kKeepRows / kStep;
+    const int g = blockIdx.y, c = blockIdx.z, tid = threadIdx.x, x = blockIdx.x;
+    const KeepRange r = keep_range(p, c, g);
+    if (x >= 2 * chunks) {
+        keep_side<INPLACE>(p, r, c, g, x - 2 * chunks, chunks);
+        return;
+    }
+    const int which = x & 1, i0 = (x >> 1) * kKeepRows + tid / kLanes;
+    int j[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) j[u] = r.rows[min(i0 + u * kStep, p.max_keep - 1)];
+    const float *src = p.src[which] + c * p.src_cs[which] + g * HD + tid % kLanes * 4;
+    float *dst = p.dst[which] + c * p.dst_cs[which] + g * HD + tid % kLanes * 4;
+    v4f v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)  // entries behind the count: a row that is there, not stored
+        v[u] = *reinterpret_cast<const v4f *>(src + keep_source<INPLACE>(p, j[u], r.first, min(i0 + u * kStep, p.max_keep - 1)) * p.src_st[which]);
+    if (INPLACE) loads_done();
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+        if (i0 + u * kStep < r.count) *reinterpret_cast<v4f *>(dst + (r.first + i0 + u * kStep) * p.dst_st[which]) = v[u];
+}
+
+// Longer lists in place.  Workgroup: one slab of 16 columns of K or V of one KV
+// head and cache, or (the last x) its weights and positions; it walks the list
+// in chunks: all loads of a chunk, then its stores.  The list ascends with
+// rows[i] >= first + i, so what a later chunk reads lies at or behind its own
+// places, past everything written before it, and only the chunk's own loads
+// have to end (the barrier) before its stores.
+template <int HD>
+__global__ void __launch_bounds__(kKeepThreads) k_cache_keep_slabs(CacheKeep p) {
+    constexpr int kSlabs = HD / kKeepSlab, kLanes = kKeepSlab / 4, kStep = kKeepThreads / kLanes, kUnroll = 8;
+    const int g = blockIdx.y, c = blockIdx.z, tid = threadIdx.x, x = blockIdx.x;
+    const KeepRange r = keep_range(p, c, g);
+    if (x == 2 * kSlabs) {
+        keep_side<true>(p, r, c, g, 0, 1);
+        return;
+    }
+    const int which = x / kSlabs, at = x % kSlabs * kKeepSlab + tid % kLanes * 4;
+    const float *src = p.src[which] + c * p.src_cs[which] + g * HD + at;
+    float *dst = p.dst[which] + c * p.dst_cs[which] + g * HD + at;
+    for (int b = tid / kLanes; b - tid / kLanes < r.count; b += kStep * kUnroll) {
+        v4f v[kUnroll];
+        int j[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) j[u] = r.rows[min(b + u * kStep, p.max_keep - 1)];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            v[u] = *reinterpret_cast<const v4f *>(src + keep_source<true>(p, j[u], r.first, min(b + u * kStep, p.max_keep - 1)) * p.src_st[which]);
+        loads_done();
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (b + u * kStep < r.count) *reinterpret_cast<v4f *>(dst + (r.first + b + u * kStep) * p.dst_st[which]) = v[u];
     }
 }
 
