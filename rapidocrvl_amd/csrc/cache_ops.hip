@@ -153,52 +153,73 @@ int round_up_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Row tiles and key shares of one attention call: `rows` query rows (token,
 // head) per sequence and KV head over at most `keys` keys.
 struct AttnShape {
-    int qt, tiles, splits, least, steps;  // steps: images of a prompt's rows, or 0
-    int64_t part_bytes, bytes;     // of the workspace
+    bool few;                       // k_cache_attn_few
+    int wg_rows, tiles, splits, least;
+    int steps;                      // images of a prompt's rows, or 0
+    int64_t part_bytes, bytes;      // of the workspace
 };
 template <int HD>
 constexpr int64_t image_bytes = StepImage<HD>::kBytes;
 AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, bool images) {
     AttnShape a;
-    a.qt = rows > 64 ? 2 : 1;
-    a.tiles = round_up_div(rows, 64 * a.qt);
+    a.few = rows <= 32;
+    a.wg_rows = a.few ? (rows <= 16 ? 16 : 32) : (rows <= 64 ? 64 : 128);
+    a.tiles = round_up_div(rows, a.wg_rows);
     const int64_t work = a.tiles * groups;
     // two workgroups a CU; prompts of many short rows (documents) leave most
     // CUs idle behind their longest tile unless that is cut too
     const int64_t want = std::max<int64_t>(1, (work < 256 ? 512 : 1024) / work);
     a.least = work < 128 ? 2 : 6;
-    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (kBlock * a.least))});
-    a.steps = images && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
-    a.part_bytes = a.splits == 1 ? 0 : work * a.splits * 64 * a.qt * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
+    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / ((a.few ? kFewStep : kBlock) * a.least))});
+    a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
+    a.part_bytes = a.splits == 1 ? 0 : work * a.splits * a.wg_rows * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
     a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
     return a;
 }
 
-template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
-int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
+AttnPlan attn_plan(const AttnShape &sh, void *work, int64_t groups, int head_dim) {
     AttnPlan pl{sh.tiles, sh.splits, sh.least, nullptr, nullptr, nullptr, sh.steps};
     if (sh.splits > 1) {
         pl.part = static_cast<float *>(work);
-        pl.parts = reinterpret_cast<int32_t *>(static_cast<float *>(work) +
-                                               (size_t)p.kvh * seqs * sh.tiles * sh.splits * 64 * QT * (HD + 2));
+        pl.parts = reinterpret_cast<int32_t *>(pl.part + groups * sh.tiles * sh.splits * sh.wg_rows * (head_dim + 2));
     }
+    return pl;
+}
+
+template <int HD, int kRows>
+int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs) {
+    if (pl.splits > 1)
+        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows>), dim3(pl.tiles * (kRows / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl, seqs);
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}
+
+template <int HD, bool TREE, bool SHAPED, int QT>
+int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
+    const AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
+    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(256), 0, s, p, pl);
+    return launch_join<HD, 16 * QT>(s, p, pl, seqs);
+}
+
+template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
+int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
+    AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
     if (IMG) {
         uint8_t *img = static_cast<uint8_t *>(work) + sh.part_bytes;
         pl.img = img;
         hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps, p.kvh), dim3(kAttnThreads), 0, s, p, img);
     }
     hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT, IMG>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(kAttnThreads), 0, s, p, pl);
-    if (sh.splits > 1)
-        hipLaunchKernelGGL((k_cache_attn_join<HD, QT>), dim3(sh.tiles * (64 * QT / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl, seqs);
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    return launch_join<HD, 64 * QT>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED>
 int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     if constexpr (!TREE)
         if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, 2, true>(s, p, sh, work, seqs);
-    return sh.qt == 2 ? launch_attn_t<HD, TREE, SHAPED, 2, false>(s, p, sh, work, seqs)
+    if (sh.few)
+        return sh.wg_rows == 16 ? launch_few<HD, TREE, SHAPED, 1>(s, p, sh, work, seqs) : launch_few<HD, TREE, SHAPED, 2>(s, p, sh, work, seqs);
+    return sh.wg_rows == 128 ? launch_attn_t<HD, TREE, SHAPED, 2, false>(s, p, sh, work, seqs)
                       : launch_attn_t<HD, TREE, SHAPED, 1, false>(s, p, sh, work, seqs);
 }
 

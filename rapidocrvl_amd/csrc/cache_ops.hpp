@@ -159,14 +159,14 @@ __device__ __forceinline__ float tanh_f(float x) {
 struct AttnTile {
     int lo, hi;        // keys some row of the tile sees: [lo, hi)
     int parts;         // shares they are cut into
-    int from, to;      // this share's steps of kBlock keys, from lo rounded down
+    int from, to;      // this share's steps, from lo rounded down to a multiple of kBlock
 };
 
-// steps of a tile cut into at most `splits` shares of at least `least` steps
+// a tile's steps of `keys` keys cut into at most `splits` shares of at least `least` steps
 constexpr int kMaxShares = 64;
-__device__ __forceinline__ void cut_tile(AttnTile &t, int splits, int least, int part) {
+__device__ __forceinline__ void cut_tile(AttnTile &t, int keys, int splits, int least, int part) {
     t.lo &= ~(kBlock - 1);
-    const int steps = max(0, (t.hi - t.lo + kBlock - 1) / kBlock);
+    const int steps = max(0, (t.hi - t.lo + keys - 1) / keys);
     t.parts = min(splits, max(1, steps / least));
     t.from = (int)((int64_t)steps * part / t.parts);
     t.to = (int)((int64_t)steps * (part + 1) / t.parts);
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         t.hi = p.rows0 + tok1 + 1;
         all_hi = p.rows0 + tok0 + 1;
     }
-    cut_tile(t, pl.splits, pl.least, part);
+    cut_tile(t, kBlock, pl.splits, pl.least, part);
     if (part >= t.parts) return;
     if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
 
@@ -742,14 +742,274 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     }
 }
 
+// Few rows (at most 32 per sequence and KV head: one token, small trees).  What
+// counts is how soon the cache is read: no wave waits for another, and K and V
+// go from memory to the fp32 matrix instruction as they are loaded.
+// Workgroup: 16·QT rows, four waves that take the share's blocks of 16 keys in
+// turn, the next block's rows requested before this one's products:
+//   K  lane 16·q + r: key r, dims 16c + 4q .. +3; product e of chunk c sums over
+//      the dims 16c + 4q + e, as the query rows are held
+//   V  lane 16·q + j: keys 4q .. 4q+3, dims 64d + 4j .. +3
+// Scores and sums come out transposed, as in k_cache_attn; the waves' sums are
+// joined in LDS.  Products, weights and sums are fp32 throughout.
+constexpr int kFewKeys = 16, kFewStep = 4 * kFewKeys;
+template <int HD, bool TREE, bool SHAPED, int QT>
+__global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAttn p, AttnPlan pl) {
+    constexpr int KC = HD / 16, D = HD / 64, kRows = 16 * QT, kPad = HD + 4;
+    __shared__ __attribute__((aligned(16))) float s_o[4][kRows][kPad];
+    __shared__ float s_m[4][kRows], s_l[4][kRows];
+    __shared__ uint64_t s_bits[64];
+    __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
+    const int part = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const size_t slot = (size_t)s * p.kvh + g;
+    int len = 0, count = p.n;
+    if (TREE) {
+        const SeqRows q = seq_rows(p, s);
+        len = q.len;
+        count = q.count;
+    }
+    const int rows = count * p.group;
+    if (rows == 0) {
+        if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = 0;
+        return;
+    }
+    AttnTile t{0, 0, 1, 0, 0};
+    int all_lo = 0, all_hi;
+    if (TREE) {
+        t.hi = len + count;
+        all_hi = len;
+        if (wave == 0) {
+            const uint64_t b = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
+            s_bits[lane] = b;
+            s_depth[lane] = __popcll(b) - 1;
+        }
+        __syncthreads();
+    } else if (p.begin) {
+        if (tid == 0) {
+            s_lo = s_hi_min = p.rows;
+            s_hi = s_lo_max = 0;
+        }
+        __syncthreads();
+        if (tid < count) {  // at most 32 tokens
+            const int b = min(max(p.begin[tid], 0), p.rows), e = min(max(p.end[tid], 0), p.rows);
+            if (b < e) {
+                atomicMin(&s_lo, b);
+                atomicMax(&s_hi, e);
+            }
+            atomicMax(&s_lo_max, b);
+            atomicMin(&s_hi_min, e);
+        }
+        __syncthreads();
+        t.lo = s_lo;
+        t.hi = s_hi;
+        all_lo = s_lo_max;
+        all_hi = s_hi_min;
+    } else {
+        t.hi = p.rows0 + count;
+        all_hi = p.rows0 + 1;
+    }
+    cut_tile(t, kFewStep, pl.splits, pl.least, part);
+    if (part >= t.parts) return;
+    if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
+
+    const float *kbase = p.k + s * p.k_ss + g * HD + 4 * kg, *vbase = p.v + s * p.v_ss + g * HD + 4 * r16;
+    const int last = t.hi - 1;
+    v4f kx[KC], vx[4][D];
+    auto load = [&](int k0) {
+        const float *ks = kbase + min(k0 + r16, last) * p.k_st;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 16 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                vx[i][d] = *reinterpret_cast<const v4f *>(vbase + min(k0 + 4 * kg + i, last) * p.v_st + 64 * d);
+    };
+    if (t.from < t.to) load(t.lo + t.from * kFewStep + wave * kFewKeys);
+
+    v4f q[QT][KC];
+    float slope[QT];
+    int row_lo[QT], row_hi[QT], row_pos[QT];
+    uint64_t bits[QT];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const int row = 16 * u + r16;
+        const bool live = row < rows;
+        const int tok = live ? row / p.group : 0, h = g * p.group + (live ? row % p.group : 0);
+        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 4 * kg;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) q[u][c] = *reinterpret_cast<const v4f *>(src + 16 * c);
+        slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+        row_lo[u] = row_hi[u] = row_pos[u] = 0;
+        bits[u] = 0;
+        if (TREE) {
+            if (live) {
+                row_hi[u] = len;
+                bits[u] = s_bits[tok];
+                if (SHAPED) row_pos[u] = p.pos ? p.pos[slot * p.side + len + tok] : len + s_depth[tok];
+            }
+        } else if (live) {
+            row_lo[u] = p.begin ? min(max(p.begin[tok], 0), p.rows) : 0;
+            row_hi[u] = p.end ? min(max(p.end[tok], 0), p.rows) : p.rows0 + tok + 1;
+            row_pos[u] = p.rows0 + tok;
+        }
+    }
+    const float scale = SHAPED ? p.scale : p.scale * kLog2e;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + slot * p.side : nullptr;
+
+    v4f o[QT][D][4];  // [..][x][i]: dim 64d + 16·kg + 4i + x
+    float m[QT], l[QT];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        m[u] = kLowest;
+        l[u] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[u][d][x] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int step = t.from; step < t.to; ++step) {
+        const int k0 = t.lo + step * kFewStep + wave * kFewKeys;
+        v4f sc[QT];
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            v4f a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+#pragma unroll
+            for (int c = 0; c < KC; c += 2)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    a = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c][e], q[u][c][e], a, 0, 0, 0);
+                    b = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c + 1][e], q[u][c + 1][e], b, 0, 0, 0);
+                }
+            sc[u] = a + b;
+        }
+        v4f v[4][D];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[i][d] = vx[i][d];
+        if (step + 1 < t.to) load(k0 + kFewStep);
+        const bool whole = k0 >= all_lo && k0 + kFewKeys <= all_hi;
+        uint32_t bad = 0;  // keys whose value row is not finite, where not every row sees all keys
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    top = umax3(top, max(abs_bits(v[i][d][0]), abs_bits(v[i][d][1])), max(abs_bits(v[i][d][2]), abs_bits(v[i][d][3])));
+                const uint64_t b = __ballot(top >= 0x7f800000u);
+                const bool here = b >> (16 * kg) & 0xffff;
+                if (here)
+#pragma unroll
+                    for (int d = 0; d < D; ++d) v[i][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                bad |= here ? 1u << i : 0u;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            uint32_t see = 0xf;  // of the lane's four keys
+            if (!whole) {
+                const int n1 = min(max(row_hi[u] - k0, 0), 16), n0 = min(max(row_lo[u] - k0, 0), 16);
+                uint32_t w = ((1u << n1) - 1) & ~((1u << n0) - 1);
+                if (TREE) {
+                    const int off = k0 - len;  // the block's first key among the drafted ones
+                    if (off > -16 && off < 64) w |= (uint32_t)(off >= 0 ? bits[u] >> off : bits[u] << -off);
+                }
+                see = w >> (4 * kg) & 0xf;
+            }
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = sc[u][i] * scale;
+                if (SHAPED) {
+                    const int key = k0 + 4 * kg + i;
+                    int at = key;
+                    if (TREE) at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
+                    if (p.cap > 0.0f) x[i] = p.cap * tanh_f(x[i] * inv_cap);
+                    x[i] = fmaf(x[i], kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)at)));
+                }
+                x[i] = see >> i & 1 ? x[i] : -INFINITY;
+            }
+            const float top = groups_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+            if (__any(top > m[u])) {
+                const float mn = top > m[u] ? top : m[u];
+                const float f = __builtin_amdgcn_exp2f(m[u] - mn);
+                l[u] *= f;
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) o[u][d][y] *= f;
+                m[u] = mn;
+            }
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(x[i] - m[u]);
+                l[u] += w[i];
+                if (!whole && (bad & see) >> i & 1) l[u] = __uint_as_float(0x7fc00000u);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        o[u][d][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d][y], w[i], o[u][d][y], 0, 0, 0);
+        }
+    }
+
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const int row = 16 * u + r16;
+        const float total = groups_sum(l[u]);
+        if (kg == 0) {
+            s_m[wave][row] = m[u];
+            s_l[wave][row] = total;
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<v4f *>(&s_o[wave][row][64 * d + 16 * kg + 4 * i]) = (v4f){o[u][d][0][i], o[u][d][1][i], o[u][d][2][i], o[u][d][3][i]};
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (HD / 4); i += 256) {
+        const int row = i / (HD / 4), at = i % (HD / 4) * 4;
+        float mm = s_m[0][row], f[4], total = 0.0f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, s_m[w][row]);
+        v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mm);
+            total = fmaf(s_l[w][row], f[w], total);
+            x += *reinterpret_cast<const v4f *>(&s_o[w][row][at]) * f[w];
+        }
+        if (t.parts > 1) {
+            *reinterpret_cast<v4f *>(pl.part + ((slot * pl.splits + part) * kRows + row) * HD + at) = x;
+            if (at == 0)
+                reinterpret_cast<float2 *>(pl.part + (size_t)p.kvh * gridDim.z * pl.splits * kRows * HD)[(slot * pl.splits + part) * kRows + row] =
+                    make_float2(mm, total);
+            continue;
+        }
+        const int tok = row / p.group, h = g * p.group + row % p.group;
+        *reinterpret_cast<v4f *>(p.out + s * p.o_ss + tok * p.o_st + h * HD + at) = x * (total == 0.0f ? 0.0f : 1.0f / total);
+        if (p.lse && at == 0)
+            p.lse[((size_t)s * p.n + tok) * p.heads + h] = (mm + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    }
+}
+
 // Joins the shares of the tiles that were cut: HD / 4 lanes of float4 per row;
 // rows of uncut tiles are done already.  The lanes first take the shares'
 // maxima and denominators, one or a few each, then all walk the shares with
 // the factors that those give, kJoin loads in flight.
 constexpr int kJoin = 8;
-template <int HD, int QT>
+template <int HD, int kRows>
 __global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan pl, int seqs) {
-    constexpr int kRows = 64 * QT, kLanes = HD / 4, kPer = 256 / kLanes, kOwn = kMaxShares / kLanes;
+    constexpr int kLanes = HD / 4, kPer = 256 / kLanes, kOwn = kMaxShares / kLanes;
     const int per_tile = kRows / kPer;
     const int tile = blockIdx.x / per_tile, local = blockIdx.x % per_tile * kPer + threadIdx.x / kLanes;
     const int g = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes;
