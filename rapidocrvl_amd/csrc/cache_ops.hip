@@ -143,6 +143,7 @@ int tree_params(const pocr_tree_args *a, const char *op, CacheAttn *p) {
     p->heads = a->heads;
     p->kvh = a->kv_heads;
     p->group = a->heads / a->kv_heads;
+    p->inv_group = 1.0f / (float)p->group;
     p->scale = default_scale(a->scale, a->head_dim);
     p->cap = a->cap;
     return POCR_OK;
@@ -169,8 +170,9 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
     // two workgroups a CU; prompts of many short rows (documents) leave most
     // CUs idle behind their longest tile unless that is cut too
     const int64_t want = std::max<int64_t>(1, (work < 256 ? 512 : 1024) / work);
-    a.least = work < 128 ? 2 : 6;
-    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / ((a.few ? kFewStep : kBlock) * a.least))});
+    const int step = !a.few ? kBlock : kFewKeys * kFewWaves;
+    a.least = a.few ? 1 : (work < 128 ? 2 : 6);
+    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
     a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
     a.part_bytes = a.splits == 1 ? 0 : work * a.splits * a.wg_rows * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
     a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
@@ -197,7 +199,7 @@ int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs)
 template <int HD, bool TREE, bool SHAPED, int QT>
 int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     const AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
-    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(256), 0, s, p, pl);
+    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
     return launch_join<HD, 16 * QT>(s, p, pl, seqs);
 }
 
@@ -296,6 +298,7 @@ extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, v
     p.heads = a->heads;
     p.kvh = a->kv_heads;
     p.group = a->heads / a->kv_heads;
+    p.inv_group = 1.0f / (float)p.group;
     p.scale = default_scale(a->scale, a->head_dim);
     p.cap = a->cap;
     return launch_attn<false>((hipStream_t)stream, p, a->head_dim, 1, shape, a->workspace);

@@ -23,7 +23,7 @@ struct CacheAttn {
     const uint64_t *take;
     int64_t q_ss, q_st, k_ss, k_st, v_ss, v_st, o_ss, o_st, side;
     int n, rows0, rows, heads, kvh, group;     // rows: prompt rows0 + n, tree max_rows
-    float scale, cap;
+    float scale, cap, inv_group;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -155,6 +155,9 @@ __device__ __forceinline__ float tanh_f(float x) {
     return copysignf(t, x);
 }
 
+// x / p.group for x below 2^20 (the quotient is at least 1/2 group away from the next)
+__device__ __forceinline__ int by_group(const CacheAttn &p, int x) { return (int)(((float)x + 0.5f) * p.inv_group); }
+
 // the rows of one tile and its share of the keys
 struct AttnTile {
     int lo, hi;        // keys some row of the tile sees: [lo, hi)
@@ -168,8 +171,8 @@ __device__ __forceinline__ void cut_tile(AttnTile &t, int keys, int splits, int 
     t.lo &= ~(kBlock - 1);
     const int steps = max(0, (t.hi - t.lo + keys - 1) / keys);
     t.parts = min(splits, max(1, steps / least));
-    t.from = (int)((int64_t)steps * part / t.parts);
-    t.to = (int)((int64_t)steps * (part + 1) / t.parts);
+    t.from = (int)((uint32_t)steps * (uint32_t)part / (uint32_t)t.parts);  // at most 2^25 steps, 64 shares
+    t.to = (int)((uint32_t)steps * (uint32_t)(part + 1) / (uint32_t)t.parts);
 }
 
 // what the launch adds to a call's arguments
@@ -466,7 +469,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     for (int u = 0; u < QT; ++u) {
         const int row = first_row + (wave * QT + u) * 16 + r16;
         const bool live = row < rows;
-        const int tok = live ? row / p.group : tok0, h = g * p.group + (live ? row % p.group : 0);
+        const int in = row - tok0 * p.group, tok = live ? tok0 + by_group(p, in) : tok0;
+        const int h = g * p.group + (live ? row - tok * p.group : 0);
         const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 8 * kg;
         float x[C][8];
         uint32_t top = 0;
@@ -717,7 +721,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         const float total = groups_sum(l[u]);
         if (row >= rows) continue;
         const bool whole_row = t.parts == 1;
-        const int tok = row / p.group, h = g * p.group + row % p.group;
+        const int tok = tok0 + by_group(p, row - tok0 * p.group), h = g * p.group + row - tok * p.group;
         const float f = whole_row ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
         float *dst = whole_row ? p.out + s * p.o_ss + tok * p.o_st + h * HD + 8 * kg
                                : pl.part + ((slot * pl.splits + part) * kRows + local) * HD + 8 * kg;
@@ -745,24 +749,36 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
 // Few rows (at most 32 per sequence and KV head: one token, small trees).  What
 // counts is how soon the cache is read: no wave waits for another, and K and V
 // go from memory to the fp32 matrix instruction as they are loaded.
-// Workgroup: 16·QT rows, four waves that take the share's blocks of 16 keys in
-// turn, the next block's rows requested before this one's products:
+// Workgroup: 16·QT rows, four waves that take the share's blocks of 16 keys in turn, the next block's rows requested before this one's products:
 //   K  lane 16·q + r: key r, dims 16c + 4q .. +3; product e of chunk c sums over
 //      the dims 16c + 4q + e, as the query rows are held
 //   V  lane 16·q + j: keys 4q .. 4q+3, dims 64d + 4j .. +3
 // Scores and sums come out transposed, as in k_cache_attn; the waves' sums are
 // joined in LDS.  Products, weights and sums are fp32 throughout.
-constexpr int kFewKeys = 16, kFewStep = 4 * kFewKeys;
+constexpr int kFewKeys = 16;
+constexpr int kFewWaves = 4;
 template <int HD, bool TREE, bool SHAPED, int QT>
-__global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAttn p, AttnPlan pl) {
-    constexpr int KC = HD / 16, D = HD / 64, kRows = 16 * QT, kPad = HD + 4;
-    __shared__ __attribute__((aligned(16))) float s_o[4][kRows][kPad];
-    __shared__ float s_m[4][kRows], s_l[4][kRows];
+__global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAttn p, AttnPlan pl) {
+    constexpr int KC = HD / 16, D = HD / 64, kRows = 16 * QT, kPad = HD + 4, W = kFewWaves, kFewStep = W * kFewKeys;
+    __shared__ __attribute__((aligned(16))) float s_o[W][kRows][kPad];
+    __shared__ float s_m[W][kRows], s_l[W][kRows];
     __shared__ uint64_t s_bits[64];
     __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
     const int part = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     const size_t slot = (size_t)s * p.kvh + g;
+    // nothing here waits for the lengths: the query rows, also of tokens that are not there
+    v4f q[QT][KC];
+    int row_tok[QT], row_head[QT];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const int row = min(16 * u + r16, p.n * p.group - 1);
+        row_tok[u] = by_group(p, row);
+        row_head[u] = g * p.group + row - row_tok[u] * p.group;
+        const float *src = p.q + s * p.q_ss + row_tok[u] * p.q_st + row_head[u] * HD + 4 * kg;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) q[u][c] = *reinterpret_cast<const v4f *>(src + 16 * c);
+    }
     int len = 0, count = p.n;
     if (TREE) {
         const SeqRows q = seq_rows(p, s);
@@ -828,18 +844,13 @@ __global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAt
     };
     if (t.from < t.to) load(t.lo + t.from * kFewStep + wave * kFewKeys);
 
-    v4f q[QT][KC];
     float slope[QT];
     int row_lo[QT], row_hi[QT], row_pos[QT];
     uint64_t bits[QT];
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-        const int row = 16 * u + r16;
-        const bool live = row < rows;
-        const int tok = live ? row / p.group : 0, h = g * p.group + (live ? row % p.group : 0);
-        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 4 * kg;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) q[u][c] = *reinterpret_cast<const v4f *>(src + 16 * c);
+        const bool live = 16 * u + r16 < rows;
+        const int tok = row_tok[u], h = row_head[u];
         slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
         row_lo[u] = row_hi[u] = row_pos[u] = 0;
         bits[u] = 0;
@@ -875,15 +886,12 @@ __global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAt
         v4f sc[QT];
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
-            v4f a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+            v4f a[4] = {};
 #pragma unroll
-            for (int c = 0; c < KC; c += 2)
+            for (int c = 0; c < KC; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    a = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c][e], q[u][c][e], a, 0, 0, 0);
-                    b = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c + 1][e], q[u][c + 1][e], b, 0, 0, 0);
-                }
-            sc[u] = a + b;
+                for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c][e], q[u][c][e], a[e], 0, 0, 0);
+            sc[u] = (a[0] + a[1]) + (a[2] + a[3]);
         }
         v4f v[4][D];
 #pragma unroll
@@ -976,17 +984,17 @@ __global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAt
                 *reinterpret_cast<v4f *>(&s_o[wave][row][64 * d + 16 * kg + 4 * i]) = (v4f){o[u][d][0][i], o[u][d][1][i], o[u][d][2][i], o[u][d][3][i]};
     }
     __syncthreads();
-    for (int i = tid; i < rows * (HD / 4); i += 256) {
+    for (int i = tid; i < rows * (HD / 4); i += 64 * W) {
         const int row = i / (HD / 4), at = i % (HD / 4) * 4;
-        float mm = s_m[0][row], f[4], total = 0.0f;
+        float mm = s_m[0][row], total = 0.0f;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, s_m[w][row]);
+        for (int w = 1; w < W; ++w) mm = fmaxf(mm, s_m[w][row]);
         v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mm);
-            total = fmaf(s_l[w][row], f[w], total);
-            x += *reinterpret_cast<const v4f *>(&s_o[w][row][at]) * f[w];
+        for (int w = 0; w < W; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][row] - mm);
+            total = fmaf(s_l[w][row], f, total);
+            x += *reinterpret_cast<const v4f *>(&s_o[w][row][at]) * f;
         }
         if (t.parts > 1) {
             *reinterpret_cast<v4f *>(pl.part + ((slot * pl.splits + part) * kRows + row) * HD + at) = x;
@@ -995,7 +1003,7 @@ __global__ void __launch_bounds__(256, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAt
                     make_float2(mm, total);
             continue;
         }
-        const int tok = row / p.group, h = g * p.group + row % p.group;
+        const int tok = by_group(p, row), h = g * p.group + row - tok * p.group;
         *reinterpret_cast<v4f *>(p.out + s * p.o_ss + tok * p.o_st + h * HD + at) = x * (total == 0.0f ? 0.0f : 1.0f / total);
         if (p.lse && at == 0)
             p.lse[((size_t)s * p.n + tok) * p.heads + h] = (mm + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
