@@ -203,7 +203,7 @@ int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *wor
     return launch_join<HD, 16 * QT>(s, p, pl, seqs);
 }
 
-template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
+template <int HD, bool TREE, bool SHAPED, int QT, bool IMG, int W>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
     if (IMG) {
@@ -211,18 +211,18 @@ int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
         pl.img = img;
         hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps, p.kvh), dim3(kAttnThreads), 0, s, p, img);
     }
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT, IMG>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(kAttnThreads), 0, s, p, pl);
-    return launch_join<HD, 64 * QT>(s, p, pl, seqs);
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT, IMG, W>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(64 * W), 0, s, p, pl);
+    return launch_join<HD, 16 * QT * W>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED>
 int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     if constexpr (!TREE)
-        if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, 2, true>(s, p, sh, work, seqs);
+        if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, 2, true, 4>(s, p, sh, work, seqs);
     if (sh.few)
         return sh.wg_rows == 16 ? launch_few<HD, TREE, SHAPED, 1>(s, p, sh, work, seqs) : launch_few<HD, TREE, SHAPED, 2>(s, p, sh, work, seqs);
-    return sh.wg_rows == 128 ? launch_attn_t<HD, TREE, SHAPED, 2, false>(s, p, sh, work, seqs)
-                      : launch_attn_t<HD, TREE, SHAPED, 1, false>(s, p, sh, work, seqs);
+    return sh.wg_rows == 128 ? launch_attn_t<HD, TREE, SHAPED, 1, false, 8>(s, p, sh, work, seqs)
+                      : launch_attn_t<HD, TREE, SHAPED, 1, false, 4>(s, p, sh, work, seqs);
 }
 
 template <bool TREE>

@@ -203,16 +203,20 @@ struct StepImage {
 };
 static_assert(sizeof(StepImage<128>) == StepImage<128>::kBytes && sizeof(StepImage<64>) == StepImage<64>::kBytes, "whole KB");
 
-// Lays a step's rows into its image: 256 threads, K keys 8·wave + lane%8 by
-// whole 128-byte lines (their pieces meet in a bank in pairs), V the keys of a lane group and two dims of the wave's
-// 32.  Two barriers in between, which the caller places: k(), barrier, v(), barrier.
-// EVEN: the image of one factor where the rows' exponents allow it.
-template <int HD, bool EVEN>
+// Lays a step's rows into its image: four waves each of K and V, the same
+// four or not (has_k, has_v), K keys 8·wave + lane%8 by whole 128-byte lines
+// (their pieces meet in a bank in pairs), V the keys of a lane group and two
+// dims of the wave's 32.  Two barriers in between, which the
+// caller places: sizes(), barrier, put(), barrier.  One exponent serves all
+// keys where theirs lie within 2^kSpread of each other.
+template <int HD>
 struct StepLayer {
     static constexpr int C = HD / 32, kVKeys = HD == 128 ? 8 : 4;
     v4f kx[C];
     v2f vx[kVKeys];
-    int wave, lane, ke;
+    int wave, lane, ke;  // wave: of the four
+    bool has_k, has_v;
+    __device__ __forceinline__ StepLayer(int w, int l, bool k, bool v) : wave(w), lane(l), ke(0), has_k(k), has_v(v) {}
     __device__ __forceinline__ int v_q() const { return HD == 128 ? wave : wave & 1; }
     __device__ __forceinline__ int v_half() const { return HD == 128 ? 0 : wave >> 1; }
     __device__ __forceinline__ int k_key() const { return 8 * wave + (lane & 7); }
@@ -223,112 +227,123 @@ struct StepLayer {
     }
     // k, v: row 0 of the KV head; keys k0 .. k0+31, those past `last` as it
     __device__ __forceinline__ void load(const float *k, int64_t k_st, const float *v, int64_t v_st, int k0, int last) {
-        const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * k_part();
+        if (has_k) {
+            const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * k_part();
 #pragma unroll
-        for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
-        const float *vs = v + 32 * v_q() + 2 * (lane & 15);
-#pragma unroll
-        for (int i = 0; i < kVKeys; ++i) vx[i] = *reinterpret_cast<const v2f *>(vs + min(k0 + v_key(i), last) * v_st);
-    }
-    // sizes of the rows: s_k[32] exponents of K, s_v[C][32] bits of V's parts
-    __device__ __forceinline__ void sizes(int *s_k, uint32_t (*s_v)[kBlock]) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 8));
-        ke = row_exp(groups_umax(top));
-        if (k_part() == 0) s_k[k_key()] = ke;
-        uint32_t m[kVKeys];
-#pragma unroll
-        for (int i = 0; i < kVKeys; ++i) {
-            m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
-            m[i] = lanes8_umax(m[i]);
-            m[i] = max(m[i], __float_as_uint(xchg<XM16>(__uint_as_float(m[i]))));
+            for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
         }
-        if ((lane & 15) == 0)
+        if (has_v) {
+            const float *vs = v + 32 * v_q() + 2 * (lane & 15);
 #pragma unroll
-            for (int i = 0; i < kVKeys; ++i) s_v[v_q()][v_key(i)] = m[i];
-    }
-    __device__ __forceinline__ void put_k(StepImage<HD> *im, int e) const {
-        uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * (k_part() >> 1) + (k_key() & 15)) * 16 + (k_part() & 1) * 8;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            v2h h0, l0, h1, l1;
-            split_h(__builtin_ldexpf(kx[c][0], kTop - e), __builtin_ldexpf(kx[c][1], kTop - e), h0, l0);
-            split_h(__builtin_ldexpf(kx[c][2], kTop - e), __builtin_ldexpf(kx[c][3], kTop - e), h1, l1);
-            *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+            for (int i = 0; i < kVKeys; ++i) vx[i] = *reinterpret_cast<const v2f *>(vs + min(k0 + v_key(i), last) * v_st);
         }
     }
-    __device__ __forceinline__ void put_v(StepImage<HD> *im, const int (&e)[kVKeys]) const {
-        float x[kVKeys], y[kVKeys];
+    // sizes of the rows: s_k[32] exponents of K, s_v[32][4] bits of V's parts
+    __device__ __forceinline__ void sizes(int *s_k, uint32_t (*s_v)[4]) {
+        if (has_k) {
+            uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < kVKeys; ++i) {
-            x[i] = e[i] > kMaxExp ? 0.0f : __builtin_ldexpf(vx[i][0], kTop - e[i]);
-            y[i] = e[i] > kMaxExp ? 0.0f : __builtin_ldexpf(vx[i][1], kTop - e[i]);
+            for (int c = 0; c < C; ++c)
+                top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xF, 0xF, false));  // lane ^ 8
+            ke = row_exp(groups_umax(top));
+            if (k_part() == 0) s_k[k_key()] = ke;
         }
-        uint8_t *dst = im->v + v_q() * 4096 + lane * 16 + v_half() * 8;
+        if (!has_v) return;
+        // 4 or 8 keys over 16 lanes: halves change hands until a lane has one key
+        uint32_t m[8];
 #pragma unroll
-        for (int i = 0; i < kVKeys; i += 4) {
-            v2h h0, l0, h1, l1;
-            split_h(x[i], x[i + 1], h0, l0);
-            split_h(x[i + 2], x[i + 3], h1, l1);
-            *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
-            split_h(y[i], y[i + 1], h0, l0);
-            split_h(y[i + 2], y[i + 3], h1, l1);
-            *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-            *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+        for (int i = 0; i < kVKeys; ++i) m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
+        if (kVKeys == 8) halve<4, XM16>(m, lane & 8);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = max(m[i], __float_as_uint(xchg<XM16>(__uint_as_float(m[i]))));
+        halve<2, XM8>(m, lane & 4);
+        halve<1, XQ2>(m, lane & 2);
+        m[0] = max(m[0], __float_as_uint(xchg<XQ1>(__uint_as_float(m[0]))));
+        const int i = (kVKeys == 8 ? (lane & 8) >> 1 : 0) + ((lane & 4) >> 1) + ((lane & 2) >> 1);
+        if ((lane & 1) == 0) s_v[v_key(i)][v_q()] = m[0];
+    }
+    template <int N, int X>
+    __device__ __forceinline__ static void halve(uint32_t (&m)[8], bool upper) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t keep = upper ? m[i + N] : m[i], give = upper ? m[i] : m[i + N];
+            m[i] = max(keep, __float_as_uint(xchg<X>(__uint_as_float(give))));
         }
     }
-    __device__ __forceinline__ static float v_factor(int e) { return e > kMaxExp ? __uint_as_float(0x7fc00000u) : pow2(e); }
-    // before the first barrier
-    __device__ __forceinline__ void k(StepImage<HD> *im, int *s_k, uint32_t (*s_v)[kBlock]) {
-        sizes(s_k, s_v);
-        if (!EVEN) {
-            if (k_part() == 0) im->kf[k_key()] = pow2(ke - kTop);
-            put_k(im, ke);
-        }
-    }
-    // after it
-    __device__ __forceinline__ void v(StepImage<HD> *im, const int *s_k, const uint32_t (*s_v)[kBlock]) {
-        int e[kVKeys];
-        if (EVEN) {  // every wave looks at all 32 keys: lane l at key l % 32
-            uint32_t bits = 0;
+    // the rows' halves and factors
+    __device__ __forceinline__ void put(StepImage<HD> *im, const int *s_k, const uint32_t (*s_v)[4]) const {
+        // every wave looks at all 32 keys: lane l at key l % 32
+        uint32_t bits = s_v[lane & 31][0];
 #pragma unroll
-            for (int c = 0; c < C; ++c) bits = max(bits, s_v[c][lane & 31]);
-            const int k1 = s_k[lane & 31], v1 = row_exp(bits);
-            int k_hi = k1, v_hi = v1;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                k_hi = max(k_hi, __shfl_xor(k_hi, o));
-                v_hi = max(v_hi, __shfl_xor(v_hi, o));
-            }
-            const bool even = __all(k1 >= k_hi - kSpread && v1 >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
+        for (int c = 1; c < C; ++c) bits = max(bits, s_v[lane & 31][c]);
+        const int k1 = s_k[lane & 31], v1 = row_exp(bits);
+        const int k_hi = max32(k1), v_hi = max32(v1);
+        const bool even = __all(k1 >= k_hi - kSpread && v1 >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
+        if (has_k) {
             const int kk = even ? k_hi : ke;
-            put_k(im, kk);
             if (k_part() == 0) im->kf[k_key()] = pow2(kk - kTop);
+            uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * (k_part() >> 1) + (k_key() & 15)) * 16 + (k_part() & 1) * 8;
 #pragma unroll
-            for (int i = 0; i < kVKeys; ++i) e[i] = even ? v_hi : __shfl(v1, v_key(i));
-            if (wave == 0 && lane == 0) {
-                im->kf_all = pow2(min(k_hi, kMaxExp) - kTop);
-                im->ve_all = v_hi;
-                im->even = even;
+            for (int c = 0; c < C; ++c) {
+                v2h h0, l0, h1, l1;
+                split_h(__builtin_ldexpf(kx[c][0], kTop - kk), __builtin_ldexpf(kx[c][1], kTop - kk), h0, l0);
+                split_h(__builtin_ldexpf(kx[c][2], kTop - kk), __builtin_ldexpf(kx[c][3], kTop - kk), h1, l1);
+                *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
             }
-        } else {
+        }
+        if (!has_v) return;
+        int e[kVKeys];
+#pragma unroll
+        for (int i = 0; i < kVKeys; ++i) e[i] = v_hi;
+        if (!even)
+#pragma unroll
+            for (int i = 0; i < kVKeys; ++i) e[i] = __shfl(v1, v_key(i));
+        {
+            float x[kVKeys], y[kVKeys];
 #pragma unroll
             for (int i = 0; i < kVKeys; ++i) {
-                uint32_t top = 0;
+                x[i] = __builtin_ldexpf(vx[i][0], kTop - e[i]);
+                y[i] = __builtin_ldexpf(vx[i][1], kTop - e[i]);
+            }
+            if (!even)
 #pragma unroll
-                for (int c = 0; c < C; ++c) top = max(top, s_v[c][v_key(i)]);
-                e[i] = row_exp(top);
+                for (int i = 0; i < kVKeys; ++i)
+                    if (e[i] > kMaxExp) x[i] = y[i] = 0.0f;
+            uint8_t *dst = im->v + v_q() * 4096 + lane * 16 + v_half() * 8;
+#pragma unroll
+            for (int i = 0; i < kVKeys; i += 4) {
+                v2h h0, l0, h1, l1;
+                split_h(x[i], x[i + 1], h0, l0);
+                split_h(x[i + 2], x[i + 3], h1, l1);
+                *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+                split_h(y[i], y[i + 1], h0, l0);
+                split_h(y[i + 2], y[i + 3], h1, l1);
+                *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
             }
         }
-        put_v(im, e);
-        if (v_q() == 0 && (lane & 15) == 0)
-#pragma unroll
-            for (int i = 0; i < kVKeys; ++i) im->vf[v_key(i)] = v_factor(e[i]);
+        if (wave == 0 && lane < kBlock) {
+            const int f = even ? v_hi : v1;
+            im->vf[lane] = f > kMaxExp ? __uint_as_float(0x7fc00000u) : pow2(f);
+        }
+        if (wave == 0 && lane == 0) {
+            im->kf_all = pow2(min(k_hi, kMaxExp) - kTop);
+            im->ve_all = v_hi;
+            im->even = even;
+        }
+    }
+    // max over 32 lanes that repeat twice
+    __device__ __forceinline__ static int max32(int v) {
+        v = max(v, __float_as_int(xchg<XQ1>(__int_as_float(v))));
+        v = max(v, __float_as_int(xchg<XQ2>(__int_as_float(v))));
+        v = max(v, __float_as_int(xchg<XM8>(__int_as_float(v))));
+        v = max(v, __float_as_int(xchg<XM16>(__int_as_float(v))));
+        const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+        return max((int)a[0], (int)a[1]);
     }
 };
 
@@ -339,23 +354,21 @@ __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, uint
     using Im = StepImage<HD>;
     __shared__ __attribute__((aligned(16))) Im im;
     __shared__ int s_k[kBlock];
-    __shared__ uint32_t s_v[Im::C][kBlock];
+    __shared__ uint32_t s_v[kBlock][4];
     const int tid = threadIdx.x, g = blockIdx.y;
-    StepLayer<HD, true> st;
-    st.wave = tid >> 6;
-    st.lane = tid & 63;
+    StepLayer<HD> st(tid >> 6, tid & 63, true, true);
     st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, blockIdx.x * kBlock, p.rows - 1);
-    st.k(&im, s_k, s_v);
+    st.sizes(s_k, s_v);
     __syncthreads();
-    st.v(&im, s_k, s_v);
+    st.put(&im, s_k, s_v);
     __syncthreads();
     const uint4 *src = reinterpret_cast<const uint4 *>(&im);
     uint4 *dst = reinterpret_cast<uint4 *>(img + ((size_t)g * gridDim.x + blockIdx.x) * Im::kBytes);
     for (int i = tid; i < Im::kBytes / 16; i += kAttnThreads) dst[i] = src[i];
 }
 
-// Workgroup: 64·QT rows (token, head of the KV head's group) of one sequence
-// and KV head, four waves of 16·QT rows; one share of the keys, 32 a step.
+// Workgroup: 16·QT·W rows (token, head of the KV head's group) of one sequence
+// and KV head, W waves of 16·QT rows; one share of the keys, 32 a step.
 // Scores come out transposed (lane l: query row l%16, keys 4·(l/16) + i of each
 // 16), so a row's maximum, denominator and weights stay with its four lanes and
 // the weights are the second product's operand as they are; the sums come out
@@ -368,14 +381,14 @@ __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, uint
 // the halves hold the products that count whatever the sizes of V's rows.  All
 // rescales are by powers of two.  Steps that every row of the tile sees, with
 // one factor for all keys, need neither masks nor factors per key.
-template <int HD, bool TREE, bool SHAPED, int QT, bool IMG>
-__global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
+template <int HD, bool TREE, bool SHAPED, int QT, bool IMG, int W>
+__global__ void __launch_bounds__(64 * W, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
     using Im = StepImage<HD>;
     constexpr int C = HD / 32;              // 32-dim chunks
-    constexpr int kRows = 64 * QT;
+    constexpr int kRows = 16 * W * QT;
     __shared__ __attribute__((aligned(16))) Im ims[2];
     __shared__ int s_ke[kBlock];
-    __shared__ uint32_t s_ve[C][kBlock];
+    __shared__ uint32_t s_ve[kBlock][4];
     __shared__ uint64_t s_bits[64];
     __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
     __shared__ int2 s_row[kRows];  // the cache rows that each row sees: [x, y)
@@ -447,12 +460,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
         const uint8_t *src = images + (size_t)step * Im::kBytes + wave_u * 1024;
         const uint32_t dst = ims_at + b * Im::kBytes + wave_u * 1024;
 #pragma unroll
-        for (int i = 0; i < (kChunks + 3) / 4; ++i)
-            if (4 * i + wave_u < kChunks) lds_load_at(src + i * 4096, 16 * lane, dst + i * 4096);
+        for (int i = 0; i < (kChunks + W - 1) / W; ++i)
+            if (W * i + wave_u < kChunks) lds_load_at(src + i * W * 1024, 16 * lane, dst + i * W * 1024);
     };
-    StepLayer<HD, false> rowsin;
-    rowsin.wave = wave;
-    rowsin.lane = lane;
+    StepLayer<HD> rowsin(wave_u & 3, lane, W == 4 || wave_u < 4, W == 4 || wave_u >= 4);
     const float *kbase = IMG ? nullptr : p.k + s * p.k_ss + g * HD, *vbase = IMG ? nullptr : p.v + s * p.v_ss + g * HD;
     const int last = t.hi - 1;
     if (t.from < t.to) {
@@ -541,9 +552,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
     };
 
     if (!IMG && t.from < t.to) {
-        rowsin.k(&ims[0], s_ke, s_ve);
+        rowsin.sizes(s_ke, s_ve);
         __syncthreads();
-        rowsin.v(&ims[0], s_ke, s_ve);
+        rowsin.put(&ims[0], s_ke, s_ve);
         __syncthreads();
     }
     for (int step = t.from; step < t.to; ++step) {
@@ -612,7 +623,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
                 return fmaf(x, kLog2e, -slope[u] * fabsf(dist));
             };
             v8h ph[QT], pL[QT];
-            if (IMG && whole && im.even) {
+            if (whole && im.even) {
                 const float kf = im.kf_all;
                 const int ve = im.ve_all;
 #pragma unroll
@@ -708,9 +719,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_attn(CacheAttn p, Att
             }
         }
         if (!IMG && more) {
-            rowsin.k(&ims[b ^ 1], s_ke, s_ve);
+            rowsin.sizes(s_ke, s_ve);
             __syncthreads();
-            rowsin.v(&ims[b ^ 1], s_ke, s_ve);
+            rowsin.put(&ims[b ^ 1], s_ke, s_ve);
             __syncthreads();
         }
     }
