@@ -164,16 +164,16 @@ constexpr int64_t image_bytes = StepImage<HD>::kBytes;
 AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, bool images) {
     AttnShape a;
     a.few = rows <= 32;
-    a.wg_rows = a.few ? (rows <= 16 ? 16 : 32) : (rows <= 64 ? 64 : 128);
+    a.wg_rows = a.few ? (rows <= 16 ? 16 : 32) : 128;
     a.tiles = round_up_div(rows, a.wg_rows);
     const int64_t work = a.tiles * groups;
     // two workgroups a CU; prompts of many short rows (documents) leave most
     // CUs idle behind their longest tile unless that is cut too
-    const int64_t want = std::max<int64_t>(1, (work < 256 ? 512 : 1024) / work);
-    const int step = !a.few ? kBlock : kFewKeys * kFewWaves;
+    a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
+    const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : (a.few || a.steps ? 512 : 256)) / work);
+    const int step = a.few ? kFewKeys * kFewWaves : kBlock;
     a.least = a.few ? 1 : (work < 128 ? 2 : 6);
     a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
-    a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
     a.part_bytes = a.splits == 1 ? 0 : work * a.splits * a.wg_rows * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
     a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
     return a;
@@ -203,7 +203,7 @@ int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *wor
     return launch_join<HD, 16 * QT>(s, p, pl, seqs);
 }
 
-template <int HD, bool TREE, bool SHAPED, int QT, bool IMG, int W>
+template <int HD, bool TREE, bool SHAPED, bool IMG>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
     if (IMG) {
@@ -211,18 +211,17 @@ int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
         pl.img = img;
         hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps, p.kvh), dim3(kAttnThreads), 0, s, p, img);
     }
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, QT, IMG, W>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(64 * W), 0, s, p, pl);
-    return launch_join<HD, 16 * QT * W>(s, p, pl, seqs);
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(IMG ? 256 : 512), 0, s, p, pl);
+    return launch_join<HD, 128>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED>
 int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     if constexpr (!TREE)
-        if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, 2, true, 4>(s, p, sh, work, seqs);
+        if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, true>(s, p, sh, work, seqs);
     if (sh.few)
         return sh.wg_rows == 16 ? launch_few<HD, TREE, SHAPED, 1>(s, p, sh, work, seqs) : launch_few<HD, TREE, SHAPED, 2>(s, p, sh, work, seqs);
-    return sh.wg_rows == 128 ? launch_attn_t<HD, TREE, SHAPED, 1, false, 8>(s, p, sh, work, seqs)
-                      : launch_attn_t<HD, TREE, SHAPED, 1, false, 4>(s, p, sh, work, seqs);
+    return launch_attn_t<HD, TREE, SHAPED, false>(s, p, sh, work, seqs);
 }
 
 template <bool TREE>

@@ -73,9 +73,22 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ void split_h(float a, float b, v2h &hi, v2h &lo) {
-    hi = __builtin_convertvector((v2f){a, b}, v2h);
-    lo = __builtin_convertvector((v2f){__builtin_fmaf((float)hi[0], -1.0f, a), __builtin_fmaf((float)hi[1], -1.0f, b)}, v2h);
+// the halves of a·f and b·f: the conversions and the remainders a·f - hi are
+// each one mixed-precision multiply-add (hi's halves are read where they lie;
+// without the empty asm the compiler makes each of them twice)
+__device__ __forceinline__ v2h whole_v2h(v2h x) {
+    uint32_t u = __builtin_bit_cast(uint32_t, x);
+    asm("" : "+v"(u));
+    return __builtin_bit_cast(v2h, u);
+}
+__device__ __forceinline__ void split_h(float a, float b, float f, v2h &hi, v2h &lo) {
+    hi = whole_v2h((v2h){(_Float16)__builtin_fmaf(a, f, 0.0f), (_Float16)__builtin_fmaf(b, f, 0.0f)});
+    lo = (v2h){(_Float16)__builtin_fmaf(a, f, -(float)hi[0]), (_Float16)__builtin_fmaf(b, f, -(float)hi[1])};
+}
+// likewise of a and b; one: 1, where the compiler does not see it
+__device__ __forceinline__ void split_one(float a, float b, float one, v2h &hi, v2h &lo) {
+    hi = whole_v2h(__builtin_convertvector((v2f){a, b}, v2h));
+    lo = (v2h){(_Float16)__builtin_fmaf(a, one, -(float)hi[0]), (_Float16)__builtin_fmaf(b, one, -(float)hi[1])};
 }
 
 constexpr int kTop = 14;        // operand rows are scaled to sizes below 2^kTop
@@ -94,12 +107,13 @@ __device__ __forceinline__ uint32_t umax3(uint32_t a, uint32_t b, uint32_t c) { 
 // a lane's share of a row, scaled by its exponent, as halves
 template <int C>
 __device__ __forceinline__ void split_row(const float (&x)[C][8], int e, v8h (&hi)[C], v8h (&lo)[C]) {
+    const float f = pow2(kTop - e);
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             v2h h, l;
-            split_h(__builtin_ldexpf(x[c][i], kTop - e), __builtin_ldexpf(x[c][i + 1], kTop - e), h, l);
+            split_h(x[c][i], x[c][i + 1], f, h, l);
             hi[c][i] = h[0];
             hi[c][i + 1] = h[1];
             lo[c][i] = l[0];
@@ -190,67 +204,59 @@ struct AttnPlan {
 // and, for prompts of many tiles, in memory:
 //   K  [16-key tile][32-dim chunk][half] lane l = 16·q + r: key r, dims 32c + 8q .. +7
 //   V  [32-dim chunk][t][half] lane l = 16·q + j: keys 4q .. +3 and 16+4q .. +3, dim 32c + 2j + t
-//   the keys' factors kf (key row = stored · kf) and vf (value row = stored · 2^-kTop · vf),
-//   and whether one factor holds for all of them.
+//   the keys' factors kf (key row = stored · kf) and vf (value row = stored · 2^-kTop · vf).
+// Scores come out with lane group q on keys 4q .. +3 and 16+4q .. +3; where the
+// exponents of these eight rows allow it, for all four groups (`even`), a
+// group's rows have one factor: a lane then needs one of each.
 template <int HD>
 struct StepImage {
     static constexpr int C = HD / 32, kK = 2 * C * 2 * 1024, kV = C * 2 * 2 * 1024, kSide = kK + kV, kBytes = kSide + 1024;
     uint8_t k[kK], v[kV];
     float kf[kBlock], vf[kBlock];
-    float kf_all;  // where `even`: every key's kf, and the exponent of every vf
-    int ve_all, even;
-    uint8_t pad[1024 - 8 * kBlock - 12];
+    float kf_group[4];
+    int ve_group[4];  // exponents of vf
+    int even[4];
+    uint8_t pad[1024 - 8 * kBlock - 48];
 };
 static_assert(sizeof(StepImage<128>) == StepImage<128>::kBytes && sizeof(StepImage<64>) == StepImage<64>::kBytes, "whole KB");
 
-// Lays a step's rows into its image: four waves each of K and V, the same
-// four or not (has_k, has_v), K keys 8·wave + lane%8 by whole 128-byte lines
-// (their pieces meet in a bank in pairs), V the keys of a lane group and two
-// dims of the wave's 32.  Two barriers in between, which the
-// caller places: sizes(), barrier, put(), barrier.  One exponent serves all
-// keys where theirs lie within 2^kSpread of each other.
+// Lays eight rows of each of K and V into a step's image, those of lane group
+// `group`, by one wave that waits for no other.  K: lane kk + 8·part holds key
+// kk's floats 4·part + 32c .. +3 (whole 128-byte lines); V: lane l dims 2l,
+// 2l + 1 of all eight keys (heads of 64: lanes l and l + 32 four keys each).
 template <int HD>
 struct StepLayer {
     static constexpr int C = HD / 32, kVKeys = HD == 128 ? 8 : 4;
     v4f kx[C];
     v2f vx[kVKeys];
-    int wave, lane, ke;  // wave: of the four
-    bool has_k, has_v;
-    __device__ __forceinline__ StepLayer(int w, int l, bool k, bool v) : wave(w), lane(l), ke(0), has_k(k), has_v(v) {}
-    __device__ __forceinline__ int v_q() const { return HD == 128 ? wave : wave & 1; }
-    __device__ __forceinline__ int v_half() const { return HD == 128 ? 0 : wave >> 1; }
-    __device__ __forceinline__ int k_key() const { return 8 * wave + (lane & 7); }
-    __device__ __forceinline__ int k_part() const { return lane >> 3; }
-    __device__ __forceinline__ int v_key(int i) const {
-        const int kg = lane >> 4;
-        return HD == 128 ? 4 * kg + (i & 3) + 4 * (i & 4) : 16 * v_half() + 4 * kg + i;
-    }
+    __device__ __forceinline__ static int key_of(int group, int i) { return 4 * group + (i & 3) + 4 * (i & 4); }
+    __device__ __forceinline__ static int v_first(int lane) { return HD == 128 ? 0 : (lane >> 5) * 4; }
     // k, v: row 0 of the KV head; keys k0 .. k0+31, those past `last` as it
-    __device__ __forceinline__ void load(const float *k, int64_t k_st, const float *v, int64_t v_st, int k0, int last) {
-        if (has_k) {
-            const float *ks = k + min(k0 + k_key(), last) * k_st + 4 * k_part();
+    __device__ __forceinline__ void load(const float *k, int64_t k_st, const float *v, int64_t v_st, int k0, int last, int group, int lane) {
+        const float *ks = k + min(k0 + key_of(group, lane & 7), last) * k_st + 4 * (lane >> 3);
 #pragma unroll
-            for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
-        }
-        if (has_v) {
-            const float *vs = v + 32 * v_q() + 2 * (lane & 15);
+        for (int c = 0; c < C; ++c) kx[c] = *reinterpret_cast<const v4f *>(ks + 32 * c);
+        const float *vs = v + 2 * (lane % (HD / 2));
 #pragma unroll
-            for (int i = 0; i < kVKeys; ++i) vx[i] = *reinterpret_cast<const v2f *>(vs + min(k0 + v_key(i), last) * v_st);
+        for (int i = 0; i < kVKeys; ++i)
+            vx[i] = *reinterpret_cast<const v2f *>(vs + min(k0 + key_of(group, v_first(lane) + i), last) * v_st);
+    }
+    template <int N, int X>
+    __device__ __forceinline__ static void halve(uint32_t (&m)[8], bool upper) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t keep = upper ? m[i + N] : m[i], give = upper ? m[i] : m[i + N];
+            m[i] = max(keep, __float_as_uint(xchg<X>(__uint_as_float(give))));
         }
     }
-    // sizes of the rows: s_k[32] exponents of K, s_v[32][4] bits of V's parts
-    __device__ __forceinline__ void sizes(int *s_k, uint32_t (*s_v)[4]) {
-        if (has_k) {
-            uint32_t top = 0;
+    __device__ __forceinline__ void put(StepImage<HD> *im, int group, int lane) const {
+        // sizes: lane's K key kk = lane & 7, and V key i
+        uint32_t kt = 0;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                top = umax3(top, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
-            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xF, 0xF, false));  // lane ^ 8
-            ke = row_exp(groups_umax(top));
-            if (k_part() == 0) s_k[k_key()] = ke;
-        }
-        if (!has_v) return;
-        // 4 or 8 keys over 16 lanes: halves change hands until a lane has one key
+        for (int c = 0; c < C; ++c)
+            kt = umax3(kt, max(abs_bits(kx[c][0]), abs_bits(kx[c][1])), max(abs_bits(kx[c][2]), abs_bits(kx[c][3])));
+        kt = max(kt, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)kt, 0x128, 0xF, 0xF, false));  // lane ^ 8
+        const int ke = row_exp(groups_umax(kt));
         uint32_t m[8];
 #pragma unroll
         for (int i = 0; i < kVKeys; ++i) m[i] = max(abs_bits(vx[i][0]), abs_bits(vx[i][1]));
@@ -261,89 +267,81 @@ struct StepLayer {
         halve<2, XM8>(m, lane & 4);
         halve<1, XQ2>(m, lane & 2);
         m[0] = max(m[0], __float_as_uint(xchg<XQ1>(__uint_as_float(m[0]))));
-        const int i = (kVKeys == 8 ? (lane & 8) >> 1 : 0) + ((lane & 4) >> 1) + ((lane & 2) >> 1);
-        if ((lane & 1) == 0) s_v[v_key(i)][v_q()] = m[0];
-    }
-    template <int N, int X>
-    __device__ __forceinline__ static void halve(uint32_t (&m)[8], bool upper) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t keep = upper ? m[i + N] : m[i], give = upper ? m[i] : m[i + N];
-            m[i] = max(keep, __float_as_uint(xchg<X>(__uint_as_float(give))));
+        const int at = (kVKeys == 8 ? (lane & 8) >> 1 : (lane >> 5) * 4) + ((lane & 4) >> 1) + ((lane & 2) >> 1);  // the key of m[0]
+        {
+            const auto a = __builtin_amdgcn_permlane16_swap(m[0], m[0], false, false);
+            m[0] = max((uint32_t)a[0], (uint32_t)a[1]);
         }
-    }
-    // the rows' halves and factors
-    __device__ __forceinline__ void put(StepImage<HD> *im, const int *s_k, const uint32_t (*s_v)[4]) const {
-        // every wave looks at all 32 keys: lane l at key l % 32
-        uint32_t bits = s_v[lane & 31][0];
-#pragma unroll
-        for (int c = 1; c < C; ++c) bits = max(bits, s_v[lane & 31][c]);
-        const int k1 = s_k[lane & 31], v1 = row_exp(bits);
-        const int k_hi = max32(k1), v_hi = max32(v1);
-        const bool even = __all(k1 >= k_hi - kSpread && v1 >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
-        if (has_k) {
-            const int kk = even ? k_hi : ke;
-            if (k_part() == 0) im->kf[k_key()] = pow2(kk - kTop);
-            uint8_t *dst = im->k + (k_key() >> 4) * C * 2048 + (16 * (k_part() >> 1) + (k_key() & 15)) * 16 + (k_part() & 1) * 8;
+        if (HD == 128) {
+            const auto a = __builtin_amdgcn_permlane32_swap(m[0], m[0], false, false);
+            m[0] = max((uint32_t)a[0], (uint32_t)a[1]);
+        }
+        const int ve = row_exp(m[0]);
+        // all eight of each: the wave's largest
+        const int k_hi = max8lanes(ke);
+        int v_hi = max8lanes(ve);  // over lanes of a row of 16
+        v_hi = max(v_hi, __float_as_int(xchg<XM16>(__int_as_float(v_hi))));
+        {
+            const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)v_hi, (uint32_t)v_hi, false, false);
+            v_hi = max((int)a[0], (int)a[1]);
+        }
+        const bool even = __all(ke >= k_hi - kSpread && ve >= v_hi - kSpread && k_hi <= kMaxExp && v_hi <= kMaxExp);
+        const int kk = even ? k_hi : ke;
+        {
+            const int key = key_of(group, lane & 7), part = lane >> 3;
+            const float f = pow2(kTop - kk);
+            uint8_t *dst = im->k + (key >> 4) * C * 2048 + (16 * (part >> 1) + (key & 15)) * 16 + (part & 1) * 8;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 v2h h0, l0, h1, l1;
-                split_h(__builtin_ldexpf(kx[c][0], kTop - kk), __builtin_ldexpf(kx[c][1], kTop - kk), h0, l0);
-                split_h(__builtin_ldexpf(kx[c][2], kTop - kk), __builtin_ldexpf(kx[c][3], kTop - kk), h1, l1);
+                split_h(kx[c][0], kx[c][1], f, h0, l0);
+                split_h(kx[c][2], kx[c][3], f, h1, l1);
                 *reinterpret_cast<v4h *>(dst + c * 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
                 *reinterpret_cast<v4h *>(dst + c * 2048 + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
             }
+            if (part == 0) im->kf[key] = pow2(kk - kTop);
         }
-        if (!has_v) return;
-        int e[kVKeys];
+        const int ee = even ? v_hi : ve;
+        if ((lane & 1) == 0 && (HD == 64 || lane < 16)) im->vf[key_of(group, at)] = ee > kMaxExp ? __uint_as_float(0x7fc00000u) : pow2(ee);
+        // rows that count as infinite are stored as zeros
+        const float mine = ee > kMaxExp ? 0.0f : pow2(kTop - ee);
+        uint8_t *dst = im->v + (lane % (HD / 2)) / 16 * 4096 + (16 * group + (lane & 15)) * 16 + v_first(lane) * 2;
 #pragma unroll
-        for (int i = 0; i < kVKeys; ++i) e[i] = v_hi;
-        if (!even)
+        for (int i = 0; i < kVKeys; i += 4) {
+            float f[4];
 #pragma unroll
-            for (int i = 0; i < kVKeys; ++i) e[i] = __shfl(v1, v_key(i));
-        {
-            float x[kVKeys], y[kVKeys];
+            for (int x = 0; x < 4; ++x) f[x] = even ? mine : __shfl(mine, key_lane(v_first(lane) + i + x));
 #pragma unroll
-            for (int i = 0; i < kVKeys; ++i) {
-                x[i] = __builtin_ldexpf(vx[i][0], kTop - e[i]);
-                y[i] = __builtin_ldexpf(vx[i][1], kTop - e[i]);
-            }
-            if (!even)
-#pragma unroll
-                for (int i = 0; i < kVKeys; ++i)
-                    if (e[i] > kMaxExp) x[i] = y[i] = 0.0f;
-            uint8_t *dst = im->v + v_q() * 4096 + lane * 16 + v_half() * 8;
-#pragma unroll
-            for (int i = 0; i < kVKeys; i += 4) {
+            for (int t = 0; t < 2; ++t) {
                 v2h h0, l0, h1, l1;
-                split_h(x[i], x[i + 1], h0, l0);
-                split_h(x[i + 2], x[i + 3], h1, l1);
-                *reinterpret_cast<v4h *>(dst + 2 * i) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-                *reinterpret_cast<v4h *>(dst + 2 * i + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
-                split_h(y[i], y[i + 1], h0, l0);
-                split_h(y[i + 2], y[i + 3], h1, l1);
-                *reinterpret_cast<v4h *>(dst + 2 * i + 2048) = (v4h){h0[0], h0[1], h1[0], h1[1]};
-                *reinterpret_cast<v4h *>(dst + 2 * i + 3072) = (v4h){l0[0], l0[1], l1[0], l1[1]};
+                if (even) {
+                    split_h(vx[i][t], vx[i + 1][t], mine, h0, l0);
+                    split_h(vx[i + 2][t], vx[i + 3][t], mine, h1, l1);
+                } else {
+                    float y[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) y[x] = f[x] != 0.0f ? vx[i + x][t] * f[x] : 0.0f;
+                    split_h(y[0], y[1], 1.0f, h0, l0);
+                    split_h(y[2], y[3], 1.0f, h1, l1);
+                }
+                *reinterpret_cast<v4h *>(dst + 2 * i + 2048 * t) = (v4h){h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<v4h *>(dst + 2 * i + 2048 * t + 1024) = (v4h){l0[0], l0[1], l1[0], l1[1]};
             }
         }
-        if (wave == 0 && lane < kBlock) {
-            const int f = even ? v_hi : v1;
-            im->vf[lane] = f > kMaxExp ? __uint_as_float(0x7fc00000u) : pow2(f);
-        }
-        if (wave == 0 && lane == 0) {
-            im->kf_all = pow2(min(k_hi, kMaxExp) - kTop);
-            im->ve_all = v_hi;
-            im->even = even;
+        if (lane == 0) {
+            im->kf_group[group] = pow2(min(k_hi, kMaxExp) - kTop);
+            im->ve_group[group] = v_hi;
+            im->even[group] = even;
         }
     }
-    // max over 32 lanes that repeat twice
-    __device__ __forceinline__ static int max32(int v) {
+    // a lane that holds V key i's size (of a half of the lanes for heads of 64)
+    __device__ __forceinline__ static int key_lane(int i) {
+        return HD == 128 ? ((i & 4) << 1) + ((i & 2) << 1) + ((i & 1) << 1) : ((i & 4) << 3) + ((i & 2) << 1) + ((i & 1) << 1);
+    }
+    __device__ __forceinline__ static int max8lanes(int v) {
         v = max(v, __float_as_int(xchg<XQ1>(__int_as_float(v))));
         v = max(v, __float_as_int(xchg<XQ2>(__int_as_float(v))));
-        v = max(v, __float_as_int(xchg<XM8>(__int_as_float(v))));
-        v = max(v, __float_as_int(xchg<XM16>(__int_as_float(v))));
-        const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-        return max((int)a[0], (int)a[1]);
+        return max(v, __float_as_int(xchg<XM8>(__int_as_float(v))));
     }
 };
 
@@ -353,42 +351,38 @@ template <int HD>
 __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, uint8_t *img) {
     using Im = StepImage<HD>;
     __shared__ __attribute__((aligned(16))) Im im;
-    __shared__ int s_k[kBlock];
-    __shared__ uint32_t s_v[kBlock][4];
     const int tid = threadIdx.x, g = blockIdx.y;
-    StepLayer<HD> st(tid >> 6, tid & 63, true, true);
-    st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, blockIdx.x * kBlock, p.rows - 1);
-    st.sizes(s_k, s_v);
-    __syncthreads();
-    st.put(&im, s_k, s_v);
+    StepLayer<HD> st;
+    st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, blockIdx.x * kBlock, p.rows - 1, tid >> 6, tid & 63);
+    st.put(&im, tid >> 6, tid & 63);
     __syncthreads();
     const uint4 *src = reinterpret_cast<const uint4 *>(&im);
     uint4 *dst = reinterpret_cast<uint4 *>(img + ((size_t)g * gridDim.x + blockIdx.x) * Im::kBytes);
     for (int i = tid; i < Im::kBytes / 16; i += kAttnThreads) dst[i] = src[i];
 }
 
-// Workgroup: 16·QT·W rows (token, head of the KV head's group) of one sequence
-// and KV head, W waves of 16·QT rows; one share of the keys, 32 a step.
-// Scores come out transposed (lane l: query row l%16, keys 4·(l/16) + i of each
-// 16), so a row's maximum, denominator and weights stay with its four lanes and
-// the weights are the second product's operand as they are; the sums come out
+// Workgroup: 128 rows (token, head of the KV head's group) of one sequence and
+// KV head, four waves of 32 rows; one share of the keys, 32 a step.  Scores come
+// out transposed (lane l: query row l%16, keys 4·(l/16) + i of each 16), so a
+// row's maximum, denominator and weights stay with its four lanes and the
+// weights are the second product's operand as they are; the sums come out
 // transposed too (lane: the same query row, 8 consecutive dims of each 32).
 // Two LDS buffers: a step's products run on one while the next step's image
-// arrives in the other (IMG: direct loads; else the rows, laid out here).
+// arrives in the other, by direct loads (IMG) or from four more waves that do
+// nothing but lay rows out: what these spend on vector instructions then runs
+// beside the others' matrix instructions.
 //
 // A row's weights are e = 2^(x - m), m an integer above its maximum so far; the
 // products take e·vf·2^(14-a) with 2^a above the row's largest e·vf so far, so
 // the halves hold the products that count whatever the sizes of V's rows.  All
 // rescales are by powers of two.  Steps that every row of the tile sees, with
-// one factor for all keys, need neither masks nor factors per key.
-template <int HD, bool TREE, bool SHAPED, int QT, bool IMG, int W>
-__global__ void __launch_bounds__(64 * W, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
+// even factors, need neither masks nor factors per key.
+template <int HD, bool TREE, bool SHAPED, bool IMG>
+__global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
     using Im = StepImage<HD>;
     constexpr int C = HD / 32;              // 32-dim chunks
-    constexpr int kRows = 16 * W * QT;
+    constexpr int QT = 2, W = 4, kRows = 16 * W * QT;
     __shared__ __attribute__((aligned(16))) Im ims[2];
-    __shared__ int s_ke[kBlock];
-    __shared__ uint32_t s_ve[kBlock][4];
     __shared__ uint64_t s_bits[64];
     __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
     __shared__ int2 s_row[kRows];  // the cache rows that each row sees: [x, y)
@@ -463,13 +457,25 @@ __global__ void __launch_bounds__(64 * W, 2) k_cache_attn(CacheAttn p, AttnPlan 
         for (int i = 0; i < (kChunks + W - 1) / W; ++i)
             if (W * i + wave_u < kChunks) lds_load_at(src + i * W * 1024, 16 * lane, dst + i * W * 1024);
     };
-    StepLayer<HD> rowsin(wave_u & 3, lane, W == 4 || wave_u < 4, W == 4 || wave_u >= 4);
-    const float *kbase = IMG ? nullptr : p.k + s * p.k_ss + g * HD, *vbase = IMG ? nullptr : p.v + s * p.v_ss + g * HD;
-    const int last = t.hi - 1;
-    if (t.from < t.to) {
-        if (IMG) fetch(t.from, 0);
-        else rowsin.load(kbase, p.k_st, vbase, p.v_st, t.lo + t.from * kBlock, last);
+    if (IMG && t.from < t.to) fetch(t.from, 0);
+    if (!IMG && wave_u >= W) {  // a producer: its group's rows of every step, two steps ahead of their use
+        const float *kbase = p.k + s * p.k_ss + g * HD, *vbase = p.v + s * p.v_ss + g * HD;
+        StepLayer<HD> x[2];
+        if (t.from < t.to) x[0].load(kbase, p.k_st, vbase, p.v_st, t.lo + t.from * kBlock, t.hi - 1, wave_u - W, lane);
+        if (t.from + 1 < t.to) x[1].load(kbase, p.k_st, vbase, p.v_st, t.lo + (t.from + 1) * kBlock, t.hi - 1, wave_u - W, lane);
+        for (int step = t.from; step < t.to; step += 2) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (step + b >= t.to) break;
+                x[b].put(&ims[b], wave_u - W, lane);
+                if (step + b + 2 < t.to)
+                    x[b].load(kbase, p.k_st, vbase, p.v_st, t.lo + (step + b + 2) * kBlock, t.hi - 1, wave_u - W, lane);
+                __syncthreads();  // the step is there, and the one before it done with
+            }
+        }
+        return;
     }
+    const int last = t.hi - 1;
 
     // query rows: halves, scale, what they see
     v8h qh[QT][C], ql[QT][C];
@@ -529,50 +535,42 @@ __global__ void __launch_bounds__(64 * W, 2) k_cache_attn(CacheAttn p, AttnPlan 
 #pragma unroll
         for (int d = 0; d < 2 * C; ++d) o[u][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // a row's maximum (in its four lanes) and the largest exponent of its weighted values
+    // a row's maximum (in its four lanes), and the largest exponent of its
+    // weighted values: the power of two that its sums are due for it
     auto raise_m = [&](int u, float top) {
-        if (__any(top > m[u])) {
-            const float mn = top > m[u] ? ceilf(top) + 2.0f : m[u];
-            l[u] *= __builtin_amdgcn_exp2f(m[u] - mn);
-            a[u] = max(a[u] - (int)fminf(mn - m[u], 16384.0f), -16384);
-            m[u] = mn;
-        }
+        const float mn = top > m[u] ? ceilf(top) + 2.0f : m[u];
+        l[u] *= __builtin_amdgcn_exp2f(m[u] - mn);
+        a[u] = max(a[u] - (int)fminf(mn - m[u], 16384.0f), -16384);
+        m[u] = mn;
     };
     auto raise_a = [&](int u, int need) {
-        if (__any(need > a[u])) {
-            const int an = need > a[u] ? need + 3 : a[u];
-            const float f = __builtin_ldexpf(1.0f, max(a[u] - an, -200));
-#pragma unroll
-            for (int d = 0; d < 2 * C; ++d) o[u][d] *= f;
-            a[u] = an;
-        }
+        const int an = need > a[u] ? need + 3 : a[u], by = max(a[u] - an, -200);
+        a[u] = an;
+        return by;
     };
     auto max8 = [](const float (&x)[8]) {
-        return groups_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+        return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     };
+    float one = 1.0f;
+    asm("" : "+s"(one));
+    const bool live_wave = first_row + wave * QT * 16 < rows;
 
-    if (!IMG && t.from < t.to) {
-        rowsin.sizes(s_ke, s_ve);
-        __syncthreads();
-        rowsin.put(&ims[0], s_ke, s_ve);
-        __syncthreads();
-    }
     for (int step = t.from; step < t.to; ++step) {
         const int b = (step - t.from) & 1, k0 = t.lo + step * kBlock;
-        const bool more = step + 1 < t.to;
         const Im &im = ims[b];
         if (IMG) {
             wait_vm<0>();   // this wave's part of the step's image is in LDS,
             lds_barrier();  // now everybody's is, and nobody reads the other buffer any more
-            if (more) fetch(step + 1, b ^ 1);
-        } else if (more) {
-            rowsin.load(kbase, p.k_st, vbase, p.v_st, k0 + kBlock, last);
+            if (step + 1 < t.to) fetch(step + 1, b ^ 1);
+        } else {
+            __syncthreads();  // the producers' image likewise
         }
+        if (!live_wave) continue;
         const bool whole = k0 >= all_lo && k0 + kBlock <= all_hi;
         // what each row sees of the step's keys, as bits
         uint32_t see[QT];
-        bool any = whole;
         if (!whole) {
+            bool any = false;
 #pragma unroll
             for (int u = 0; u < QT; ++u) {
                 const int2 sees = s_row[(wave * QT + u) * 16 + r16];
@@ -584,145 +582,136 @@ __global__ void __launch_bounds__(64 * W, 2) k_cache_attn(CacheAttn p, AttnPlan 
                 }
                 any = any || see[u];
             }
-            any = __any(any);
+            if (!__any(any)) continue;
         }
-        if (any) {
-            v4f sc[QT][2];
+        v4f sc[QT][2];
 #pragma unroll
-            for (int u = 0; u < QT; ++u) sc[u][0] = sc[u][1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < QT; ++u) sc[u][0] = sc[u][1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int c = 0; c < C; ++c) {  // neighbouring products go to different sums
-                v8h kh[2], kl[2];
+        for (int c = 0; c < C; ++c) {  // neighbouring products go to different sums
+            v8h kh[2], kl[2];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    kh[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + lane * 16);
-                    kl[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + 1024 + lane * 16);
-                }
-#pragma unroll
-                for (int x = 0; x < 3; ++x)
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                        for (int u = 0; u < QT; ++u)
-                            sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? kl[kt] : kh[kt], x == 1 ? ql[u][c] : qh[u][c],
-                                                                               sc[u][kt], 0, 0, 0);
+            for (int kt = 0; kt < 2; ++kt) {
+                kh[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + lane * 16);
+                kl[kt] = *reinterpret_cast<const v8h *>(im.k + (kt * C + c) * 2048 + 1024 + lane * 16);
             }
-            int kpos[8];
-            if (TREE && SHAPED) {
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int u = 0; u < QT; ++u)
+                        sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? kl[kt] : kh[kt], x == 1 ? ql[u][c] : qh[u][c],
+                                                                           sc[u][kt], 0, 0, 0);
+        }
+        // capped and biased scores, to the base 2, of key k0 + 16(e/4) + 4kg + e%4
+        auto shape = [&](int u, float x, int e) {
+            if (p.cap > 0.0f) x = p.cap * tanh_f(x * inv_cap);
+            if (!p.slopes) return x * kLog2e;
+            const int in = 16 * (e >> 2) + (e & 3);
+            float dist = (float)(row_pos[u] - k0 - 4 * kg) - (float)in;
+            if (TREE) {
+                const int key = k0 + 4 * kg + in;
+                const int at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
+                dist = (float)(int)((uint32_t)row_pos[u] - (uint32_t)at);
+            }
+            return fmaf(x, kLog2e, -slope[u] * fabsf(dist));
+        };
+        v8h ph[QT], pL[QT];
+        int by[QT];
+        auto weights = [&](int u, const float (&w)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                v2h hi, lo;
+                split_one(w[e], w[e + 1], one, hi, lo);
+                ph[u][e] = hi[0];
+                ph[u][e + 1] = hi[1];
+                pL[u][e] = lo[0];
+                pL[u][e + 1] = lo[1];
+            }
+        };
+        if (whole && __all(im.even[kg])) {  // all rows see all keys, the lane's keys have one factor
+            const float kf = im.kf_group[kg];
+            const int ve = im.ve_group[kg];
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+                const float f = kf * qf[u];
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = SHAPED ? shape(u, sc[u][e >> 2][e & 3] * f, e) : sc[u][e >> 2][e & 3];
+                const float mine = SHAPED ? max8(x) : max8(x) * f;
+                raise_m(u, groups_max(mine));
+                by[u] = raise_a(u, (int)groups_max(ceilf(fmaxf(mine - m[u], -16000.0f)) + (float)ve));
+                // weights below 2^-60 of the largest come out 0 either way
+                const int sh = max(14 + ve - a[u], -60);
+                const float mm = m[u] - (float)sh;
+                float w[8], sum = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int key = k0 + 16 * (e >> 2) + 4 * kg + (e & 3);
-                    kpos[e] = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
+                    w[e] = __builtin_amdgcn_exp2f(SHAPED ? x[e] - mm : __builtin_fmaf(x[e], f, -mm));
+                    sum += w[e];
                 }
+                l[u] += __builtin_ldexpf(sum, -sh);
+                weights(u, w);
             }
-            // capped and biased scores, to the base 2
-            auto shape = [&](int u, float x, int e) {
-                if (p.cap > 0.0f) x = p.cap * tanh_f(x * inv_cap);
-                const float dist = TREE ? (float)(int)((uint32_t)row_pos[u] - (uint32_t)kpos[e])
-                                        : (float)(row_pos[u] - k0 - 4 * kg) - (float)(16 * (e >> 2) + (e & 3));
-                return fmaf(x, kLog2e, -slope[u] * fabsf(dist));
-            };
-            v8h ph[QT], pL[QT];
-            if (whole && im.even) {
-                const float kf = im.kf_all;
-                const int ve = im.ve_all;
+        } else {
 #pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    const float f = kf * qf[u];
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = SHAPED ? shape(u, sc[u][e >> 2][e & 3] * f, e) : sc[u][e >> 2][e & 3];
-                    const float top = SHAPED ? max8(x) : max8(x) * f;
-                    raise_m(u, top);
-                    raise_a(u, ve + (int)ceilf(fmaxf(top - m[u], -16000.0f)));
-                    // weights below 2^-60 of the largest come out 0 either way
-                    const int sh = max(14 + ve - a[u], -60);
-                    const float mm = m[u] - (float)sh;
-                    float w[8], sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        w[e] = __builtin_amdgcn_exp2f(SHAPED ? x[e] - mm : fmaf(x[e], f, -mm));
-                        sum += w[e];
-                    }
-                    l[u] += __builtin_ldexpf(sum, -sh);
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        v2h hi, lo;
-                        split_h(w[e], w[e + 1], hi, lo);
-                        ph[u][e] = hi[0];
-                        ph[u][e + 1] = hi[1];
-                        pL[u][e] = lo[0];
-                        pL[u][e + 1] = lo[1];
-                    }
-                }
-            } else {
-                float kf[8], vf[8];
+            for (int u = 0; u < QT; ++u) {
+                const uint32_t mine = whole ? ~0u : see[u] >> (4 * kg);
+                float x[8], vf[8];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
                     const v4f fk = *reinterpret_cast<const v4f *>(&im.kf[16 * kt + 4 * kg]);
                     const v4f fv = *reinterpret_cast<const v4f *>(&im.vf[16 * kt + 4 * kg]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        kf[4 * kt + i] = fk[i];
-                        vf[4 * kt + i] = fv[i];
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    const uint32_t mine = whole ? ~0u : see[u] >> (4 * kg);
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = sc[u][e >> 2][e & 3] * (kf[e] * qf[u]);
+                        const int e = 4 * kt + i;
+                        x[e] = sc[u][kt][i] * (fk[i] * qf[u]);
                         if (SHAPED) x[e] = shape(u, x[e], e);
-                        x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
-                    }
-                    raise_m(u, max8(x));
-                    float w[8], sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        w[e] = __builtin_amdgcn_exp2f(x[e] - m[u]);
-                        sum += w[e];
-                        // a bad value row is NaN, for the rows that see it only
-                        w[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? w[e] * vf[e] : 0.0f;
-                    }
-                    l[u] += sum;
-                    const float big = max8(w);
-                    raise_a(u, big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -16384);  // big < 2^that
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        v2h hi, lo;
-                        split_h(__builtin_ldexpf(w[e], 14 - a[u]), __builtin_ldexpf(w[e + 1], 14 - a[u]), hi, lo);
-                        ph[u][e] = hi[0];
-                        ph[u][e + 1] = hi[1];
-                        pL[u][e] = lo[0];
-                        pL[u][e + 1] = lo[1];
+                        x[e] = mine >> (16 * kt + i) & 1 ? x[e] : -INFINITY;
+                        vf[e] = fv[i];
                     }
                 }
-            }
+                raise_m(u, groups_max(max8(x)));
+                float w[8], sum = 0.0f;
 #pragma unroll
-            for (int d = 0; d < 2 * C; d += 2) {
-                v8h vh[2], vl[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    vh[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + lane * 16);
-                    vl[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + 1024 + lane * 16);
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(x[e] - m[u]);
+                    sum += w[e];
+                    // a bad value row is NaN, for the rows that see it only
+                    w[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? w[e] * vf[e] : 0.0f;
                 }
+                l[u] += sum;
+                const float big = groups_max(max8(w));
+                by[u] = raise_a(u, big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -16384);  // big < 2^that
 #pragma unroll
-                for (int x = 0; x < 3; ++x)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int u = 0; u < QT; ++u)
-                            o[u][d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? vl[y] : vh[y], x == 1 ? pL[u] : ph[u],
-                                                                                 o[u][d + y], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) w[e] = __builtin_ldexpf(w[e], 14 - a[u]);
+                weights(u, w);
             }
         }
-        if (!IMG && more) {
-            rowsin.sizes(s_ke, s_ve);
-            __syncthreads();
-            rowsin.put(&ims[b ^ 1], s_ke, s_ve);
-            __syncthreads();
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+            if (__any(by[u] < 0)) {
+                const float f = __builtin_ldexpf(1.0f, by[u]);
+#pragma unroll
+                for (int d = 0; d < 2 * C; ++d) o[u][d] *= f;
+            }
+#pragma unroll
+        for (int d = 0; d < 2 * C; d += 2) {
+            v8h vh[2], vl[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                vh[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + lane * 16);
+                vl[y] = *reinterpret_cast<const v8h *>(im.v + (d + y) * 2048 + 1024 + lane * 16);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int u = 0; u < QT; ++u)
+                        o[u][d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? vl[y] : vh[y], x == 1 ? pL[u] : ph[u],
+                                                                             o[u][d + y], 0, 0, 0);
         }
     }
 
