@@ -153,20 +153,36 @@ __device__ __forceinline__ uint32_t lanes8_umax(uint32_t v) {
     return max(v, __float_as_uint(xchg<XM8>(__uint_as_float(v))));
 }
 
-// tanh to about 2^-23 of its value: below 1.75 Lambert's continued fraction
-// x/(1 + x²/(3 + x²/(5 + … x²/13))) as a quotient of polynomials (off by 2^-27
-// at 1.75), above it 1 − 2/(e^2x + 1), where the difference no longer cancels
-__device__ __forceinline__ float tanh_f(float x) {
-    const float a = fabsf(x), z = a * a;
-    const bool low = a < 1.75f;
-    const float e = __builtin_amdgcn_exp2f(fminf(a, 20.0f) * (2.0f * kLog2e));
-    const float num = a * fmaf(z, fmaf(z, z + 378.0f, 17325.0f), 135135.0f);
-    const float den = fmaf(z, fmaf(z, fmaf(z, 28.0f, 3150.0f), 62370.0f), 135135.0f);
-    const float d = low ? den : e + 1.0f, n = low ? num : 2.0f;
-    float r = __builtin_amdgcn_rcpf(d);
-    r = fmaf(fmaf(-d, r, 1.0f), r, r);
-    const float t = low ? n * r : fmaf(-n, r, 1.0f);
-    return copysignf(t, x);
+// tanh of N numbers, to 2.5 · 2^-24 of its value; NaN stays NaN.  Up to 0.85, x +
+// x³·P(x²) with a P fitted to (tanh(x)/x − 1)/x² there (least largest error,
+// 2^-27 of tanh); above, 1 − 2/(e^2x + 1), where the difference no longer
+// cancels.  Scores are mostly far below their cap: a wave whose numbers all are
+// takes the polynomial alone, 9 instructions a number instead of 22.
+template <int N>
+__device__ __forceinline__ void tanh_all(float (&x)[N]) {
+    float top = fabsf(x[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+    const bool some_high = __any(top > 0.85f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float z = x[i] * x[i];
+        float q = fmaf(z, 0.00144017930142581463f, -0.00714282691478729248f);
+        q = fmaf(z, q, 0.0211210921406745911f);
+        q = fmaf(z, q, -0.0537964627146720886f);
+        q = fmaf(z, q, 0.133314788341522217f);
+        q = fmaf(z, q, -0.333332657814025879f);
+        const float low = fmaf(x[i] * z, q, x[i]);
+        if (some_high) {
+            const float a = fabsf(x[i]);
+            const float d = __builtin_amdgcn_exp2f((a > 20.0f ? 20.0f : a) * (2.0f * kLog2e)) + 1.0f;
+            float r = __builtin_amdgcn_rcpf(d);
+            r = fmaf(fmaf(-d, r, 1.0f), r, r);
+            x[i] = a > 0.85f ? copysignf(fmaf(-2.0f, r, 1.0f), x[i]) : low;
+        } else {
+            x[i] = low;
+        }
+    }
 }
 
 // x / p.group for x below 2^20 (the quotient is at least 1/2 group away from the next)
@@ -521,7 +537,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
         }
         if (kg == 0) s_row[row - first_row] = sees;  // for this wave alone
     }
-    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
     const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
 
     v4f o[QT][2 * C];
@@ -604,18 +620,28 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
                         sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? kl[kt] : kh[kt], x == 1 ? ql[u][c] : qh[u][c],
                                                                            sc[u][kt], 0, 0, 0);
         }
-        // capped and biased scores, to the base 2, of key k0 + 16(e/4) + 4kg + e%4
-        auto shape = [&](int u, float x, int e) {
-            if (p.cap > 0.0f) x = p.cap * tanh_f(x * inv_cap);
-            if (!p.slopes) return x * kLog2e;
-            const int in = 16 * (e >> 2) + (e & 3);
-            float dist = (float)(row_pos[u] - k0 - 4 * kg) - (float)in;
-            if (TREE) {
-                const int key = k0 + 4 * kg + in;
-                const int at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
-                dist = (float)(int)((uint32_t)row_pos[u] - (uint32_t)at);
+        // capped and biased scores, to the base 2, of keys k0 + 16(e/4) + 4kg + e%4
+        auto shape = [&](int u, float (&x)[8]) {
+            if (p.cap > 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= inv_cap;
+                tanh_all(x);
             }
-            return fmaf(x, kLog2e, -slope[u] * fabsf(dist));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= cap2;
+            if (!p.slopes) return;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int in = 16 * (e >> 2) + (e & 3);
+                float dist = (float)(row_pos[u] - k0 - 4 * kg) - (float)in;
+                if (TREE) {
+                    if (e == 4) __builtin_amdgcn_sched_barrier(0);  // not all eight loads at once: registers
+                    const int key = k0 + 4 * kg + in;
+                    const int at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
+                    dist = (float)(int)((uint32_t)row_pos[u] - (uint32_t)at);
+                }
+                x[e] = fmaf(-slope[u], fabsf(dist), x[e]);
+            }
         };
         v8h ph[QT], pL[QT];
         int by[QT];
@@ -638,7 +664,8 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
                 const float f = kf * qf[u];
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = SHAPED ? shape(u, sc[u][e >> 2][e & 3] * f, e) : sc[u][e >> 2][e & 3];
+                for (int e = 0; e < 8; ++e) x[e] = sc[u][e >> 2][e & 3] * (SHAPED ? f : 1.0f);
+                if (SHAPED) shape(u, x);
                 const float mine = SHAPED ? max8(x) : max8(x) * f;
                 raise_m(u, groups_max(mine));
                 by[u] = raise_a(u, (int)groups_max(ceilf(fmaxf(mine - m[u], -16000.0f)) + (float)ve));
@@ -667,11 +694,12 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
                     for (int i = 0; i < 4; ++i) {
                         const int e = 4 * kt + i;
                         x[e] = sc[u][kt][i] * (fk[i] * qf[u]);
-                        if (SHAPED) x[e] = shape(u, x[e], e);
-                        x[e] = mine >> (16 * kt + i) & 1 ? x[e] : -INFINITY;
                         vf[e] = fv[i];
                     }
                 }
+                if (SHAPED) shape(u, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
                 raise_m(u, groups_max(max8(x)));
                 float w[8], sum = 0.0f;
 #pragma unroll
@@ -867,7 +895,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
         }
     }
     const float scale = SHAPED ? p.scale : p.scale * kLog2e;
-    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
     const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + slot * p.side : nullptr;
 
     v4f o[QT][D][4];  // [..][x][i]: dim 64d + 16·kg + 4i + x
@@ -930,17 +958,23 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
             }
             float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = sc[u][i] * scale;
-                if (SHAPED) {
+            for (int i = 0; i < 4; ++i) x[i] = sc[u][i] * scale;
+            if (SHAPED) {
+                if (p.cap > 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] *= inv_cap;
+                    tanh_all(x);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
                     const int key = k0 + 4 * kg + i;
                     int at = key;
                     if (TREE) at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
-                    if (p.cap > 0.0f) x[i] = p.cap * tanh_f(x[i] * inv_cap);
-                    x[i] = fmaf(x[i], kLog2e, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)at)));
+                    x[i] = fmaf(x[i], cap2, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)at)));
                 }
-                x[i] = see >> i & 1 ? x[i] : -INFINITY;
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = see >> i & 1 ? x[i] : -INFINITY;
             const float top = groups_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
             if (__any(top > m[u])) {
                 const float mn = top > m[u] ? top : m[u];
@@ -1126,7 +1160,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) 
             }
         }
     }
-    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
     const int rows = q.count * p.group;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     float x[C][8];
@@ -1191,16 +1225,24 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) 
             const int local = 16 * t + r16;
             const float qf = s_qf[local], lse = s_lse[local];
             const uint64_t see = s_see[local];
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = sc[i] * (kf[i] * qf);
+            if (SHAPED) {
+                if (p.cap > 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] *= inv_cap;
+                    tanh_all(y);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[i] = fmaf(y[i], cap2, -s_slope[local] * fabsf((float)(int)((uint32_t)s_pos[local] - (uint32_t)kpos[i])));
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float y = sc[i] * (kf[i] * qf);
-                if (SHAPED) {
-                    if (p.cap > 0.0f) y = p.cap * tanh_f(y * inv_cap);
-                    y = fmaf(y, kLog2e, -s_slope[local] * fabsf((float)(int)((uint32_t)s_pos[local] - (uint32_t)kpos[i])));
-                }
                 const int draft = key0 + 16 * wave + 4 * kg + i - q.len;
                 const bool seen = lse != INFINITY && (draft < 0 || (draft < 64 && (see >> draft & 1)));
-                acc[i] += seen ? __builtin_amdgcn_exp2f(fmaf(lse, -kLog2e, y)) : 0.0f;
+                acc[i] += seen ? __builtin_amdgcn_exp2f(fmaf(lse, -kLog2e, y[i])) : 0.0f;
             }
         }
     }

@@ -189,6 +189,31 @@ def test_prompt_masked_values_do_not_leak(ctx, rng, bad, where):
             assert not np.isfinite(out[at - rows0:, :256]).all(1).any()
 
 
+@pytest.mark.parametrize("where", ["q", "k"])
+@pytest.mark.parametrize("n", [1, 45])
+def test_prompt_nan_passes_the_cap(ctx, rng, n, where):
+    """A capped score of NaN is NaN: its row is not finite."""
+    with ref.Hip() as hip:
+        q = rng.standard_normal((n, 256)).astype(F32)
+        k = rng.standard_normal((n + 30, 128)).astype(F32)
+        (q if where == "q" else k)[0, 5] = np.nan
+        a, q, k, v = prompt_case(hip, rng, n, 30, 2, 1, 128, None, cap=9.0, q=q, k=k)
+        ctx.prompt_attention(a)
+        out = hip.down(a.out, (n, 2, 128))
+        assert not np.isfinite(out[:, 0] if where == "k" else out[:1, 0]).all(-1).any()
+
+
+@pytest.mark.parametrize("size", [0.01, 0.5, 4.0, 60.0])
+@pytest.mark.parametrize("n", [1, 70])
+def test_prompt_caps_of_all_sizes(ctx, rng, n, size):
+    """Scores far below their cap, around it and far above it."""
+    with ref.Hip() as hip:
+        q = rng.standard_normal((n, 256)).astype(F32) * F32(size)
+        a, q, k, v = prompt_case(hip, rng, n, 50, 2, 1, 128, None, cap=3.0, q=q)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, None)
+
+
 def test_prompt_rows_that_see_nothing_read_nothing(ctx, rng):
     """A whole prompt of padding: zeros and -inf, whatever the cache holds."""
     with ref.Hip() as hip:
