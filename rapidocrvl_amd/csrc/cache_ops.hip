@@ -224,6 +224,24 @@ int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
     return launch_attn_t<HD, TREE, SHAPED, false>(s, p, sh, work, seqs);
 }
 
+template <int HD, bool SHAPED>
+int launch_weights(hipStream_t s, const CacheAttn &p, int seqs) {
+    const int64_t groups = (int64_t)p.kvh * seqs;
+    auto launch = [&](auto kernel, int keys, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(round_up_div(p.rows, keys), p.kvh, seqs), dim3(threads), 0, s, p);
+    };
+    // A workgroup lays all query rows out by itself and takes about as long for
+    // 32, 64 or 96 keys (512 query rows: 15, 17, 19 us), so one round on 256 CUs
+    // is what counts: 64 tokens of 16 heads over 8,256 rows took 35 us as 516
+    // workgroups of 32 keys, 33 as 258 of 64, 21 as 172 of 96; over 4,064 rows 16, 18, 19.
+    if (p.n * p.group <= kWRows) launch(k_cache_weights<HD, SHAPED, 0>, 64, 256);
+    else if (round_up_div(p.rows, 32) * groups <= 256) launch(k_cache_weights<HD, SHAPED, 1>, 32, 512);
+    else if (round_up_div(p.rows, 64) * groups <= 256) launch(k_cache_weights<HD, SHAPED, 2>, 64, 512);
+    else launch(k_cache_weights<HD, SHAPED, 3>, 96, 512);
+    HIP_TRY(hipGetLastError());
+    return POCR_OK;
+}
+
 template <bool TREE>
 int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, const AttnShape &sh, void *work) {
     const bool shaped = p.cap > 0.0f || p.slopes;
@@ -333,18 +351,10 @@ extern "C" int pocr_cache_weights(pocr_ctx *ctx, const pocr_tree_args *a, void *
     CACHE_OP_ENTER(ctx, stream, op);
     p.weights = a->weights;
     p.take = a->take;
-    const dim3 grid((p.rows + kWKeys - 1) / kWKeys, p.kvh, a->seqs);
     hipStream_t s = (hipStream_t)stream;
     const bool shaped = p.cap > 0.0f || p.slopes;
-    if (a->head_dim == 128) {
-        if (shaped) hipLaunchKernelGGL((k_cache_weights<128, true>), grid, dim3(kAttnThreads), 0, s, p);
-        else hipLaunchKernelGGL((k_cache_weights<128, false>), grid, dim3(kAttnThreads), 0, s, p);
-    } else {
-        if (shaped) hipLaunchKernelGGL((k_cache_weights<64, true>), grid, dim3(kAttnThreads), 0, s, p);
-        else hipLaunchKernelGGL((k_cache_weights<64, false>), grid, dim3(kAttnThreads), 0, s, p);
-    }
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    if (a->head_dim == 128) return shaped ? launch_weights<128, true>(s, p, a->seqs) : launch_weights<128, false>(s, p, a->seqs);
+    return shaped ? launch_weights<64, true>(s, p, a->seqs) : launch_weights<64, false>(s, p, a->seqs);
 }
 
 extern "C" int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *a, void *stream) {

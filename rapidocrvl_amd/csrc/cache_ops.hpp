@@ -1104,35 +1104,123 @@ __global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan p
         p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
 }
 
-// The weights of cache rows.  Workgroup: 64 rows of one sequence and KV head,
-// 16 a wave, their halves in registers throughout; the query rows (token, head)
-// pass through LDS 64 at a time, laid out as the matrix instructions take them.
-// A lane sums its query row of each 16 for four keys; the sum over a key's 16
-// lanes ends the kernel, so the order of every sum is fixed.
-constexpr int kWKeys = 64, kWRows = 64;
-template <int HD, bool SHAPED>
-__global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) {
-    constexpr int C = HD / 32;
-    __shared__ __attribute__((aligned(16))) uint8_t sq[4 * C * 2 * 1024];
-    __shared__ float s_qf[kWRows], s_lse[kWRows], s_slope[kWRows];
-    __shared__ int s_pos[kWRows];
-    __shared__ uint64_t s_see[kWRows];
-    __shared__ uint64_t s_bits[64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
-    const int g = blockIdx.y, s = blockIdx.z, key0 = blockIdx.x * kWKeys;
+// The weights of cache rows.  Workgroup: 64 rows (MANY·32) of one sequence and
+// KV head, their halves in four waves' registers throughout; the query rows
+// (token, head) pass through LDS 64 at a time, laid out as the matrix
+// instructions take them.  A lane sums its query row of each 16 for four keys;
+// the sum over a key's 16 lanes ends the kernel, so the order of every sum is
+// fixed.
+//
+// Up to 64 query rows there is one step, and four waves of 16 keys lay the rows
+// out themselves (16 single tokens of 16 heads over 1,610 rows: 11 us, the keys
+// at 2.4 TB/s).  For more (MANY), four more waves do so in two buffers, two
+// steps ahead of their use; the others hold 16·MANY keys each and take every
+// other 32 query rows.
+constexpr int kWRows = 64;
+template <int HD>
+struct WeightRows {
+    uint8_t q[4 * (HD / 32) * 2 * 1024];  // [16-row tile][32-dim chunk][half] lane l = 16·q + r: row r, dims 32c + 8q .. +7
+    float qf[kWRows], lse[kWRows];        // scale; log2 of the denominator, +inf for rows that do not count
+    float slope[kWRows];
+    int pos[kWRows];
+    uint64_t see[kWRows];
+};
+template <int HD, bool SHAPED, int MANY>
+__global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn p) {
+    constexpr int C = HD / 32, KT = MANY ? MANY : 1, kKeys = MANY ? 32 * MANY : 64;
+    __shared__ __attribute__((aligned(16))) WeightRows<HD> steps[MANY ? 2 : 1];
+    __shared__ float s_sum[kKeys];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
+    const int g = blockIdx.y, s = blockIdx.z, key0 = blockIdx.x * kKeys;
     const SeqRows q = seq_rows(p, s);
-    const int end = q.len + q.count;
+    const int end = q.len + q.count, rows = q.count * p.group;
     if (key0 >= end || q.count == 0) return;
     const uint64_t mine = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
-    if (wave == 0) s_bits[lane] = mine;
     const uint64_t take = p.take ? p.take[s] : ~0ull;
     const int32_t *pos = SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
 
-    v8h kh[C], kl[C];
-    float kf[4];
-    int kpos[4];
-    {
-        const float *src = p.k + s * p.k_ss + min(key0 + 16 * wave + r16, end - 1) * p.k_st + g * HD + 8 * kg;
+    // 16 query rows as a wave loads and lays them out
+    struct Row {
+        float x[C][8], lse;
+        int pos;
+    };
+    auto load = [&](Row &r, int first) {
+        const int row = min(first + r16, rows - 1), tok = by_group(p, row), h = g * p.group + row - tok * p.group;
+        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 8 * kg;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r.x[c][i] = a[i];
+                r.x[c][4 + i] = b[i];
+            }
+        }
+        r.lse = p.lse[((size_t)s * p.n + tok) * p.heads + h];
+        if (SHAPED) r.pos = pos ? pos[q.len + tok] : 0;
+    };
+    auto put = [&](const Row &r, WeightRows<HD> &to, int first, int tile) {
+        const int row = min(first + r16, rows - 1), tok = by_group(p, row), local = 16 * tile + r16;
+        if (first < rows) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) top = umax3(top, abs_bits(r.x[c][i]), abs_bits(r.x[c][i + 1]));
+            const int e = row_exp(groups_umax(top));
+            v8h hi[C], lo[C];
+            split_row<C>(r.x, e, hi, lo);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                *reinterpret_cast<v8h *>(to.q + ((tile * C + c) * 2) * 1024 + lane * 16) = hi[c];
+                *reinterpret_cast<v8h *>(to.q + ((tile * C + c) * 2 + 1) * 1024 + lane * 16) = lo[c];
+            }
+            const uint64_t b = __shfl((unsigned long long)mine, tok);
+            if (kg == 0) {
+                to.qf[local] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
+                to.see[local] = b;
+                if (SHAPED) {
+                    to.slope[local] = p.slopes ? p.slopes[g * p.group + row - tok * p.group] * kLog2e : 0.0f;
+                    to.pos[local] = pos ? r.pos : q.len + __popcll(b) - 1;
+                }
+            }
+        }
+        const bool live = first + r16 < rows && (take >> tok & 1) && r.lse != -INFINITY;
+        if (kg == 0) to.lse[local] = live ? r.lse * kLog2e : INFINITY;
+    };
+    if (MANY && wave >= 4) {
+        const int mine16 = 16 * (wave - 4);
+        Row r[2];
+        load(r[0], mine16);
+        load(r[1], kWRows + mine16);
+        for (int row0 = 0; row0 < rows; row0 += 2 * kWRows) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int at = row0 + b * kWRows;
+                if (at >= rows) break;
+                put(r[b], steps[b], at + mine16, wave - 4);
+                if (at + 2 * kWRows < rows) load(r[b], at + 2 * kWRows + mine16);
+                __syncthreads();  // the step is there, and the one before it done with
+            }
+        }
+        __syncthreads();  // the others' last
+        return;
+    }
+
+    Row own;
+    if (!MANY) load(own, 16 * wave);
+    const int first_key = key0 + 16 * KT * (MANY ? wave & 1 : wave), half = MANY ? wave >> 1 : 0;
+    // a lane writes at most one sum; what it adds to is on its way
+    const int out_key = first_key + (r16 < 4 * KT ? 16 * (r16 >> 2) + 4 * kg + (r16 & 3) : kKeys);
+    float *out = p.weights + ((size_t)s * p.kvh + g) * p.side + out_key;
+    const bool writes = half == 0 && out_key < min(first_key + 16 * KT, end);
+    const float before = writes ? *out : 0.0f;
+    v8h kh[KT][C], kl[KT][C];
+    float kf[KT][4];
+    int kpos[KT][4];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        const float *src = p.k + s * p.k_ss + min(first_key + 16 * kt + r16, end - 1) * p.k_st + g * HD + 8 * kg;
         float x[C][8];
         uint32_t top = 0;
 #pragma unroll
@@ -1146,118 +1234,102 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_cache_weights(CacheAttn p) 
             }
         }
         const int e = row_exp(groups_umax(top));
-        split_row<C>(x, e, kh, kl);
+        split_row<C>(x, e, kh[kt], kl[kt]);
         const float f = pow2(e - kTop);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * wave + 4 * kg + i;
-            kf[i] = __shfl(f, 4 * kg + i);
-            kpos[i] = key;
+            const int key = first_key + 16 * kt + 4 * kg + i;
+            kf[kt][i] = __shfl(f, 4 * kg + i);
+            kpos[kt][i] = key;
             if (SHAPED) {
                 const int depth = __popcll(__shfl((unsigned long long)mine, min(max(key - q.len, 0), 63))) - 1;
-                if (pos) kpos[i] = pos[min(key, end - 1)];
-                else if (key >= q.len) kpos[i] = q.len + depth;
+                if (pos) kpos[kt][i] = pos[min(key, end - 1)];
+                else if (key >= q.len) kpos[kt][i] = q.len + depth;
             }
         }
     }
     const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
-    const int rows = q.count * p.group;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    float x[C][8];
-    auto load = [&](int row) {
-        const int tok = min(row, rows - 1) / p.group, h = g * p.group + min(row, rows - 1) % p.group;
-        const float *src = p.q + s * p.q_ss + tok * p.q_st + h * HD + 8 * kg;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[c][i] = a[i];
-                x[c][4 + i] = b[i];
-            }
-        }
-    };
-    load(16 * wave + r16);
+    const bool drafts = key0 + kKeys > q.len;  // some key is a drafted token's
+    float acc[KT][4] = {};
     for (int row0 = 0; row0 < rows; row0 += kWRows) {
+        if (!MANY) put(own, steps[0], 16 * wave, wave);
         __syncthreads();
-        {
-            uint32_t top = 0;
+        const WeightRows<HD> &in = steps[MANY ? row0 / kWRows & 1 : 0];
+        for (int pair = half; row0 + 32 * pair < rows && pair < 2; pair += MANY ? 2 : 1) {
+            v4f sc[2][KT];
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) top = umax3(top, abs_bits(x[c][i]), abs_bits(x[c][i + 1]));
-            const int e = row_exp(groups_umax(top));
-            v8h hi[C], lo[C];
-            split_row<C>(x, e, hi, lo);
+                for (int kt = 0; kt < KT; ++kt) sc[t][kt] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                *reinterpret_cast<v8h *>(sq + ((wave * C + c) * 2) * 1024 + lane * 16) = hi[c];
-                *reinterpret_cast<v8h *>(sq + ((wave * C + c) * 2 + 1) * 1024 + lane * 16) = lo[c];
+                v8h qh[2], ql[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    qh[t] = *reinterpret_cast<const v8h *>(in.q + (((2 * pair + t) * C + c) * 2) * 1024 + lane * 16);
+                    ql[t] = *reinterpret_cast<const v8h *>(in.q + (((2 * pair + t) * C + c) * 2 + 1) * 1024 + lane * 16);
+                }
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+                            sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x == 0 ? kl[kt][c] : kh[kt][c], x == 1 ? ql[t] : qh[t],
+                                                                               sc[t][kt], 0, 0, 0);
             }
-            const int local = 16 * wave + r16, row = row0 + local;
-            if (kg == 0) {
-                const int tok = min(row, rows - 1) / p.group, h = g * p.group + min(row, rows - 1) % p.group;
-                const float lse = p.lse[((size_t)s * p.n + tok) * p.heads + h];
-                const bool live = row < rows && (take >> tok & 1) && lse != -INFINITY;
-                s_qf[local] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
-                s_lse[local] = live ? lse : INFINITY;
-                const uint64_t b = s_bits[tok];
-                s_see[local] = b;
-                if (SHAPED) {
-                    s_slope[local] = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-                    s_pos[local] = pos ? pos[q.len + tok] : q.len + __popcll(b) - 1;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int local = 32 * pair + 16 * t + r16;
+                const float qf = in.qf[local], lse = in.lse[local];
+                const uint64_t see = drafts ? in.see[local] : 0;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    float y[4];
+                    if (SHAPED) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = sc[t][kt][i] * (kf[kt][i] * qf);
+                        if (p.cap > 0.0f) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] *= inv_cap;
+                            tanh_all(y);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            y[i] = fmaf(y[i], cap2, -in.slope[local] * fabsf((float)(int)((uint32_t)in.pos[local] - (uint32_t)kpos[kt][i]))) - lse;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = fmaf(sc[t][kt][i], kf[kt][i] * qf, -lse);
+                    }
+                    uint32_t take4 = lse != INFINITY ? 0xf : 0;  // which of the lane's keys the row sees
+                    if (drafts) {
+                        const int off = first_key + 16 * kt + 4 * kg - q.len, up = min(max(off, 0), 63), down = min(max(-off, 0), 4);
+                        take4 &= (off < 64 ? (uint32_t)(see >> up) << down : 0u) | ((1u << down) - 1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[kt][i] += __builtin_amdgcn_exp2f(take4 >> i & 1 ? y[i] : -INFINITY);
                 }
             }
         }
-        __syncthreads();
-        if (row0 + kWRows < rows) load(row0 + kWRows + 16 * wave + r16);
-        const int tiles = min(4, (rows - row0 + 15) / 16);
-        for (int t = 0; t < tiles; ++t) {
-            v4f sc = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float sum = 0.0f;
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const v8h qh = *reinterpret_cast<const v8h *>(sq + ((t * C + c) * 2) * 1024 + lane * 16);
-                const v8h ql = *reinterpret_cast<const v8h *>(sq + ((t * C + c) * 2 + 1) * 1024 + lane * 16);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[c], qh, sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c], ql, sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c], qh, sc, 0, 0, 0);
-            }
-            const int local = 16 * t + r16;
-            const float qf = s_qf[local], lse = s_lse[local];
-            const uint64_t see = s_see[local];
-            float y[4];
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = sc[i] * (kf[i] * qf);
-            if (SHAPED) {
-                if (p.cap > 0.0f) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] *= inv_cap;
-                    tanh_all(y);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[i] = fmaf(y[i], cap2, -s_slope[local] * fabsf((float)(int)((uint32_t)s_pos[local] - (uint32_t)kpos[i])));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int draft = key0 + 16 * wave + 4 * kg + i - q.len;
-                const bool seen = lse != INFINITY && (draft < 0 || (draft < 64 && (see >> draft & 1)));
-                acc[i] += seen ? __builtin_amdgcn_exp2f(fmaf(lse, -kLog2e, y[i])) : 0.0f;
-            }
+        for (int i = 0; i < 4; ++i) {
+            float a = acc[kt][i];
+            a += xchg<XQ1>(a);
+            a += xchg<XQ2>(a);
+            a += xchg<XM8>(a);
+            a += xchg<XM16>(a);
+            sum = r16 == 4 * kt + i ? a : sum;
         }
+    if (MANY) {
+        if (half && r16 < 4 * KT) s_sum[out_key - key0] = sum;
+        __syncthreads();
+        if (writes) sum += s_sum[out_key - key0];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        acc[i] += xchg<XQ1>(acc[i]);
-        acc[i] += xchg<XQ2>(acc[i]);
-        acc[i] += xchg<XM8>(acc[i]);
-        acc[i] += xchg<XM16>(acc[i]);
-    }
-    const int key = key0 + 16 * wave + 4 * kg + r16;
-    if (r16 < 4 && key < end) {
-        const float w = r16 == 0 ? acc[0] : (r16 == 1 ? acc[1] : (r16 == 2 ? acc[2] : acc[3]));
-        p.weights[((size_t)s * p.kvh + g) * p.side + key] += w;
-    }
+    if (writes) *out = before + sum;
 }
 
 // ---------------------------------------------------------------------------
