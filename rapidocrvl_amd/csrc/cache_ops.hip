@@ -157,7 +157,9 @@ struct AttnShape {
     bool few;                       // k_cache_attn_few
     int wg_rows, tiles, splits, least;
     int steps;                      // images of a prompt's rows, or 0
-    int64_t part_bytes, bytes;      // of the workspace
+    int jobs;                       // with images: workgroups per KV head
+    int64_t slots;                  // shares with partial sums, or 0
+    int64_t part_bytes, cut_bytes, bytes;  // of the workspace: partial sums and their counts or jobs, images
 };
 template <int HD>
 constexpr int64_t image_bytes = StepImage<HD>::kBytes;
@@ -170,48 +172,70 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
     // two workgroups a CU; prompts of many short rows (documents) leave most
     // CUs idle behind their longest tile unless that is cut too
     a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
-    const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : (a.few || a.steps ? 512 : 256)) / work);
     const int step = a.few ? kFewKeys * kFewWaves : kBlock;
-    a.least = a.few ? 1 : (work < 128 ? 2 : 6);
-    a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
-    a.part_bytes = a.splits == 1 ? 0 : work * a.splits * a.wg_rows * (head_dim + 2) * 4 + (work * 4 + 15) / 16 * 16;
-    a.bytes = a.part_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
+    if (a.steps) {
+        a.least = 2;
+        a.splits = 1;
+        a.jobs = work <= 512 ? (int)(512 / groups) : a.tiles;
+        a.slots = a.jobs > a.tiles ? a.jobs * groups : 0;
+        a.cut_bytes = (a.tiles * (int64_t)sizeof(TileCut) + a.jobs * 4 + 15) / 16 * 16;
+    } else {
+        const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : (a.few ? 512 : 256)) / work);
+        a.least = a.few ? 1 : (work < 128 ? 2 : 6);
+        a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
+        a.jobs = 0;
+        a.slots = a.splits > 1 ? work * a.splits : 0;
+        a.cut_bytes = a.slots ? (work * 4 + 15) / 16 * 16 : 0;
+    }
+    a.part_bytes = a.slots * a.wg_rows * (head_dim + 2) * 4;
+    a.bytes = a.part_bytes + a.cut_bytes + a.steps * groups * (head_dim == 128 ? image_bytes<128> : image_bytes<64>);
     return a;
 }
 
-AttnPlan attn_plan(const AttnShape &sh, void *work, int64_t groups, int head_dim) {
-    AttnPlan pl{sh.tiles, sh.splits, sh.least, nullptr, nullptr, nullptr, sh.steps};
-    if (sh.splits > 1) {
+AttnPlan attn_plan(const AttnShape &sh, void *work, int head_dim) {
+    AttnPlan pl{};
+    pl.tiles = sh.tiles;
+    pl.splits = sh.splits;
+    pl.least = sh.least;
+    pl.steps = sh.steps;
+    pl.max_jobs = sh.jobs;
+    if (sh.slots) {
         pl.part = static_cast<float *>(work);
-        pl.parts = reinterpret_cast<int32_t *>(pl.part + groups * sh.tiles * sh.splits * sh.wg_rows * (head_dim + 2));
+        pl.stat = reinterpret_cast<float2 *>(pl.part + sh.slots * sh.wg_rows * head_dim);
+    }
+    char *at = static_cast<char *>(work) + sh.part_bytes;
+    if (sh.steps) {
+        pl.cuts = reinterpret_cast<TileCut *>(at);
+        pl.jobs = reinterpret_cast<int32_t *>(pl.cuts + sh.tiles);
+        pl.img = reinterpret_cast<uint8_t *>(at + sh.cut_bytes);
+    } else if (sh.slots) {
+        pl.parts = reinterpret_cast<int32_t *>(at);
     }
     return pl;
 }
 
 template <int HD, int kRows>
 int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs) {
-    if (pl.splits > 1)
-        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows>), dim3(pl.tiles * (kRows / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl, seqs);
+    if (pl.part)
+        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows>), dim3(pl.tiles * (kRows / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl);
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }
 
 template <int HD, bool TREE, bool SHAPED, int QT>
 int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
-    const AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
+    const AttnPlan pl = attn_plan(sh, work, HD);
     hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
     return launch_join<HD, 16 * QT>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED, bool IMG>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
-    AttnPlan pl = attn_plan(sh, work, (int64_t)p.kvh * seqs, HD);
-    if (IMG) {
-        uint8_t *img = static_cast<uint8_t *>(work) + sh.part_bytes;
-        pl.img = img;
-        hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps, p.kvh), dim3(kAttnThreads), 0, s, p, img);
-    }
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(sh.tiles * sh.splits, p.kvh, seqs), dim3(IMG ? 256 : 512), 0, s, p, pl);
+    const AttnPlan pl = attn_plan(sh, work, HD);
+    if (IMG)
+        hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps + 1, p.kvh), dim3(kAttnThreads), 0, s, p, pl, const_cast<uint8_t *>(pl.img));
+    const int x = IMG ? sh.jobs : sh.tiles * sh.splits;
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(x, p.kvh, seqs), dim3(IMG ? 256 : 512), 0, s, p, pl);
     return launch_join<HD, 128>(s, p, pl, seqs);
 }
 

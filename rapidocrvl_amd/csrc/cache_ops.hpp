@@ -197,23 +197,36 @@ struct AttnTile {
 
 // a tile's steps of `keys` keys cut into at most `splits` shares of at least `least` steps
 constexpr int kMaxShares = 64;
+__device__ __forceinline__ void share_tile(AttnTile &t, int keys, int parts, int part) {
+    const int steps = max(0, (t.hi - t.lo + keys - 1) / keys);
+    t.parts = parts;
+    t.from = (int)((uint32_t)steps * (uint32_t)part / (uint32_t)parts);  // at most 2^25 steps, 64 shares
+    t.to = (int)((uint32_t)steps * (uint32_t)(part + 1) / (uint32_t)parts);
+}
 __device__ __forceinline__ void cut_tile(AttnTile &t, int keys, int splits, int least, int part) {
     t.lo &= ~(kBlock - 1);
     const int steps = max(0, (t.hi - t.lo + keys - 1) / keys);
-    t.parts = min(splits, max(1, steps / least));
-    t.from = (int)((uint32_t)steps * (uint32_t)part / (uint32_t)t.parts);  // at most 2^25 steps, 64 shares
-    t.to = (int)((uint32_t)steps * (uint32_t)(part + 1) / (uint32_t)t.parts);
+    share_tile(t, keys, min(splits, max(1, steps / least)), part);
 }
 
 // what the launch adds to a call's arguments
+struct TileCut {
+    int lo, hi, all_lo, all_hi;  // keys some row of the tile sees, and all its rows see
+    int first, parts;            // its jobs
+};
 struct AttnPlan {
     int tiles;        // row tiles per (sequence, KV head)
     int splits;       // shares a tile's keys may be cut into; 1: no partial sums
     int least;        // steps of a share
-    float *part;      // [tile][split][64·QT rows][HD] sums, then [rows][2] maximum and denominator
+    float *part;      // sums of a share [128 or 16·QT rows][HD]: [tile][split], with images [KV head][job]
+    float2 *stat;     // their rows' maxima and denominators
     int32_t *parts;   // [tile] shares in use
-    const uint8_t *img;  // [kv head][step] images of all rows, or null: the rows are laid out here
+    // with images
+    const uint8_t *img;  // [kv head][step] images of all rows
     int steps;        // images per KV head
+    TileCut *cuts;    // [tile]
+    int32_t *jobs;    // [max_jobs] a job's tile, long rows first, or -1
+    int max_jobs;     // workgroups per KV head; tiles: their keys are not cut
 };
 
 // A step's 32 key and value rows as the matrix instructions take them, in LDS
@@ -361,19 +374,110 @@ struct StepLayer {
     }
 };
 
+// The jobs of a prompt's tiles: the spans of each, and shares as even as
+// max_jobs workgroups allow, by bisecting the length of a share.  One workgroup.
+constexpr int kCutTiles = 512;  // tiles that may be cut
+constexpr int kTileRows = 128;
+__device__ __forceinline__ void cut_prompt(const CacheAttn &p, const AttnPlan &pl) {
+    __shared__ int s_steps[kCutTiles], s_wave[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = p.n * p.group;
+    const bool cut = pl.max_jobs > pl.tiles;
+    int most = 1;
+    for (int tile = tid; tile < pl.tiles; tile += kAttnThreads) {
+        const int tok0 = tile * kTileRows / p.group, tok1 = (min((tile + 1) * kTileRows, rows) - 1) / p.group;
+        TileCut c{0, p.rows0 + tok1 + 1, 0, p.rows0 + tok0 + 1, pl.tiles - 1 - tile, 1};
+        if (p.begin) {
+            c.lo = c.all_hi = p.rows;
+            c.hi = c.all_lo = 0;
+#pragma unroll 8
+            for (int tok = tok0; tok <= tok1; ++tok) {
+                const int b = min(max(p.begin[tok], 0), p.rows), e = min(max(p.end[tok], 0), p.rows);
+                c.lo = b < e ? min(c.lo, b) : c.lo;
+                c.hi = b < e ? max(c.hi, e) : c.hi;
+                c.all_lo = max(c.all_lo, b);
+                c.all_hi = min(c.all_hi, e);
+            }
+            c.lo = c.lo < c.hi ? c.lo & ~(kBlock - 1) : c.hi;
+        }
+        pl.cuts[tile] = c;
+        if (!cut) pl.jobs[c.first] = tile;
+        const int steps = (c.hi - c.lo + kBlock - 1) / kBlock;
+        if (cut) s_steps[tile] = steps;
+        most = max(most, steps);
+    }
+    if (!cut) return;
+    __syncthreads();
+    auto parts_of = [&](int steps, int length) {  // steps / length rounded up, 1 to kMaxShares; both at most 2^25
+        const uint32_t n = steps + length - 1;
+        if (n >= (uint32_t)kMaxShares * length) return kMaxShares;
+        int parts = (int)((float)n * __builtin_amdgcn_rcpf((float)length));
+        parts -= parts * length > (int)n;
+        parts += (parts + 1) * length <= (int)n;
+        return max(parts, 1);
+    };
+    // every wave by itself, eight tiles a lane
+    int own[kCutTiles / 64];
+#pragma unroll
+    for (int i = 0; i < kCutTiles / 64; ++i) {
+        const int tile = 64 * i + lane;
+        own[i] = tile < pl.tiles ? s_steps[tile] : -1;
+        most = max(most, own[i]);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+    int lo = pl.least, hi = max(lo, most);
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        float jobs = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kCutTiles / 64; ++i) jobs += own[i] < 0 ? 0.0f : (float)parts_of(own[i], mid);
+        if (wave_sum(jobs) <= (float)pl.max_jobs) hi = mid;
+        else lo = mid + 1;
+    }
+    // jobs in order, the last tile's first: two tiles a thread
+    const int at = pl.tiles - 1 - 2 * tid;
+    const int n0 = at >= 0 ? parts_of(s_steps[at], lo) : 0, n1 = at >= 1 ? parts_of(s_steps[at - 1], lo) : 0;
+    int before = n0 + n1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(before, o);
+        if (lane >= o) before += y;
+    }
+    if (lane == 63) s_wave[wave] = before;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) before += s_wave[w];
+    before -= n0 + n1;
+    for (int i = 0; i < n0 + n1; ++i) pl.jobs[before + i] = i < n0 ? at : at - 1;
+    if (at >= 0) {
+        pl.cuts[at].first = before;
+        pl.cuts[at].parts = n0;
+    }
+    if (at >= 1) {
+        pl.cuts[at - 1].first = before + n0;
+        pl.cuts[at - 1].parts = n1;
+    }
+    const int jobs = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    for (int i = jobs + tid; i < pl.max_jobs; i += kAttnThreads) pl.jobs[i] = -1;
+}
+
 // Images of all of a prompt's rows, for prompts of so many tiles that laying
-// every step out in each of them would cost more.  Workgroup: one step of one KV head.
+// every step out in each of them would cost more, and the tiles' jobs.
+// Workgroup: the jobs, or one step of one KV head.
 template <int HD>
-__global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, uint8_t *img) {
+__global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, AttnPlan pl, uint8_t *img) {
     using Im = StepImage<HD>;
     __shared__ __attribute__((aligned(16))) Im im;
-    const int tid = threadIdx.x, g = blockIdx.y;
+    const int tid = threadIdx.x, g = blockIdx.y, step = (int)blockIdx.x - 1;
+    if (step < 0) {
+        if (g == 0) cut_prompt(p, pl);
+        return;
+    }
     StepLayer<HD> st;
-    st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, blockIdx.x * kBlock, p.rows - 1, tid >> 6, tid & 63);
+    st.load(p.k + g * HD, p.k_st, p.v + g * HD, p.v_st, step * kBlock, p.rows - 1, tid >> 6, tid & 63);
     st.put(&im, tid >> 6, tid & 63);
     __syncthreads();
     const uint4 *src = reinterpret_cast<const uint4 *>(&im);
-    uint4 *dst = reinterpret_cast<uint4 *>(img + ((size_t)g * gridDim.x + blockIdx.x) * Im::kBytes);
+    uint4 *dst = reinterpret_cast<uint4 *>(img + ((size_t)g * pl.steps + step) * Im::kBytes);
     for (int i = tid; i < Im::kBytes / 16; i += kAttnThreads) dst[i] = src[i];
 }
 
@@ -405,7 +509,14 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
-    const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
+    int tile, part;
+    if (IMG) {
+        tile = pl.jobs[blockIdx.x];
+        if (tile < 0) return;
+        part = (int)blockIdx.x - pl.cuts[tile].first;
+    } else {
+        tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
+    }
     const int first_row = tile * kRows;
     int len = 0, count = p.n;
     if (TREE) {
@@ -423,43 +534,53 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
     AttnTile t{0, 0, 1, 0, 0};
     int all_lo = 0, all_hi;
     const int tok0 = first_row / p.group, tok1 = (min(first_row + kRows, rows) - 1) / p.group;
-    if (TREE) {
-        t.hi = len + count;
-        all_hi = len;
-        if (wave == 0) {
-            const uint64_t b = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
-            s_bits[lane] = b;
-            s_depth[lane] = __popcll(b) - 1;
-        }
-        __syncthreads();
-    } else if (p.begin) {
-        if (tid == 0) {
-            s_lo = s_hi_min = p.rows;
-            s_hi = s_lo_max = 0;
-        }
-        __syncthreads();
-        const int tok = tok0 + tid;
-        if (tok <= tok1) {  // at most kRows tokens
-            const int b = min(max(p.begin[tok], 0), p.rows), e = min(max(p.end[tok], 0), p.rows);
-            if (b < e) {
-                atomicMin(&s_lo, b);
-                atomicMax(&s_hi, e);
-            }
-            atomicMax(&s_lo_max, b);
-            atomicMin(&s_hi_min, e);
-        }
-        __syncthreads();
-        t.lo = s_lo;
-        t.hi = s_hi;
-        all_lo = s_lo_max;
-        all_hi = s_hi_min;
+    if (IMG) {
+        const TileCut c = pl.cuts[tile];
+        t.lo = c.lo;
+        t.hi = c.hi;
+        all_lo = c.all_lo;
+        all_hi = c.all_hi;
+        share_tile(t, kBlock, c.parts, part);
     } else {
-        t.hi = p.rows0 + tok1 + 1;
-        all_hi = p.rows0 + tok0 + 1;
+        if (TREE) {
+            t.hi = len + count;
+            all_hi = len;
+            if (wave == 0) {
+                const uint64_t b = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
+                s_bits[lane] = b;
+                s_depth[lane] = __popcll(b) - 1;
+            }
+            __syncthreads();
+        } else if (p.begin) {
+            if (tid == 0) {
+                s_lo = s_hi_min = p.rows;
+                s_hi = s_lo_max = 0;
+            }
+            __syncthreads();
+            const int tok = tok0 + tid;
+            if (tok <= tok1) {  // at most kRows tokens
+                const int b = min(max(p.begin[tok], 0), p.rows), e = min(max(p.end[tok], 0), p.rows);
+                if (b < e) {
+                    atomicMin(&s_lo, b);
+                    atomicMax(&s_hi, e);
+                }
+                atomicMax(&s_lo_max, b);
+                atomicMin(&s_hi_min, e);
+            }
+            __syncthreads();
+            t.lo = s_lo & ~(kBlock - 1);
+            t.hi = s_hi;
+            all_lo = s_lo_max;
+            all_hi = s_hi_min;
+        } else {
+            t.hi = p.rows0 + tok1 + 1;
+            all_hi = p.rows0 + tok0 + 1;
+        }
+        cut_tile(t, kBlock, pl.splits, pl.least, part);
+        if (part >= t.parts) return;
+        if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
     }
-    cut_tile(t, kBlock, pl.splits, pl.least, part);
-    if (part >= t.parts) return;
-    if (pl.parts && part == 0 && tid == 0) pl.parts[slot] = t.parts;
+    const size_t share = IMG ? (size_t)g * pl.max_jobs + blockIdx.x : slot * pl.splits + part;
 
     // the first step's rows are on their way before the query rows
     const uint8_t *images = IMG ? pl.img + ((size_t)g * pl.steps + t.lo / kBlock) * Im::kBytes : nullptr;
@@ -752,7 +873,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
         const int tok = tok0 + by_group(p, row - tok0 * p.group), h = g * p.group + row - tok * p.group;
         const float f = whole_row ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
         float *dst = whole_row ? p.out + s * p.o_ss + tok * p.o_st + h * HD + 8 * kg
-                               : pl.part + ((slot * pl.splits + part) * kRows + local) * HD + 8 * kg;
+                               : pl.part + (share * kRows + local) * HD + 8 * kg;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -764,10 +885,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, 
             }
         if (kg != 0) continue;
         if (!whole_row) {
-            float *st = pl.part + (size_t)p.kvh * gridDim.z * pl.tiles * pl.splits * kRows * HD +
-                        ((slot * pl.splits + part) * kRows + local) * 2;
-            st[0] = m[u];
-            st[1] = total;
+            pl.stat[share * kRows + local] = make_float2(m[u], total);
         } else if (p.lse) {
             p.lse[((size_t)s * p.n + tok) * p.heads + h] = (m[u] + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
         }
@@ -1033,7 +1151,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
         if (t.parts > 1) {
             *reinterpret_cast<v4f *>(pl.part + ((slot * pl.splits + part) * kRows + row) * HD + at) = x;
             if (at == 0)
-                reinterpret_cast<float2 *>(pl.part + (size_t)p.kvh * gridDim.z * pl.splits * kRows * HD)[(slot * pl.splits + part) * kRows + row] =
+                pl.stat[(slot * pl.splits + part) * kRows + row] =
                     make_float2(mm, total);
             continue;
         }
@@ -1050,18 +1168,18 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
 // the factors that those give, kJoin loads in flight.
 constexpr int kJoin = 8;
 template <int HD, int kRows>
-__global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan pl, int seqs) {
+__global__ void __launch_bounds__(256) k_cache_attn_join(CacheAttn p, AttnPlan pl) {
     constexpr int kLanes = HD / 4, kPer = 256 / kLanes, kOwn = kMaxShares / kLanes;
     const int per_tile = kRows / kPer;
     const int tile = blockIdx.x / per_tile, local = blockIdx.x % per_tile * kPer + threadIdx.x / kLanes;
     const int g = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes;
     const size_t slot = ((size_t)s * p.kvh + g) * pl.tiles + tile;
-    const int parts = pl.parts[slot];
+    const int parts = pl.cuts ? pl.cuts[tile].parts : pl.parts[slot];
+    const size_t first = pl.cuts ? (size_t)g * pl.max_jobs + pl.cuts[tile].first : slot * pl.splits;
     const int rows = (p.lens ? seq_rows(p, s).count : p.n) * p.group, row = tile * kRows + local;
     if (parts < 2 || row >= rows) return;  // the same for a row's lanes
-    const float2 *st = reinterpret_cast<const float2 *>(pl.part + (size_t)p.kvh * seqs * pl.tiles * pl.splits * kRows * HD) +
-                       slot * pl.splits * kRows + local;
-    const float *src = pl.part + (slot * pl.splits * kRows + local) * HD + 4 * lane;
+    const float2 *st = pl.stat + first * kRows + local;
+    const float *src = pl.part + (first * kRows + local) * HD + 4 * lane;
     float2 mine[kOwn];
     float m = kLowest;
 #pragma unroll
