@@ -1253,9 +1253,9 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
     const SeqRows q = seq_rows(p, s);
     const int end = q.len + q.count, rows = q.count * p.group;
     if (key0 >= end || q.count == 0) return;
-    const uint64_t mine = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
     const uint64_t take = p.take ? p.take[s] : ~0ull;
     const int32_t *pos = SHAPED && p.pos ? p.pos + ((size_t)s * p.kvh + g) * p.side : nullptr;
+    uint64_t mine = 0;
 
     // 16 query rows as a wave loads and lays them out
     struct Row {
@@ -1311,6 +1311,7 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
         Row r[2];
         load(r[0], mine16);
         load(r[1], kWRows + mine16);
+        mine = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
         for (int row0 = 0; row0 < rows; row0 += 2 * kWRows) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -1334,25 +1335,31 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
     const bool writes = half == 0 && out_key < min(first_key + 16 * KT, end);
     const float before = writes ? *out : 0.0f;
     v8h kh[KT][C], kl[KT][C];
-    float kf[KT][4];
+    float kf[KT][4], x[KT][C][8];
     int kpos[KT][4];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
         const float *src = p.k + s * p.k_ss + min(first_key + 16 * kt + r16, end - 1) * p.k_st + g * HD + 8 * kg;
-        float x[C][8];
-        uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const v4f a = *reinterpret_cast<const v4f *>(src + 32 * c), b = *reinterpret_cast<const v4f *>(src + 32 * c + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[c][i] = a[i];
-                x[c][4 + i] = b[i];
-                top = umax3(top, abs_bits(a[i]), abs_bits(b[i]));
+                x[kt][c][i] = a[i];
+                x[kt][c][4 + i] = b[i];
             }
         }
+    }
+    mine = tree_bits(p.parents ? p.parents + (size_t)s * p.n : nullptr, p.n, lane);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) top = umax3(top, abs_bits(x[kt][c][i]), abs_bits(x[kt][c][i + 1]));
         const int e = row_exp(groups_umax(top));
-        split_row<C>(x, e, kh[kt], kl[kt]);
+        split_row<C>(x[kt], e, kh[kt], kl[kt]);
         const float f = pow2(e - kTop);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1475,7 +1482,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // between sinks and recent by three histogram passes over 11, 11 and 10 of its
 // bits (integer counts: the order of the atomics does not matter; eleven bits
 // hold two of the mantissa, which spreads weights of few exponents over the
-// bins), then one pass that writes the kept rows in order: a wave owns 64·KPT
+// bins; a pass whose bin is taken whole is the last, as the second mostly is
+// among weights that differ), then one pass that writes the kept rows in order: a wave owns 64·KPT
 // consecutive rows of a tile, so a row's place is a count of ballots.  KPT rows
 // per thread and tile; where one tile holds the cache its keys are read once
 // and stay in registers.
@@ -1483,7 +1491,7 @@ template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     constexpr int kTile = kSelThreads * KPT, kBins = 2048;
     __shared__ int hist[kBins];
-    __shared__ int s_bin, s_need;
+    __shared__ int s_bin, s_need, s_all;
     __shared__ int s_eq[kSelWaves], s_gt[kSelWaves];
     const int g = blockIdx.x, c = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = min(max(p.lens[c], 0), p.max_rows);
@@ -1538,11 +1546,17 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
                 const bool lower = above + n0 < need;
                 s_bin = kBins - 1 - 2 * tid - (lower ? 1 : 0);
                 s_need = need - above - (lower ? n0 : 0);
+                s_all = s_need == (lower ? n1 : n0);
             }
             __syncthreads();
             prefix |= (uint32_t)s_bin << shift;
             mask |= (uint32_t)(bins - 1) << shift;
             need = s_need;  // how many keys equal to prefix are taken, after the last pass
+            if (s_all && prefix) {  // the whole bin is taken: every key above the one below it
+                prefix -= 1;
+                need = 0;
+                break;
+            }
         }
     const bool none = p.budget == p.sinks + p.recent;
     int done = 0, eq_done = 0;  // rows written, equal keys met
