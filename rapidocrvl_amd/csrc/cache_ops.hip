@@ -235,7 +235,7 @@ int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
     if (IMG)
         hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps + 1, p.kvh), dim3(kAttnThreads), 0, s, p, pl, const_cast<uint8_t *>(pl.img));
     const int x = IMG ? sh.jobs : sh.tiles * sh.splits;
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(x, p.kvh, seqs), dim3(IMG ? 256 : 512), 0, s, p, pl);
+    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(x, p.kvh, seqs), dim3(IMG ? 256 : 768), 0, s, p, pl);
     return launch_join<HD, 128>(s, p, pl, seqs);
 }
 

@@ -482,15 +482,22 @@ __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, Attn
 }
 
 // Workgroup: 128 rows (token, head of the KV head's group) of one sequence and
-// KV head, four waves of 32 rows; one share of the keys, 32 a step.  Scores come
-// out transposed (lane l: query row l%16, keys 4·(l/16) + i of each 16), so a
-// row's maximum, denominator and weights stay with its four lanes and the
-// weights are the second product's operand as they are; the sums come out
-// transposed too (lane: the same query row, 8 consecutive dims of each 32).
-// Two LDS buffers: a step's products run on one while the next step's image
-// arrives in the other, by direct loads (IMG) or from four more waves that do
-// nothing but lay rows out: what these spend on vector instructions then runs
-// beside the others' matrix instructions.
+// KV head; one share of the keys, 32 a step.  Scores come out transposed (lane
+// l: query row l%16, keys 4·(l/16) + i of each 16), so a row's maximum,
+// denominator and weights stay with its four lanes and the weights are the
+// second product's operand as they are; the sums come out transposed too (lane:
+// the same query row, 8 consecutive dims of each 32).  Two LDS buffers: a step's
+// products run on one while the next step's image arrives in the other.
+//
+// IMG: images come ready from memory by direct loads; four waves of 32 rows (a
+// value read from LDS serves two products), two workgroups a CU, so one's
+// softmax runs beside the other's products.  8,192 causal rows of 16 heads:
+// 825 GFLOP of fp16 products in 0.78 ms, 1,058 TFLOP/s where a large matrix
+// product of the library reaches 1,159.
+// Otherwise one workgroup a CU: four waves do nothing but lay rows out, eight of
+// 16 rows multiply.  What the ones spend on vector instructions runs beside the
+// others' matrix instructions; eight waves that did both in turn took 65 us for
+// one tree of 64 over 8,192 rows, four of each 38, four and eight 33.
 //
 // A row's weights are e = 2^(x - m), m an integer above its maximum so far; the
 // products take e·vf·2^(14-a) with 2^a above the row's largest e·vf so far, so
@@ -498,10 +505,10 @@ __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, Attn
 // rescales are by powers of two.  Steps that every row of the tile sees, with
 // even factors, need neither masks nor factors per key.
 template <int HD, bool TREE, bool SHAPED, bool IMG>
-__global__ void __launch_bounds__(IMG ? 256 : 512, 2) k_cache_attn(CacheAttn p, AttnPlan pl) {
+__global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(CacheAttn p, AttnPlan pl) {
     using Im = StepImage<HD>;
     constexpr int C = HD / 32;              // 32-dim chunks
-    constexpr int QT = 2, W = 4, kRows = 16 * W * QT;
+    constexpr int QT = IMG ? 2 : 1, W = IMG ? 4 : 8, kRows = 16 * W * QT;
     __shared__ __attribute__((aligned(16))) Im ims[2];
     __shared__ uint64_t s_bits[64];
     __shared__ int s_depth[64], s_lo, s_hi, s_lo_max, s_hi_min;
