@@ -214,10 +214,10 @@ AttnPlan attn_plan(const AttnShape &sh, void *work, int head_dim) {
     return pl;
 }
 
-template <int HD, int kRows>
+template <int HD, int kRows, int kSub>
 int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs) {
     if (pl.part)
-        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows>), dim3(pl.tiles * (kRows / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl);
+        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows, kSub>), dim3(pl.tiles * (kRows * kSub / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl);
     HIP_TRY(hipGetLastError());
     return POCR_OK;
 }
@@ -226,7 +226,7 @@ template <int HD, bool TREE, bool SHAPED, int QT>
 int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     const AttnPlan pl = attn_plan(sh, work, HD);
     hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
-    return launch_join<HD, 16 * QT>(s, p, pl, seqs);
+    return launch_join<HD, 16 * QT, 4>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED, bool IMG>
@@ -236,7 +236,7 @@ int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
         hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps + 1, p.kvh), dim3(kAttnThreads), 0, s, p, pl, const_cast<uint8_t *>(pl.img));
     const int x = IMG ? sh.jobs : sh.tiles * sh.splits;
     hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(x, p.kvh, seqs), dim3(IMG ? 256 : 768), 0, s, p, pl);
-    return launch_join<HD, 128>(s, p, pl, seqs);
+    return launch_join<HD, 128, 1>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED>
