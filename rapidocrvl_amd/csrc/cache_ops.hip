@@ -165,8 +165,8 @@ template <int HD>
 constexpr int64_t image_bytes = StepImage<HD>::kBytes;
 AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, bool images) {
     AttnShape a;
-    a.few = rows <= 32;
-    a.wg_rows = a.few ? (rows <= 16 ? 16 : 32) : 128;
+    a.few = rows <= 16;
+    a.wg_rows = a.few ? 16 : kTileRows;
     a.tiles = round_up_div(rows, a.wg_rows);
     const int64_t work = a.tiles * groups;
     // two workgroups a CU; prompts of many short rows (documents) leave most
@@ -180,7 +180,7 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
         a.slots = a.jobs > a.tiles ? a.jobs * groups : 0;
         a.cut_bytes = (a.tiles * (int64_t)sizeof(TileCut) + a.jobs * 4 + 15) / 16 * 16;
     } else {
-        const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : (a.few ? 512 : 256)) / work);
+        const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : 256) / work);
         a.least = a.few ? 1 : (work < 128 ? 2 : 6);
         a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
         a.jobs = 0;
@@ -222,11 +222,11 @@ int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs)
     return POCR_OK;
 }
 
-template <int HD, bool TREE, bool SHAPED, int QT>
+template <int HD, bool TREE, bool SHAPED>
 int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     const AttnPlan pl = attn_plan(sh, work, HD);
-    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED, QT>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
-    return launch_join<HD, 16 * QT, 4>(s, p, pl, seqs);
+    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
+    return launch_join<HD, 16, 4>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED, bool IMG>
@@ -243,8 +243,7 @@ template <int HD, bool TREE, bool SHAPED>
 int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     if constexpr (!TREE)
         if (sh.steps) return launch_attn_t<HD, TREE, SHAPED, true>(s, p, sh, work, seqs);
-    if (sh.few)
-        return sh.wg_rows == 16 ? launch_few<HD, TREE, SHAPED, 1>(s, p, sh, work, seqs) : launch_few<HD, TREE, SHAPED, 2>(s, p, sh, work, seqs);
+    if (sh.few) return launch_few<HD, TREE, SHAPED>(s, p, sh, work, seqs);
     return launch_attn_t<HD, TREE, SHAPED, false>(s, p, sh, work, seqs);
 }
 

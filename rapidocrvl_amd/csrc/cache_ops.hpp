@@ -218,7 +218,7 @@ struct AttnPlan {
     int tiles;        // row tiles per (sequence, KV head)
     int splits;       // shares a tile's keys may be cut into; 1: no partial sums
     int least;        // steps of a share
-    float *part;      // sums of a share [128 or 16·QT rows][HD]: [tile][split], with images [KV head][job]
+    float *part;      // sums of a share [128 or 16 rows][HD]: [tile][split], with images [KV head][job]
     float2 *stat;     // their rows' maxima and denominators
     int32_t *parts;   // [tile] shares in use
     // with images
@@ -899,20 +899,24 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
     }
 }
 
-// Few rows (at most 32 per sequence and KV head: one token, small trees).  What
+// Few rows (at most 16 per sequence and KV head: one token, small trees).  What
 // counts is how soon the cache is read: no wave waits for another, and K and V
 // go from memory to the fp32 matrix instruction as they are loaded.
-// Workgroup: 16·QT rows, four waves that take the share's blocks of 16 keys in turn, the next block's rows requested before this one's products:
+// Workgroup: 16 rows, four waves that take the share's blocks of 16 keys in
+// turn, the next block's rows requested before this one's products:
 //   K  lane 16·q + r: key r, dims 16c + 4q .. +3; product e of chunk c sums over
 //      the dims 16c + 4q + e, as the query rows are held
 //   V  lane 16·q + j: keys 4q .. 4q+3, dims 64d + 4j .. +3
 // Scores and sums come out transposed, as in k_cache_attn; the waves' sums are
 // joined in LDS.  Products, weights and sums are fp32 throughout.
+// One token of 16 heads and 2 KV heads over 1,609 rows of 128: 7.9 us and 4.2 of
+// the join, 3.3 MB; of 16 sequences 15 us, of 64 41 us (5.1 TB/s), of 256 143 us
+// (5.9 TB/s).
 constexpr int kFewKeys = 16;
 constexpr int kFewWaves = 4;
-template <int HD, bool TREE, bool SHAPED, int QT>
-__global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_few(CacheAttn p, AttnPlan pl) {
-    constexpr int KC = HD / 16, D = HD / 64, kRows = 16 * QT, kPad = HD + 4, W = kFewWaves, kFewStep = W * kFewKeys;
+template <int HD, bool TREE, bool SHAPED>
+__global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn p, AttnPlan pl) {
+    constexpr int KC = HD / 16, D = HD / 64, kRows = 16, kPad = HD + 4, W = kFewWaves, kFewStep = W * kFewKeys;
     __shared__ __attribute__((aligned(16))) float s_o[W][kRows][kPad];
     __shared__ float s_m[W][kRows], s_l[W][kRows];
     __shared__ uint64_t s_bits[64];
@@ -921,17 +925,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
     const int part = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     const size_t slot = (size_t)s * p.kvh + g;
     // nothing here waits for the lengths: the query rows, also of tokens that are not there
-    v4f q[QT][KC];
-    int row_tok[QT], row_head[QT];
+    v4f q[KC];
+    const int in = min(r16, p.n * p.group - 1), row_tok = by_group(p, in), row_head = g * p.group + in - row_tok * p.group;
+    const float *src = p.q + s * p.q_ss + row_tok * p.q_st + row_head * HD + 4 * kg;
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        const int row = min(16 * u + r16, p.n * p.group - 1);
-        row_tok[u] = by_group(p, row);
-        row_head[u] = g * p.group + row - row_tok[u] * p.group;
-        const float *src = p.q + s * p.q_ss + row_tok[u] * p.q_st + row_head[u] * HD + 4 * kg;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) q[u][c] = *reinterpret_cast<const v4f *>(src + 16 * c);
-    }
+    for (int c = 0; c < KC; ++c) q[c] = *reinterpret_cast<const v4f *>(src + 16 * c);
     int len = 0, count = p.n;
     if (TREE) {
         const SeqRows q = seq_rows(p, s);
@@ -960,7 +958,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
             s_hi = s_lo_max = 0;
         }
         __syncthreads();
-        if (tid < count) {  // at most 32 tokens
+        if (tid < count) {  // at most 16 tokens
             const int b = min(max(p.begin[tid], 0), p.rows), e = min(max(p.end[tid], 0), p.rows);
             if (b < e) {
                 atomicMin(&s_lo, b);
@@ -997,55 +995,39 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
     };
     if (t.from < t.to) load(t.lo + t.from * kFewStep + wave * kFewKeys);
 
-    float slope[QT];
-    int row_lo[QT], row_hi[QT], row_pos[QT];
-    uint64_t bits[QT];
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        const bool live = 16 * u + r16 < rows;
-        const int tok = row_tok[u], h = row_head[u];
-        slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-        row_lo[u] = row_hi[u] = row_pos[u] = 0;
-        bits[u] = 0;
-        if (TREE) {
-            if (live) {
-                row_hi[u] = len;
-                bits[u] = s_bits[tok];
-                if (SHAPED) row_pos[u] = p.pos ? p.pos[slot * p.side + len + tok] : len + s_depth[tok];
-            }
-        } else if (live) {
-            row_lo[u] = p.begin ? min(max(p.begin[tok], 0), p.rows) : 0;
-            row_hi[u] = p.end ? min(max(p.end[tok], 0), p.rows) : p.rows0 + tok + 1;
-            row_pos[u] = p.rows0 + tok;
+    const bool live = r16 < rows;
+    const float slope = SHAPED && p.slopes ? p.slopes[row_head] * kLog2e : 0.0f;
+    int row_lo = 0, row_hi = 0, row_pos = 0;
+    uint64_t bits = 0;
+    if (TREE) {
+        if (live) {
+            row_hi = len;
+            bits = s_bits[row_tok];
+            if (SHAPED) row_pos = p.pos ? p.pos[slot * p.side + len + row_tok] : len + s_depth[row_tok];
         }
+    } else if (live) {
+        row_lo = p.begin ? min(max(p.begin[row_tok], 0), p.rows) : 0;
+        row_hi = p.end ? min(max(p.end[row_tok], 0), p.rows) : p.rows0 + row_tok + 1;
+        row_pos = p.rows0 + row_tok;
     }
     const float scale = SHAPED ? p.scale : p.scale * kLog2e;
     const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
     const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + slot * p.side : nullptr;
 
-    v4f o[QT][D][4];  // [..][x][i]: dim 64d + 16·kg + 4i + x
-    float m[QT], l[QT];
+    v4f o[D][4];  // [..][x][i]: dim 64d + 16·kg + 4i + x
+    float m = kLowest, l = 0.0f;
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        m[u] = kLowest;
-        l[u] = 0.0f;
+    for (int d = 0; d < D; ++d)
 #pragma unroll
-        for (int d = 0; d < D; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[u][d][x] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    }
+        for (int x = 0; x < 4; ++x) o[d][x] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     for (int step = t.from; step < t.to; ++step) {
         const int k0 = t.lo + step * kFewStep + wave * kFewKeys;
-        v4f sc[QT];
+        v4f a[4] = {};
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            v4f a[4] = {};
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c][e], q[u][c][e], a[e], 0, 0, 0);
-            sc[u] = (a[0] + a[1]) + (a[2] + a[3]);
-        }
+            for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[c][e], q[c][e], a[e], 0, 0, 0);
+        const v4f sc = (a[0] + a[1]) + (a[2] + a[3]);
         v4f v[4][D];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -1069,79 +1051,72 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
                 bad |= here ? 1u << i : 0u;
             }
         }
-#pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            uint32_t see = 0xf;  // of the lane's four keys
-            if (!whole) {
-                const int n1 = min(max(row_hi[u] - k0, 0), 16), n0 = min(max(row_lo[u] - k0, 0), 16);
-                uint32_t w = ((1u << n1) - 1) & ~((1u << n0) - 1);
-                if (TREE) {
-                    const int off = k0 - len;  // the block's first key among the drafted ones
-                    if (off > -16 && off < 64) w |= (uint32_t)(off >= 0 ? bits[u] >> off : bits[u] << -off);
-                }
-                see = w >> (4 * kg) & 0xf;
+        uint32_t see = 0xf;  // of the lane's four keys
+        if (!whole) {
+            const int n1 = min(max(row_hi - k0, 0), 16), n0 = min(max(row_lo - k0, 0), 16);
+            uint32_t w = ((1u << n1) - 1) & ~((1u << n0) - 1);
+            if (TREE) {
+                const int off = k0 - len;  // the block's first key among the drafted ones
+                if (off > -16 && off < 64) w |= (uint32_t)(off >= 0 ? bits >> off : bits << -off);
             }
-            float x[4];
+            see = w >> (4 * kg) & 0xf;
+        }
+        float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = sc[u][i] * scale;
-            if (SHAPED) {
-                if (p.cap > 0.0f) {
+        for (int i = 0; i < 4; ++i) x[i] = sc[i] * scale;
+        if (SHAPED) {
+            if (p.cap > 0.0f) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] *= inv_cap;
-                    tanh_all(x);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = k0 + 4 * kg + i;
-                    int at = key;
-                    if (TREE) at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
-                    x[i] = fmaf(x[i], cap2, -slope[u] * fabsf((float)(int)((uint32_t)row_pos[u] - (uint32_t)at)));
-                }
+                for (int i = 0; i < 4; ++i) x[i] *= inv_cap;
+                tanh_all(x);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = see >> i & 1 ? x[i] : -INFINITY;
-            const float top = groups_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if (__any(top > m[u])) {
-                const float mn = top > m[u] ? top : m[u];
-                const float f = __builtin_amdgcn_exp2f(m[u] - mn);
-                l[u] *= f;
-#pragma unroll
-                for (int d = 0; d < D; ++d)
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) o[u][d][y] *= f;
-                m[u] = mn;
-            }
-            float w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(x[i] - m[u]);
-                l[u] += w[i];
-                if (!whole && (bad & see) >> i & 1) l[u] = __uint_as_float(0x7fc00000u);
+                const int key = k0 + 4 * kg + i;
+                int at = key;
+                if (TREE) at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
+                x[i] = fmaf(x[i], cap2, -slope * fabsf((float)(int)((uint32_t)row_pos - (uint32_t)at)));
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int d = 0; d < D; ++d)
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        o[u][d][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d][y], w[i], o[u][d][y], 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = see >> i & 1 ? x[i] : -INFINITY;
+        const float top = groups_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        if (__any(top > m)) {
+            const float mn = top > m ? top : m;
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) o[d][y] *= f;
+            m = mn;
+        }
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(x[i] - m);
+            l += w[i];
+            if (!whole && (bad & see) >> i & 1) l = __uint_as_float(0x7fc00000u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    o[d][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d][y], w[i], o[d][y], 0, 0, 0);
     }
 
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        const int row = 16 * u + r16;
-        const float total = groups_sum(l[u]);
-        if (kg == 0) {
-            s_m[wave][row] = m[u];
-            s_l[wave][row] = total;
-        }
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<v4f *>(&s_o[wave][row][64 * d + 16 * kg + 4 * i]) = (v4f){o[u][d][0][i], o[u][d][1][i], o[u][d][2][i], o[u][d][3][i]};
+    const float total = groups_sum(l);
+    if (kg == 0) {
+        s_m[wave][r16] = m;
+        s_l[wave][r16] = total;
     }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<v4f *>(&s_o[wave][r16][64 * d + 16 * kg + 4 * i]) = (v4f){o[d][0][i], o[d][1][i], o[d][2][i], o[d][3][i]};
     __syncthreads();
     for (int i = tid; i < rows * (HD / 4); i += 64 * W) {
         const int row = i / (HD / 4), at = i % (HD / 4) * 4;
@@ -1157,9 +1132,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, QT == 1 ? 2 : 1) k_cache_attn_
         }
         if (t.parts > 1) {
             *reinterpret_cast<v4f *>(pl.part + ((slot * pl.splits + part) * kRows + row) * HD + at) = x;
-            if (at == 0)
-                pl.stat[(slot * pl.splits + part) * kRows + row] =
-                    make_float2(mm, total);
+            if (at == 0) pl.stat[(slot * pl.splits + part) * kRows + row] = make_float2(mm, total);
             continue;
         }
         const int tok = by_group(p, row), h = g * p.group + row - tok * p.group;
