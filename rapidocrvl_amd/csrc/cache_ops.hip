@@ -14,7 +14,16 @@ constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kMaxPromptRows = 1 << 22;
 constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
 constexpr int kMaxQueryHeads = 1024;
-constexpr int kImageTiles = 4;
+// Images cost a launch and a pass over the rows, and pay by the steps that all
+// tiles take (of 128 rows and 32 keys): images, attention and join against
+// attention and join took, 16 heads over 2 KV heads of 128, causal, in us:
+//   600 rows                   1,444 steps at most   32 : 30
+//   256 rows behind 2,000      2,272                 43 : 37
+//   800 rows                   2,500                 36 : 42
+//   128 rows behind 8,000      4,064                 56 : 54
+//   1,200 rows                 5,700                 49 : 88
+//   256 rows behind 8,000      8,256                 82 : 94
+constexpr int kImageTiles = 8, kImageSteps = 2400;
 
 // The calling thread's device becomes the context's for one call.
 struct DeviceScope {
@@ -90,7 +99,8 @@ int prompt_shape(const pocr_prompt_args *a, const char *op) {
     if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
     RC(check_heads(a->heads, a->kv_heads, a->head_dim, op));
     RC(check_scores(a->scale, a->cap, op));
-    if (a->n < 1 || a->n > kMaxPromptRows) return fail(POCR_ERR_ARG, "%s: %d rows", op, a->n);
+    if (a->n < 1 || a->n > kMaxPromptRows || (int64_t)a->n * (a->heads / a->kv_heads) > kMaxCacheRows)
+        return fail(POCR_ERR_ARG, "%s: %d rows of %d heads", op, a->n, a->heads);
     if (a->rows_before < 0 || a->rows_before > kMaxCacheRows - a->n) return fail(POCR_ERR_ARG, "%s: %d rows before", op, a->rows_before);
     return POCR_OK;
 }
@@ -165,21 +175,31 @@ template <int HD>
 constexpr int64_t image_bytes = StepImage<HD>::kBytes;
 AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, bool images) {
     AttnShape a;
+    // 16 rows by either form, 16 sequences of 2 tokens over 1,609 rows: 16 us in
+    // fp32 straight from the cache, 19 laid out; beyond, the fp32 products of two
+    // tiles took 29 us where laying out takes 20
     a.few = rows <= 16;
     a.wg_rows = a.few ? 16 : kTileRows;
     a.tiles = round_up_div(rows, a.wg_rows);
     const int64_t work = a.tiles * groups;
-    // two workgroups a CU; prompts of many short rows (documents) leave most
-    // CUs idle behind their longest tile unless that is cut too
-    a.steps = images && !a.few && a.tiles >= kImageTiles ? round_up_div(keys, kBlock) : 0;
+    const int steps = round_up_div(keys, kBlock);
+    a.steps = images && a.tiles >= kImageTiles && work * steps >= kImageSteps ? steps : 0;
     const int step = a.few ? kFewKeys * kFewWaves : kBlock;
     if (a.steps) {
+        // Two workgroups a CU run at once; the device cuts the tiles into shares of
+        // at least two steps that fill them once (480 or 768 workgroups for the
+        // same prompts: 15 to 25% more time).  More tiles than that stay whole.
         a.least = 2;
         a.splits = 1;
-        a.jobs = work <= 512 ? (int)(512 / groups) : a.tiles;
+        a.jobs = work <= kCutTiles ? (int)(kCutTiles / groups) : a.tiles;
         a.slots = a.jobs > a.tiles ? a.jobs * groups : 0;
         a.cut_bytes = (a.tiles * (int64_t)sizeof(TileCut) + a.jobs * 4 + 15) / 16 * 16;
     } else {
+        // One workgroup a CU at a time (512 for 16 trees of 12 over 1,609 rows: 41
+        // us, 256: 32, by the form that both were measured with; 256 and 512 are
+        // alike for few rows).  From 256 tiles on, whose lengths may differ, shares
+        // for four rounds.  Shares of fewer steps than `least` cost more in sums
+        // than they save where the tiles fill half of the chip anyway.
         const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : 256) / work);
         a.least = a.few ? 1 : (work < 128 ? 2 : 6);
         a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
