@@ -69,7 +69,8 @@ BAD_SCORES = [(dict(scale=-1.0), ARG, "scale"), (dict(scale=float("nan")), ARG, 
 
 
 @pytest.mark.parametrize("kw,want,text", BAD_HEADS + BAD_SCORES + [
-    (dict(n=0), ARG, "rows"), (dict(n=(1 << 22) + 1), ARG, "rows"), (dict(rows_before=-1), ARG, "rows before"),
+    (dict(n=0), ARG, "rows"), (dict(n=(1 << 22) + 1), ARG, "rows"), (dict(n=1 << 22, heads=1024, kv_heads=1), ARG, "rows"),
+    (dict(rows_before=-1), ARG, "rows before"),
     (dict(rows_before=1 << 30), ARG, "rows before"), (dict(q=None), ARG, "null q"), (dict(k=None), ARG, "null k"),
     (dict(v=None), ARG, "null v"), (dict(out=None), ARG, "null out"), (dict(q=P + 4), ARG, "aligned"),
     (dict(k=P + 8), ARG, "aligned"), (dict(lse=P + 2), ARG, "aligned"), (dict(q_stride=2044), ARG, "q rows"),

@@ -235,6 +235,114 @@ def test_prompt_extreme_spans(ctx, rng, edge):
         check_prompt(hip, a, q, k, v, spans)
 
 
+# Prompts of many tiles take another way: images of the rows, laid out once, and
+# shares that the device cuts (from 8 tiles of 128 query rows and 2,400 steps of
+# a tile and 32 keys: 840 tokens of 16 heads over one KV head, 105 tiles of up to
+# 28 steps).
+
+
+@pytest.mark.parametrize("kind", ["causal", "prefix", "docs", "window", "holes"])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (12.0, False), (25.0, True)], ids=["plain", "cap", "cap-bias"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_many_tiles(ctx, rng, kind, cap, bias, hd):
+    with ref.Hip() as hip:
+        n, rows0 = 840, 37
+        spans = spans_of(kind, n, rows0, rng)
+        slopes = alibi(16) if bias else None
+        a, q, k, v = prompt_case(hip, rng, n, rows0, 16, 1, hd, spans, cap, slopes, pad=4)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans, slopes, rows=np.unique(np.r_[0:20, 20:820:11, 820:840]))
+
+
+@pytest.mark.parametrize("n,rows0,heads,kvh", [(900, 0, 21, 3), (64, 10000, 16, 1), (1100, 0, 64, 4), (700, 5000, 5, 5)],
+                         ids=["groups-of-7", "few-tiles-long", "uncut", "group-of-1"])
+@pytest.mark.parametrize("kind", ["causal", "docs"])
+def test_prompt_many_tiles_shapes(ctx, rng, n, rows0, heads, kvh, kind):
+    with ref.Hip() as hip:
+        spans = spans_of(kind, n, rows0, rng)
+        a, q, k, v = prompt_case(hip, rng, n, rows0, heads, kvh, 64, spans)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans, rows=np.unique(np.r_[0:5, 5:n - 5:23, n - 5:n]))
+
+
+def test_prompt_many_tiles_all_rows(ctx, rng):
+    """No row is left out or written twice, whatever its tile's shares."""
+    with ref.Hip() as hip:
+        n = 803
+        spans = spans_of("holes", n, 0, rng)
+        a, q, k, v = prompt_case(hip, rng, n, 0, 16, 1, 64, spans)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans)
+
+
+def test_prompt_many_tiles_wide_ranges(ctx, rng):
+    """Rows of very different size in one step, and of one size in the next."""
+    with ref.Hip() as hip:
+        n, rows0 = 830, 30
+        rows = rows0 + n
+        size = np.exp2(np.where(np.arange(rows) // 96 % 2, rng.integers(-14, 15, rows), 3)).astype(F32)[:, None]
+        k = rng.standard_normal((rows, 64)).astype(F32) * size * F32(2.0 ** -8)
+        v = rng.standard_normal((rows, 64)).astype(F32) * size
+        q = rng.standard_normal((n, 1024)).astype(F32) * np.exp2(rng.integers(-12, 3, (n, 1))).astype(F32)
+        k[rows // 2], v[rows // 3], q[n // 2, :128] = 0.0, 0.0, 0.0
+        a, q, k, v = prompt_case(hip, rng, n, rows0, 16, 1, 64, None, q=q, k=k, v=v)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, None, rows=np.unique(np.r_[0:830:7, 829]))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_prompt_many_tiles_masked_values_do_not_leak(ctx, rng, bad, where):
+    with ref.Hip() as hip:
+        n, at = 840, 500
+        k = rng.standard_normal((n, 64)).astype(F32)
+        v = rng.standard_normal((n, 64)).astype(F32)
+        (k if where == "k" else v)[at, 5] = bad
+        a, q, k, v = prompt_case(hip, rng, n, 0, 16, 1, 64, None, k=k, v=v)
+        ctx.prompt_attention(a)
+        out = hip.down(a.out, (n, 1024))
+        (k if where == "k" else v)[at, 5] = 0.0
+        check_prompt(hip, a, q, k, v, None, rows=np.unique(np.r_[0:at:9, at - 20:at]))
+        if np.isnan(bad) or where == "v":
+            assert not np.isfinite(out[at:].reshape(-1, 16, 64)).all(-1).any()
+
+
+@pytest.mark.parametrize("edge", [2 ** 31 - 1, -2 ** 31])
+def test_prompt_many_tiles_extreme_spans(ctx, rng, edge):
+    with ref.Hip() as hip:
+        n = 840
+        i = np.arange(n)
+        spans = (np.where(i % 2, -2 ** 31, edge).astype(I32), np.where(i % 4 < 2, 2 ** 31 - 1, edge).astype(I32))
+        spans[0][300:600] = spans[1][300:600] = edge  # whole tiles that see nothing
+        a, q, k, v = prompt_case(hip, rng, n, 7, 16, 1, 64, spans)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans, rows=np.unique(np.r_[0:840:13, 838:840]))
+
+
+def test_prompt_many_tiles_captured_and_replayed(ctx, rng):
+    """A graph cuts its tiles by the spans that each replay finds, an eager call of another workspace between."""
+    with ref.Hip() as hip:
+        s = hip.stream()
+        n, rows0 = 820, 20
+        spans = spans_of("causal", n, rows0, rng) or (np.zeros(n, I32), (rows0 + 1 + np.arange(n)).astype(I32))
+        a, q, k, v = prompt_case(hip, rng, n, rows0, 16, 1, 64, spans)
+        b, bq, bk, bv = prompt_case(hip, rng, 810, 0, 16, 1, 64, None)
+        hip.sync()
+        g = hip.capture(s, lambda: ctx.prompt_attention(a, s))
+        rows = np.unique(np.r_[0:n:17, n - 1])
+        for kind in ("causal", "docs", "holes", "window", "docs"):
+            spans = spans_of(kind, n, rows0, rng) or (np.zeros(n, I32), (rows0 + 1 + np.arange(n)).astype(I32))
+            hip.write(a.row_begin, spans[0])
+            hip.write(a.row_end, spans[1])
+            k[:] = rng.standard_normal(k.shape) * 0.64
+            hip.write(a.k, k)
+            hip.replay(g, s)
+            check_prompt(hip, a, q, k, v, spans, rows=rows)
+            ctx.prompt_attention(b, s)
+            hip.sync()
+            check_prompt(hip, b, bq, bk, bv, None, rows=rows[rows < 810])
+
+
 # ---------------------------------------------------------------------------
 # drafted trees
 # ---------------------------------------------------------------------------
@@ -371,6 +479,22 @@ def test_tree_bias_cap_take(ctx, rng, cap, moved, n):
     with ref.Hip() as hip:
         t = Tree(hip, rng, [130, 0, 41], [n, n, 1], n, 16, 2, 128, random_trees(rng, 3, n), cap, alibi(16),
                  positions if moved else None, take=[0b10110101101, 2 ** 64 - 1, 0])
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
+
+
+@pytest.mark.parametrize("seqs,room", [(1, 0), (40, 20), (90, 20)], ids=["32-keys", "64-keys", "96-keys"])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (18.0, True)], ids=["plain", "cap-bias"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [9, 33])
+def test_weights_of_many_rows(ctx, rng, seqs, room, cap, bias, hd, n):
+    """More than 64 query rows, by workgroups of 32, 64 and 96 cache rows; lengths that end anywhere in them."""
+    with ref.Hip() as hip:
+        lens = rng.integers(0, 70, seqs)
+        t = Tree(hip, rng, lens, rng.integers(0, n + 1, seqs), n, 16, 2, hd, random_trees(rng, seqs, n), cap,
+                 alibi(16) if bias else None, room=room)
         ctx.tree_attention(t.a)
         t.check()
         ctx.cache_weights(t.a)
