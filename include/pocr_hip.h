@@ -297,10 +297,11 @@ int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters
  *  - head_dim is 64 or 128 (POCR_ERR_UNSUPPORTED otherwise); heads is a
  *    multiple of kv_heads, query head h reads KV head h / (heads / kv_heads).
  *  - Sums and softmax statistics are fp32; products keep 22 bits of each
- *    operand, or 2^-32 of the largest of its row and head.  A row whose query is NaN, or that sees a NaN or an infinite
- *    value, comes out not finite; what an infinite query or key gives its rows
- *    is unspecified (sizes of 2^110 and more count as infinite).  Rows that do
- *    not see such a key or value do not change.
+ *    operand, or 2^-32 of the largest of its row and head.  A row whose query
+ *    is NaN, or that sees a NaN or an infinite value, comes out not finite;
+ *    what an infinite query or key gives its rows is unspecified (sizes of
+ *    2^110 and more count as infinite).  Rows that do not see such a key or
+ *    value do not change.
  *
  * Scores of query row i and cache row j:
  *   s = scale * q·k, then cap * tanh(s / cap) where cap > 0, then
@@ -322,7 +323,7 @@ typedef struct {
     void *workspace;          /* pocr_prompt_attention_workspace bytes, 16-byte aligned */
     int64_t workspace_bytes;
     int64_t q_stride, k_stride, v_stride, out_stride;
-    int32_t n;                /* 1 .. 2^22 rows */
+    int32_t n;                /* 1 .. 2^22 rows, n * (heads / kv_heads) <= 2^30 */
     int32_t rows_before;      /* rows_before + n <= 2^30 */
     int32_t heads, kv_heads, head_dim;
     float scale;              /* > 0; 0: 1 / sqrt(head_dim) */

@@ -305,11 +305,11 @@ AttnShape tree_attn(const pocr_tree_args *a) {
 }
 
 // the addresses of `caches` blocks of `rows` rows overlap
-bool overlap(const void *a, int64_t acs, int64_t ast, int arows, const void *b, int64_t bcs, int64_t bst, int brows,
-             int caches, int64_t width) {
+bool overlap(const void *a, int64_t acs, int64_t ast, int arows, int64_t awidth, const void *b, int64_t bcs, int64_t bst,
+             int brows, int64_t bwidth, int caches) {
     const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
-    const char *a1 = a0 + 4 * ((caches - 1) * acs + (arows - 1) * ast + width);
-    const char *b1 = b0 + 4 * ((caches - 1) * bcs + (brows - 1) * bst + width);
+    const char *a1 = a0 + 4 * ((caches - 1) * acs + (arows - 1) * ast + awidth);
+    const char *b1 = b0 + 4 * ((caches - 1) * bcs + (brows - 1) * bst + bwidth);
     return a0 < b1 && b0 < a1;
 }
 
@@ -474,11 +474,16 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
             a->max_rows != a->max_rows_out || ((a->weights || a->positions) && p.side != p.side_out))
             return fail(POCR_ERR_ARG, "%s: in place, the strides and row counts of source and destination are equal", op);
     } else {
-        const int64_t heads = (int64_t)a->kv_heads;
-        if (overlap(a->k, a->k_cache_stride, a->k_stride, a->max_rows, a->k_out, a->k_out_cache_stride, a->k_out_stride, a->max_rows_out, a->caches, kvd) ||
-            overlap(a->v, a->v_cache_stride, a->v_stride, a->max_rows, a->v_out, a->v_out_cache_stride, a->v_out_stride, a->max_rows_out, a->caches, kvd) ||
-            (a->weights && overlap(a->weights, heads * p.side, 1, 1, a->weights_out, heads * p.side_out, 1, 1, a->caches, (heads - 1) * p.side + a->max_rows)) ||
-            (a->positions && overlap(a->positions, heads * p.side, 1, 1, a->positions_out, heads * p.side_out, 1, 1, a->caches, (heads - 1) * p.side + a->max_rows)))
+        const int64_t heads = a->kv_heads, in = (heads - 1) * p.side + a->max_rows, out = (heads - 1) * p.side_out + a->max_rows_out;
+        auto rows = [&](const void *x, int64_t xcs, int64_t xst, const void *y, int64_t ycs, int64_t yst) {
+            return overlap(x, xcs, xst, a->max_rows, kvd, y, ycs, yst, a->max_rows_out, kvd, a->caches);
+        };
+        auto sides = [&](const void *x, const void *y) {
+            return x && overlap(x, heads * p.side, 0, 1, in, y, heads * p.side_out, 0, 1, out, a->caches);
+        };
+        if (rows(a->k, a->k_cache_stride, a->k_stride, a->k_out, a->k_out_cache_stride, a->k_out_stride) ||
+            rows(a->v, a->v_cache_stride, a->v_stride, a->v_out, a->v_out_cache_stride, a->v_out_stride) ||
+            sides(a->weights, a->weights_out) || sides(a->positions, a->positions_out))
             return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
     }
     CACHE_OP_ENTER(ctx, stream, op);
