@@ -135,8 +135,8 @@ def test_keep_refusals(kw, text):
 
 def test_keep_overlap_counts_the_destinations_own_stride():
     """Side buffers of other strides: 2,600 floats at the destination, of which the last 200 are the source's first."""
-    refused("keep", ARG, "overlaps", weights=P, weights_out=P - 4 * 2400, side_out_stride=500, **OUT)
-    refused("keep", ARG, "null context", weights=P, weights_out=P - 4 * 2600, side_out_stride=500, **OUT)
+    refused("keep", ARG, "overlaps", weights=1 << 20, weights_out=(1 << 20) - 4 * 2400, side_out_stride=500, **OUT)
+    refused("keep", ARG, "null context", weights=1 << 20, weights_out=(1 << 20) - 4 * 2600, side_out_stride=500, **OUT)
 
 
 def test_keep_head_dim():
