@@ -1,5 +1,6 @@
 // cache_ops.hip — the cache operators' entry points (cache_ops.hpp): argument
 // checks, launch shapes, and the device and stream they run on.
+#include <cfloat>
 #include <cmath>
 
 #include "cache_ops.hpp"
@@ -67,7 +68,8 @@ int check_heads(int heads, int kv_heads, int head_dim, const char *op) {
 
 int check_scores(float scale, float cap, const char *op) {
     if (!(scale >= 0.0f) || std::isinf(scale)) return fail(POCR_ERR_ARG, "%s: scale must be finite and >= 0", op);
-    if (!(cap >= 0.0f) || std::isinf(cap)) return fail(POCR_ERR_ARG, "%s: cap must be finite and >= 0", op);
+    // 1 / cap is a factor of the scores
+    if (!(cap >= 0.0f) || std::isinf(cap) || (cap > 0.0f && cap < FLT_MIN)) return fail(POCR_ERR_ARG, "%s: cap must be finite and 0 or at least 2^-126", op);
     return POCR_OK;
 }
 

@@ -65,7 +65,8 @@ BAD_HEADS = [(dict(heads=0), ARG, "heads"), (dict(kv_heads=0), ARG, "heads"), (d
              (dict(heads=2048, kv_heads=2), ARG, "heads"), (dict(head_dim=96), UNS, "head_dim"),
              (dict(head_dim=0), UNS, "head_dim"), (dict(head_dim=-128), UNS, "head_dim")]
 BAD_SCORES = [(dict(scale=-1.0), ARG, "scale"), (dict(scale=float("nan")), ARG, "scale"),
-              (dict(scale=float("inf")), ARG, "scale"), (dict(cap=-3.0), ARG, "cap"), (dict(cap=float("nan")), ARG, "cap")]
+              (dict(scale=float("inf")), ARG, "scale"), (dict(cap=-3.0), ARG, "cap"), (dict(cap=float("nan")), ARG, "cap"),
+              (dict(cap=1e-40), ARG, "cap")]
 
 
 @pytest.mark.parametrize("kw,want,text", BAD_HEADS + BAD_SCORES + [
