@@ -285,7 +285,9 @@ int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters
  *    floats are 16-byte aligned and their strides, counted in floats, are
  *    multiples of 4 (POCR_ERR_ARG otherwise); index buffers are 4-byte aligned.
  *  - `stream` is the hipStream_t the work is queued on, null HIP's default
- *    stream; a stream of another device is POCR_ERR_ARG.  A call returns once
+ *    stream, of the HIP runtime that the library runs on (a process that loads
+ *    the library and then a package with a runtime of its own holds two); a
+ *    stream of another device is POCR_ERR_ARG.  A call returns once
  *    its kernels are queued, allocates nothing, keeps nothing, waits for
  *    nothing and leaves the calling thread's current device as it was: it may
  *    be captured into a HIP graph.

@@ -45,7 +45,7 @@ struct DeviceScope {
 int check_stream(const pocr_ctx *ctx, hipStream_t s, const char *op) {
     if (!s) return POCR_OK;
     hipDevice_t dev = 0;
-    if (hipStreamGetDevice(s, &dev) != hipSuccess) return fail(POCR_ERR_ARG, "%s: not a stream", op);
+    if (hipStreamGetDevice(s, &dev) != hipSuccess) return fail(POCR_ERR_ARG, "%s: not a stream of the HIP runtime that this library runs on", op);
     if (dev != ctx->device) return fail(POCR_ERR_ARG, "%s: a stream of device %d, the context is on %d", op, dev, ctx->device);
     return POCR_OK;
 }

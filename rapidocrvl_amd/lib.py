@@ -358,25 +358,6 @@ def tree_attention_workspace(args: TreeArgs) -> int:
     return check(load().pocr_tree_attention_workspace(C.byref(args)))
 
 
-_known_streams = set()
-
-
-def _stream(stream):
-    """A hipStream_t handle for the cache operators (0: HIP's default stream).
-    A handle, and the buffers, have to come from the HIP runtime that the
-    library itself runs on: a process that loads the library and only then
-    another package with a HIP runtime of its own holds two."""
-    if stream and stream not in _known_streams:
-        load()
-        with open("/proc/self/maps") as f:
-            runtimes = {os.path.realpath(ln.split()[-1]) for ln in f if "libamdhip64" in ln}
-        if len(runtimes) > 1:
-            raise RuntimeError("two HIP runtimes are loaded (" + ", ".join(sorted(runtimes)) + "): a stream of one is "
-                               "not known to the other; import the package that made it before this library is loaded")
-        _known_streams.add(stream)
-    return stream
-
-
 def device_count() -> int:
     return int(load().pocr_device_count())
 
@@ -639,27 +620,26 @@ class Context:
         check(load().pocr_text_attention_noalloc(self.h, C.c_void_p(q_dev), C.c_void_p(k_dev), C.c_void_p(v_dev),
                                                  cache_len, heads, kv_heads, head_dim, C.c_void_p(out_dev)))
 
-
     # -- cache operators: device buffers, queued on the caller's stream --------
     def prompt_attention(self, args: PromptArgs, stream=0):
         """Attention of a prompt's rows (masks as spans, capped scores, distance biases)."""
-        check(load().pocr_prompt_attention(self.h, C.byref(args), _stream(stream)))
+        check(load().pocr_prompt_attention(self.h, C.byref(args), stream))
 
     def tree_attention(self, args: TreeArgs, stream=0):
         """Attention of drafted trees over their sequences' caches."""
-        check(load().pocr_tree_attention(self.h, C.byref(args), _stream(stream)))
+        check(load().pocr_tree_attention(self.h, C.byref(args), stream))
 
     def cache_weights(self, args: TreeArgs, stream=0):
         """Adds what each cache row weighs for the taken tokens to args.weights."""
-        check(load().pocr_cache_weights(self.h, C.byref(args), _stream(stream)))
+        check(load().pocr_cache_weights(self.h, C.byref(args), stream))
 
     def cache_select(self, args: SelectArgs, stream=0):
         """Lists the rows that stay when each cache falls to args.budget rows."""
-        check(load().pocr_cache_select(self.h, C.byref(args), _stream(stream)))
+        check(load().pocr_cache_select(self.h, C.byref(args), stream))
 
     def cache_keep(self, args: KeepArgs, stream=0):
         """Moves the listed rows of each cache together."""
-        check(load().pocr_cache_keep(self.h, C.byref(args), _stream(stream)))
+        check(load().pocr_cache_keep(self.h, C.byref(args), stream))
 
 
 class Model:
