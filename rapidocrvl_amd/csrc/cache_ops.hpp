@@ -498,12 +498,11 @@ __global__ void __launch_bounds__(kAttnThreads) k_cache_images(CacheAttn p, Attn
 // IMG: images come ready from memory by direct loads; four waves of 32 rows (a
 // value read from LDS serves two products), two workgroups a CU, so one's
 // softmax runs beside the other's products.  8,192 causal rows of 16 heads:
-// 825 GFLOP of fp16 products in 0.77 ms, 1,070 TFLOP/s where a large matrix
+// 825 GFLOP of fp16 products in 0.75 ms, 1,103 TFLOP/s where a large matrix
 // product of the library reaches 1,159.  Its products alone, with no softmax and
 // no LDS reads between them, take 0.57 ms: the clock falls under them.
 // (256 rows in eight waves, whose halves take turns at products and softmax
-// behind barriers: the same 0.77 ms, but 80 us for 61 at 1,345 rows, whose
-// shares are twice as long to start and end.)
+// behind barriers, were no faster there and took 80 us for 61 at 1,345 rows.)
 // Otherwise one workgroup a CU: four waves do nothing but lay rows out, eight of
 // 16 rows multiply.  What the ones spend on vector instructions runs beside the
 // others' matrix instructions; eight waves that did both in turn took 65 us for
