@@ -148,13 +148,6 @@ __device__ __forceinline__ float groups_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// max over 8 consecutive lanes
-__device__ __forceinline__ uint32_t lanes8_umax(uint32_t v) {
-    v = max(v, __float_as_uint(xchg<XQ1>(__uint_as_float(v))));
-    v = max(v, __float_as_uint(xchg<XQ2>(__uint_as_float(v))));
-    return max(v, __float_as_uint(xchg<XM8>(__uint_as_float(v))));
-}
-
 // tanh of N numbers, to 2.5 · 2^-24 of its value; NaN stays NaN.  Up to 0.85, x +
 // x³·P(x²) with a P fitted to (tanh(x)/x − 1)/x² there (least largest error,
 // 2^-27 of tanh); above, 1 − 2/(e^2x + 1), where the difference no longer
