@@ -1490,8 +1490,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // among weights that differ), then one pass that writes the kept rows in order: a wave owns 64·KPT
 // consecutive rows of a tile, so a row's place is a count of ballots.  KPT rows
 // per thread and tile; where one tile holds the cache its keys are read once
-// and stay in registers.  36 selections, one workgroup each: 6.8 us of 1,609
-// rows, 10.7 of 8,192, nearly all of it the chain of load, passes and barriers.
+// and stay in registers.  36 selections, one workgroup each: 6.6 us of 1,609
+// rows, 10.6 of 8,192, nearly all of it the chain of load, passes and barriers.
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     constexpr int kTile = kSelThreads * KPT, kBins = 2048;
@@ -1499,6 +1499,15 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     __shared__ int s_bin, s_need, s_all;
     __shared__ int s_eq[kSelWaves], s_gt[kSelWaves];
     const int g = blockIdx.x, c = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float *w = p.weights + ((size_t)c * p.kvh + g) * p.side;
+    const bool one = p.max_rows <= kTile;  // one tile holds any cache: its weights wait for no length
+    float x[KPT];
+    auto load = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < KPT; ++i)  // all on their way at once
+            x[i] = w[min(tile * kTile + (wave * KPT + i) * 64 + lane, p.max_rows - 1)];
+    };
+    if (one) load(0);
     const int len = min(max(p.lens[c], 0), p.max_rows);
     int32_t *kept = p.kept + ((size_t)c * p.kvh + g) * p.budget;
     if (g == 0 && tid == 0) p.counts[c] = min(len, p.budget);
@@ -1506,29 +1515,27 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
         for (int j = tid; j < len; j += kSelThreads) kept[j] = j;
         return;
     }
-    const float *w = p.weights + ((size_t)c * p.kvh + g) * p.side;
     const int first = p.sinks, last = len - p.recent;  // candidates [first, last): more than `need` of them
     int need = p.budget - p.sinks - p.recent;
     const int tiles = (len + kTile - 1) / kTile;
-    uint32_t key[KPT] = {};
-    auto load = [&](int tile) {
-        float x[KPT];
-#pragma unroll
-        for (int i = 0; i < KPT; ++i)  // all on their way at once
-            x[i] = w[min(tile * kTile + (wave * KPT + i) * 64 + lane, len - 1)];
+    uint32_t key[KPT];
+    auto keys = [&] {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) key[i] = weight_key(x[i]);
     };
+    if (one) keys();
     uint32_t prefix = 0, mask = 0;
     if (need > 0)
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : kBins;
             hist[tid] = 0;
             hist[tid + kSelThreads] = 0;
-            if (tiles == 1 && pass == 0) load(0);
             __syncthreads();
             for (int tile = 0; tile < tiles; ++tile) {
-                if (tiles > 1) load(tile);
+                if (!one) {
+                    load(tile);
+                    keys();
+                }
 #pragma unroll
                 for (int i = 0; i < KPT; ++i) {
                     const int j = tile * kTile + (wave * KPT + i) * 64 + lane;
@@ -1567,7 +1574,10 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     const bool some = p.budget > p.sinks + p.recent;
     int done = 0, eq_done = 0;  // rows written, equal keys met
     for (int tile = 0; tile < tiles; ++tile) {
-        if (tiles > 1) load(tile);
+        if (!one) {
+            load(tile);
+            keys();
+        }
         int gt = 0, eq = 0;
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
