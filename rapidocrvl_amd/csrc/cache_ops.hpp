@@ -93,10 +93,21 @@ __device__ __forceinline__ void split_one(float a, float b, float one, v2h &hi, 
     lo = (v2h){(_Float16)__builtin_fmaf(a, one, -(float)hi[0]), (_Float16)__builtin_fmaf(b, one, -(float)hi[1])};
 }
 
+// x as rounded: no part of a multiply-add
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 constexpr int kTop = 14;        // operand rows are scaled to sizes below 2^kTop
 constexpr int kSpread = 4;      // key (value) rows of one exponent's scale lie within 2^kSpread
 constexpr int kMaxExp = 110;    // rows of larger exponents count as infinite
 constexpr float kLowest = -3.0e38f;
+// Up to here a score's last bit is 1/4 and whole numbers are exact: a weight's
+// argument may be one multiply-add of the unrounded product and carry a power
+// of two with the maximum.  Beyond, what that rounds away is more than the
+// weights' room in fp16 (2^14 of 2^16), and each operation rounds for itself.
+constexpr float kFarScore = 4194304.0f;
 constexpr int kBlock = 32;      // keys per step
 constexpr int kAttnThreads = 256;
 
@@ -808,16 +819,23 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = sc[u][e >> 2][e & 3] * (SHAPED ? f : 1.0f);
                 if (SHAPED) shape(u, x);
-                const float mine = SHAPED ? max8(x) : max8(x) * f;
+                const float mine = rounded(SHAPED ? max8(x) : max8(x) * f);
                 raise_m(u, groups_max(mine));
                 by[u] = raise_a(u, (int)groups_max(ceilf(fmaxf(mine - m[u], -16000.0f)) + (float)ve));
                 // weights below 2^-60 of the largest come out 0 either way
                 const int sh = max(14 + ve - a[u], -60);
                 const float mm = m[u] - (float)sh;
                 float w[8], sum = 0.0f;
+                if (__any(fabsf(m[u]) > kFarScore)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = rounded(SHAPED ? x[e] : x[e] * f) - m[u] + (float)sh;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = SHAPED ? x[e] - mm : __builtin_fmaf(x[e], f, -mm);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(SHAPED ? x[e] - mm : __builtin_fmaf(x[e], f, -mm));
+                    w[e] = __builtin_amdgcn_exp2f(w[e]);
                     sum += w[e];
                 }
                 l[u] += __builtin_ldexpf(sum, -sh);

@@ -1,0 +1,64 @@
+"""The cache operators at the ends of the ranges that their header states.
+Definitions and bounds: cache_ops_f64.py."""
+import cache_ops_f64 as ref
+import numpy as np
+import pytest
+from test_gpu_cache_ops import F32, I32, alibi, prompt_case, visible
+
+pytestmark = pytest.mark.gpu
+
+
+def check_one_hot(out, lse, s, seen, v):
+    """Rows whose largest score stands far above the next: their key's value row.
+
+    A score of 22-bit operands is off by at most 2^-15 of the largest (2^-19 of
+    the sum of its 64 products' sizes, which stays below 16 times the largest
+    score).  Where the next is 2^-12 of that and at least 2^7 further down, its
+    weight is below e^-90.  The value row keeps 22 bits (2^-19 with its sums),
+    and the logarithm of the sum what the score does."""
+    order = np.sort(np.where(seen, s, -np.inf), 1)
+    size = np.abs(np.where(seen, s, 0.0)).max(1)
+    clear = order[:, -1] - order[:, -2] > np.maximum(size * 2.0 ** -12, 2.0 ** 7)
+    assert clear.sum() > len(s) / 2
+    at = np.where(seen, s, -np.inf).argmax(1)
+    assert np.isfinite(out).all() and np.isfinite(lse).all()
+    err = np.abs(out - v[at])[clear]
+    assert np.all(err <= np.abs(v[at])[clear] * 2.0 ** -19 + np.abs(v[at]).max(1)[clear, None] * 2.0 ** -28)
+    assert np.all(np.abs(lse - order[:, -1]) <= size * 2.0 ** -15)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 13, 2.0 ** 14, 2.0 ** 20, 2.0 ** 40])
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+@pytest.mark.parametrize("n,rows0,heads", [(1, 200, 2), (20, 200, 2), (840, 37, 16)], ids=["few", "tiles", "images"])
+def test_prompt_far_scores(ctx, rng, n, rows0, heads, size, bias):
+    """Finite scores of 2^24 and far more: a step of fp32 there is more than an exponent of fp16 holds."""
+    with ref.Hip() as hip:
+        q = (rng.standard_normal((n, heads * 64)) * size).astype(F32)
+        k = (rng.standard_normal((rows0 + n, 64)) * size).astype(F32)
+        slopes = alibi(heads) if bias else None
+        a, q, k, v = prompt_case(hip, rng, n, rows0, heads, 1, 64, None, 0.0, slopes, q=q, k=k)
+        ctx.prompt_attention(a)
+        out, lse = hip.down(a.out, (n, heads * 64)), hip.down(a.lse, (n, heads))
+        dist = rows0 + np.arange(n)[:, None] - np.arange(rows0 + n)
+        for h in range(heads):
+            s = q[:, h * 64:(h + 1) * 64].astype(np.float64) @ k.T.astype(np.float64) * 0.125
+            if bias:
+                s -= slopes[h].astype(np.float64) * np.abs(dist)
+            check_one_hot(out[:, h * 64:(h + 1) * 64], lse[:, h], s, visible(None, n, rows0), v)
+
+
+@pytest.mark.parametrize("slope", [2.0 ** 18, 2.0 ** 19, 2.0 ** 20, 2.0 ** 21, 2.0 ** 24])
+@pytest.mark.parametrize("n,rows0,heads", [(1, 400, 2), (20, 400, 2), (840, 237, 16)], ids=["few", "tiles", "images"])
+def test_prompt_far_biases(ctx, rng, n, rows0, heads, slope):
+    """Rows that see none of their nearest 100 keys: all their scores lie far below zero."""
+    with ref.Hip() as hip:
+        i = np.arange(n)
+        spans = np.zeros(n, I32), (rows0 + i - 100).astype(I32)
+        slopes = np.full(heads, slope, F32)
+        a, q, k, v = prompt_case(hip, rng, n, rows0, heads, 1, 64, spans, 0.0, slopes)
+        ctx.prompt_attention(a)
+        out, lse = hip.down(a.out, (n, heads * 64)), hip.down(a.lse, (n, heads))
+        dist = rows0 + i[:, None] - np.arange(rows0 + n)
+        for h in range(heads):
+            s = q[:, h * 64:(h + 1) * 64].astype(np.float64) @ k.T.astype(np.float64) * 0.125 - slope * np.abs(dist)
+            check_one_hot(out[:, h * 64:(h + 1) * 64], lse[:, h], s, visible(spans, n, rows0), v)
