@@ -1045,6 +1045,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
 
     v4f o[D][4];  // [..][x][i]: dim 64d + 16·kg + 4i + x
     float m = kLowest, l = 0.0f;
+    uint32_t sees_bad = 0;
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
@@ -1120,12 +1121,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
                 for (int y = 0; y < 4; ++y) o[d][y] *= f;
             m = mn;
         }
+        sees_bad |= bad & see;
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             w[i] = __builtin_amdgcn_exp2f(x[i] - m);
             l += w[i];
-            if (!whole && (bad & see) >> i & 1) l = __uint_as_float(0x7fc00000u);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -1136,6 +1137,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
                     o[d][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d][y], w[i], o[d][y], 0, 0, 0);
     }
 
+    if (groups_umax(sees_bad))  // the sums alone: the denominator is of the scores
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[d][x] = (v4f){NAN, NAN, NAN, NAN};
     const float total = groups_sum(l);
     if (kg == 0) {
         s_m[wave][r16] = m;

@@ -3,7 +3,7 @@ Definitions and bounds: cache_ops_f64.py."""
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, alibi, prompt_case, visible
+from test_gpu_cache_ops import F32, I32, Tree, alibi, prompt_case, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,38 @@ def test_prompt_far_biases(ctx, rng, n, rows0, heads, slope):
         for h in range(heads):
             s = q[:, h * 64:(h + 1) * 64].astype(np.float64) @ k.T.astype(np.float64) * 0.125 - slope * np.abs(dist)
             check_one_hot(out[:, h * 64:(h + 1) * 64], lse[:, h], s, visible(spans, n, rows0), v)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("at", [5, 70, 103], ids=["first", "middle", "last"])
+@pytest.mark.parametrize("n,rows0,heads", [(1, 103, 2), (4, 100, 2), (30, 74, 2), (840, 20, 16)],
+                         ids=["one", "few", "tiles", "images"])
+def test_prompt_bad_values_leave_the_lse(ctx, rng, n, rows0, heads, at, bad):
+    """lse is of the scores alone, whatever a visible value row holds; out is not finite there."""
+    with ref.Hip() as hip:
+        v = rng.standard_normal((rows0 + n, 64)).astype(F32)
+        clean = v.copy()
+        v[at, 9], clean[at] = bad, 0.0
+        a, q, k, v = prompt_case(hip, rng, n, rows0, heads, 1, 64, None, v=v)
+        ctx.prompt_attention(a)
+        out, lse = hip.down(a.out, (n, heads, 64)), hip.down(a.lse, (n, heads))
+        sees = rows0 + np.arange(n) >= at
+        assert not np.isfinite(out[sees]).all(-1).any()
+        assert np.isfinite(out[~sees]).all()
+        for h in range(heads):
+            _, e, _, _, eb, _ = ref.attention(q[:, h * 64:(h + 1) * 64], k, clean, visible(None, n, rows0), 0.125)
+            ref.close(lse[:, h], e, eb, f"lse of head {h}")
+
+
+@pytest.mark.parametrize("at", [3, 300, 601], ids=["first", "middle", "draft"])
+@pytest.mark.parametrize("n", [2, 20])
+def test_tree_bad_values_leave_the_weights(ctx, rng, n, at):
+    """The lse that pocr_cache_weights takes stays that of the scores: weights are those of finite values."""
+    with ref.Hip() as hip:
+        t = Tree(hip, rng, [600, 601], None, n, 4, 2, 128)
+        x = t.v.copy()
+        x[:, at, 7] = np.nan  # KV head 0
+        hip.write(t.a.v, x)
+        ctx.tree_attention(t.a)
+        ctx.cache_weights(t.a)
+        t.check_weights()
