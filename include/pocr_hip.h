@@ -299,11 +299,14 @@ int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters
  *  - head_dim is 64 or 128 (POCR_ERR_UNSUPPORTED otherwise); heads is a
  *    multiple of kv_heads, query head h reads KV head h / (heads / kv_heads).
  *  - Sums and softmax statistics are fp32; products keep 22 bits of each
- *    operand, or 2^-32 of the largest of its row and head.  A row whose query
- *    is NaN, or that sees a NaN or an infinite value, comes out not finite;
- *    what an infinite query or key gives its rows is unspecified (sizes of
- *    2^110 and more, also of scale times a query, count as infinite).  Rows
- *    that do not see such a key or value do not change.
+ *    operand, or 2^-32 of the largest of its row and head (less where that, or
+ *    scale times it for a query, is below 2^-110).  A row whose query is NaN, or
+ *    that sees a NaN or an infinite value, comes out not finite; its lse is that
+ *    of its scores.  What an infinite query or key gives its rows is unspecified
+ *    (sizes of 2^110 and more, also of scale times a query, count as infinite;
+ *    so do a score, a bias, and scale times the largest of a query row times the
+ *    largest of a key row, beyond 2^126).  Rows that do not see such a key or
+ *    value do not change.
  *
  * Scores of query row i and cache row j:
  *   s = scale * q·k, then cap * tanh(s / cap) where cap > 0, then
@@ -328,8 +331,8 @@ typedef struct {
     int32_t n;                /* 1 .. 2^22 rows, n * (heads / kv_heads) <= 2^30 */
     int32_t rows_before;      /* rows_before + n <= 2^30 */
     int32_t heads, kv_heads, head_dim;
-    float scale;              /* > 0; 0: 1 / sqrt(head_dim) */
-    float cap;                /* 2^-126 and more; 0: scores as they are */
+    float scale;              /* 2^-126 to 2^126; 0: 1 / sqrt(head_dim) */
+    float cap;                /* 2^-126 to 2^126; 0: scores as they are */
 } pocr_prompt_args;
 int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *args, void *stream);
 /* workspace bytes of such a call (pointers and strides are not looked at), or an error status */

@@ -15,6 +15,7 @@ constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kMaxPromptRows = 1 << 22;
 constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
 constexpr int kMaxQueryHeads = 1024;
+constexpr float kLeast = FLT_MIN, kMost = 0x1p126f;  // of scale and cap
 // Images cost a launch and a pass over the rows, and pay by the steps that all
 // tiles take (of 128 rows and 32 keys): images, attention and join against
 // attention and join took, 16 heads over 2 KV heads of 128, causal, in us:
@@ -66,10 +67,10 @@ int check_heads(int heads, int kv_heads, int head_dim, const char *op) {
     return POCR_OK;
 }
 
+// Both meet log2(e), and a cap its reciprocal, as factors in fp32.
 int check_scores(float scale, float cap, const char *op) {
-    if (!(scale >= 0.0f) || std::isinf(scale)) return fail(POCR_ERR_ARG, "%s: scale must be finite and >= 0", op);
-    // 1 / cap is a factor of the scores
-    if (!(cap >= 0.0f) || std::isinf(cap) || (cap > 0.0f && cap < FLT_MIN)) return fail(POCR_ERR_ARG, "%s: cap must be finite and 0 or at least 2^-126", op);
+    if (!(scale == 0.0f || (scale >= kLeast && scale <= kMost))) return fail(POCR_ERR_ARG, "%s: scale must be 0 or 2^-126 to 2^126", op);
+    if (!(cap == 0.0f || (cap >= kLeast && cap <= kMost))) return fail(POCR_ERR_ARG, "%s: cap must be 0 or 2^-126 to 2^126", op);
     return POCR_OK;
 }
 

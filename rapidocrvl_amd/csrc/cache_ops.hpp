@@ -30,6 +30,12 @@ struct CacheAttn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// slope[h] to the base 2; the largest ones stay finite, so that distance 0 costs nothing
+__device__ __forceinline__ float slope_of(const CacheAttn &p, int h) {
+    const float x = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    return fabsf(x) == INFINITY ? copysignf(3.4028235e38f, x) : x;
+}
+
 // lane t of a full wave: token t of a drafted tree, the bits of itself and its
 // ancestors (pointer doubling: after k rounds the bits cover 2^k generations)
 __device__ __forceinline__ uint64_t tree_bits(const int32_t *parents, int n, int lane) {
@@ -661,7 +667,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
         const int e = row_exp(groups_umax(top));
         split_row<C>(x, e, qh[u], ql[u]);
         qf[u] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
-        slope[u] = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+        slope[u] = SHAPED ? slope_of(p, h) : 0.0f;
         row_pos[u] = 0;
         bits[u] = 0;
         int2 sees = {0, 0};
@@ -1025,7 +1031,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
     if (t.from < t.to) load(t.lo + t.from * kFewStep + wave * kFewKeys);
 
     const bool live = r16 < rows;
-    const float slope = SHAPED && p.slopes ? p.slopes[row_head] * kLog2e : 0.0f;
+    const float slope = SHAPED ? slope_of(p, row_head) : 0.0f;
     int row_lo = 0, row_hi = 0, row_pos = 0;
     uint64_t bits = 0;
     if (TREE) {
@@ -1326,7 +1332,7 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
                 to.qf[local] = pow2(e - kTop) * (SHAPED ? p.scale : p.scale * kLog2e);
                 to.see[local] = b;
                 if (SHAPED) {
-                    to.slope[local] = p.slopes ? p.slopes[g * p.group + row - tok * p.group] * kLog2e : 0.0f;
+                    to.slope[local] = slope_of(p, g * p.group + row - tok * p.group);
                     to.pos[local] = pos ? r.pos : q.len + __popcll(b) - 1;
                 }
             }

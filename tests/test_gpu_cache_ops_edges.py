@@ -3,7 +3,7 @@ Definitions and bounds: cache_ops_f64.py."""
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, Tree, alibi, prompt_case, visible
+from test_gpu_cache_ops import F32, I32, Tree, alibi, check_prompt, prompt_case, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,36 @@ def test_tree_bad_values_leave_the_weights(ctx, rng, n, at):
         ctx.tree_attention(t.a)
         ctx.cache_weights(t.a)
         t.check_weights()
+
+
+@pytest.mark.parametrize("slope", [3e38, -3e38])
+@pytest.mark.parametrize("n,heads", [(1, 2), (20, 2), (840, 16)], ids=["few", "tiles", "images"])
+def test_prompt_largest_slopes(ctx, rng, n, heads, slope):
+    """A slope near fp32's end: a row's own key has no distance and no bias.  Rows see themselves alone."""
+    with ref.Hip() as hip:
+        i = np.arange(n)
+        spans = i.astype(I32), (i + 1).astype(I32)
+        a, q, k, v = prompt_case(hip, rng, n, 0, heads, 1, 64, spans, 0.0, np.full(heads, slope, F32))
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_tree_largest_slopes(ctx, rng, n):
+    with ref.Hip() as hip:
+        t = Tree(hip, rng, [0, 0], None, n, 2, 1, 64, np.full((2, n), -1, I32))  # every token sees itself alone
+        t.a.slopes = hip.up(np.full(2, 3e38, F32))
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
+
+
+@pytest.mark.parametrize("cap", [2.0 ** -126, 2.0 ** 126])
+@pytest.mark.parametrize("n,heads", [(1, 2), (20, 2), (840, 16)], ids=["few", "tiles", "images"])
+def test_prompt_caps_at_the_ends(ctx, rng, n, heads, cap):
+    """The least cap makes all scores alike, the largest leaves them as they are."""
+    with ref.Hip() as hip:
+        a, q, k, v = prompt_case(hip, rng, n, 60, heads, 1, 64, None, cap)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, None)
