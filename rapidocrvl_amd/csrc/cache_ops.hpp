@@ -30,6 +30,14 @@ struct CacheAttn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// |a - b| of any two positions, up to 2^32: one instruction in the order of the
+// unsigned (selects for it: 64 biased tokens' weights of 8,256 rows 22.9 us for 22.3)
+__device__ __forceinline__ float distance(int a, int b) {
+    uint32_t d;
+    asm("v_sad_u32 %0, %1, %2, 0" : "=v"(d) : "v"((uint32_t)a ^ 0x80000000u), "v"((uint32_t)b ^ 0x80000000u));
+    return (float)d;
+}
+
 // slope[h] to the base 2; the largest ones stay finite, so that distance 0 costs nothing
 __device__ __forceinline__ float slope_of(const CacheAttn &p, int h) {
     const float x = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
@@ -798,7 +806,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
                     if (e == 4) __builtin_amdgcn_sched_barrier(0);  // not all eight loads at once: registers
                     const int key = k0 + 4 * kg + in;
                     const int at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
-                    dist = (float)(int)((uint32_t)row_pos[u] - (uint32_t)at);
+                    dist = distance(row_pos[u], at);
                 }
                 x[e] = fmaf(-slope[u], fabsf(dist), x[e]);
             }
@@ -1111,7 +1119,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
                 const int key = k0 + 4 * kg + i;
                 int at = key;
                 if (TREE) at = pos ? pos[min(key, last)] : (key < len ? key : len + s_depth[min(key - len, 63)]);
-                x[i] = fmaf(x[i], cap2, -slope * fabsf((float)(int)((uint32_t)row_pos - (uint32_t)at)));
+                x[i] = fmaf(x[i], cap2, -slope * distance(row_pos, at));
             }
         }
 #pragma unroll
@@ -1455,7 +1463,7 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            y[i] = fmaf(y[i], cap2, -in.slope[local] * fabsf((float)(int)((uint32_t)in.pos[local] - (uint32_t)kpos[kt][i]))) - lse;
+                            y[i] = fmaf(y[i], cap2, -in.slope[local] * distance(in.pos[local], kpos[kt][i])) - lse;
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) y[i] = fmaf(sc[t][kt][i], kf[kt][i] * qf, -lse);

@@ -130,3 +130,17 @@ def test_prompt_caps_at_the_ends(ctx, rng, n, heads, cap):
         a, q, k, v = prompt_case(hip, rng, n, 60, heads, 1, 64, None, cap)
         ctx.prompt_attention(a)
         check_prompt(hip, a, q, k, v, None)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_tree_positions_of_the_whole_range(ctx, rng, n):
+    """Positions further apart than 2^31."""
+    def positions(s, kvh, side):
+        return rng.integers(-2 ** 31, 2 ** 31, (s, kvh, side)).astype(I32)
+
+    with ref.Hip() as hip:
+        t = Tree(hip, rng, [90, 33], None, n, 4, 2, 64, slopes=np.array([1e-9, 2e-9, 4e-10, 1e-9], F32), positions=positions)
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
