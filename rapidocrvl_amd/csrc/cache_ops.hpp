@@ -1053,7 +1053,13 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
         row_hi = p.end ? min(max(p.end[row_tok], 0), p.rows) : p.rows0 + row_tok + 1;
         row_pos = p.rows0 + row_tok;
     }
-    const float scale = SHAPED ? p.scale : p.scale * kLog2e;
+    // the scale's power of two goes into the query rows (no bit changes): a score
+    // that fp32 holds has products that it holds
+    const uint32_t scale_bits = __float_as_uint(p.scale);
+    const float power = __uint_as_float(scale_bits & 0x7f800000u), rest = __uint_as_float((scale_bits & 0x7fffffu) | 0x3f800000u);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) q[c] *= power;
+    const float scale = SHAPED ? rest : rest * kLog2e;
     const float inv_cap = SHAPED && p.cap > 0.0f ? 1.0f / p.cap : 0.0f, cap2 = SHAPED && p.cap > 0.0f ? p.cap * kLog2e : kLog2e;
     const int32_t *pos = TREE && SHAPED && p.pos ? p.pos + slot * p.side : nullptr;
 

@@ -144,3 +144,16 @@ def test_tree_positions_of_the_whole_range(ctx, rng, n):
         t.check()
         ctx.cache_weights(t.a)
         t.check_weights()
+
+
+@pytest.mark.parametrize("up,down", [(64, 63), (100, 27), (27, 100)])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("n", [1, 20])
+def test_prompt_products_that_need_their_scale(ctx, rng, n, cap, up, down):
+    """q·k passes fp32's range where scale·q·k does not."""
+    with ref.Hip() as hip:
+        q = (rng.standard_normal((n, 128)) * 2.0 ** up).astype(F32)
+        k = (rng.standard_normal((n + 50, 64)) * 2.0 ** down).astype(F32)
+        a, q, k, v = prompt_case(hip, rng, n, 50, 2, 1, 64, None, cap, scale=2.0 ** -126, q=q, k=k)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, None)
