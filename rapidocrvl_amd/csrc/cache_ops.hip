@@ -2,6 +2,7 @@
 // checks, launch shapes, and the device and stream they run on.
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "cache_ops.hpp"
 #include "internal.hpp"
@@ -46,7 +47,10 @@ struct DeviceScope {
 int check_stream(const pocr_ctx *ctx, hipStream_t s, const char *op) {
     if (!s) return POCR_OK;
     hipDevice_t dev = 0;
-    if (hipStreamGetDevice(s, &dev) != hipSuccess) return fail(POCR_ERR_ARG, "%s: not a stream of the HIP runtime that this library runs on", op);
+    if (hipStreamGetDevice(s, &dev) != hipSuccess) {
+        (void)hipGetLastError();  // answered here: no later check finds it
+        return fail(POCR_ERR_ARG, "%s: not a stream of the HIP runtime that this library runs on", op);
+    }
     if (dev != ctx->device) return fail(POCR_ERR_ARG, "%s: a stream of device %d, the context is on %d", op, dev, ctx->device);
     return POCR_OK;
 }
@@ -57,6 +61,16 @@ int check_stream(const pocr_ctx *ctx, hipStream_t s, const char *op) {
     DeviceScope scope_;                                        \
     RC(scope_.enter((ctx)->device));                           \
     RC(check_stream(ctx, (hipStream_t)(stream), op))
+
+// Queues a kernel and answers for that alone: the thread's last error may be
+// anyone's, an application's handled one or another call's.
+template <class... P, class... A>
+int launch(hipStream_t s, dim3 grid, int threads, void (*kernel)(P...), A... args) {
+    static_assert((std::is_same_v<P, A> && ...), "arguments are passed by address");
+    void *at[] = {&args...};
+    HIP_TRY(hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(threads), at, 0, s));
+    return POCR_OK;
+}
 
 bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -239,26 +253,23 @@ AttnPlan attn_plan(const AttnShape &sh, void *work, int head_dim) {
 
 template <int HD, int kRows, int kSub>
 int launch_join(hipStream_t s, const CacheAttn &p, const AttnPlan &pl, int seqs) {
-    if (pl.part)
-        hipLaunchKernelGGL((k_cache_attn_join<HD, kRows, kSub>), dim3(pl.tiles * (kRows * kSub / (1024 / HD)), p.kvh, seqs), dim3(256), 0, s, p, pl);
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    if (!pl.part) return POCR_OK;
+    return launch(s, dim3(pl.tiles * (kRows * kSub / (1024 / HD)), p.kvh, seqs), 256, k_cache_attn_join<HD, kRows, kSub>, p, pl);
 }
 
 template <int HD, bool TREE, bool SHAPED>
 int launch_few(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     const AttnPlan pl = attn_plan(sh, work, HD);
-    hipLaunchKernelGGL((k_cache_attn_few<HD, TREE, SHAPED>), dim3(sh.splits, p.kvh, seqs), dim3(64 * kFewWaves), 0, s, p, pl);
+    RC(launch(s, dim3(sh.splits, p.kvh, seqs), 64 * kFewWaves, k_cache_attn_few<HD, TREE, SHAPED>, p, pl));
     return launch_join<HD, 16, 4>(s, p, pl, seqs);
 }
 
 template <int HD, bool TREE, bool SHAPED, bool IMG>
 int launch_attn_t(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *work, int seqs) {
     const AttnPlan pl = attn_plan(sh, work, HD);
-    if (IMG)
-        hipLaunchKernelGGL(k_cache_images<HD>, dim3(sh.steps + 1, p.kvh), dim3(kAttnThreads), 0, s, p, pl, const_cast<uint8_t *>(pl.img));
+    if (IMG) RC(launch(s, dim3(sh.steps + 1, p.kvh), kAttnThreads, k_cache_images<HD>, p, pl, const_cast<uint8_t *>(pl.img)));
     const int x = IMG ? sh.jobs : sh.tiles * sh.splits;
-    hipLaunchKernelGGL((k_cache_attn<HD, TREE, SHAPED, IMG>), dim3(x, p.kvh, seqs), dim3(IMG ? 256 : 768), 0, s, p, pl);
+    RC(launch(s, dim3(x, p.kvh, seqs), IMG ? 256 : 768, k_cache_attn<HD, TREE, SHAPED, IMG>, p, pl));
     return launch_join<HD, 128, 1>(s, p, pl, seqs);
 }
 
@@ -273,19 +284,17 @@ int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
 template <int HD, bool SHAPED>
 int launch_weights(hipStream_t s, const CacheAttn &p, int seqs) {
     const int64_t groups = (int64_t)p.kvh * seqs;
-    auto launch = [&](auto kernel, int keys, int threads) {
-        hipLaunchKernelGGL(kernel, dim3(round_up_div(p.rows, keys), p.kvh, seqs), dim3(threads), 0, s, p);
+    auto run = [&](auto kernel, int keys, int threads) {
+        return launch(s, dim3(round_up_div(p.rows, keys), p.kvh, seqs), threads, kernel, p);
     };
     // A workgroup lays all query rows out by itself and takes about as long for
     // 32, 64 or 96 keys (512 query rows: 15, 17, 19 us), so one round on 256 CUs
     // is what counts: 64 tokens of 16 heads over 8,256 rows took 35 us as 516
     // workgroups of 32 keys, 33 as 258 of 64, 21 as 172 of 96; over 4,064 rows 16, 18, 19.
-    if (p.n * p.group <= kWRows) launch(k_cache_weights<HD, SHAPED, 0>, 64, 256);
-    else if (round_up_div(p.rows, 32) * groups <= 256) launch(k_cache_weights<HD, SHAPED, 1>, 32, 512);
-    else if (round_up_div(p.rows, 64) * groups <= 256) launch(k_cache_weights<HD, SHAPED, 2>, 64, 512);
-    else launch(k_cache_weights<HD, SHAPED, 3>, 96, 512);
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    if (p.n * p.group <= kWRows) return run(k_cache_weights<HD, SHAPED, 0>, 64, 256);
+    if (round_up_div(p.rows, 32) * groups <= 256) return run(k_cache_weights<HD, SHAPED, 1>, 32, 512);
+    if (round_up_div(p.rows, 64) * groups <= 256) return run(k_cache_weights<HD, SHAPED, 2>, 64, 512);
+    return run(k_cache_weights<HD, SHAPED, 3>, 96, 512);
 }
 
 template <bool TREE>
@@ -432,11 +441,9 @@ extern "C" int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *a, void 
     // rows per thread: the fewest that hold the cache in registers (1,609 rows: 2)
     const dim3 grid(a->kv_heads, a->caches);
     hipStream_t s = (hipStream_t)stream;
-    if (a->max_rows <= 2 * kSelThreads) hipLaunchKernelGGL(k_cache_select<2>, grid, dim3(kSelThreads), 0, s, p);
-    else if (a->max_rows <= 8 * kSelThreads) hipLaunchKernelGGL(k_cache_select<8>, grid, dim3(kSelThreads), 0, s, p);
-    else hipLaunchKernelGGL(k_cache_select<16>, grid, dim3(kSelThreads), 0, s, p);
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    if (a->max_rows <= 2 * kSelThreads) return launch(s, grid, kSelThreads, k_cache_select<2>, p);
+    if (a->max_rows <= 8 * kSelThreads) return launch(s, grid, kSelThreads, k_cache_select<8>, p);
+    return launch(s, grid, kSelThreads, k_cache_select<16>, p);
 }
 
 extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *stream) {
@@ -515,23 +522,13 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
     p.max_rows = a->max_rows;
     p.max_rows_out = a->max_rows_out;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 threads(kKeepThreads);
     const int side = a->weights || a->positions ? 1 : 0;
     if (inplace && a->max_keep > kKeepRows) {
         const dim3 grid(2 * a->head_dim / kKeepSlab + side, a->kv_heads, a->caches);
-        if (a->head_dim == 128) hipLaunchKernelGGL(k_cache_keep_slabs<128>, grid, threads, 0, s, p);
-        else hipLaunchKernelGGL(k_cache_keep_slabs<64>, grid, threads, 0, s, p);
-    } else {
-        const int chunks = (a->max_keep + kKeepRows - 1) / kKeepRows;
-        const dim3 grid((2 + side) * chunks, a->kv_heads, a->caches);
-        if (a->head_dim == 128) {
-            if (inplace) hipLaunchKernelGGL((k_cache_keep<128, true>), grid, threads, 0, s, p, chunks);
-            else hipLaunchKernelGGL((k_cache_keep<128, false>), grid, threads, 0, s, p, chunks);
-        } else {
-            if (inplace) hipLaunchKernelGGL((k_cache_keep<64, true>), grid, threads, 0, s, p, chunks);
-            else hipLaunchKernelGGL((k_cache_keep<64, false>), grid, threads, 0, s, p, chunks);
-        }
+        return launch(s, grid, kKeepThreads, a->head_dim == 128 ? k_cache_keep_slabs<128> : k_cache_keep_slabs<64>, p);
     }
-    HIP_TRY(hipGetLastError());
-    return POCR_OK;
+    const int chunks = (a->max_keep + kKeepRows - 1) / kKeepRows;
+    const dim3 grid((2 + side) * chunks, a->kv_heads, a->caches);
+    if (a->head_dim == 128) return launch(s, grid, kKeepThreads, inplace ? k_cache_keep<128, true> : k_cache_keep<128, false>, p, chunks);
+    return launch(s, grid, kKeepThreads, inplace ? k_cache_keep<64, true> : k_cache_keep<64, false>, p, chunks);
 }

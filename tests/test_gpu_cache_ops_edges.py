@@ -1,9 +1,13 @@
 """The cache operators at the ends of the ranges that their header states.
 Definitions and bounds: cache_ops_f64.py."""
+import ctypes as C
+
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, Tree, alibi, check_prompt, prompt_case, visible
+from test_gpu_cache_ops import F32, I32, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, visible
+
+from rapidocrvl_amd import lib
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +161,40 @@ def test_prompt_products_that_need_their_scale(ctx, rng, n, cap, up, down):
         a, q, k, v = prompt_case(hip, rng, n, 50, 2, 1, 64, None, cap, scale=2.0 ** -126, q=q, k=k)
         ctx.prompt_attention(a)
         check_prompt(hip, a, q, k, v, None)
+
+
+def all_calls(ctx, hip, rng):
+    """One small call of each operator and of each of its forms, with its check."""
+    t, big = Tree(hip, rng, [70], None, 2, 4, 2, 64), Tree(hip, rng, [500], None, 20, 4, 2, 64)
+    a, q, k, v = prompt_case(hip, rng, 840, 0, 16, 1, 64, None)
+    w = rng.random((2, 2, 100)).astype(F32)
+    sel = lib.SelectArgs(weights=hip.up(w), lens=hip.up(np.array([100, 60], I32)), kept=hip.up(np.full((2, 2, 50), -9, I32)),
+                         counts=hip.up(np.zeros(2, I32)), caches=2, kv_heads=2, max_rows=100, budget=50, sinks=1, recent=7)
+    kp = Keep(rng, 2, 200, 2, 64)
+    lists = ascending(rng, (2, 2), 100, 200)
+    keep = kp.args(hip, lists, [100, 40], None, rows_out=120)
+    return [(ctx.tree_attention, t.a, t.check), (ctx.cache_weights, t.a, t.check_weights),
+            (ctx.tree_attention, big.a, big.check), (ctx.cache_weights, big.a, big.check_weights),
+            (ctx.prompt_attention, a, lambda: check_prompt(hip, a, q, k, v, None, rows=np.arange(0, 840, 41))),
+            (ctx.cache_select, sel, lambda: check_select(hip, sel, w, [100, 60])),
+            (ctx.cache_keep, keep, lambda: kp.check(hip, keep, lists, [100, 40], None))]
+
+
+def test_errors_of_others_are_theirs(ctx, rng):
+    """A call that follows an error of the application's own, or one that these
+    calls answered themselves (a stream they do not know), succeeds and says so."""
+    with ref.Hip() as hip:
+        calls = all_calls(ctx, hip, rng)
+        hip.sync()
+        no_stream = C.create_string_buffer(4096)  # an address that no stream has
+        for call, args, check in calls:
+            assert hip.rt.hipSetDevice(4711) != 0  # handled, and left behind as the thread's last error
+            call(args)
+            check()
+            with pytest.raises(lib.PocrError) as e:
+                call(args, C.addressof(no_stream))
+            assert e.value.code == lib.POCR_ERR_ARG
+        for call, args, check in all_calls(ctx, hip, rng):
+            call(args)
+            check()
+        hip.rt.hipGetLastError()
