@@ -12,6 +12,7 @@ using namespace pocr;
 namespace {
 
 constexpr int kMaxGridYZ = 65535;
+constexpr int64_t kMaxGrid = 0xffffffff;  // threads along x
 constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kMaxPromptRows = 1 << 22;
 constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
@@ -527,8 +528,14 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
         const dim3 grid(2 * a->head_dim / kKeepSlab + side, a->kv_heads, a->caches);
         return launch(s, grid, kKeepThreads, a->head_dim == 128 ? k_cache_keep_slabs<128> : k_cache_keep_slabs<64>, p);
     }
-    const int chunks = (a->max_keep + kKeepRows - 1) / kKeepRows;
-    const dim3 grid((2 + side) * chunks, a->kv_heads, a->caches);
-    if (a->head_dim == 128) return launch(s, grid, kKeepThreads, inplace ? k_cache_keep<128, true> : k_cache_keep<128, false>, p, chunks);
-    return launch(s, grid, kKeepThreads, inplace ? k_cache_keep<64, true> : k_cache_keep<64, false>, p, chunks);
+    // no list is longer than its destination; lists of more workgroups than a grid holds take several
+    const int chunks = round_up_div(std::min(a->max_keep, a->max_rows_out), kKeepRows), most = kMaxGrid / ((2 + side) * kKeepThreads);
+    auto run = [&](auto kernel) {
+        for (int at = 0; at < chunks; at += most)
+            RC(launch(s, dim3((2 + side) * std::min(most, chunks - at), a->kv_heads, a->caches), kKeepThreads, kernel, p, at,
+                      std::min(most, chunks - at), chunks));
+        return (int)POCR_OK;
+    };
+    if (a->head_dim == 128) return run(inplace ? k_cache_keep<128, true> : k_cache_keep<128, false>);
+    return run(inplace ? k_cache_keep<64, true> : k_cache_keep<64, false>);
 }

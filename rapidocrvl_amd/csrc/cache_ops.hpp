@@ -1703,15 +1703,17 @@ __device__ __forceinline__ int keep_source(const CacheKeep &p, int listed, int f
 }
 
 // weights and positions of list entries from, from + step, ... chunks of 256
+// (their numbers pass 31 bits behind the longest lists)
 template <bool INPLACE>
 __device__ __forceinline__ void keep_side(const CacheKeep &p, const KeepRange &r, int c, int g, int from, int step) {
     const size_t in = ((size_t)c * p.kvh + g) * p.side, out = ((size_t)c * p.kvh + g) * p.side_out + r.first;
-    for (int b = from * kKeepThreads; b < r.count; b += step * kKeepThreads) {
-        const int i = b + threadIdx.x;
+    const int64_t stride = (int64_t)step * kKeepThreads;
+    for (int64_t b = (int64_t)from * kKeepThreads; b < r.count; b += stride) {
+        const int64_t i = b + threadIdx.x;
         float w = 0.0f;
         int32_t at = 0;
         if (i < r.count) {
-            const int j = keep_source<INPLACE>(p, r.rows[i], r.first, i);
+            const int j = keep_source<INPLACE>(p, r.rows[i], r.first, (int)i);
             if (p.weights) w = p.weights[in + j];
             if (p.pos) at = p.pos[in + j];
         }
@@ -1723,26 +1725,27 @@ __device__ __forceinline__ void keep_side(const CacheKeep &p, const KeepRange &r
     }
     if (INPLACE) __syncthreads();
     if (p.weights)
-        for (int i = r.count + from * kKeepThreads + threadIdx.x; r.first + i < p.max_rows_out; i += step * kKeepThreads)
+        for (int64_t i = r.count + (int64_t)from * kKeepThreads + threadIdx.x; r.first + i < p.max_rows_out; i += stride)
             p.weights_out[out + i] = 0.0f;
 }
 
 // Workgroup: 64 listed rows of K or V of one KV head and cache (x even, odd),
 // HD / 4 lanes a row, all loads before the first store; or (the last x's) their
 // weights and positions.  In place for lists of at most 64 rows, which one
-// workgroup holds whole.  2,048 rows of 18 caches with two KV heads into others:
+// workgroup holds whole.  A grid has `chunks` of a list's all_chunks, from chunk0
+// on.  2,048 rows of 18 caches with two KV heads into others:
 // 151 MB read and written in 35.7 us, 4.2 TB/s of a large copy's 4.8; 768 rows,
 // 57 MB, in 11.6 us, 4.9 TB/s.
 template <int HD, bool INPLACE>
-__global__ void __launch_bounds__(kKeepThreads) k_cache_keep(CacheKeep p, int chunks) {
+__global__ void __launch_bounds__(kKeepThreads) k_cache_keep(CacheKeep p, int chunk0, int chunks, int all_chunks) {
     constexpr int kLanes = HD / 4, kStep = kKeepThreads / kLanes, kUnroll = kKeepRows / kStep;
     const int g = blockIdx.y, c = blockIdx.z, tid = threadIdx.x, x = blockIdx.x;
     const KeepRange r = keep_range(p, c, g);
     if (x >= 2 * chunks) {
-        keep_side<INPLACE>(p, r, c, g, x - 2 * chunks, chunks);
+        keep_side<INPLACE>(p, r, c, g, chunk0 + x - 2 * chunks, all_chunks);
         return;
     }
-    const int which = x & 1, i0 = (x >> 1) * kKeepRows + tid / kLanes;
+    const int which = x & 1, i0 = (chunk0 + (x >> 1)) * kKeepRows + tid / kLanes;
     int j[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) j[u] = r.rows[min(i0 + u * kStep, p.max_keep - 1)];

@@ -5,7 +5,7 @@ import ctypes as C
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, visible
+from test_gpu_cache_ops import F32, I32, SENTINEL, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, visible
 
 from rapidocrvl_amd import lib
 
@@ -198,3 +198,43 @@ def test_errors_of_others_are_theirs(ctx, rng):
             call(args)
             check()
         hip.rt.hipGetLastError()
+
+
+@pytest.mark.parametrize("rows_out,first,side", [(1000, 3, False), (1000, 985, True), (360_000_000, 359_999_990, True)],
+                         ids=["short", "short-weights", "long-weights"])
+def test_keep_longest_lists(ctx, rng, rows_out, first, side):
+    """Lists as long as the header allows, few of whose entries are in use; destinations
+    whose workgroups pass 2^32 threads and whose weights' tail passes 31 bits with its steps."""
+    with ref.Hip() as hip:
+        free, total = C.c_size_t(), C.c_size_t()
+        assert hip.rt.hipMemGetInfo(C.byref(free), C.byref(total)) == 0
+        if free.value < (200 << 30) and rows_out > 1000:
+            pytest.skip("needs 200 GiB of device memory")
+        count = min(20, rows_out - first)
+        src = rng.standard_normal((2, 40, 64)).astype(F32)
+        w = rng.random(40).astype(F32)
+        pick = np.sort(rng.choice(40, 20, replace=False)).astype(I32)
+        a = lib.KeepArgs(k=hip.up(src[0]), v=hip.up(src[1]), k_out=hip.raw(256 * rows_out), v_out=hip.raw(256 * rows_out),
+                         rows=hip.raw(4 << 30), counts=hip.up(np.array([20], I32)), first=hip.up(np.array([first], I32)),
+                         caches=1, kv_heads=1, head_dim=64, max_keep=2 ** 30, max_rows=40, max_rows_out=rows_out,
+                         k_stride=64, v_stride=64, k_out_stride=64, v_out_stride=64)
+        hip.write(a.rows, pick)
+        at = max(0, first - 5)  # a window of the destination around the moved rows
+        size = min(first + count + 5, rows_out) - at
+        for p in (a.k_out, a.v_out):
+            hip.write(p + 256 * at, np.full((size, 64), SENTINEL, F32))
+        tails = {at, rows_out // 3, rows_out - 900} & set(range(rows_out - 899))
+        if side:
+            a.weights, a.weights_out = hip.up(w), hip.raw(4 * rows_out)
+            for t in tails:
+                hip.write(a.weights_out + 4 * t, np.full(900, SENTINEL, F32))
+        ctx.cache_keep(a)
+        for x, p in enumerate((a.k_out, a.v_out)):
+            want = np.full((size, 64), SENTINEL, F32)
+            want[first - at:first - at + count] = src[x, pick[:count]]
+            assert np.array_equal(hip.down(p + 256 * at, (size, 64)), want)
+        for t in tails if side else ():
+            i = t + np.arange(900)
+            moved = w[pick[np.clip(i - first, 0, count - 1)]]
+            want = np.where(i < first, SENTINEL, np.where(i < first + count, moved, F32(0.0)))
+            assert np.array_equal(hip.down(a.weights_out + 4 * t, 900), want), t
