@@ -283,10 +283,15 @@ int launch_attn_s(hipStream_t s, const CacheAttn &p, const AttnShape &sh, void *
 }
 
 template <int HD, bool SHAPED>
-int launch_weights(hipStream_t s, const CacheAttn &p, int seqs) {
+int launch_weights(hipStream_t s, CacheAttn p, int seqs) {
     const int64_t groups = (int64_t)p.kvh * seqs;
     auto run = [&](auto kernel, int keys, int threads) {
-        return launch(s, dim3(round_up_div(p.rows, keys), p.kvh, seqs), threads, kernel, p);
+        const int blocks = round_up_div(p.rows, keys), most = kMaxGrid / threads;  // max_rows is a bound, lengths are on the device
+        for (int at = 0; at < blocks; at += most) {
+            p.key0 = at * keys;
+            RC(launch(s, dim3(std::min(most, blocks - at), p.kvh, seqs), threads, kernel, p));
+        }
+        return (int)POCR_OK;
     };
     // A workgroup lays all query rows out by itself and takes about as long for
     // 32, 64 or 96 keys (512 query rows: 15, 17, 19 us), so one round on 256 CUs

@@ -25,6 +25,7 @@ struct CacheAttn {
     const uint64_t *take;
     int64_t q_ss, q_st, k_ss, k_st, v_ss, v_st, o_ss, o_st, side;
     int n, rows0, rows, heads, kvh, group;     // rows: prompt rows0 + n, tree max_rows
+    int key0;                                  // weights: first key of the grid
     float scale, cap, inv_group;
 };
 
@@ -1297,7 +1298,7 @@ __global__ void __launch_bounds__(MANY ? 512 : 256, 2) k_cache_weights(CacheAttn
     __shared__ __attribute__((aligned(16))) WeightRows<HD> steps[MANY ? 2 : 1];
     __shared__ float s_sum[kKeys];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
-    const int g = blockIdx.y, s = blockIdx.z, key0 = blockIdx.x * kKeys;
+    const int g = blockIdx.y, s = blockIdx.z, key0 = p.key0 + blockIdx.x * kKeys;
     const SeqRows q = seq_rows(p, s);
     const int end = q.len + q.count, rows = q.count * p.group;
     if (key0 >= end || q.count == 0) return;

@@ -238,3 +238,18 @@ def test_keep_longest_lists(ctx, rng, rows_out, first, side):
             moved = w[pick[np.clip(i - first, 0, count - 1)]]
             want = np.where(i < first, SENTINEL, np.where(i < first + count, moved, F32(0.0)))
             assert np.array_equal(hip.down(a.weights_out + 4 * t, 900), want), t
+
+
+@pytest.mark.parametrize("n,heads", [(1, 2), (16, 2), (20, 16)], ids=["one", "few", "many"])
+def test_tree_of_the_largest_bound(ctx, rng, n, heads):
+    """max_rows is a bound: lengths far below it, workgroups past 2^32 threads."""
+    with ref.Hip() as hip:
+        t = Tree(hip, rng, [300], None, n, heads, 1, 64)
+        t.a.max_rows, t.a.weights = 2 ** 30, hip.raw(4 << 30)
+        hip.write(t.a.weights, t.weights)
+        t.a.workspace_bytes = lib.tree_attention_workspace(t.a)
+        t.a.workspace = hip.raw(t.a.workspace_bytes)
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
