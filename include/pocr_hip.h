@@ -328,7 +328,7 @@ typedef struct {
     void *workspace;          /* pocr_prompt_attention_workspace bytes, 16-byte aligned */
     int64_t workspace_bytes;
     int64_t q_stride, k_stride, v_stride, out_stride;
-    int32_t n;                /* 1 .. 2^22 rows, n * (heads / kv_heads) <= 2^30 */
+    int32_t n;                /* 1 .. 2^22 rows, n * (heads / kv_heads) <= 2^29 */
     int32_t rows_before;      /* rows_before + n <= 2^30 */
     int32_t heads, kv_heads, head_dim;
     float scale;              /* 2^-126 to 2^126; 0: 1 / sqrt(head_dim) */

@@ -15,6 +15,7 @@ constexpr int kMaxGridYZ = 65535;
 constexpr int64_t kMaxGrid = 0xffffffff;  // threads along x
 constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kMaxPromptRows = 1 << 22;
+constexpr int kMaxQueryRows = 1 << 29;  // of a KV head: 2^22 tiles, 768 threads each
 constexpr int kMaxTreeTokens = 64;  // a token's ancestors are the bits of one 64-bit word
 constexpr int kMaxQueryHeads = 1024;
 constexpr float kLeast = FLT_MIN, kMost = 0x1p126f;  // of scale and cap
@@ -117,7 +118,7 @@ int prompt_shape(const pocr_prompt_args *a, const char *op) {
     if (!a) return fail(POCR_ERR_ARG, "%s: null arguments", op);
     RC(check_heads(a->heads, a->kv_heads, a->head_dim, op));
     RC(check_scores(a->scale, a->cap, op));
-    if (a->n < 1 || a->n > kMaxPromptRows || (int64_t)a->n * (a->heads / a->kv_heads) > kMaxCacheRows)
+    if (a->n < 1 || a->n > kMaxPromptRows || (int64_t)a->n * (a->heads / a->kv_heads) > kMaxQueryRows)
         return fail(POCR_ERR_ARG, "%s: %d rows of %d heads", op, a->n, a->heads);
     if (a->rows_before < 0 || a->rows_before > kMaxCacheRows - a->n) return fail(POCR_ERR_ARG, "%s: %d rows before", op, a->rows_before);
     return POCR_OK;

@@ -16,3 +16,10 @@ def test_scores_out_of_range(call, kw, text):
 @pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** 126])
 def test_scores_at_the_ends(call, size):
     refused(call, ARG, "null context", cap=size, scale=size)
+
+
+def test_prompt_query_rows():
+    """2^29 query rows of a KV head are 2^22 tiles of 768 threads; twice as many pass a grid."""
+    wide = dict(q_stride=1 << 18, out_stride=1 << 18, kv_heads=1, k_stride=128, v_stride=128, n=1 << 22)
+    refused("prompt", ARG, "rows", heads=256, **wide)
+    refused("prompt", ARG, "null context", heads=128, **wide)
