@@ -406,7 +406,9 @@ int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *args, void *stream)
  * strides) each list must ascend with rows[i] >= first + i, as
  * pocr_cache_select's lists and the path of accepted tokens behind first =
  * lens do; a list that does not leaves unspecified rows.  Otherwise a
- * destination may not overlap its source (POCR_ERR_ARG). */
+ * destination may not overlap its source (POCR_ERR_ARG): rows of both that
+ * alternate in one pool do not where their strides are equal; where they
+ * differ, the whole ranges count. */
 typedef struct {
     const float *k, *v;       /* cache c, row j, KV head g: k + c*k_cache_stride + j*k_stride + g*head_dim */
     const float *weights;     /* [caches][kv_heads][side_stride], or null */

@@ -323,13 +323,48 @@ AttnShape tree_attn(const pocr_tree_args *a) {
     return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), a->max_rows, (int64_t)a->kv_heads * a->seqs, a->head_dim, false);
 }
 
-// the addresses of `caches` blocks of `rows` rows overlap
-bool overlap(const void *a, int64_t acs, int64_t ast, int arows, int64_t awidth, const void *b, int64_t bcs, int64_t bst,
-             int brows, int64_t bwidth, int caches) {
-    const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
-    const char *a1 = a0 + 4 * ((caches - 1) * acs + (arows - 1) * ast + awidth);
-    const char *b1 = b0 + 4 * ((caches - 1) * bcs + (brows - 1) * bst + bwidth);
-    return a0 < b1 && b0 < a1;
+// Memory of one buffer: `blocks` blocks of `rows` rows of `width` floats.
+struct Area {
+    const void *at;
+    int64_t outer, inner;  // floats from block to block and from row to row
+    int64_t blocks, rows, width;
+    int64_t block() const { return (rows - 1) * inner + width; }
+};
+
+// The numbers k in [least, most] for which a span of `a` floats and one of `b`
+// floats, d - k * step behind its start, share some: [*from, *to] (step > 0).
+bool meeting(int64_t d, int64_t step, int64_t least, int64_t most, int64_t a, int64_t b, int64_t *from, int64_t *to) {
+    auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    *from = std::max(least, floor_div(d - a, step) + 1);  // d - k * step < a
+    *to = std::min(most, -floor_div(-d - b, step) - 1);   // d - k * step > -b
+    return *from <= *to;
+}
+
+// Rows of a block of x and of one of y, d floats behind it, share memory.
+// Rows of two strides count as meeting where their blocks do.
+bool rows_meet(const Area &x, const Area &y, int64_t d) {
+    if (d >= x.block() || d <= -y.block()) return false;
+    if (x.rows > 1 && y.rows > 1 && x.inner != y.inner) return true;
+    const int64_t step = x.rows > 1 ? x.inner : (y.rows > 1 ? y.inner : 1);
+    int64_t from, to;
+    return x.rows == 1 && y.rows == 1 ? true : meeting(d, step, 1 - y.rows, x.rows - 1, x.width, y.width, &from, &to);
+}
+
+// x and y share memory (other: of two different blocks, x and y being one
+// buffer).  Interleaved blocks and rows do not meet, as where several caches lie
+// in one pool; blocks of two strides count as meeting where their ranges do.
+bool overlap(const Area &x, const Area &y, bool other = false) {
+    const int64_t bytes = (int64_t)(reinterpret_cast<uintptr_t>(y.at) - reinterpret_cast<uintptr_t>(x.at));
+    const int64_t d = bytes / 4 - (bytes % 4 < 0);  // addresses are multiples of 4
+    if (d >= (x.blocks - 1) * x.outer + x.block() || d <= -((y.blocks - 1) * y.outer + y.block())) return false;
+    if (x.blocks > 1 && y.blocks > 1 && x.outer != y.outer) return true;
+    if (x.blocks == 1 && y.blocks == 1) return !other && rows_meet(x, y, d);
+    const int64_t step = x.blocks > 1 ? x.outer : y.outer;
+    int64_t from, to;
+    if (!meeting(d, step, 1 - y.blocks, x.blocks - 1, x.block(), y.block(), &from, &to)) return false;
+    for (int64_t k = from; k <= to; ++k)
+        if (!(other && k == 0) && rows_meet(x, y, d - k * step)) return true;
+    return false;
 }
 
 }  // namespace
@@ -491,16 +526,14 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
             a->max_rows != a->max_rows_out || ((a->weights || a->positions) && p.side != p.side_out))
             return fail(POCR_ERR_ARG, "%s: in place, the strides and row counts of source and destination are equal", op);
     } else {
-        const int64_t heads = a->kv_heads, in = (heads - 1) * p.side + a->max_rows, out = (heads - 1) * p.side_out + a->max_rows_out;
-        auto rows = [&](const void *x, int64_t xcs, int64_t xst, const void *y, int64_t ycs, int64_t yst) {
-            return overlap(x, xcs, xst, a->max_rows, kvd, y, ycs, yst, a->max_rows_out, kvd, a->caches);
+        const int64_t sides = (int64_t)a->caches * a->kv_heads;
+        const Area k{a->k, a->k_cache_stride, a->k_stride, a->caches, a->max_rows, kvd}, v{a->v, a->v_cache_stride, a->v_stride, a->caches, a->max_rows, kvd},
+            k_out{a->k_out, a->k_out_cache_stride, a->k_out_stride, a->caches, a->max_rows_out, kvd},
+            v_out{a->v_out, a->v_out_cache_stride, a->v_out_stride, a->caches, a->max_rows_out, kvd};
+        auto side = [&](const void *x, const void *y) {
+            return x && overlap({x, 0, p.side, 1, sides, a->max_rows}, {y, 0, p.side_out, 1, sides, a->max_rows_out});
         };
-        auto sides = [&](const void *x, const void *y) {
-            return x && overlap(x, heads * p.side, 0, 1, in, y, heads * p.side_out, 0, 1, out, a->caches);
-        };
-        if (rows(a->k, a->k_cache_stride, a->k_stride, a->k_out, a->k_out_cache_stride, a->k_out_stride) ||
-            rows(a->v, a->v_cache_stride, a->v_stride, a->v_out, a->v_out_cache_stride, a->v_out_stride) ||
-            sides(a->weights, a->weights_out) || sides(a->positions, a->positions_out))
+        if (overlap(k, k_out) || overlap(v, v_out) || side(a->weights, a->weights_out) || side(a->positions, a->positions_out))
             return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
     }
     CACHE_OP_ENTER(ctx, stream, op);

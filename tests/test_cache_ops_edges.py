@@ -1,7 +1,12 @@
 """Refusals of the cache operators at the ends of their ranges, where buffers
 meet, and what their workspace queries look at.  No GPU needed."""
+import ctypes as C
+
+import numpy as np
 import pytest
-from test_cache_ops import ARG, refused
+from test_cache_ops import ARG, keep, refused
+
+from rapidocrvl_amd import lib
 
 
 @pytest.mark.parametrize("call", ["prompt", "tree", "weights"])
@@ -23,3 +28,54 @@ def test_prompt_query_rows():
     wide = dict(q_stride=1 << 18, out_stride=1 << 18, kv_heads=1, k_stride=128, v_stride=128, n=1 << 22)
     refused("prompt", ARG, "rows", heads=256, **wide)
     refused("prompt", ARG, "null context", heads=128, **wide)
+
+
+def memory(at, outer, inner, blocks, rows, width):
+    """The floats of `blocks` blocks of `rows` rows, by address / 4."""
+    return {at + b * outer + r * inner + i for b in range(blocks) for r in range(rows) for i in range(width)}
+
+
+def keep_answer(**kw):
+    L = lib.load()
+    rc = L.pocr_cache_keep(None, C.byref(keep(**kw)), None)
+    assert rc == ARG
+    return L.pocr_last_error().decode()
+
+
+@pytest.mark.parametrize("seed", range(20))
+@pytest.mark.parametrize("alike", [True, False], ids=["one-stride", "two-strides"])
+def test_keep_overlap_of_interleaved_rows(seed, alike):
+    """Source and destination anywhere in one pool: refused where they share memory and, strides being alike, only there."""
+    rng = np.random.default_rng(seed)
+    far = dict(v=1 << 30, v_out=1 << 31, kv_heads=1, head_dim=64, max_keep=3)
+    for _ in range(40):
+        caches, rows, rows_out = (int(x) for x in rng.integers(1, 5, 3))
+        inner = 64 + 4 * int(rng.integers(0, 40))
+        outer = max(4, rows * inner + 4 * int(rng.integers(-40, 200))) if rng.random() < 0.7 else 4 * int(rng.integers(1, 60))
+        inner2, outer2 = (inner, outer) if alike else (64 + 4 * int(rng.integers(0, 40)), 4 * int(rng.integers(1, 300)))
+        src, dst = 1 << 20, (1 << 20) + 4 * int(rng.integers(-500, 500))
+        if src == dst:
+            continue
+        text = keep_answer(k=4 * src, k_out=4 * dst, caches=caches, max_rows=rows, max_rows_out=rows_out, k_cache_stride=outer,
+                           k_stride=inner, k_out_cache_stride=outer2, k_out_stride=inner2, **far)
+        a = memory(src, outer, inner, caches, rows, 64)
+        b = memory(dst, outer2, inner2, caches, rows_out, 64)
+        if a & b:
+            assert "overlaps" in text
+        elif alike or min(a) > max(b) or min(b) > max(a):
+            assert "null context" in text
+
+
+def test_keep_from_slot_to_slot():
+    """A pool [layer][slot][row]: all layers of one slot into the next; then one row further, into the source's last."""
+    slot = 100 * 256
+    pool = {n: 4 * slot for n in ("k_cache_stride", "v_cache_stride", "k_out_cache_stride", "v_out_cache_stride")}
+    for shift, text in ((0, "null context"), (-256, "overlaps")):
+        refused("keep", ARG, text, k=1 << 30, k_out=(1 << 30) + 4 * (slot + shift), v=1 << 34, v_out=(1 << 34) + 8 * slot, **pool)
+
+
+def test_keep_interleaved_side_buffers():
+    """Weights of source and destination row by row in one buffer [cache][KV head][2][100]."""
+    out = dict(k_out=1 << 30, v_out=1 << 31, side_stride=200, side_out_stride=200)
+    refused("keep", ARG, "null context", weights=1 << 20, weights_out=(1 << 20) + 400, **out)
+    refused("keep", ARG, "overlaps", weights=1 << 20, weights_out=(1 << 20) + 396, **out)

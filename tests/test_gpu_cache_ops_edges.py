@@ -253,3 +253,25 @@ def test_tree_of_the_largest_bound(ctx, rng, n, heads):
         t.check()
         ctx.cache_weights(t.a)
         t.check_weights()
+
+
+def test_keep_within_a_pool(ctx, rng):
+    """Caches of all layers from one slot of a pool [layer][slot][K, V][row] into another; the other slots stay."""
+    with ref.Hip() as hip:
+        layers, slots, rows, st = 3, 4, 90, 2 * 64
+        pool = rng.standard_normal((layers, slots, 2, rows, st)).astype(F32)
+        lists = ascending(rng, (layers, 2), 70, rows)
+        base, size = hip.up(pool), 4 * rows * st
+        at = lambda slot, x: base + (2 * slot + x) * size  # noqa: E731
+        a = lib.KeepArgs(k=at(2, 0), v=at(2, 1), k_out=at(1, 0), v_out=at(1, 1), rows=hip.up(lists), counts=hip.up(np.full(layers, 70, I32)),
+                         caches=layers, kv_heads=2, head_dim=64, max_keep=70, per_head=1, max_rows=rows, max_rows_out=rows)
+        for n in ("k", "v", "k_out", "v_out"):
+            setattr(a, n + "_cache_stride", slots * 2 * rows * st)
+            setattr(a, n + "_stride", st)
+        ctx.cache_keep(a)
+        want = pool.copy().reshape(layers, slots, 2, rows, 2, 64)
+        src = want.copy()
+        for c in range(layers):
+            for g in range(2):
+                want[c, 1, :, :70, g] = src[c, 2][:, lists[c, g], g]
+        assert np.array_equal(hip.down(base, want.shape), want)
