@@ -408,7 +408,9 @@ int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *args, void *stream)
  * lens do; a list that does not leaves unspecified rows.  Otherwise a
  * destination may not overlap its source (POCR_ERR_ARG): rows of both that
  * alternate in one pool do not where their strides are equal; where they
- * differ, the whole ranges count. */
+ * differ, the whole ranges count.  Nor may a destination overlap another
+ * destination, another's source or the lists; but one buffer as K and V may go
+ * to one destination as both, elsewhere. */
 typedef struct {
     const float *k, *v;       /* cache c, row j, KV head g: k + c*k_cache_stride + j*k_stride + g*head_dim */
     const float *weights;     /* [caches][kv_heads][side_stride], or null */

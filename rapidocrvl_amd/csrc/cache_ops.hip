@@ -57,12 +57,18 @@ int check_stream(const pocr_ctx *ctx, hipStream_t s, const char *op) {
     return POCR_OK;
 }
 
-#define CACHE_OP_ENTER(ctx, stream, op)                        \
+#define CACHE_OP_CONTEXT(ctx, op)                                  \
     if (!(ctx)) return fail(POCR_ERR_ARG, "%s: null context", op); \
-    CHECK_INJECT((op) + 5); /* the name without pocr_ */       \
-    DeviceScope scope_;                                        \
-    RC(scope_.enter((ctx)->device));                           \
+    CHECK_INJECT((op) + 5) /* the name without pocr_ */
+
+#define CACHE_OP_DEVICE(ctx, stream, op) \
+    DeviceScope scope_;                  \
+    RC(scope_.enter((ctx)->device));     \
     RC(check_stream(ctx, (hipStream_t)(stream), op))
+
+#define CACHE_OP_ENTER(ctx, stream, op) \
+    CACHE_OP_CONTEXT(ctx, op);          \
+    CACHE_OP_DEVICE(ctx, stream, op)
 
 // Queues a kernel and answers for that alone: the thread's last error may be
 // anyone's, an application's handled one or another call's.
@@ -525,18 +531,36 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
             (a->caches > 1 && (a->k_cache_stride != a->k_out_cache_stride || a->v_cache_stride != a->v_out_cache_stride)) ||
             a->max_rows != a->max_rows_out || ((a->weights || a->positions) && p.side != p.side_out))
             return fail(POCR_ERR_ARG, "%s: in place, the strides and row counts of source and destination are equal", op);
-    } else {
-        const int64_t sides = (int64_t)a->caches * a->kv_heads;
-        const Area k{a->k, a->k_cache_stride, a->k_stride, a->caches, a->max_rows, kvd}, v{a->v, a->v_cache_stride, a->v_stride, a->caches, a->max_rows, kvd},
-            k_out{a->k_out, a->k_out_cache_stride, a->k_out_stride, a->caches, a->max_rows_out, kvd},
-            v_out{a->v_out, a->v_out_cache_stride, a->v_out_stride, a->caches, a->max_rows_out, kvd};
-        auto side = [&](const void *x, const void *y) {
-            return x && overlap({x, 0, p.side, 1, sides, a->max_rows}, {y, 0, p.side_out, 1, sides, a->max_rows_out});
-        };
-        if (overlap(k, k_out) || overlap(v, v_out) || side(a->weights, a->weights_out) || side(a->positions, a->positions_out))
-            return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
     }
-    CACHE_OP_ENTER(ctx, stream, op);
+    const int64_t sides = (int64_t)a->caches * a->kv_heads;
+    const Area src[4] = {{a->k, a->k_cache_stride, a->k_stride, a->caches, a->max_rows, kvd},
+                         {a->v, a->v_cache_stride, a->v_stride, a->caches, a->max_rows, kvd},
+                         {a->weights, 0, p.side, 1, sides, a->max_rows},
+                         {a->positions, 0, p.side, 1, sides, a->max_rows}};
+    const Area dst[4] = {{a->k_out, a->k_out_cache_stride, a->k_out_stride, a->caches, a->max_rows_out, kvd},
+                         {a->v_out, a->v_out_cache_stride, a->v_out_stride, a->caches, a->max_rows_out, kvd},
+                         {a->weights_out, 0, p.side_out, 1, sides, a->max_rows_out},
+                         {a->positions_out, 0, p.side_out, 1, sides, a->max_rows_out}};
+    if (!inplace)
+        for (int i = 0; i < 4; ++i)
+            if (dst[i].at && overlap(src[i], dst[i])) return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
+    CACHE_OP_CONTEXT(ctx, op);
+    // What one workgroup writes no other reads, or writes otherwise: one buffer as
+    // K and V goes to one destination elsewhere (the same values twice), not in place.
+    const Area lists[3] = {{a->rows, 0, 0, 1, 1, (a->per_head ? sides : a->caches) * a->max_keep},
+                           {a->counts, 0, 0, 1, 1, a->caches},
+                           {a->first, 0, 0, 1, 1, a->caches}};
+    const char *names[7] = {"K", "V", "weights", "positions", "rows", "counts", "first"};
+    const bool twice = !inplace && a->k == a->v && a->k_out == a->v_out && a->k_stride == a->v_stride && a->k_out_stride == a->v_out_stride &&
+                       (a->caches == 1 || (a->k_cache_stride == a->v_cache_stride && a->k_out_cache_stride == a->v_out_cache_stride));
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; dst[i].at && j < 7; ++j) {
+            const Area &read = j < 4 ? src[j] : lists[j - 4];
+            if (j == i || !read.at || (twice && i + j == 1)) continue;
+            if (overlap(dst[i], read) || (j < i && overlap(dst[i], dst[j])))
+                return fail(POCR_ERR_ARG, "%s: the destination of %s overlaps %s", op, names[i], names[j]);
+        }
+    CACHE_OP_DEVICE(ctx, stream, op);
     p.src[0] = a->k;
     p.src[1] = a->v;
     p.dst[0] = a->k_out;

@@ -79,3 +79,47 @@ def test_keep_interleaved_side_buffers():
     out = dict(k_out=1 << 30, v_out=1 << 31, side_stride=200, side_out_stride=200)
     refused("keep", ARG, "null context", weights=1 << 20, weights_out=(1 << 20) + 400, **out)
     refused("keep", ARG, "overlaps", weights=1 << 20, weights_out=(1 << 20) + 396, **out)
+
+
+# K, V, weights and positions at places of their own, in place and elsewhere, and lists
+APART = dict(k=1 << 30, v=1 << 31, k_out=1 << 30, v_out=1 << 31, rows=1 << 20, counts=1 << 21, first=1 << 22)
+SIDES = dict(weights=1 << 23, weights_out=1 << 23, positions=1 << 24, positions_out=1 << 24)
+ELSEWHERE = dict(k_out=1 << 32, v_out=1 << 33)
+CACHE = 4 << 16  # bytes from cache to cache
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(v=1 << 30, v_out=1 << 30), "destination of K overlaps V"),
+    (dict(v=(1 << 30) + 1024 * 99, v_out=(1 << 30) + 1024 * 99), "destination of K overlaps V"),
+    (dict(v=(1 << 30) + 2 * CACHE, v_out=(1 << 30) + 2 * CACHE), "destination of K overlaps V"),
+    (dict(SIDES, positions=1 << 23, positions_out=1 << 23), "destination of weights overlaps positions"),
+    (dict(SIDES, weights=(1 << 31) + 64, weights_out=(1 << 31) + 64), "destination of V overlaps weights"),
+    (dict(rows=(1 << 30) + 512), "destination of K overlaps rows"),
+    (dict(counts=(1 << 31) + CACHE), "destination of V overlaps counts"),
+    (dict(SIDES, first=(1 << 23) + 4 * 599), "destination of weights overlaps first"),
+    (dict(ELSEWHERE, k_out=(1 << 31) + 1024 * 99), "destination of K overlaps V"),
+    (dict(ELSEWHERE, v_out=(1 << 32) + CACHE), "destination of V overlaps K"),
+    (dict(ELSEWHERE, v_out=1 << 32), "destination of V overlaps K"),  # two sources, one destination
+    (dict(ELSEWHERE, **dict(SIDES, weights_out=1 << 25, positions_out=1 << 25)), "destination of positions overlaps weights")])
+def test_keep_destinations_meet_nothing_else(kw, text):
+    """Found once there is a context (never looked into: the refusal comes before the device)."""
+    L = lib.load()
+    if L.pocr_device_count() > 0:
+        pytest.skip("a call that was not refused would run")
+    ctx = C.create_string_buffer(4096)
+    a = keep(**{**APART, **kw})
+    rc = L.pocr_cache_keep(C.cast(ctx, C.c_void_p), C.byref(a), None)
+    assert rc == ARG and text in L.pocr_last_error().decode(), L.pocr_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [{}, SIDES, ELSEWHERE, dict(v=(1 << 30) + 1024 * 100, v_out=(1 << 30) + 1024 * 100),
+                                dict(v=(1 << 30) + 512, v_out=(1 << 30) + 512, kv_heads=1), dict(ELSEWHERE, v=1 << 30, v_out=1 << 32)])
+def test_keep_buffers_side_by_side(kw):
+    """K and V behind each other in each cache, row by row, and one buffer as both: these calls get as far as the device."""
+    L = lib.load()
+    if L.pocr_device_count() > 0:
+        pytest.skip("the call would run")
+    ctx = C.create_string_buffer(4096)
+    a = keep(**{**APART, **kw})
+    rc = L.pocr_cache_keep(C.cast(ctx, C.c_void_p), C.byref(a), None)
+    assert rc == lib.POCR_ERR_DEVICE, L.pocr_last_error().decode()

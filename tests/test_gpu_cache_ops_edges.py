@@ -275,3 +275,26 @@ def test_keep_within_a_pool(ctx, rng):
             for g in range(2):
                 want[c, 1, :, :70, g] = src[c, 2][:, lists[c, g], g]
         assert np.array_equal(hip.down(base, want.shape), want)
+
+
+@pytest.mark.parametrize("n", [20, 300])
+def test_keep_one_buffer_as_k_and_v(ctx, rng, n):
+    """Elsewhere it moves to one destination as both; in place, where two workgroups would move each row, it is refused."""
+    with ref.Hip() as hip:
+        kp = Keep(rng, 2, 400, 2, 64)
+        lists = ascending(rng, (2, 2), n, 400)
+        a = kp.args(hip, lists, [n, n // 2], None, side=False)
+        b = lib.KeepArgs.from_buffer_copy(a)
+        a.v = a.v_out = a.k
+        with pytest.raises(lib.PocrError) as e:
+            ctx.cache_keep(a)
+        assert e.value.code == lib.POCR_ERR_ARG
+        assert np.array_equal(hip.down(a.k, kp.kv.shape), kp.kv)
+        b.v, b.k_out = b.k, hip.up(np.full((2, n, 128), SENTINEL, F32))
+        b.v_out, b.max_rows_out, b.k_out_cache_stride, b.v_out_cache_stride = b.k_out, n, n * 128, n * 128
+        ctx.cache_keep(b)
+        got = hip.down(b.k_out, (2, n, 2, 64))
+        for c, count in enumerate((n, n // 2)):
+            assert np.all(got[c, count:] == SENTINEL)
+            for g in range(2):
+                assert np.array_equal(got[c, :count, g], kp.part(kp.kv, 0)[c, lists[c, g, :count], g])
