@@ -354,7 +354,7 @@ typedef struct {
     const int32_t *parents;   /* [seqs][n], outside [-1, t): -1; null: chains (t - 1) */
     const float *slopes;      /* [heads], or null */
     const int32_t *positions; /* [seqs][kv_heads][side_stride], or null */
-    float *out;               /* as q, by out_seq_stride and out_stride */
+    float *out;               /* as q, by out_seq_stride and out_stride; no two rows overlap */
     float *lse;               /* [seqs][n][heads]: written where not null; read by pocr_cache_weights */
     float *weights;           /* pocr_cache_weights: [seqs][kv_heads][side_stride] */
     const uint64_t *take;     /* pocr_cache_weights: [seqs] bit t: token t counts; null: all */
@@ -409,7 +409,7 @@ int pocr_cache_select(pocr_ctx *ctx, const pocr_select_args *args, void *stream)
  * destination may not overlap its source (POCR_ERR_ARG): rows of both that
  * alternate in one pool do not where their strides are equal; where they
  * differ, the whole ranges count.  Nor may a destination overlap another
- * destination, another's source or the lists; but one buffer as K and V may go
+ * destination, another's source or the lists, or its caches each other; but one buffer as K and V may go
  * to one destination as both, elsewhere. */
 typedef struct {
     const float *k, *v;       /* cache c, row j, KV head g: k + c*k_cache_stride + j*k_stride + g*head_dim */

@@ -432,6 +432,8 @@ extern "C" int pocr_tree_attention(pocr_ctx *ctx, const pocr_tree_args *a, void 
     RC(check_rows(a->out, a->out_stride, (int64_t)a->heads * a->head_dim, "out", op));
     RC(check_outer(a->v_seq_stride, a->seqs, "v", op));
     RC(check_outer(a->out_seq_stride, a->seqs, "out", op));
+    const Area out{a->out, a->out_seq_stride, a->out_stride, a->seqs, a->n, (int64_t)a->heads * a->head_dim};
+    if (overlap(out, out, true)) return fail(POCR_ERR_ARG, "%s: out rows of two sequences overlap", op);
     const AttnShape shape = tree_attn(a);
     RC(check_workspace(a->workspace, a->workspace_bytes, shape.bytes, op));
     CACHE_OP_ENTER(ctx, stream, op);
@@ -545,6 +547,8 @@ extern "C" int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *a, void *str
         for (int i = 0; i < 4; ++i)
             if (dst[i].at && overlap(src[i], dst[i])) return fail(POCR_ERR_ARG, "%s: a destination overlaps its source", op);
     CACHE_OP_CONTEXT(ctx, op);
+    for (int i = 0; i < 2; ++i)
+        if (overlap(dst[i], dst[i], true)) return fail(POCR_ERR_ARG, "%s: caches of the destination overlap", op);
     // What one workgroup writes no other reads, or writes otherwise: one buffer as
     // K and V goes to one destination elsewhere (the same values twice), not in place.
     const Area lists[3] = {{a->rows, 0, 0, 1, 1, (a->per_head ? sides : a->caches) * a->max_keep},

@@ -88,6 +88,18 @@ ELSEWHERE = dict(k_out=1 << 32, v_out=1 << 33)
 CACHE = 4 << 16  # bytes from cache to cache
 
 
+def answer_behind_the_context(args, want):
+    """The answer to a call with a context, which is never looked into: refused before the device, or the device's own error."""
+    L = lib.load()
+    if L.pocr_device_count() > 0:
+        pytest.skip("a call that was not refused would run")
+    ctx = C.create_string_buffer(4096)
+    rc = L.pocr_cache_keep(C.cast(ctx, C.c_void_p), C.byref(args), None)
+    msg = L.pocr_last_error().decode()
+    assert rc == want, msg
+    return msg
+
+
 @pytest.mark.parametrize("kw,text", [
     (dict(v=1 << 30, v_out=1 << 30), "destination of K overlaps V"),
     (dict(v=(1 << 30) + 1024 * 99, v_out=(1 << 30) + 1024 * 99), "destination of K overlaps V"),
@@ -102,24 +114,32 @@ CACHE = 4 << 16  # bytes from cache to cache
     (dict(ELSEWHERE, v_out=1 << 32), "destination of V overlaps K"),  # two sources, one destination
     (dict(ELSEWHERE, **dict(SIDES, weights_out=1 << 25, positions_out=1 << 25)), "destination of positions overlaps weights")])
 def test_keep_destinations_meet_nothing_else(kw, text):
-    """Found once there is a context (never looked into: the refusal comes before the device)."""
-    L = lib.load()
-    if L.pocr_device_count() > 0:
-        pytest.skip("a call that was not refused would run")
-    ctx = C.create_string_buffer(4096)
-    a = keep(**{**APART, **kw})
-    rc = L.pocr_cache_keep(C.cast(ctx, C.c_void_p), C.byref(a), None)
-    assert rc == ARG and text in L.pocr_last_error().decode(), L.pocr_last_error().decode()
+    assert text in answer_behind_the_context(keep(**{**APART, **kw}), ARG)
 
 
 @pytest.mark.parametrize("kw", [{}, SIDES, ELSEWHERE, dict(v=(1 << 30) + 1024 * 100, v_out=(1 << 30) + 1024 * 100),
                                 dict(v=(1 << 30) + 512, v_out=(1 << 30) + 512, kv_heads=1), dict(ELSEWHERE, v=1 << 30, v_out=1 << 32)])
 def test_keep_buffers_side_by_side(kw):
-    """K and V behind each other in each cache, row by row, and one buffer as both: these calls get as far as the device."""
-    L = lib.load()
-    if L.pocr_device_count() > 0:
-        pytest.skip("the call would run")
-    ctx = C.create_string_buffer(4096)
-    a = keep(**{**APART, **kw})
-    rc = L.pocr_cache_keep(C.cast(ctx, C.c_void_p), C.byref(a), None)
-    assert rc == lib.POCR_ERR_DEVICE, L.pocr_last_error().decode()
+    """K and V behind each other in each cache, row by row, and one buffer as both."""
+    answer_behind_the_context(keep(**{**APART, **kw}), lib.POCR_ERR_DEVICE)
+
+
+def test_outputs_that_overlap_themselves():
+    """Two sequences' or caches' rows in one place; rows that alternate are in places of their own."""
+    refused("tree", ARG, "two sequences", out_seq_stride=2048 * 4)
+    refused("tree", ARG, "two sequences", out_seq_stride=2044, out_stride=3 * 2048)
+    refused("tree", ARG, "null context", out_seq_stride=2048 * 5)
+    refused("tree", ARG, "null context", out_seq_stride=2048, out_stride=3 * 2048)
+
+
+@pytest.mark.parametrize("kw", [dict(ELSEWHERE, k_out_cache_stride=256 * 99),
+                                dict(ELSEWHERE, v_out_cache_stride=256, v_out_stride=512),
+                                dict(k_cache_stride=256 * 99, k_out_cache_stride=256 * 99)])
+def test_keep_caches_that_overlap(kw):
+    assert "caches of the destination" in answer_behind_the_context(keep(**{**APART, **kw}), ARG)
+
+
+@pytest.mark.parametrize("kw", [dict(ELSEWHERE, v_out_cache_stride=256, v_out_stride=768),
+                                dict(k_cache_stride=256 * 100, k_out_cache_stride=256 * 100)])
+def test_keep_caches_that_touch_or_alternate(kw):
+    answer_behind_the_context(keep(**{**APART, **kw}), lib.POCR_ERR_DEVICE)
