@@ -318,11 +318,11 @@ int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, const
     return shaped ? launch_attn_s<64, TREE, true>(s, p, sh, work, seqs) : launch_attn_s<64, TREE, false>(s, p, sh, work, seqs);
 }
 
-AttnShape prompt_attn(const pocr_prompt_args *a) {
+AttnShape prompt_attn(const pocr_prompt_args *a, bool spans) {
     const int64_t rows = (int64_t)a->rows_before + a->n;
     // spans may leave out most of a long cache: its images are worth their
     // making where all rows are seen, or not many more than the prompt's own
-    const bool images = !a->row_begin || a->rows_before <= 4 * (int64_t)a->n;
+    const bool images = !spans || a->rows_before <= 4 * (int64_t)a->n;
     return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), rows, a->kv_heads, a->head_dim, images);
 }
 AttnShape tree_attn(const pocr_tree_args *a) {
@@ -377,7 +377,7 @@ bool overlap(const Area &x, const Area &y, bool other = false) {
 
 extern "C" int64_t pocr_prompt_attention_workspace(const pocr_prompt_args *a) {
     RC(prompt_shape(a, "pocr_prompt_attention_workspace"));
-    return prompt_attn(a).bytes;
+    return std::max(prompt_attn(a, false).bytes, prompt_attn(a, true).bytes);  // shapes alone: with spans or without
 }
 
 extern "C" int64_t pocr_tree_attention_workspace(const pocr_tree_args *a) {
@@ -396,7 +396,7 @@ extern "C" int pocr_prompt_attention(pocr_ctx *ctx, const pocr_prompt_args *a, v
     if (!a->row_begin != !a->row_end) return fail(POCR_ERR_ARG, "%s: row_begin and row_end come together", op);
     for (const void *x : {(const void *)a->row_begin, (const void *)a->row_end, (const void *)a->slopes, (const void *)a->lse})
         RC(check_index(x, "an index or side buffer", op));
-    const AttnShape shape = prompt_attn(a);
+    const AttnShape shape = prompt_attn(a, a->row_begin);
     RC(check_workspace(a->workspace, a->workspace_bytes, shape.bytes, op));
     CACHE_OP_ENTER(ctx, stream, op);
     CacheAttn p{};

@@ -4,7 +4,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
-from test_cache_ops import ARG, keep, refused
+from test_cache_ops import ARG, keep, prompt, refused
 
 from rapidocrvl_amd import lib
 
@@ -143,3 +143,15 @@ def test_keep_caches_that_overlap(kw):
                                 dict(k_cache_stride=256 * 100, k_out_cache_stride=256 * 100)])
 def test_keep_caches_that_touch_or_alternate(kw):
     answer_behind_the_context(keep(**{**APART, **kw}), lib.POCR_ERR_DEVICE)
+
+
+@pytest.mark.parametrize("shape", [dict(n=64, rows_before=9000), dict(n=300, rows_before=5000), dict(n=7, rows_before=5000),
+                                   dict(n=2000, rows_before=100), dict(n=1, rows_before=0), dict(n=128, rows_before=8000)])
+def test_prompt_workspace_of_shapes_alone(shape):
+    """What the query names without pointers is enough with them, spans or none."""
+    L = lib.load()
+    need = L.pocr_prompt_attention_workspace(C.byref(prompt(q=None, k=None, v=None, out=None, workspace=None, **shape)))
+    spans = dict(row_begin=4096, row_end=4096)
+    assert L.pocr_prompt_attention_workspace(C.byref(prompt(**spans, **shape))) == need
+    for kw in ({}, spans):
+        refused("prompt", ARG, "null context", workspace_bytes=need, **kw, **shape)
