@@ -1534,8 +1534,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // bins; a pass whose bin is taken whole is the last, as the second mostly is
 // among weights that differ), then one pass that writes the kept rows in order: a wave owns 64·KPT
 // consecutive rows of a tile, so a row's place is a count of ballots.  KPT rows
-// per thread and tile; where one tile holds the cache its keys are read once
-// and stay in registers.  36 selections, one workgroup each: 6.6 us of 1,609
+// per thread and tile; a cache of one tile is read once, its keys stay in
+// registers (8,192 rows in a buffer of 32,768: 15.3 us, 18.1 read by each pass).  36 selections, one workgroup each: 6.6 us of 1,609
 // rows, 10.6 of 8,192, nearly all of it the chain of load, passes and barriers.
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
@@ -1545,14 +1545,14 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     __shared__ int s_eq[kSelWaves], s_gt[kSelWaves];
     const int g = blockIdx.x, c = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float *w = p.weights + ((size_t)c * p.kvh + g) * p.side;
-    const bool one = p.max_rows <= kTile;  // one tile holds any cache: its weights wait for no length
+    const bool early = p.max_rows <= kTile;  // one tile holds any cache: its weights wait for no length
     float x[KPT];
     auto load = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i)  // all on their way at once
             x[i] = w[min(tile * kTile + (wave * KPT + i) * 64 + lane, p.max_rows - 1)];
     };
-    if (one) load(0);
+    if (early) load(0);
     const int len = min(max(p.lens[c], 0), p.max_rows);
     int32_t *kept = p.kept + ((size_t)c * p.kvh + g) * p.budget;
     if (g == 0 && tid == 0) p.counts[c] = min(len, p.budget);
@@ -1568,6 +1568,8 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) key[i] = weight_key(x[i]);
     };
+    const bool one = tiles == 1;  // this cache's keys stay in registers
+    if (one && !early) load(0);
     if (one) keys();
     uint32_t prefix = 0, mask = 0;
     if (need > 0)

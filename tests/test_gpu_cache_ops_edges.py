@@ -5,7 +5,7 @@ import ctypes as C
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, SENTINEL, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, visible
+from test_gpu_cache_ops import F32, I32, SENTINEL, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, run_select, visible
 
 from rapidocrvl_amd import lib
 
@@ -298,3 +298,15 @@ def test_keep_one_buffer_as_k_and_v(ctx, rng, n):
             assert np.all(got[c, count:] == SENTINEL)
             for g in range(2):
                 assert np.array_equal(got[c, :count, g], kp.part(kp.kv, 0)[c, lists[c, g, :count], g])
+
+
+@pytest.mark.parametrize("max_rows", [2048, 2049, 8193, 16384, 16385, 70000])
+def test_select_of_short_caches_in_long_buffers(ctx, rng, max_rows):
+    """Lengths far below what the buffers hold, on both sides of one and of several tiles, in one call."""
+    with ref.Hip() as hip:
+        lens = [0, 51, 700, 2048, min(8192, max_rows), min(16384, max_rows), min(16385, max_rows), max_rows]
+        w = rng.integers(0, 400, (len(lens), 2, max_rows)).astype(F32)
+        for c, length in enumerate(lens):
+            w[c, :, length:] = 1e6  # rows behind a cache's end weigh nothing
+        a = run_select(ctx, hip, w, lens, 50, 4, 16)
+        check_select(hip, a, w, lens)
