@@ -5,7 +5,8 @@ import ctypes as C
 import cache_ops_f64 as ref
 import numpy as np
 import pytest
-from test_gpu_cache_ops import F32, I32, SENTINEL, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case, run_select, visible
+from test_gpu_cache_ops import (F32, I32, SENTINEL, Keep, Tree, alibi, ascending, check_prompt, check_select, prompt_case,
+                                random_trees, run_select, spans_of, visible)
 
 from rapidocrvl_amd import lib
 
@@ -310,3 +311,51 @@ def test_select_of_short_caches_in_long_buffers(ctx, rng, max_rows):
             w[c, :, length:] = 1e6  # rows behind a cache's end weigh nothing
         a = run_select(ctx, hip, w, lens, 50, 4, 16)
         check_select(hip, a, w, lens)
+
+
+@pytest.mark.parametrize("seqs,kvh,n,longest", [(140, 2, 1, 600), (300, 1, 3, 1500), (256, 1, 1, 4000)])
+def test_tree_many_ragged_sequences(ctx, rng, seqs, kvh, n, longest):
+    """Few rows of so many sequences that a tile has at most four shares: lengths from 0 on, sequences without tokens."""
+    with ref.Hip() as hip:
+        lens = rng.integers(0, longest, seqs)
+        lens[:4] = 0, 1, longest - 1, longest
+        t = Tree(hip, rng, lens, rng.integers(0, n + 1, seqs), n, 4 * kvh, kvh, 64, random_trees(rng, seqs, n))
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
+
+
+@pytest.mark.parametrize("seqs,kvh,n,longest", [(60, 2, 33, 900), (130, 1, 20, 1300), (90, 2, 33, 900)])
+def test_tree_many_ragged_trees(ctx, rng, seqs, kvh, n, longest):
+    """More rows: two or three tiles a sequence, of which counts leave some or all without rows, in two, three shares or one."""
+    with ref.Hip() as hip:
+        lens, counts = rng.integers(0, longest, seqs), rng.integers(0, n + 1, seqs)
+        lens[:4], counts[:8] = (0, 1, longest - 1, longest), (n, n, n, n, 0, 1, 2, n)
+        t = Tree(hip, rng, lens, counts, n, 8 * kvh, kvh, 64, random_trees(rng, seqs, n), slopes=alibi(8 * kvh))
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
+
+
+@pytest.mark.parametrize("n", [1, 12, 24])
+def test_tree_one_long_sequence_among_short_ones(ctx, rng, n):
+    with ref.Hip() as hip:
+        lens = np.r_[rng.integers(0, 500, 15), 7900]
+        t = Tree(hip, rng, lens, None, n, 8, 1, 64, random_trees(rng, 16, n))
+        ctx.tree_attention(t.a)
+        t.check()
+        ctx.cache_weights(t.a)
+        t.check_weights()
+
+
+@pytest.mark.parametrize("n,rows0", [(33, 2000), (64, 8000), (300, 2000), (600, 0)])
+@pytest.mark.parametrize("kind", ["causal", "docs"])
+def test_prompt_chunks_behind_a_prefix(ctx, rng, n, rows0, kind):
+    """Prompts of few tiles whose keys are cut into shares."""
+    with ref.Hip() as hip:
+        spans = spans_of(kind, n, rows0, rng)
+        a, q, k, v = prompt_case(hip, rng, n, rows0, 16, 2, 64, spans)
+        ctx.prompt_attention(a)
+        check_prompt(hip, a, q, k, v, spans, rows=np.unique(np.r_[0, 1, np.arange(0, n, 17), n - 1]))
