@@ -108,7 +108,7 @@ __device__ __forceinline__ void split_one(float a, float b, float one, v2h &hi, 
     lo = (v2h){(_Float16)__builtin_fmaf(a, one, -(float)hi[0]), (_Float16)__builtin_fmaf(b, one, -(float)hi[1])};
 }
 
-// x as rounded: no part of a multiply-add
+// x as rounded: no part of a multiply-add (a score less its row's rounded maximum is then at most 0)
 __device__ __forceinline__ float rounded(float x) {
     asm("" : "+v"(x));
     return x;
@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
                 }
                 if (SHAPED) shape(u, x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
+                for (int e = 0; e < 8; ++e) x[e] = rounded(mine >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY);
                 raise_m(u, groups_max(max8(x)));
                 float w[8], sum = 0.0f;
 #pragma unroll
@@ -1130,7 +1130,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_cache_attn_few(CacheAttn 
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = see >> i & 1 ? x[i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) x[i] = rounded(see >> i & 1 ? x[i] : -INFINITY);
         const float top = groups_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
         if (__any(top > m)) {
             const float mn = top > m ? top : m;
