@@ -282,8 +282,10 @@ int pocr_time_stream_read(pocr_ctx *ctx, int64_t bytes, int n_buffers, int iters
  *
  * Conventions of this section:
  *  - Every pointer is a device address on the context's device.  Buffers of
- *    floats are 16-byte aligned and their strides, counted in floats, are
- *    multiples of 4 (POCR_ERR_ARG otherwise); index buffers are 4-byte aligned.
+ *    rows (q, k, v, out and their like) and workspaces are 16-byte aligned and
+ *    row strides, counted in floats, multiples of 4 (POCR_ERR_ARG otherwise);
+ *    lse, slopes, weights and index buffers are 4-byte aligned, take 8.  What a
+ *    call writes overlaps none of its other buffers, where not said otherwise.
  *  - `stream` is the hipStream_t the work is queued on, null HIP's default
  *    stream, of the HIP runtime that the library runs on (a process that loads
  *    the library and then a package with a runtime of its own holds two); a

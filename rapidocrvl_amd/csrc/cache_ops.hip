@@ -28,6 +28,7 @@ constexpr float kLeast = FLT_MIN, kMost = 0x1p126f;  // of scale and cap
 //   128 rows behind 8,000      4,064                 56 : 54
 //   1,200 rows                 5,700                 49 : 88
 //   256 rows behind 8,000      8,256                 82 : 94
+// (what counts is steps; 128 rows behind 8,000, few tiles with long shares, lose 2 us)
 constexpr int kImageTiles = 8, kImageSteps = 2400;
 
 // The calling thread's device becomes the context's for one call.
@@ -224,7 +225,10 @@ AttnShape attn_shape(int64_t rows, int64_t keys, int64_t groups, int head_dim, b
         // us, 256: 32, by the form that both were measured with; 256 and 512 are
         // alike for few rows).  From 256 tiles on, whose lengths may differ, shares
         // for four rounds.  Shares of fewer steps than `least` cost more in sums
-        // than they save where the tiles fill half of the chip anyway.
+        // than they save where the tiles fill half of the chip anyway (least 2 and
+        // 6, us: 16 trees of 12 over 250 rows, 32 tiles, 17.5 and 24.0, over 800 rows
+        // 22.9 and 25.8; 64 trees, 128 tiles, over 250 rows 25.9 and 24.8; 128 trees
+        // over 250 rows 68 and 29, over 500 rows 82 and 63; 1,609 rows alike).
         const int64_t want = std::max<int64_t>(1, (work >= 256 ? 1024 : 256) / work);
         a.least = a.few ? 1 : (work < 128 ? 2 : 6);
         a.splits = (int)std::min<int64_t>({want, kMaxShares, std::max<int64_t>(1, keys / (step * a.least))});
@@ -320,8 +324,15 @@ int launch_attn(hipStream_t s, const CacheAttn &p, int head_dim, int seqs, const
 
 AttnShape prompt_attn(const pocr_prompt_args *a, bool spans) {
     const int64_t rows = (int64_t)a->rows_before + a->n;
-    // spans may leave out most of a long cache: its images are worth their
-    // making where all rows are seen, or not many more than the prompt's own
+    // Spans may leave out most of a long cache, whose images are made all the
+    // same: worth it where all rows are seen, or not many more than the prompt's
+    // own.  Images against none, us, spans that see all rows, the latter half or
+    // the prompt's own alone:
+    //   600 rows behind 1,200      50 : 58    43 : 45    33 : 31
+    //   600 rows behind 9,600     167 : 245  102 : 139   36 : 31
+    //   300 rows behind 4,800      65 : 75    49 : 47    28 : 21
+    // The spans are on the device: far behind, where images may cost a third, none
+    // are made, which costs up to half as much again where spans see everything.
     const bool images = !spans || a->rows_before <= 4 * (int64_t)a->n;
     return attn_shape((int64_t)a->n * (a->heads / a->kv_heads), rows, a->kv_heads, a->head_dim, images);
 }

@@ -217,6 +217,11 @@ struct AttnTile {
 };
 
 // a tile's steps of `keys` keys cut into at most `splits` shares of at least `least` steps
+// 32, 64 or 128 shares, us: one token over 6,400 rows and one KV head 14.6, 12.6,
+// 14.1; 20,000 rows 23.6, 17.6, 17.0; 64,000 rows 53.5, 33.8, 24.9; one tree of 12
+// over 8,192 rows and two KV heads 30.5, 26.1, 29.7; 30,000 rows 71.2, 47.1, 41.1.
+// 64 do best up to about 20,000 rows; from four KV heads on the 256 workgroups of
+// a call are the bound instead.
 constexpr int kMaxShares = 64;
 __device__ __forceinline__ void share_tile(AttnTile &t, int keys, int parts, int part) {
     const int steps = max(0, (t.hi - t.lo + keys - 1) / keys);
@@ -953,7 +958,7 @@ __global__ void __launch_bounds__(IMG ? 256 : 768, IMG ? 2 : 3) k_cache_attn(Cac
 //   V  lane 16·q + j: keys 4q .. 4q+3, dims 64d + 4j .. +3
 // Scores and sums come out transposed, as in k_cache_attn; the waves' sums are
 // joined in LDS.  Products, weights and sums are fp32 throughout.
-// One token of 16 heads and 2 KV heads over 1,609 rows of 128: 7.9 us and 4.2 of
+// One token of 16 heads and 2 KV heads over 1,609 rows of 128: 8.4 us and 3.8 of
 // the join, 3.3 MB; of 16 sequences 15 us, of 64 41 us (5.1 TB/s), of 256 143 us
 // (5.9 TB/s).
 constexpr int kFewKeys = 16;
@@ -1532,11 +1537,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // bits (integer counts: the order of the atomics does not matter; eleven bits
 // hold two of the mantissa, which spreads weights of few exponents over the
 // bins; a pass whose bin is taken whole is the last, as the second mostly is
-// among weights that differ), then one pass that writes the kept rows in order: a wave owns 64·KPT
-// consecutive rows of a tile, so a row's place is a count of ballots.  KPT rows
-// per thread and tile; a cache of one tile is read once, its keys stay in
-// registers (8,192 rows in a buffer of 32,768: 15.3 us, 18.1 read by each pass).  36 selections, one workgroup each: 6.6 us of 1,609
-// rows, 10.6 of 8,192, nearly all of it the chain of load, passes and barriers.
+// among weights that differ), then one pass that writes the kept rows in order:
+// a wave owns 64·KPT consecutive rows of a tile, so a row's place is a count of
+// ballots.  KPT rows per thread and tile; a cache of one tile is read once, its
+// keys stay in registers (8,192 rows in a buffer of 32,768: 15.3 us, 18.1 read by
+// each pass).  36 selections, one workgroup each: 6.5 us of 1,609 rows, 10.6 of
+// 8,192, nearly all of it the chain of load, passes and barriers.
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) k_cache_select(CacheSelect p) {
     constexpr int kTile = kSelThreads * KPT, kBins = 2048;
@@ -1769,7 +1775,9 @@ __global__ void __launch_bounds__(kKeepThreads) k_cache_keep(CacheKeep p, int ch
 // in chunks: all loads of a chunk, then its stores.  The list ascends with
 // rows[i] >= first + i, so what a later chunk reads lies at or behind its own
 // places, past everything written before it, and only the chunk's own loads
-// have to end (the barrier) before its stores.
+// have to end (the barrier) before its stores.  18 caches with two KV heads,
+// 8,192 -> 2,048 rows: 48 us, 3.1 TB/s read and written (elsewhere, by
+// k_cache_keep, 36 us); 1,609 -> 768 rows 16.7 us, 3.4 TB/s (11.2).
 template <int HD>
 __global__ void __launch_bounds__(kKeepThreads) k_cache_keep_slabs(CacheKeep p) {
     constexpr int kSlabs = HD / kKeepSlab, kLanes = kKeepSlab / 4, kStep = kKeepThreads / kLanes, kUnroll = 8;
