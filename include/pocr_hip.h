@@ -436,6 +436,130 @@ typedef struct {
 } pocr_keep_args;
 int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *args, void *stream);
 
+/* ---------------- K/V caches in 4 or 8 bits (device buffers, caller's stream) ---------------- */
+/* No counterpart in the reference: rows normed, rotated and appended to a cache,
+ * caches whose rows are held in 4 or 8 bits, and the attention over those.  The
+ * conventions of the section above hold here too: pointers, alignment, streams,
+ * workspaces, numbers that live on the device.  Strides are at most 2^40. */
+
+/* Rows of seqs sequences of up to n tokens each, of q, k and v, on their way to
+ * where attention reads them.  Each may be left out (null, with its destination).
+ *  - Every head x of q (k) becomes x * q_norm / sqrt(mean(x^2) + eps) where q_norm
+ *    (k_norm) is given;
+ *  - where positions are given (rotary_dim > 0), pair i < rotary_dim / 2 of its
+ *    elements, (i, i + rotary_dim / 2) or, adjacent, (2i, 2i + 1), is turned by
+ *    position[axis(i)] * freqs[i] radians: (a, b) -> (a cos - b sin, b cos + a sin).
+ *    Elements from rotary_dim on stay.  The first sections[0] pairs turn by axis 0,
+ *    the next sections[1] by axis 1, and so on; interleaved, axis a > 0 has pairs
+ *    a, a + axes, ..., sections[a] of them, and axis 0 the others.
+ *  - v is taken as it is.
+ * All of it is computed in 64 bits and rounded once, to fp32: a row does not
+ * depend on which call made it.  Angles are exact to 2^-20 of a turn up to
+ * positions times frequencies of 2^31.
+ * Tokens from counts[s] on are not looked at and what would be theirs is left as
+ * it was. */
+typedef struct {
+    const float *q, *k, *v;   /* sequence s, token t, head h: q + s*q_seq_stride + t*q_stride + h*head_dim */
+    float *q_out;             /* likewise; q itself (equal strides) or elsewhere */
+    float *k_out, *v_out;     /* pocr_rotate_rows: row first[s] + t of sequence s; k itself (v itself) without first */
+    const int32_t *positions; /* [seqs][n][axes], or null */
+    const double *freqs;      /* [rotary_dim / 2] radians a position, 8-byte aligned */
+    const float *q_norm, *k_norm; /* [head_dim], or null */
+    const int32_t *counts;    /* [seqs] tokens of each sequence, forced into [0, n]; null: n */
+    const int32_t *first;     /* [seqs] rows before the tokens', forced into [0, rows - count]; null: 0 */
+    int64_t q_seq_stride, q_stride, k_seq_stride, k_stride, v_seq_stride, v_stride;
+    int64_t q_out_seq_stride, q_out_stride, k_out_seq_stride, k_out_stride, v_out_seq_stride, v_out_stride;
+    int32_t seqs;             /* 1 .. 65535 */
+    int32_t n;                /* 1 .. 2^22 */
+    int32_t heads, kv_heads;  /* 1 .. 1024 where q (k or v) is given */
+    int32_t head_dim;         /* 64 or 128 */
+    int32_t rotary_dim;       /* 0, or a multiple of 16 up to head_dim */
+    int32_t axes;             /* 1 .. 4 */
+    int32_t sections[4];      /* pairs of each axis, rotary_dim / 2 together */
+    int32_t interleaved, adjacent;
+    int32_t max_rows;         /* rows of k_out and of v_out a sequence, n .. 2^30; pocr_qcache_write: not looked at */
+    float eps;                /* of the norms, 0 .. 1 */
+} pocr_rows_args;
+int pocr_rotate_rows(pocr_ctx *ctx, const pocr_rows_args *args, void *stream);
+
+/* A K/V cache of `capacity` rows for each sequence and KV head, in memory the
+ * caller owns.  Of every 64 elements of a row: codes c in [-8, 7] (8 bits: [-128,
+ * 127]), a midpoint and a step in fp16; an element's value is mid + step * c.
+ * From elements of lo to hi (sizes beyond 65504 count as that), in 64 bits, by
+ * reciprocals that are rounded themselves:
+ *   mid = (7 lo + 8 hi) * (1/15) (8 bits: (127 lo + 128 hi) * (1/255)), rounded to fp32 and that to fp16,
+ *   step = the least fp16 number that is at least (hi - mid) * (1/7) and (mid - lo) * (1/8) (127 and 128),
+ *   c = the whole number nearest to (x - mid) * (1/step), ties to even,
+ * so a value is within half a step.  A group with a NaN or an infinity reads back
+ * as NaN.
+ * Row j of KV head g of sequence s: its codes, plus 8 (128), at byte
+ *   (s * seq_stride + g * capacity + j) * head_dim * bits / 8
+ * and its parameters at number (s * seq_stride + g * capacity + j) * head_dim / 32: the
+ * steps of its groups, then their midpoints.  Codes lie in the order in which the
+ * attention's matrix instructions take them:
+ *   K, 4 bits: word w = 8 codes, elements 32c + 8u + (0 2 4 6 1 3 5 7) from the low
+ *     bits on, u = w / (head_dim / 32), c = w % (head_dim / 32);
+ *   K, 8 bits: 8 bytes m, elements 32c + 8u .. +7, c = 2 (m / 8) + m % 2, u = m / 2 % 4;
+ *   V, heads of 128: 8 codes m, elements 4m .. +3 and 64 + 4m .. +3; heads of 64: as they come. */
+typedef struct {
+    uint8_t *k_codes, *v_codes;    /* 16-byte aligned */
+    uint16_t *k_params, *v_params; /* 16-byte aligned */
+    int64_t seq_stride;            /* rows from sequence to sequence, >= kv_heads * capacity; 0: that */
+    int32_t seqs;                  /* 1 .. 65535 */
+    int32_t kv_heads;              /* 1 .. 1024 */
+    int32_t head_dim;              /* 64 or 128 */
+    int32_t capacity;              /* 1 .. 2^30 rows */
+    int32_t bits;                  /* 4 or 8 */
+} pocr_qcache;
+
+/* rows into a cache: K and V rows of args as above, into rows first[s] + t, in
+ * place of k_out and v_out (null here).  K rows are held as pocr_rotate_rows gives
+ * them; q rows, where given, go to q_out in the same pass.  seqs, kv_heads and
+ * head_dim are the cache's, n is at most its capacity.  No other row changes. */
+int pocr_qcache_write(pocr_ctx *ctx, const pocr_rows_args *args, const pocr_qcache *cache, void *stream);
+
+/* rows of a cache as fp32: row t < counts[s] of a destination is cache row
+ * first[s] + t, or, with a list, rows[s][t] */
+typedef struct {
+    float *k_out, *v_out;     /* sequence s, row t, KV head g: k_out + s*k_out_seq_stride + t*k_out_stride + g*head_dim;
+                                 one may be null */
+    const int32_t *rows;      /* [seqs][n], per_head: [seqs][kv_heads][n]; forced into [0, capacity); or null */
+    const int32_t *counts;    /* [seqs], forced into [0, n] (without a list: [0, min(n, capacity)]); null: n */
+    const int32_t *first;     /* [seqs], without a list, forced into [0, capacity - count]; null: 0 */
+    int64_t k_out_seq_stride, k_out_stride, v_out_seq_stride, v_out_stride;
+    int32_t n;                /* 1 .. 2^30 */
+    int32_t per_head;         /* each KV head has its own list */
+} pocr_qread_args;
+int pocr_qcache_read(pocr_ctx *ctx, const pocr_qread_args *args, const pocr_qcache *cache, void *stream);
+
+/* softmax attention of the last counts[s] of lens[s] cached tokens, written
+ * before: token t is at position lens[s] - counts[s] + t and sees the rows up to
+ * its own, with a window the last `window` of those.  Scores as in the section
+ * above, |position(i) - position(j)| the distance in rows.  A token that sees
+ * nothing (its position is negative) has an out row of zeros and -inf for its
+ * lse.  Rows of out and lse behind a sequence's last token are left as they were.
+ * A row that sees a group of NaN comes out not finite: the whole of it for a
+ * key's group, with its lse, that group's elements for a value's. */
+typedef struct {
+    const float *q;           /* sequence s, token t, head h: q + s*q_seq_stride + t*q_stride + h*head_dim */
+    float *out;               /* likewise, no two rows overlap */
+    float *lse;               /* [seqs][n][heads] log-sum-exp of the scores, or null */
+    const int32_t *lens;      /* [seqs] rows in the cache, the tokens' own among them, forced into [0, max_rows] */
+    const int32_t *counts;    /* [seqs], forced into [0, n]; null: n */
+    const float *slopes;      /* [heads], or null */
+    void *workspace;          /* pocr_qcache_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t q_seq_stride, q_stride, out_seq_stride, out_stride;
+    int32_t n;                /* 1 .. 2^22 tokens, n * (heads / kv_heads) <= 2^24 */
+    int32_t heads;            /* a multiple of the cache's kv_heads, up to 1024 */
+    int32_t max_rows;         /* no sequence has more rows; 1 .. capacity */
+    int32_t window;           /* >= 0; 0: all rows */
+    float scale, cap;         /* as above */
+} pocr_qattention_args;
+int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *args, const pocr_qcache *cache, void *stream);
+/* workspace bytes of such a call (pointers and strides are not looked at), or an error status */
+int64_t pocr_qcache_attention_workspace(const pocr_qattention_args *args, const pocr_qcache *cache);
+
 /* ---------------- model / step level (device-resident) ---------------- */
 int pocr_model_create(pocr_ctx *ctx, const pocr_config *cfg, pocr_model **out);
 void pocr_model_destroy(pocr_model *m);

@@ -90,6 +90,44 @@ class KeepArgs(C.Structure):
                                           "max_rows_out")]
 
 
+class RowsArgs(C.Structure):
+    """pocr_rows_args: rows of q, k and v normed, rotated and put where attention
+    reads them."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out", "v_out", "positions", "freqs", "q_norm",
+                                          "k_norm", "counts", "first")]
+    _fields_ += [(n, C.c_int64) for n in ("q_seq_stride", "q_stride", "k_seq_stride", "k_stride", "v_seq_stride",
+                                          "v_stride", "q_out_seq_stride", "q_out_stride", "k_out_seq_stride",
+                                          "k_out_stride", "v_out_seq_stride", "v_out_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("seqs", "n", "heads", "kv_heads", "head_dim", "rotary_dim", "axes")]
+    _fields_ += [("sections", C.c_int32 * 4)]
+    _fields_ += [(n, C.c_int32) for n in ("interleaved", "adjacent", "max_rows")] + [("eps", C.c_float)]
+
+
+class QCache(C.Structure):
+    """pocr_qcache: a K/V cache whose rows are held in 4 or 8 bits."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "v_codes", "k_params", "v_params")] + [("seq_stride", C.c_int64)]
+    _fields_ += [(n, C.c_int32) for n in ("seqs", "kv_heads", "head_dim", "capacity", "bits")]
+
+
+class QReadArgs(C.Structure):
+    """pocr_qread_args: rows of a QCache as fp32."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k_out", "v_out", "rows", "counts", "first")]
+    _fields_ += [(n, C.c_int64) for n in ("k_out_seq_stride", "k_out_stride", "v_out_seq_stride", "v_out_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("n", "per_head")]
+
+
+class QAttentionArgs(C.Structure):
+    """pocr_qattention_args: attention of a QCache's last tokens."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse", "lens", "counts", "slopes", "workspace")]
+    _fields_ += [(n, C.c_int64) for n in ("workspace_bytes", "q_seq_stride", "q_stride", "out_seq_stride", "out_stride")]
+    _fields_ += [(n, C.c_int32) for n in ("n", "heads", "max_rows", "window")]
+    _fields_ += [("scale", C.c_float), ("cap", C.c_float)]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _SIGS = {
@@ -132,6 +170,11 @@ _SIGS = {
     "pocr_cache_weights": (_i, [_vp, C.POINTER(TreeArgs), _vp]),
     "pocr_cache_select": (_i, [_vp, C.POINTER(SelectArgs), _vp]),
     "pocr_cache_keep": (_i, [_vp, C.POINTER(KeepArgs), _vp]),
+    "pocr_rotate_rows": (_i, [_vp, C.POINTER(RowsArgs), _vp]),
+    "pocr_qcache_write": (_i, [_vp, C.POINTER(RowsArgs), C.POINTER(QCache), _vp]),
+    "pocr_qcache_read": (_i, [_vp, C.POINTER(QReadArgs), C.POINTER(QCache), _vp]),
+    "pocr_qcache_attention": (_i, [_vp, C.POINTER(QAttentionArgs), C.POINTER(QCache), _vp]),
+    "pocr_qcache_attention_workspace": (C.c_int64, [C.POINTER(QAttentionArgs), C.POINTER(QCache)]),
     "pocr_model_create": (_i, [_vp, C.POINTER(PocrConfig), C.POINTER(_vp)]),
     "pocr_model_destroy": (None, [_vp]),
     "pocr_model_set_weight": (_i, [_vp, _i, _i, _vp]),
@@ -356,6 +399,11 @@ def prompt_attention_workspace(args: PromptArgs) -> int:
 def tree_attention_workspace(args: TreeArgs) -> int:
     """Workspace bytes of Context.tree_attention for these shapes."""
     return check(load().pocr_tree_attention_workspace(C.byref(args)))
+
+
+def qcache_attention_workspace(args: QAttentionArgs, cache: QCache) -> int:
+    """Workspace bytes of Context.qcache_attention for these shapes."""
+    return check(load().pocr_qcache_attention_workspace(C.byref(args), C.byref(cache)))
 
 
 def device_count() -> int:
@@ -640,6 +688,24 @@ class Context:
     def cache_keep(self, args: KeepArgs, stream=0):
         """Moves the listed rows of each cache together."""
         check(load().pocr_cache_keep(self.h, C.byref(args), stream))
+
+    # -- K/V caches in 4 or 8 bits: device buffers, queued on the caller's stream --
+    def rotate_rows(self, args: RowsArgs, stream=0):
+        """Rows of q, k and v, normed and rotated, to where attention reads them."""
+        check(load().pocr_rotate_rows(self.h, C.byref(args), stream))
+
+    def qcache_write(self, args: RowsArgs, cache: QCache, stream=0):
+        """The same with K and V rows going into a cache of few bits."""
+        check(load().pocr_qcache_write(self.h, C.byref(args), C.byref(cache), stream))
+
+    def qcache_read(self, args: QReadArgs, cache: QCache, stream=0):
+        """Rows of a cache of few bits as fp32."""
+        check(load().pocr_qcache_read(self.h, C.byref(args), C.byref(cache), stream))
+
+    def qcache_attention(self, args: QAttentionArgs, cache: QCache, stream=0):
+        """Attention of a cache's last tokens over its rows."""
+        check(load().pocr_qcache_attention(self.h, C.byref(args), C.byref(cache), stream))
+
 
 
 class Model:
