@@ -202,6 +202,53 @@ int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const c
     return POCR_OK;
 }
 
+// Row tiles and key shares of one attention call.
+struct QShape {
+    int rt;       // row tiles of 16 a wave
+    bool keys;    // a workgroup's waves share its rows
+    int rows;     // of a workgroup
+    int tiles, splits, least;
+    int64_t slots, bytes;
+};
+QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
+    QShape q;
+    const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
+    q.rt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    q.keys = rows < 1024;
+    q.rows = 16 * q.rt * (q.keys ? 1 : 4);
+    q.tiles = round_up_div(rows, q.rows);
+    const int64_t work = q.tiles * groups, blocks = round_up_div(a->max_rows, kQBlock);
+    q.least = q.keys ? 4 : 8;
+    q.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 512 / work), 64, std::max<int64_t>(1, blocks / q.least)});
+    q.slots = q.splits > 1 ? work * q.splits : 0;
+    q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
+    return q;
+}
+
+template <int HD, int BITS, int RT, bool KEYS>
+int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
+    QAttnPlan pl{};
+    pl.tiles = q.tiles;
+    pl.splits = q.splits;
+    pl.least = q.least;
+    pl.part = static_cast<float *>(work);
+    pl.stat = reinterpret_cast<float2 *>(pl.part + q.slots * q.rows * HD);
+    const dim3 grid(q.tiles * q.splits, p.cache.kvh, seqs);
+    if (p.cap > 0.0f || p.slopes) RC(launch(s, grid, 256, k_qcache_attn<HD, BITS, RT, true, KEYS>, p, pl));
+    else RC(launch(s, grid, 256, k_qcache_attn<HD, BITS, RT, false, KEYS>, p, pl));
+    if (!q.slots) return POCR_OK;
+    constexpr int kRows = 16 * RT * (KEYS ? 1 : 4);
+    return launch(s, dim3(q.tiles * (kRows / (1024 / HD)), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows>, p, pl);
+}
+
+template <int HD, int BITS>
+int launch_qattn_t(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
+    if (q.rt == 1) return launch_qattn<HD, BITS, 1, true>(s, p, q, work, seqs);
+    if (q.rt == 2) return launch_qattn<HD, BITS, 2, true>(s, p, q, work, seqs);
+    if (q.keys) return launch_qattn<HD, BITS, 4, true>(s, p, q, work, seqs);
+    return launch_qattn<HD, BITS, 4, false>(s, p, q, work, seqs);
+}
+
 }  // namespace
 
 extern "C" int pocr_rotate_rows(pocr_ctx *ctx, const pocr_rows_args *a, void *stream) {
@@ -275,7 +322,7 @@ extern "C" int pocr_qcache_read(pocr_ctx *ctx, const pocr_qread_args *a, const p
 
 extern "C" int64_t pocr_qcache_attention_workspace(const pocr_qattention_args *a, const pocr_qcache *c) {
     RC(attention_shape(a, c, "pocr_qcache_attention_workspace"));
-    return 0;
+    return qattn_shape(a, c).bytes;
 }
 
 extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *a, const pocr_qcache *c, void *stream) {
@@ -290,6 +337,8 @@ extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *
         RC(check_index(x, "an index or side buffer", op));
     const Area out{a->out, a->out_seq_stride, a->out_stride, c->seqs, a->n, width};
     if (overlap(out, out, true)) return fail(POCR_ERR_ARG, "%s: out rows of two sequences overlap", op);
+    const QShape shape = qattn_shape(a, c);
+    RC(check_workspace(a->workspace, a->workspace_bytes, shape.bytes, op));
     CACHE_OP_ENTER(ctx, stream, op);
     QAttnCall p{};
     p.q = a->q;
@@ -311,7 +360,7 @@ extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *
     p.scale = default_scale(a->scale, c->head_dim);
     p.cap = a->cap;
     hipStream_t s = (hipStream_t)stream;
-    auto run = [&](auto kernel) { return launch(s, dim3(a->n, a->heads, c->seqs), 256, kernel, p); };
-    if (c->head_dim == 128) return c->bits == 4 ? run(k_qcache_attn<128, 4>) : run(k_qcache_attn<128, 8>);
-    return c->bits == 4 ? run(k_qcache_attn<64, 4>) : run(k_qcache_attn<64, 8>);
+    if (c->head_dim == 128)
+        return c->bits == 4 ? launch_qattn_t<128, 4>(s, p, shape, a->workspace, c->seqs) : launch_qattn_t<128, 8>(s, p, shape, a->workspace, c->seqs);
+    return c->bits == 4 ? launch_qattn_t<64, 4>(s, p, shape, a->workspace, c->seqs) : launch_qattn_t<64, 8>(s, p, shape, a->workspace, c->seqs);
 }

@@ -364,65 +364,533 @@ struct QAttnCall {
     float scale, cap;
 };
 
-// One query row (token, head) a workgroup, HD / 8 lanes a key: products, softmax
-// and sums in fp32, one pass.
+// Row tiles and key shares of a call.
+struct QAttnPlan {
+    int tiles, splits;  // of a (sequence, KV head); shares a tile's keys may be cut into
+    int least;          // blocks of a share
+    float *part;        // [sequence][KV head][tile][split][rows][HD] sums
+    float2 *stat;       // their rows' reference exponents and denominators
+};
+
+constexpr int kQBlock = 32;      // keys per step of a wave
+constexpr int kQTop = 13;        // weights times steps stay below 2^(kQTop + kQSlack)
+constexpr int kQSlack = 2;       // a score may pass its row's reference by this before that moves
+constexpr float kQFar = 4194304.0f;  // up to here whole numbers and their differences are exact
+
+// the query rows of a tile: [first, last] and what they see
+struct QTile {
+    int count, len;
+    int lo, hi;          // keys some row sees
+    int all_lo, all_hi;  // keys all rows see
+};
+__device__ __forceinline__ QTile q_tile(const QAttnCall &p, int s, int first, int rows) {
+    QTile t;
+    t.count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
+    t.len = min(max(p.lens[s], 0), p.max_rows);
+    const int all = t.count * p.group;
+    if (first >= all) {
+        t.lo = t.hi = t.all_lo = t.all_hi = 0;
+        t.count = 0;
+        return t;
+    }
+    const int tok0 = first / p.group, tok1 = (min(first + rows, all) - 1) / p.group, pos = t.len - t.count;
+    t.hi = max(0, pos + tok1 + 1);
+    t.all_hi = max(0, pos + tok0 + 1);
+    t.lo = p.window ? min(t.hi, max(0, pos + tok0 - p.window + 1)) : 0;
+    t.all_lo = p.window ? max(0, pos + tok1 - p.window + 1) : 0;
+    return t;
+}
+
+// the blocks of one share of a tile's keys
+struct QShare {
+    int parts, from, to;
+};
+__device__ __forceinline__ QShare q_share(const QAttnPlan &pl, const QTile &t, int part) {
+    const int first = t.lo / kQBlock, blocks = max(0, (t.hi + kQBlock - 1) / kQBlock - first);
+    QShare h;
+    h.parts = min(pl.splits, max(1, blocks / pl.least));
+    h.from = first + (int)((int64_t)blocks * part / h.parts);
+    h.to = first + (int)((int64_t)blocks * (part + 1) / h.parts);
+    return h;
+}
+
+// Codes as fp16 numbers: 1024 + code is a bit pattern away, and the subtraction exact.
+__device__ __forceinline__ v2h code_pair(uint32_t bits, int half) {
+    return __builtin_bit_cast(v2h, bits | 0x64006400u) - (v2h){(_Float16)(1024 + half), (_Float16)(1024 + half)};
+}
+
+// One block of 32 keys as a lane loads it.  Lane l = 16u + i.  K: codes of keys i
+// and 16 + i, elements 32c + 8u .. +7 of each 32 (a matrix instruction's operand);
+// V: keys 4u .. +3 and 16 + 4u .. +3, elements 4i .. +3 of each 64.  Parameters: a
+// word of the block's 32 keys' each, to be spread over the lanes through LDS.
 template <int HD, int BITS>
-__global__ void __launch_bounds__(256) k_qcache_attn(QAttnCall p) {
+struct QBlockRegs {
     using F = QFormat<HD, BITS>;
-    constexpr int L = HD / 8, U = 256 / L;
-    __shared__ float s_m[U], s_l[U], s_acc[U][HD];
-    const int i = threadIdx.x % L, unit = threadIdx.x / L, tok = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
-    const int count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
-    if (tok >= count) return;
-    const int len = min(max(p.lens[s], 0), p.max_rows), pos = len - count + tok;
-    const int from = p.window ? max(0, pos - p.window + 1) : 0;
-    const float slope = p.slopes ? p.slopes[h] : 0.0f;
-    float q[8], acc[8] = {};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = p.q[s * p.q_ss + tok * p.q_st + h * HD + 8 * i + e];
-    float m = -INFINITY, l = 0.0f;
-    const int64_t base = s * p.cache.seq_rows + (int64_t)(h / p.group) * p.cache.capacity;
-    for (int j = from + unit; j <= pos; j += U) {
-        const int64_t at = base + j;
-        float x[8];
-        q_values<HD, BITS, false>(p.cache.codes[0] + at * F::kCodes, p.cache.params[0] + at * F::kParams, i, x);
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d = fmaf(q[e], x[e], d);
-        d += xchg<XQ1>(d);
-        d += xchg<XQ2>(d);
-        d += xchg<XM8>(d);
-        if (HD == 128) d += xchg<XM16>(d);
-        d *= p.scale;
-        if (p.cap > 0.0f) d = p.cap * tanhf(d / p.cap);
-        d -= slope * (float)(pos - j);
-        const float top = fmaxf(m, d);
-        const float keep = m == top ? 1.0f : expf(m - top), w = expf(d - top);
-        l = l * keep + w;
-        m = top;
-        q_values<HD, BITS, true>(p.cache.codes[1] + at * F::kCodes, p.cache.params[1] + at * F::kParams, i, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, x[e], acc[e] * keep);
+    static constexpr int C = HD / 32, G = F::kGroups;
+    static constexpr int kKWords = C * BITS / 4;           // of a key's codes in a lane
+    static constexpr int kVWords = HD == 64 && BITS == 4 ? 1 : HD * BITS / 512;  // (16 bits for heads of 64 in 4 bits)
+    uint32_t k[2][kKWords], v[8][kVWords], kp, vp;
+
+    template <int W>
+    __device__ __forceinline__ static void words(const uint8_t *at, uint32_t *to) {
+        if constexpr (W == 8) {
+            words<4>(at, to);
+            words<4>(at + 64, to + 4);
+        } else if constexpr (W == 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(at);
+            to[0] = x.x;
+            to[1] = x.y;
+            to[2] = x.z;
+            to[3] = x.w;
+        } else if constexpr (W == 2) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+            to[0] = x.x;
+            to[1] = x.y;
+        } else {
+            to[0] = *reinterpret_cast<const uint32_t *>(at);
+        }
     }
-    if (i == 0) {
-        s_m[unit] = m;
-        s_l[unit] = l;
-    }
+    // rows from k0 on, those past `last` as that
+    __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *vc, const uint8_t *kpar, const uint8_t *vpar, int k0, int last, int lane) {
+        const int i = lane & 15, u = lane >> 4;
+        auto row = [&](int r) { return (int64_t)min(k0 + r, last); };
+        auto get = [&](auto row_of) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s_acc[unit][8 * i + e] = acc[e];
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= HD) return;
-    float top = -INFINITY, total = 0.0f, sum = 0.0f;
-    for (int k = 0; k < U; ++k) top = fmaxf(top, s_m[k]);
-    for (int k = 0; k < U; ++k) {
-        if (s_l[k] == 0.0f) continue;
-        const float f = s_m[k] == top ? 1.0f : expf(s_m[k] - top);
-        total += s_l[k] * f;
-        sum += s_acc[k][d] * f;
+            for (int t = 0; t < 2; ++t) words<kKWords>(kc + row_of(16 * t + i) * F::kCodes + 16 * u / (kKWords == 2 ? 2 : 1), k[t]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint8_t *at = vc + row_of(16 * (j >> 2) + 4 * u + (j & 3)) * F::kCodes;
+                if constexpr (HD == 64 && BITS == 4) v[j][0] = *reinterpret_cast<const uint16_t *>(at + 2 * i);
+                else words<kVWords>(at + 4 * kVWords * i, v[j]);
+            }
+            const int key = HD == 128 ? lane >> 1 : lane & 31, word = HD == 128 ? lane & 1 : 0;
+            kp = *reinterpret_cast<const uint32_t *>(kpar + row_of(key) * (4 * G) + 4 * word);
+            vp = *reinterpret_cast<const uint32_t *>(vpar + row_of(key) * (4 * G) + 4 * word);
+        };
+        get(row);
     }
-    p.out[s * p.o_ss + tok * p.o_st + h * HD + d] = total == 0.0f ? 0.0f : sum / total;
-    if (p.lse && d == 0) p.lse[((int64_t)s * p.n + tok) * p.heads + h] = total == 0.0f ? -INFINITY : top + logf(total);
+    // K's operand of chunk c, key tile t
+    __device__ __forceinline__ v8h key(int t, int c) const {
+        v8h r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v2h x;
+            if constexpr (BITS == 4) x = code_pair(k[t][c] >> 4 * e & 0x000f000fu, 8);
+            else x = code_pair(__builtin_amdgcn_perm(0u, k[t][2 * c + e / 2], e & 1 ? 0x0c030c02u : 0x0c010c00u), 128);
+            r[2 * e] = x[0];
+            r[2 * e + 1] = x[1];
+        }
+        return r;
+    }
+    // V's operand of dim tile t: element 64 (t / 4) + 4i + t % 4 of eight keys
+    __device__ __forceinline__ v8h value(int t) const {
+        v8h r;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            v2h x;
+            if constexpr (BITS == 4) {
+                const uint32_t b = t >> 1;  // the byte that holds it
+                const uint32_t two = __builtin_amdgcn_perm(v[j + 1][0], v[j][0], 0x0c040c00u + 0x00010001u * b);
+                x = code_pair(two >> 4 * (t & 1) & 0x000f000fu, 8);
+            } else {
+                const uint32_t b = t & 3;
+                x = code_pair(__builtin_amdgcn_perm(v[j + 1][t >> 2], v[j][t >> 2], 0x0c040c00u + 0x00010001u * b), 128);
+            }
+            r[j] = x[0];
+            r[j + 1] = x[1];
+        }
+        return r;
+    }
+};
+
+// a weight times a step as halves
+__device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Float16 sb, v2h &hi, v2h &lo) {
+    hi = whole_v2h((v2h){(_Float16)__builtin_fmaf(a, (float)sa, 0.0f), (_Float16)__builtin_fmaf(b, (float)sb, 0.0f)});
+    lo = (v2h){(_Float16)__builtin_fmaf(a, (float)sa, -(float)hi[0]), (_Float16)__builtin_fmaf(b, (float)sb, -(float)hi[1])};
+}
+
+// Attention over codes.  Workgroup: a tile of query rows (token, head of the KV
+// head's group) of one sequence and KV head, and a share of its keys.  KEYS: 16 ·
+// RT rows, the four waves take its blocks of 32 keys in turn and join; otherwise
+// 16 · RT rows a wave, all of the share's blocks.
+//
+// Codes go to the matrix instructions as they are, exact in fp16, and meet query
+// rows and weights as two fp16 halves each.  Scores come out transposed (lane l:
+// query row l % 16, keys 4 (l / 16) + r of each 16), so a row's statistics stay
+// with its four lanes and its weights are the second product's operand:
+//   q . k = sum over groups of step (q . c) + mid (sum of q),
+//   out = sum over keys of (p step) . c + sum of p mid.
+// p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
+// exponent that brings V's largest step so far to 2^kQTop, so that the halves of p
+// step hold the products that count whatever V's size.  All rescales are by powers
+// of two.  NaN parameters of rows that a row does not see meet a select, never a
+// product.
+template <int HD, int BITS, int RT, bool SHAPED, bool KEYS>
+__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
+    using F = QFormat<HD, BITS>;
+    using B = QBlockRegs<HD, BITS>;
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16;
+    constexpr int kRows = 16 * RT * (KEYS ? 1 : 4);
+    constexpr int kPar = 32 * 4 * G;  // bytes of a block's parameters of K or V
+    __shared__ __attribute__((aligned(16))) uint8_t s_par[4][2 * kPar];
+    __shared__ v4f s_acc[KEYS ? 2 : 1][KEYS ? RT * T : 1][64];
+    __shared__ float s_ref[KEYS ? 4 : 1][16 * RT], s_sum[KEYS ? 4 : 1][16 * RT];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
+    const int g = blockIdx.y, s = blockIdx.z;
+    const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
+    const QTile wt = q_tile(p, s, tile * kRows, kRows);
+    if (!wt.count) return;
+    const QShare share = q_share(pl, wt, part);
+    if (part >= share.parts) return;
+    const int first = tile * kRows + (KEYS ? 0 : wave * 16 * RT), all = wt.count * p.group;
+    if (first >= all) return;  // no barriers without KEYS
+    const QTile t = KEYS ? wt : q_tile(p, s, first, 16 * RT);
+
+    const int64_t base = s * p.cache.seq_rows + (int64_t)g * p.cache.capacity;
+    const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
+    const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
+    const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
+    const int last = p.cache.capacity - 1;
+    int block = share.from, end = share.to;
+    if (KEYS) {
+        block += wave;
+    } else {
+        block = max(block, t.lo / kQBlock);
+        end = min(end, (t.hi + kQBlock - 1) / kQBlock);
+    }
+    constexpr int kStep = KEYS ? 4 : 1;
+    B cur;
+    if (block < end) cur.load(kc, vc, kp, vp, block * kQBlock, last, lane);
+
+    // query rows as halves below 2^kTop, their sums of each group
+    v8h qh[RT][C], ql[RT][C];
+    float qs[RT][G], f[RT], slope[RT];
+    int pos[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = first + 16 * rt + i;
+        const bool live = r < all;
+        const int tok = live ? r / p.group : 0, head = g * p.group + (live ? r - tok * p.group : 0);
+        pos[rt] = live ? wt.len - wt.count + tok : -1;
+        float x[C][8];
+        const float *src = p.q + s * p.q_ss + tok * p.q_st + head * HD + 8 * u;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const v4f y = *reinterpret_cast<const v4f *>(src + 32 * c + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[c][e + k] = live ? y[k] : 0.0f;
+            }
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[c][e]));
+        const int e = row_exp(groups_umax(top));
+        split_row<C>(x, e, qh[rt], ql[rt]);
+        const float up = pow2(kTop - e);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 2 * gr; c < 2 * gr + 2; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += x[c][k] * up;
+            qs[rt][gr] = groups_sum(sum);
+        }
+        // score = product · f; with a cap: tanh(product · f) · cap
+        const float size = pow2(e - kTop);
+        f[rt] = SHAPED && p.cap > 0.0f ? fminf(p.scale * size * (1.0f / p.cap), 3.0e38f) : p.scale * kLog2e * size;
+        slope[rt] = 0.0f;
+        if (SHAPED && p.slopes) {
+            const float y = p.slopes[head] * kLog2e;
+            slope[rt] = fabsf(y) == INFINITY ? copysignf(3.4028235e38f, y) : y;
+        }
+    }
+
+    v4f acc[RT][T];
+    float ref[RT], m[RT], sum[RT], mids[RT][G];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int k = 0; k < T; ++k) acc[rt][k] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        m[rt] = ref[rt] = kLowest;
+        sum[rt] = 0.0f;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) mids[rt][gr] = 0.0f;
+    }
+    uint32_t step_top = 0;  // bits of V's largest step so far
+    int raise = kQTop + 14;  // exponent that brings it below 2^kQTop
+
+    for (; block < end; block += kStep) {
+        const int k0 = block * kQBlock;
+        const bool masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
+        // parameters of keys outside the tile's are zero
+        uint32_t kw = cur.kp, vw = cur.vp;
+        if (masked) {
+            const int key = k0 + (HD == 128 ? lane >> 1 : lane & 31);
+            if (key < t.lo || key >= t.hi) kw = vw = 0;
+        }
+        // V's largest step (NaN is none)
+        const uint32_t w = HD == 128 && (lane & 1) ? 0u : vw;
+        uint32_t s0 = w & 0xffffu, s1 = HD == 128 ? w >> 16 : 0u;
+        s0 = s0 > 0x7c00u ? 0u : s0;
+        s1 = s1 > 0x7c00u ? 0u : s1;
+        const uint32_t lane_top = max(s0, s1);
+        bool moved = false;
+        if (__any(lane_top > step_top)) {
+            uint32_t y = groups_umax(lane_top);
+#pragma unroll
+            for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
+            step_top = y;
+            // step < 2^(exponent - 14), subnormal ones < 2^-14
+            const int now = kQTop + 14 - (int)(y >> 10);
+            moved = now != raise;
+            raise = now;
+        }
+        uint32_t *par = reinterpret_cast<uint32_t *>(s_par[wave]);
+        if (HD == 128 || lane < 32) {
+            par[lane] = kw;
+            par[kPar / 4 + lane] = vw;
+        }
+        wave_lds_order();
+        B next;
+        if (block + kStep < end) next.load(kc, vc, kp, vp, (block + kStep) * kQBlock, last, lane);
+
+        // scores of tile t, keys 4u .. +3
+        v8h kf[2][C];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int c = 0; c < C; ++c) kf[kt][c] = cur.key(kt, c);
+        v8h kpar[2][G], vpar[2][G];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                kpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + (16 * kt + 4 * u) * 4 * G + 16 * k);
+                vpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + kPar + (16 * kt + 4 * u) * 4 * G + 16 * k);
+            }
+        auto step_of = [&](const v8h (&x)[2][G], int j, int gr) { const int at = (j & 3) * 2 * G + gr; return x[j >> 2][at >> 3][at & 7]; };
+        auto mid_of = [&](const v8h (&x)[2][G], int j, int gr) { const int at = (j & 3) * 2 * G + G + gr; return x[j >> 2][at >> 3][at & 7]; };
+        float w8[RT][8];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float sc[8];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                v4f d[G];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    d[gr] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 2 * gr; c < 2 * gr + 2; ++c) {
+                        d[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][c], qh[rt][c], d[gr], 0, 0, 0);
+                        d[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][c], ql[rt][c], d[gr], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = 4 * kt + k;
+                    float x = 0.0f;
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        x = fmaf((float)mid_of(kpar, j, gr), qs[rt][gr], x);
+                        x = fmaf((float)step_of(kpar, j, gr), d[gr][k], x);
+                    }
+                    sc[j] = rounded(x * f[rt]);
+                }
+            }
+            if (SHAPED) {
+                if (p.cap > 0.0f) {
+                    tanh_all<8>(sc);
+                    const float up = p.cap * kLog2e;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sc[j] *= up;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sc[j] = rounded(fmaf(-slope[rt], (float)(pos[rt] - (k0 + 16 * (j >> 2) + 4 * u + (j & 3))), sc[j]));
+            }
+            if (masked) {
+                const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = k0 + 16 * (j >> 2) + 4 * u + (j & 3);
+                    sc[j] = key >= from && key <= pos[rt] ? sc[j] : -INFINITY;
+                }
+            }
+            float top = sc[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
+            if (moved || __any(top > m[rt] + kQSlack)) {
+                top = groups_max(top);
+                if (top > m[rt]) m[rt] = fminf(ceilf(top), 3.0e38f);
+                const float now = fabsf(m[rt]) < kQFar ? m[rt] - (float)raise : m[rt];
+                const float by = __builtin_amdgcn_exp2f(ref[rt] - now);
+                ref[rt] = now;
+                sum[rt] *= by;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) mids[rt][gr] *= by;
+#pragma unroll
+                for (int k = 0; k < T; ++k) acc[rt][k] *= by;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w8[rt][j] = __builtin_amdgcn_exp2f(sc[j] - ref[rt]);
+                sum[rt] += w8[rt][j];
+            }
+        }
+        // A NaN among V's parameters stays with the rows that see it: others' weights are zeros.
+        v8h wh[RT][G], wl[RT][G];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    _Float16 sa = step_of(vpar, j, gr), sb = step_of(vpar, j + 1, gr);
+                    _Float16 ma = mid_of(vpar, j, gr), mb = mid_of(vpar, j + 1, gr);
+                    if (masked) {
+                        const int key = k0 + 16 * (j >> 2) + 4 * u + (j & 3);
+                        const bool a = key >= from && key <= pos[rt], b = key + 1 >= from && key + 1 <= pos[rt];
+                        sa = a ? sa : (_Float16)0;
+                        ma = a ? ma : (_Float16)0;
+                        sb = b ? sb : (_Float16)0;
+                        mb = b ? mb : (_Float16)0;
+                    }
+                    v2h h, l;
+                    split_steps(w8[rt][j], sa, w8[rt][j + 1], sb, h, l);
+                    wh[rt][gr][j] = h[0];
+                    wh[rt][gr][j + 1] = h[1];
+                    wl[rt][gr][j] = l[0];
+                    wl[rt][gr][j + 1] = l[1];
+                    mids[rt][gr] = fmaf((float)ma, w8[rt][j], mids[rt][gr]);
+                    mids[rt][gr] = fmaf((float)mb, w8[rt][j + 1], mids[rt][gr]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < T; ++k) {
+            const v8h v = cur.value(k);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh[rt][k / 4], acc[rt][k], 0, 0, 0);
+                acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl[rt][k / 4], acc[rt][k], 0, 0, 0);
+            }
+        }
+        wave_lds_order();
+        cur = next;
+    }
+
+    // denominators and midpoints over a row's four lanes
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        sum[rt] = groups_sum(sum[rt]);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            mids[rt][gr] = groups_sum(mids[rt][gr]);
+#pragma unroll
+            for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[rt][k] += mids[rt][gr];
+        }
+    }
+    if (KEYS) {  // four waves' sums: 2 and 3 to 0 and 1, then 1 to 0
+        if (u == 0)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                s_ref[wave][16 * rt + i] = sum[rt] == 0.0f ? kLowest : ref[rt];
+                s_sum[wave][16 * rt + i] = sum[rt];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float top = kLowest, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ref[w][16 * rt + i]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) total += s_sum[w][16 * rt + i] * __builtin_amdgcn_exp2f(s_ref[w][16 * rt + i] - top);
+            const float by = __builtin_amdgcn_exp2f((sum[rt] == 0.0f ? kLowest : ref[rt]) - top);
+#pragma unroll
+            for (int k = 0; k < T; ++k) acc[rt][k] *= by;
+            sum[rt] = total;
+            ref[rt] = top;
+        }
+#pragma unroll
+        for (int half = 2; half; half >>= 1) {
+            if (wave >= half && wave < 2 * half)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int k = 0; k < T; ++k) s_acc[wave - half][rt * T + k][lane] = acc[rt][k];
+            __syncthreads();
+            if (wave < half)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int k = 0; k < T; ++k) acc[rt][k] += s_acc[wave][rt * T + k][lane];
+            __syncthreads();
+        }
+        if (wave) return;
+    }
+    const int64_t slot = (((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = first + 16 * rt + i;
+        if (r >= all) continue;
+        float *dst;
+        float by = 1.0f;
+        if (share.parts > 1) {
+            const int64_t at = slot * kRows + (r - tile * kRows);
+            dst = pl.part + at * HD;
+            if (u == 0) pl.stat[at] = make_float2(sum[rt] == 0.0f ? kLowest : ref[rt], sum[rt]);
+        } else {
+            const int tok = r / p.group, head = g * p.group + r - tok * p.group;
+            dst = p.out + s * p.o_ss + tok * p.o_st + head * HD;
+            by = sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
+            if (p.lse && u == 0)
+                p.lse[((int64_t)s * p.n + tok) * p.heads + head] =
+                    sum[rt] == 0.0f ? -INFINITY : (ref[rt] + __builtin_amdgcn_logf(sum[rt])) * 0.69314718055994531f;
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<v4f *>(dst + 64 * gr + 16 * u + 4 * k) =
+                    (v4f){acc[rt][4 * gr][k] * by, acc[rt][4 * gr + 1][k] * by, acc[rt][4 * gr + 2][k] * by, acc[rt][4 * gr + 3][k] * by};
+    }
+}
+
+// A tile's shares joined: HD / 4 lanes a row.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(256) k_qcache_join(QAttnCall p, QAttnPlan pl) {
+    constexpr int L = HD / 4, U = 256 / L;
+    const int i = threadIdx.x % L, g = blockIdx.y, s = blockIdx.z;
+    const int tile = blockIdx.x / (ROWS / U), row = (int)(blockIdx.x % (ROWS / U)) * U + (int)threadIdx.x / L;
+    const QTile t = q_tile(p, s, tile * ROWS, ROWS);
+    const int r = tile * ROWS + row;
+    if (r >= t.count * p.group) return;
+    const int parts = q_share(pl, t, 0).parts;
+    if (parts == 1) return;
+    const int64_t at = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits) * ROWS + row;
+    const float2 *stat = pl.stat + at;
+    const float *part = pl.part + at * HD + 4 * i;
+    float top = kLowest, total = 0.0f;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, stat[(int64_t)k * ROWS].x);
+    v4f sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+        const float2 st = stat[(int64_t)k * ROWS];
+        const float by = __builtin_amdgcn_exp2f(st.x - top);
+        total += st.y * by;
+        sum += *reinterpret_cast<const v4f *>(part + (int64_t)k * ROWS * HD) * by;
+    }
+    const int tok = r / p.group, head = g * p.group + r - tok * p.group;
+    *reinterpret_cast<v4f *>(p.out + s * p.o_ss + tok * p.o_st + head * HD + 4 * i) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
+    if (p.lse && i == 0)
+        p.lse[((int64_t)s * p.n + tok) * p.heads + head] =
+            total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
 }
 
 }  // namespace pocr
