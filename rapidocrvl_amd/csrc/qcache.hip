@@ -182,12 +182,22 @@ int rows_call(const pocr_rows_args *a, const pocr_qcache *c, const char *op, Row
 }
 
 int launch_rows(hipStream_t s, RowsCall p, int head_dim, int bits, int seqs) {
-    p.per = p.end[2];
-    p.chunks = 1;
+    const int own = 512 / head_dim;  // heads of a wave at a time
+    const char *ev = getenv("QC_CHUNK");
+    p.chunks = ev && (int64_t)p.n * seqs < atoi(ev) ? round_up_div(p.end[2], own) : 1;
+    p.per = round_up_div(round_up_div(p.end[2], own), p.chunks) * own;
     const dim3 grid(round_up_div((int64_t)p.n * p.chunks, 4), seqs);
+    const bool whole = !p.positions || p.adjacent || 2 * p.half == head_dim;
     auto run = [&](auto kernel) { return launch(s, grid, 256, kernel, p); };
-    if (head_dim == 128) return bits == 0 ? run(k_rows<128, 0>) : (bits == 4 ? run(k_rows<128, 4>) : run(k_rows<128, 8>));
-    return bits == 0 ? run(k_rows<64, 0>) : (bits == 4 ? run(k_rows<64, 4>) : run(k_rows<64, 8>));
+    auto with = [&](auto hd, auto b) {
+        constexpr int HD = decltype(hd)::value, B = decltype(b)::value;
+        return whole ? run(k_rows<HD, B, true>) : run(k_rows<HD, B, false>);
+    };
+    auto of = [&](auto hd) {
+        if (bits == 4) return with(hd, std::integral_constant<int, 4>{});
+        return bits == 8 ? with(hd, std::integral_constant<int, 8>{}) : with(hd, std::integral_constant<int, 0>{});
+    };
+    return head_dim == 128 ? of(std::integral_constant<int, 128>{}) : of(std::integral_constant<int, 64>{});
 }
 
 int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const char *op) {

@@ -31,111 +31,151 @@ struct QFormat {
     static constexpr int kLanes = HD / 8;             // lanes of 8 neighbouring elements
 };
 
-// Where lane i's elements 8i .. 8i+7 of a row lie among its codes: K's in one
-// piece of BITS bytes; V's, for heads of 128, as halves of two pieces, which lane
-// i ^ 8 shares.
+// A lane's elements: HD / 8 lanes hold a row of a head, lane i elements 4i .. +3 and
+// HD / 2 + 4i .. +3.  A wave's loads and stores are then whole lines, the pairs of a
+// rotation of the whole head lie in one lane, and so does V's word of eight codes.
+
+// where the codes of elements 8b .. 8b+7 of a K row begin
 template <int HD, int BITS>
-__device__ __forceinline__ int k_place(int i) {
-    const int c = i >> 2, u = i & 3;  // elements 32c + 8u
+__device__ __forceinline__ int k_place(int b) {
+    const int c = b >> 2, u = b & 3;  // elements 32c + 8u
     return BITS == 4 ? 4 * (u * (HD / 32) + c) : 64 * (c >> 1) + 16 * u + 8 * (c & 1);
 }
 
-// lane i's 8 elements of a K (V) row: mid + step * code, one rounding
+// lane i's elements of a K (V) row: mid + step * code, one rounding
 template <int HD, int BITS, bool V>
 __device__ __forceinline__ void q_values(const uint8_t *codes, const _Float16 *params, int i, float (&x)[8]) {
     using F = QFormat<HD, BITS>;
-    const float step = params[i >> 3], mid = params[F::kGroups + (i >> 3)];
-    int c[8];
-    if constexpr (BITS == 4) {
-        uint32_t w;
-        if (V && HD == 128) {
-            const uint32_t sh = 16 * (i >> 3);
-            const uint2 d = *reinterpret_cast<const uint2 *>(codes + 8 * (i & 7));
-            w = (d.x >> sh & 0xffffu) | (d.y >> sh) << 16;
-        } else {
-            w = *reinterpret_cast<const uint32_t *>(codes + (V ? 4 * i : k_place<HD, BITS>(i)));
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = w >> 4 * (V ? e : (e >> 1) + 4 * (e & 1)) & 15;
+    float step[2], mid[2];
+    if constexpr (HD == 128) {
+        const v4h y = *reinterpret_cast<const v4h *>(params);
+        step[0] = y[0], step[1] = y[1], mid[0] = y[2], mid[1] = y[3];
     } else {
-        uint2 d;
-        if (V && HD == 128) {
-            const uint8_t *at = codes + 16 * (i & 7) + 4 * (i >> 3);
-            d = make_uint2(*reinterpret_cast<const uint32_t *>(at), *reinterpret_cast<const uint32_t *>(at + 8));
-        } else {
-            d = *reinterpret_cast<const uint2 *>(codes + (V ? 8 * i : k_place<HD, BITS>(i)));
-        }
+        const v2h y = *reinterpret_cast<const v2h *>(params);
+        step[0] = step[1] = y[0], mid[0] = mid[1] = y[1];
+    }
+    const int odd = i & 1;
+    int c[8];
+    if constexpr (V && HD == 128) {
+        uint32_t w[BITS / 4];
+        if constexpr (BITS == 4) w[0] = *reinterpret_cast<const uint32_t *>(codes + 4 * i);
+        else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(codes + 8 * i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = (e < 4 ? d.x : d.y) >> 8 * (e & 3) & 255;
+        for (int e = 0; e < 8; ++e) c[e] = BITS == 4 ? w[0] >> 4 * e & 15 : w[e >> 2] >> 8 * (e & 3) & 255;
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // half a word of eight (half of 8 bytes)
+            const int b = h * (HD / 16) + (i >> 1);
+            if constexpr (BITS == 4) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + (V ? 4 * b : k_place<HD, BITS>(b))) >> (V ? 16 * odd : 8 * odd);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[4 * h + e] = w >> 4 * (V ? e : (e >> 1) + 4 * (e & 1)) & 15;
+            } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + (V ? 8 * b : k_place<HD, BITS>(b)) + 4 * odd);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[4 * h + e] = w >> 8 * e & 255;
+            }
+        }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)(c[e] - F::kHalf), step, mid);
+    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)(c[e] - F::kHalf), step[e >> 2], mid[e >> 2]);
 }
 
-// Eight lanes hold a group's 64 elements; writes lane i's codes and the group's
-// parameters.  64-bit arithmetic, so that a code next to a border is the one of
-// the definition whatever computed it.
+// midpoint and step of a group whose elements are lo to hi, and 1 / step
+template <int BITS>
+__device__ __forceinline__ void q_grid(float lo, float hi, bool bad, _Float16 &step, _Float16 &mid, double &inv) {
+    constexpr double kUp = (1 << (BITS - 1)) - 1, kDown = 1 << (BITS - 1);
+    // `rounded`: to fp32 first, which the compiler would skip
+    mid = (_Float16)rounded((float)((kUp * (double)lo + kDown * (double)hi) * (1.0 / (kUp + kDown))));
+    const double need = fmax(((double)hi - (double)mid) * (1.0 / kUp), ((double)mid - (double)lo) * (1.0 / kDown));
+    step = (_Float16)rounded((float)need);
+    if ((double)step < need) step = __builtin_bit_cast(_Float16, (uint16_t)(__builtin_bit_cast(uint16_t, step) + 1));
+    inv = step > (_Float16)0 ? 1.0 / (double)step : 0.0;
+    if (bad) step = mid = __builtin_bit_cast(_Float16, (uint16_t)0x7e00);
+}
+
+// Lane i's elements into a row's codes, with the parameters of its groups.
+// 64-bit arithmetic, so that a code next to a border is the one of the definition
+// whatever computed it.
 template <int HD, int BITS, bool V>
 __device__ __forceinline__ void q_store(float (&x)[8], uint8_t *codes, _Float16 *params, int i) {
     using F = QFormat<HD, BITS>;
-    uint32_t top = 0;
+    constexpr int G = F::kGroups, N = 8 / G;  // a lane's elements of a group
+    float lo[G], hi[G];
+    uint32_t top[G];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[e]));
-    float lo = INFINITY, hi = -INFINITY;
+    for (int g = 0; g < G; ++g) {
+        lo[g] = INFINITY;
+        hi[g] = -INFINITY;
+        top[g] = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
+        for (int e = N * g; e < N * g + N; ++e) {
+            top[g] = max(top[g], abs_bits(x[e]));
+            x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            lo[g] = fminf(lo[g], x[e]);
+            hi[g] = fmaxf(hi[g], x[e]);
+        }
     }
-    auto over = [&](auto step) {
-        constexpr int S = decltype(step)::value;
-        top = max(top, __float_as_uint(xchg<S>(__uint_as_float(top))));
-        lo = fminf(lo, xchg<S>(lo));
-        hi = fmaxf(hi, xchg<S>(hi));
+    auto over = [&](auto which) {
+        constexpr int S = decltype(which)::value;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            top[g] = max(top[g], __float_as_uint(xchg<S>(__uint_as_float(top[g]))));
+            lo[g] = fminf(lo[g], xchg<S>(lo[g]));
+            hi[g] = fmaxf(hi[g], xchg<S>(hi[g]));
+        }
     };
     over(std::integral_constant<int, XQ1>{});
     over(std::integral_constant<int, XQ2>{});
     over(std::integral_constant<int, XM8>{});
-    const bool bad = top >= 0x7f800000u;  // a NaN or an infinity
-    constexpr double kUp = F::kHalf - 1, kDown = F::kHalf;
-    // `rounded`: to fp32 first, which the compiler would skip
-    _Float16 mid = (_Float16)rounded((float)((kUp * (double)lo + kDown * (double)hi) * (1.0 / (kUp + kDown))));
-    const double need = fmax(((double)hi - (double)mid) * (1.0 / kUp), ((double)mid - (double)lo) * (1.0 / kDown));
-    _Float16 step = (_Float16)rounded((float)need);
-    if ((double)step < need) step = __builtin_bit_cast(_Float16, (uint16_t)(__builtin_bit_cast(uint16_t, step) + 1));
-    const double inv = step > (_Float16)0 ? 1.0 / (double)step : 0.0;
-    if (bad) step = mid = __builtin_bit_cast(_Float16, (uint16_t)0x7e00);
+    if constexpr (HD == 128) over(std::integral_constant<int, XM16>{});
+    _Float16 step[G], mid[G];
     uint32_t c[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const double t = fmin(fmax(rint(((double)x[e] - (double)mid) * inv), -kDown), kUp);
-        c[e] = bad ? 0u : (uint32_t)((int)t + F::kHalf);
-    }
-    if ((i & 7) == 0) {
-        params[i >> 3] = step;
-        params[F::kGroups + (i >> 3)] = mid;
-    }
-    if constexpr (BITS == 4) {
-        uint32_t w = 0;
+    for (int g = 0; g < G; ++g) {
+        const bool bad = top[g] >= 0x7f800000u;  // a NaN or an infinity
+        double inv;
+        q_grid<BITS>(lo[g], hi[g], bad, step[g], mid[g], inv);
+        // Step and reciprocal are exact to 2^-52, so no quotient rounds past the
+        // outermost codes.  Adding 3 · 2^51 rounds to a whole number, ties to even.
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w |= c[e] << 4 * (V ? e : (e >> 1) + 4 * (e & 1));
-        if (V && HD == 128) {  // words 2i' and 2i'+1 of lanes i' and i' + 8: each writes one
-            const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xF, 0xF, false);  // lane ^ 8
-            w = i < 8 ? (w & 0xffffu) | other << 16 : (other >> 16) | (w & 0xffff0000u);
-            *reinterpret_cast<uint32_t *>(codes + 8 * (i & 7) + 4 * (i >> 3)) = w;
+        for (int e = N * g; e < N * g + N; ++e) {
+            double t = ((double)x[e] - (double)mid[g]) * inv;
+            asm("" : "+v"(t));  // rounded by itself: no multiply-add with what follows
+            const uint32_t code = (uint32_t)__builtin_bit_cast(uint64_t, t + 6755399441055744.0) + F::kHalf;
+            c[e] = bad ? 0u : code;
+        }
+    }
+    if (i == 0) {
+        if constexpr (HD == 128) *reinterpret_cast<v4h *>(params) = (v4h){step[0], step[1], mid[0], mid[1]};
+        else *reinterpret_cast<v2h *>(params) = (v2h){step[0], mid[0]};
+    }
+    if constexpr (V && HD == 128) {
+        if constexpr (BITS == 4) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w |= c[e] << 4 * e;
+            *reinterpret_cast<uint32_t *>(codes + 4 * i) = w;
         } else {
-            *reinterpret_cast<uint32_t *>(codes + (V ? 4 * i : k_place<HD, BITS>(i))) = w;
+            *reinterpret_cast<uint2 *>(codes + 8 * i) =
+                make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
         }
     } else {
-        const uint2 d = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-        if (V && HD == 128) {
-            uint8_t *at = codes + 16 * (i & 7) + 4 * (i >> 3);
-            *reinterpret_cast<uint32_t *>(at) = d.x;
-            *reinterpret_cast<uint32_t *>(at + 8) = d.y;
-        } else {
-            *reinterpret_cast<uint2 *>(codes + (V ? 8 * i : k_place<HD, BITS>(i))) = d;
+        // lanes i and i ^ 1 have halves of two pieces: the even lane writes the lower elements' one
+        const int odd = i & 1, b = odd * (HD / 16) + (i >> 1);
+        uint32_t w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            w[h] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[h] |= c[4 * h + e] << (BITS == 8 ? 8 * e : 4 * (V ? e : (e >> 1) + 4 * (e & 1)));
         }
+        const uint32_t give = odd ? w[0] : w[1], keep = odd ? w[1] : w[0];
+        const uint32_t got = __float_as_uint(xchg<XQ1>(__uint_as_float(give)));
+        const uint32_t first = odd ? got : keep, second = odd ? keep : got;
+        uint8_t *at = codes + (V ? b * BITS : k_place<HD, BITS>(b));
+        if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(at) = first | second << (V ? 16 : 8);
+        else *reinterpret_cast<uint2 *>(at) = make_uint2(first, second);
     }
 }
 
@@ -213,94 +253,132 @@ __device__ __forceinline__ double xchg(double v) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Wave: one token, `per` of its heads.  A lane has 8 neighbouring elements of a
-// head (a head of 128: 16 lanes); the token's angles are computed once, one a
-// lane, and go through LDS to the lanes of every head.
-template <int HD, int BITS>  // BITS 0: fp32 destinations
+// Wave: one token, `per` of its heads, HD / 8 lanes a head.  The token's angles are
+// computed once, one a lane, and go through LDS to the lanes of every head.
+// WHOLE: pairs, where there are any, lie in one lane (all but rotations of part of
+// a head by halves).
+template <int HD, int BITS, bool WHOLE>  // BITS 0: fp32 destinations
 __global__ void __launch_bounds__(256) k_rows(RowsCall p) {
-    constexpr int L = HD / 8, U = 64 / L;
-    __shared__ double2 s_turn[4][HD / 2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.y, i = lane % L;
-    const int64_t job = (int64_t)blockIdx.x * 4 + wave;
-    const int tok = (int)(job / p.chunks), chunk = (int)(job % p.chunks);
+    constexpr int L = HD / 8, U = 64 / L, H = HD / 2;
+    __shared__ double2 s_turn[4][H];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y, i = lane % L;
+    const uint32_t job = blockIdx.x * 4 + wave;  // at most 2^22 tokens, 2^9 chunks
+    const int tok = job / (uint32_t)p.chunks, chunk = job - tok * p.chunks;
     const int count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
     if (tok >= count) return;
     const int64_t row = (p.first ? min(max(p.first[s], 0), p.rows - count) : 0) + tok;
+    const int last = min(p.end[2], (chunk + 1) * p.per);
+    struct Unit {
+        int kind, head;
+        bool live;
+    };
+    auto unit = [&](int u0) {
+        const int u = u0 + lane / L;
+        Unit t;
+        t.live = u < last;
+        t.kind = u < p.end[0] ? 0 : (u < p.end[1] ? 1 : 2);
+        t.head = u - (t.kind == 0 ? 0 : (t.kind == 1 ? p.end[0] : p.end[1]));
+        return t;
+    };
+    auto fetch = [&](int u0, v4f (&x)[2]) {
+        const Unit t = unit(u0);
+        x[0] = x[1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        if (t.live) {
+            const float *src = p.src[t.kind] + s * p.src_ss[t.kind] + tok * p.src_st[t.kind] + t.head * HD + 4 * i;
+            x[0] = *reinterpret_cast<const v4f *>(src);
+            x[1] = *reinterpret_cast<const v4f *>(src + H);
+        }
+    };
+    v4f next[2];
+    fetch(chunk * p.per, next);
     if (p.positions) {
         if (lane < p.half)
             s_turn[wave][lane] = turn((double)p.positions[((int64_t)s * p.n + tok) * p.axes + axis_of(p, lane)] * p.freqs[lane]);
         wave_lds_order();
     }
-    const int last = min(p.end[2], (chunk + 1) * p.per);
-    for (int u0 = chunk * p.per; u0 < last; u0 += U) {
-        const int u = u0 + lane / L;
-        const bool live = u < last;
-        const int kind = u < p.end[0] ? 0 : (u < p.end[1] ? 1 : 2), head = !live ? 0 : u - (kind ? p.end[kind - 1] : 0);
-        float x[8];
-        if (live) {
-            const float *src = p.src[kind] + s * p.src_ss[kind] + tok * p.src_st[kind] + head * HD + 8 * i;
+    // the turns of this lane's pairs: (4i + e, H + 4i + e), or adjacent ones
+    double2 t4[4];
+    bool turns[2] = {true, true};  // of each half of the lane's elements: are they turned at all
+    if (WHOLE && p.positions) {
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) *reinterpret_cast<v4f *>(x + e) = *reinterpret_cast<const v4f *>(src + e);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        for (int e = 0; e < 4; ++e) t4[e] = s_turn[wave][p.adjacent ? (e < 2 ? 2 * i + e : H / 2 + 2 * i + e - 2) : 4 * i + e];
+        if (p.adjacent) {
+            turns[0] = 2 * i < p.half;
+            turns[1] = H / 2 + 2 * i < p.half;
         }
-        if (kind < 2) {
-            const float *w = p.norm[kind];
-            double r = 1.0, y[8];
+    }
+    for (int u0 = chunk * p.per; u0 < last; u0 += U) {
+        const Unit t = unit(u0);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = next[e >> 2][e & 3];
+        if (u0 + U < last) fetch(u0 + U, next);
+        if (t.kind < 2) {
+            const float *w = p.norm[t.kind];
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
             if (w) {
                 double sum = 0.0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
+                for (int e = 0; e < 8; ++e) sum = fma(y[e], y[e], sum);
                 sum += xchg<XQ1>(sum);
                 sum += xchg<XQ2>(sum);
                 sum += xchg<XM8>(sum);
                 if (HD == 128) sum += xchg<XM16>(sum);
-                r = 1.0 / sqrt(sum / HD + (double)p.eps);
-            }
+                const double r = 1.0 / sqrt(sum * (1.0 / HD) + (double)p.eps);
+                const v4f w0 = *reinterpret_cast<const v4f *>(w + 4 * i), w1 = *reinterpret_cast<const v4f *>(w + H + 4 * i);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = w ? (double)x[e] * r * (double)w[8 * i + e] : (double)x[e];
+                for (int e = 0; e < 8; ++e) y[e] = y[e] * r * (double)(e < 4 ? w0 : w1)[e & 3];
+            }
             if (p.positions) {
-                if (p.adjacent) {
-                    if (8 * i < 2 * p.half)
+                if (WHOLE) {
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const double2 t = s_turn[wave][4 * i + e / 2];
-                            const double a = y[e], b = y[e + 1];
-                            y[e] = a * t.x - b * t.y;
-                            y[e + 1] = b * t.x + a * t.y;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        // one instruction stream for both orders: adjacent pairs are (0,1) (2,3) (4,5) (6,7)
+                        const double a = p.adjacent ? y[2 * e] : y[e], b = p.adjacent ? y[2 * e + 1] : y[e + 4];
+                        const bool on = turns[e >> 1];
+                        x[p.adjacent ? 2 * e : e] = (float)(on ? a * t4[e].x - b * t4[e].y : a);
+                        x[p.adjacent ? 2 * e + 1 : e + 4] = (float)(on ? b * t4[e].x + a * t4[e].y : b);
+                    }
                 } else {
-                    const int far = p.half / 8;  // lanes to a pair's other element
-                    const bool low = i < far;
-                    const int from = (lane & ~(L - 1)) + (low ? i + far : i - far);
-                    float o[8];
+                    // elements d and d + half, half a multiple of 8: chunks of four `far` chunks apart
+                    const int far = p.half / 4;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = __shfl(x[e], from & 63);
-                    if (i < 2 * far)
+                    for (int h = 0; h < 2; ++h) {
+                        const int q = h * L + i, mate = q < far ? q + far : q - far;
+                        const int from = (lane & ~(L - 1)) + (mate & (L - 1));
+                        double z[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int at = 8 * (low ? i + far : i - far) + e;
-                            const double2 t = s_turn[wave][8 * (low ? i : i - far) + e];
-                            const double b = w ? (double)o[e] * r * (double)w[at] : (double)o[e];
-                            y[e] = low ? y[e] * t.x - b * t.y : y[e] * t.x + b * t.y;
+                        for (int e = 0; e < 4; ++e) {
+                            const double lower = __shfl(y[e], from & 63), upper = __shfl(y[4 + e], from & 63);
+                            z[e] = mate & L ? upper : lower;
                         }
-                }
-            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+                        for (int e = 0; e < 4; ++e) {
+                            const double own = y[4 * h + e];
+                            const int at = 4 * (q < far ? q : q - far) + e;
+                            const double2 tr = s_turn[wave][min(at, H - 1)];
+                            x[4 * h + e] = (float)(q < far ? own * tr.x - z[e] * tr.y : (q < 2 * far ? own * tr.x + z[e] * tr.y : own));
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+            }
         }
-        if (!live) continue;
-        if (BITS && kind) {
+        if (!t.live) continue;
+        if (BITS && t.kind) {
             constexpr int B = BITS ? BITS : 4;
             using F = QFormat<HD, B>;
-            const int64_t at = s * p.cache.seq_rows + (int64_t)head * p.cache.capacity + row;
-            if (kind == 1) q_store<HD, B, false>(x, p.cache.codes[0] + at * F::kCodes, p.cache.params[0] + at * F::kParams, i);
+            const int64_t at = s * p.cache.seq_rows + (int64_t)t.head * p.cache.capacity + row;
+            if (t.kind == 1) q_store<HD, B, false>(x, p.cache.codes[0] + at * F::kCodes, p.cache.params[0] + at * F::kParams, i);
             else q_store<HD, B, true>(x, p.cache.codes[1] + at * F::kCodes, p.cache.params[1] + at * F::kParams, i);
         } else {
-            float *dst = p.dst[kind] + s * p.dst_ss[kind] + (kind ? row : tok) * p.dst_st[kind] + head * HD + 8 * i;
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) *reinterpret_cast<v4f *>(dst + e) = *reinterpret_cast<const v4f *>(x + e);
+            float *dst = p.dst[t.kind] + s * p.dst_ss[t.kind] + (t.kind ? row : tok) * p.dst_st[t.kind] + t.head * HD + 4 * i;
+            *reinterpret_cast<v4f *>(dst) = (v4f){x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<v4f *>(dst + H) = (v4f){x[4], x[5], x[6], x[7]};
         }
     }
 }
@@ -341,9 +419,9 @@ __global__ void __launch_bounds__(256) k_qcache_read(QReadCall p) {
         if (!p.dst[V]) return;
         float x[8];
         q_values<HD, BITS, V == 1>(p.cache.codes[V] + at * F::kCodes, p.cache.params[V] + at * F::kParams, i, x);
-        float *dst = p.dst[V] + s * p.dst_ss[V] + t * p.dst_st[V] + g * HD + 8 * i;
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) *reinterpret_cast<v4f *>(dst + e) = *reinterpret_cast<const v4f *>(x + e);
+        float *dst = p.dst[V] + s * p.dst_ss[V] + t * p.dst_st[V] + g * HD + 4 * i;
+        *reinterpret_cast<v4f *>(dst) = (v4f){x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<v4f *>(dst + HD / 2) = (v4f){x[4], x[5], x[6], x[7]};
     };
     one(std::integral_constant<int, 0>{});
     one(std::integral_constant<int, 1>{});
