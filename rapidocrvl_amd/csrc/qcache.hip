@@ -183,15 +183,20 @@ int rows_call(const pocr_rows_args *a, const pocr_qcache *c, const char *op, Row
 
 int launch_rows(hipStream_t s, RowsCall p, int head_dim, int bits, int seqs) {
     const int own = 512 / head_dim;  // heads of a wave at a time
-    const char *ev = getenv("QC_CHUNK");
-    p.chunks = ev && (int64_t)p.n * seqs < atoi(ev) ? round_up_div(p.end[2], own) : 1;
+    const int64_t total = (int64_t)p.n * seqs;
+    // Few tokens: a wave for each four heads (1,345 tokens of 20 heads 8.74 us in one
+    // wave a token, 8.50 in five; 8,192 tokens 48.6 : 49.6).  Many: several tokens a
+    // wave, as long as 8,192 waves are left (18 x 1,345 tokens of 4 heads in 2,048,
+    // 4,096, 8,192 and 16,384 waves 28, 24, 19 and 20 us).
+    p.chunks = total < 2048 ? round_up_div(p.end[2], own) : 1;
     p.per = round_up_div(round_up_div(p.end[2], own), p.chunks) * own;
-    const dim3 grid(round_up_div((int64_t)p.n * p.chunks, 4), seqs);
-    const bool whole = !p.positions || p.adjacent || 2 * p.half == head_dim;
-    auto run = [&](auto kernel) { return launch(s, grid, 256, kernel, p); };
+    p.tokens = (int)std::min<int64_t>(p.n, std::max<int64_t>(1, total * p.chunks / 8192));
+    const dim3 grid(round_up_div((int64_t)round_up_div(p.n, p.tokens) * p.chunks, 4), seqs);
+    const int pairs = p.adjacent ? kPairsAdjacent : (!p.positions || 2 * p.half == head_dim ? kPairsWhole : kPairsPart);
     auto with = [&](auto hd, auto b) {
         constexpr int HD = decltype(hd)::value, B = decltype(b)::value;
-        return whole ? run(k_rows<HD, B, true>) : run(k_rows<HD, B, false>);
+        auto *kernel = pairs == kPairsWhole ? k_rows<HD, B, kPairsWhole> : (pairs == kPairsAdjacent ? k_rows<HD, B, kPairsAdjacent> : k_rows<HD, B, kPairsPart>);
+        return launch(s, grid, 256, kernel, p);
     };
     auto of = [&](auto hd) {
         if (bits == 4) return with(hd, std::integral_constant<int, 4>{});
@@ -223,7 +228,7 @@ struct QShape {
 QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     QShape q;
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
-    q.rt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    q.rt = rows <= 16 ? 1 : 2;
     q.keys = rows < 1024;
     q.rows = 16 * q.rt * (q.keys ? 1 : 4);
     q.tiles = round_up_div(rows, q.rows);
@@ -254,9 +259,8 @@ int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work,
 template <int HD, int BITS>
 int launch_qattn_t(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
     if (q.rt == 1) return launch_qattn<HD, BITS, 1, true>(s, p, q, work, seqs);
-    if (q.rt == 2) return launch_qattn<HD, BITS, 2, true>(s, p, q, work, seqs);
-    if (q.keys) return launch_qattn<HD, BITS, 4, true>(s, p, q, work, seqs);
-    return launch_qattn<HD, BITS, 4, false>(s, p, q, work, seqs);
+    if (q.keys) return launch_qattn<HD, BITS, 2, true>(s, p, q, work, seqs);
+    return launch_qattn<HD, BITS, 2, false>(s, p, q, work, seqs);
 }
 
 }  // namespace

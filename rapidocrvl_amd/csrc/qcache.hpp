@@ -83,7 +83,7 @@ __device__ __forceinline__ void q_values(const uint8_t *codes, const _Float16 *p
 
 // midpoint and step of a group whose elements are lo to hi, and 1 / step
 template <int BITS>
-__device__ __forceinline__ void q_grid(float lo, float hi, bool bad, _Float16 &step, _Float16 &mid, double &inv) {
+__device__ __forceinline__ void q_grid(float lo, float hi, _Float16 &step, _Float16 &mid, double &inv) {
     constexpr double kUp = (1 << (BITS - 1)) - 1, kDown = 1 << (BITS - 1);
     // `rounded`: to fp32 first, which the compiler would skip
     mid = (_Float16)rounded((float)((kUp * (double)lo + kDown * (double)hi) * (1.0 / (kUp + kDown))));
@@ -91,92 +91,121 @@ __device__ __forceinline__ void q_grid(float lo, float hi, bool bad, _Float16 &s
     step = (_Float16)rounded((float)need);
     if ((double)step < need) step = __builtin_bit_cast(_Float16, (uint16_t)(__builtin_bit_cast(uint16_t, step) + 1));
     inv = step > (_Float16)0 ? 1.0 / (double)step : 0.0;
-    if (bad) step = mid = __builtin_bit_cast(_Float16, (uint16_t)0x7e00);
 }
 
 // Lane i's elements into a row's codes, with the parameters of its groups.
 // 64-bit arithmetic, so that a code next to a border is the one of the definition
-// whatever computed it.
-template <int HD, int BITS, bool V>
-__device__ __forceinline__ void q_store(float (&x)[8], uint8_t *codes, _Float16 *params, int i) {
+// whatever computed it.  K and V rows side by side in a wave take one instruction
+// stream (`v`: this lane's is a V row): they differ in the order of what is packed.
+template <int HD, int BITS>
+__device__ __forceinline__ void q_store(const float (&x)[8], uint8_t *codes, _Float16 *params, int i, bool v) {
     using F = QFormat<HD, BITS>;
-    constexpr int G = F::kGroups, N = 8 / G;  // a lane's elements of a group
-    float lo[G], hi[G];
-    uint32_t top[G];
+    constexpr int G = F::kGroups;
+    float y[8], lo, hi, odd_sum = 0.0f;  // of the lane's group: HD 128: lanes 0-7 the first, 8-15 the second
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        lo[g] = INFINITY;
-        hi[g] = -INFINITY;
-        top[g] = 0;
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_fmed3f(x[e], -65504.0f, 65504.0f);
+    // NaN where an element is NaN or infinite
+    float bad_sum[2];
 #pragma unroll
-        for (int e = N * g; e < N * g + N; ++e) {
-            top[g] = max(top[g], abs_bits(x[e]));
-            x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-            lo[g] = fminf(lo[g], x[e]);
-            hi[g] = fmaxf(hi[g], x[e]);
-        }
+    for (int h = 0; h < 2; ++h) {
+        bad_sum[h] = x[4 * h] * 0.0f;
+#pragma unroll
+        for (int e = 1; e < 4; ++e) bad_sum[h] = fmaf(x[4 * h + e], 0.0f, bad_sum[h]);
+    }
+    auto lowest = [&](int h) { return fminf(fminf(y[4 * h], y[4 * h + 1]), fminf(y[4 * h + 2], y[4 * h + 3])); };
+    auto highest = [&](int h) { return fmaxf(fmaxf(y[4 * h], y[4 * h + 1]), fmaxf(y[4 * h + 2], y[4 * h + 3])); };
+    const float l0 = lowest(0), l1 = lowest(1), h0 = highest(0), h1 = highest(1);
+    const bool upper = HD == 128 && i >= 8;
+    auto swap8 = [](float a) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0x128, 0xF, 0xF, false)); };  // lane ^ 8
+    if constexpr (G == 2) {
+        lo = fminf(upper ? l1 : l0, swap8(upper ? l0 : l1));
+        hi = fmaxf(upper ? h1 : h0, swap8(upper ? h0 : h1));
+        odd_sum = (upper ? bad_sum[1] : bad_sum[0]) + swap8(upper ? bad_sum[0] : bad_sum[1]);
+    } else {
+        lo = fminf(l0, l1);
+        hi = fmaxf(h0, h1);
+        odd_sum = bad_sum[0] + bad_sum[1];
     }
     auto over = [&](auto which) {
         constexpr int S = decltype(which)::value;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            top[g] = max(top[g], __float_as_uint(xchg<S>(__uint_as_float(top[g]))));
-            lo[g] = fminf(lo[g], xchg<S>(lo[g]));
-            hi[g] = fmaxf(hi[g], xchg<S>(hi[g]));
-        }
+        lo = fminf(lo, xchg<S>(lo));
+        hi = fmaxf(hi, xchg<S>(hi));
+        odd_sum += xchg<S>(odd_sum);
     };
     over(std::integral_constant<int, XQ1>{});
     over(std::integral_constant<int, XQ2>{});
     over(std::integral_constant<int, XM8>{});
-    if constexpr (HD == 128) over(std::integral_constant<int, XM16>{});
-    _Float16 step[G], mid[G];
+    _Float16 own_step, own_mid;
+    double own_inv;
+    q_grid<BITS>(lo, hi, own_step, own_mid, own_inv);
+    v2h grid[2];  // step and midpoint of each half's group
+    double inv[2];
+    bool bad[2];
+    const bool own_bad = odd_sum != odd_sum;
+    const v2h nan = __builtin_bit_cast(v2h, 0x7e007e00u);
+    grid[0] = grid[1] = own_bad ? nan : (v2h){own_step, own_mid};
+    inv[0] = inv[1] = own_inv;
+    bad[0] = bad[1] = own_bad;
+    if constexpr (G == 2) {
+        const v2h other = __builtin_bit_cast(v2h, swap8(__builtin_bit_cast(float, grid[0])));
+        const uint64_t w = __builtin_bit_cast(uint64_t, own_inv);
+        const uint32_t w0 = __float_as_uint(swap8(__uint_as_float((uint32_t)w))), w1 = __float_as_uint(swap8(__uint_as_float((uint32_t)(w >> 32))));
+        const double other_inv = __builtin_bit_cast(double, (uint64_t)w1 << 32 | w0);
+        grid[0] = upper ? other : grid[0];
+        grid[1] = upper ? grid[1] : other;
+        inv[0] = upper ? other_inv : own_inv;
+        inv[1] = upper ? own_inv : other_inv;
+        bad[0] = grid[0][1] != grid[0][1];
+        bad[1] = grid[1][1] != grid[1][1];
+    }
+    // Step and reciprocal are exact to 2^-52, so no quotient rounds past the outermost
+    // codes.  Adding 3 · 2^51 rounds to a whole number, ties to even, into the low bits.
     uint32_t c[8];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const bool bad = top[g] >= 0x7f800000u;  // a NaN or an infinity
-        double inv;
-        q_grid<BITS>(lo[g], hi[g], bad, step[g], mid[g], inv);
-        // Step and reciprocal are exact to 2^-52, so no quotient rounds past the
-        // outermost codes.  Adding 3 · 2^51 rounds to a whole number, ties to even.
-#pragma unroll
-        for (int e = N * g; e < N * g + N; ++e) {
-            double t = ((double)x[e] - (double)mid[g]) * inv;
-            asm("" : "+v"(t));  // rounded by itself: no multiply-add with what follows
-            const uint32_t code = (uint32_t)__builtin_bit_cast(uint64_t, t + 6755399441055744.0) + F::kHalf;
-            c[e] = bad ? 0u : code;
-        }
+    for (int e = 0; e < 8; ++e) {
+        double t = ((double)y[e] - (double)grid[e >> 2][1]) * inv[e >> 2];
+        asm("" : "+v"(t));  // rounded by itself: no multiply-add with what follows
+        c[e] = (uint32_t)__builtin_bit_cast(uint64_t, t + (6755399441055744.0 + F::kHalf));
     }
     if (i == 0) {
-        if constexpr (HD == 128) *reinterpret_cast<v4h *>(params) = (v4h){step[0], step[1], mid[0], mid[1]};
-        else *reinterpret_cast<v2h *>(params) = (v2h){step[0], mid[0]};
+        if constexpr (G == 2) *reinterpret_cast<v4h *>(params) = (v4h){grid[0][0], grid[1][0], grid[0][1], grid[1][1]};
+        else *reinterpret_cast<v2h *>(params) = grid[0];
     }
-    if constexpr (V && HD == 128) {
-        if constexpr (BITS == 4) {
-            uint32_t w = 0;
+    uint32_t kw[2], vw[2];  // the halves' codes as K and as V packs them
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w |= c[e] << 4 * e;
-            *reinterpret_cast<uint32_t *>(codes + 4 * i) = w;
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t *d = c + 4 * h;
+        if constexpr (BITS == 8) {
+            kw[h] = vw[h] = bad[h] ? 0u : d[0] | d[1] << 8 | d[2] << 16 | d[3] << 24;
         } else {
-            *reinterpret_cast<uint2 *>(codes + 8 * i) =
-                make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+            kw[h] = bad[h] ? 0u : d[0] | d[1] << 16 | d[2] << 4 | d[3] << 20;
+            vw[h] = bad[h] ? 0u : d[0] | d[1] << 4 | d[2] << 8 | d[3] << 12;
         }
-    } else {
-        // lanes i and i ^ 1 have halves of two pieces: the even lane writes the lower elements' one
-        const int odd = i & 1, b = odd * (HD / 16) + (i >> 1);
-        uint32_t w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            w[h] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[h] |= c[4 * h + e] << (BITS == 8 ? 8 * e : 4 * (V ? e : (e >> 1) + 4 * (e & 1)));
-        }
-        const uint32_t give = odd ? w[0] : w[1], keep = odd ? w[1] : w[0];
-        const uint32_t got = __float_as_uint(xchg<XQ1>(__uint_as_float(give)));
-        const uint32_t first = odd ? got : keep, second = odd ? keep : got;
-        uint8_t *at = codes + (V ? b * BITS : k_place<HD, BITS>(b));
-        if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(at) = first | second << (V ? 16 : 8);
-        else *reinterpret_cast<uint2 *>(at) = make_uint2(first, second);
     }
+    // Lanes i and i ^ 1 have halves of two pieces of eight neighbours: the even lane
+    // writes the lower elements' one.  V's pieces for heads of 128 are the lane's own.
+    const int odd = i & 1, b = odd * (HD / 16) + (i >> 1);
+    auto pieces = [&](const uint32_t (&w)[2], uint32_t &first, uint32_t &second) {
+        const uint32_t got = __float_as_uint(xchg<XQ1>(__uint_as_float(odd ? w[0] : w[1])));
+        first = odd ? got : w[0];
+        second = odd ? w[1] : got;
+    };
+    uint32_t first, second;
+    pieces(kw, first, second);
+    int at = k_place<HD, BITS>(b);
+    if constexpr (HD == 128) {
+        first = v ? vw[0] : first;
+        second = v ? vw[1] : second;
+        at = v ? BITS * i : at;
+    } else {
+        uint32_t vf, vs;
+        pieces(vw, vf, vs);
+        first = v ? vf : first;
+        second = v ? vs : second;
+        at = v ? BITS * b : at;
+    }
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(codes + at) = first | second << (v ? 16 : 8);
+    else *reinterpret_cast<uint2 *>(codes + at) = make_uint2(first, second);
 }
 
 // ---------------------------------------------------------------------------
@@ -195,6 +224,7 @@ struct RowsCall {
     int n, half, axes, sections[4], interleaved, adjacent;
     int rows;             // of a destination
     int per, chunks;      // heads of a wave, waves of a token
+    int tokens;           // of a wave, one after the other
     float eps;
 };
 
@@ -253,93 +283,117 @@ __device__ __forceinline__ double xchg(double v) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Wave: one token, `per` of its heads, HD / 8 lanes a head.  The token's angles are
-// computed once, one a lane, and go through LDS to the lanes of every head.
-// WHOLE: pairs, where there are any, lie in one lane (all but rotations of part of
-// a head by halves).
-template <int HD, int BITS, bool WHOLE>  // BITS 0: fp32 destinations
+// 1 / sqrt(x): the instruction's estimate, then a step of third and one of second order
+__device__ __forceinline__ double inverse_root(double x) {
+    double r = __builtin_amdgcn_rsq(x);
+    double e = fma(-x * r, r, 1.0);
+    r = fma(r * e, fma(e, 0.375, 0.5), r);
+    e = fma(-x * r, r, 1.0);
+    return fma(r * e, 0.5, r);
+}
+
+// how a head's pairs lie: (i, H + i) over the whole of it, (2i, 2i + 1), or over part of it by halves
+enum : int { kPairsWhole = 0, kPairsAdjacent = 1, kPairsPart = 2 };
+
+// Wave: `tokens` tokens one after the other, `per` heads of each, HD / 8 lanes a
+// head; the next heads are on their way meanwhile.  A token's angles are computed
+// once, one a lane, and go through LDS to the lanes of every head.
+template <int HD, int BITS, int PAIRS>  // BITS 0: fp32 destinations
 __global__ void __launch_bounds__(256) k_rows(RowsCall p) {
     constexpr int L = HD / 8, U = 64 / L, H = HD / 2;
     __shared__ double2 s_turn[4][H];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y, i = lane % L;
     const uint32_t job = blockIdx.x * 4 + wave;  // at most 2^22 tokens, 2^9 chunks
-    const int tok = job / (uint32_t)p.chunks, chunk = job - tok * p.chunks;
+    const int step = job / (uint32_t)p.chunks, chunk = job - step * p.chunks;
     const int count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
-    if (tok >= count) return;
-    const int64_t row = (p.first ? min(max(p.first[s], 0), p.rows - count) : 0) + tok;
-    const int last = min(p.end[2], (chunk + 1) * p.per);
-    struct Unit {
-        int kind, head;
-        bool live;
-    };
-    auto unit = [&](int u0) {
-        const int u = u0 + lane / L;
-        Unit t;
-        t.live = u < last;
-        t.kind = u < p.end[0] ? 0 : (u < p.end[1] ? 1 : 2);
-        t.head = u - (t.kind == 0 ? 0 : (t.kind == 1 ? p.end[0] : p.end[1]));
-        return t;
-    };
-    auto fetch = [&](int u0, v4f (&x)[2]) {
-        const Unit t = unit(u0);
+    int tok = step * p.tokens;
+    const int end = min(count, tok + p.tokens), begin = chunk * p.per, last = min(p.end[2], begin + p.per);
+    if (tok >= end) return;
+    const int64_t row0 = p.first ? min(max(p.first[s], 0), p.rows - count) : 0;
+    // of a token's unit u0 + lane / L: 0 q, 1 k, 2 v, and the head
+    auto kind_of = [&](int u) { return u < p.end[0] ? 0 : (u < p.end[1] ? 1 : 2); };
+    auto pick = [](int kind, auto a, auto b, auto c) { return kind == 0 ? a : (kind == 1 ? b : c); };
+    auto fetch = [&](int t, int u0, v4f (&x)[2]) {
+        const int u = u0 + lane / L, kind = kind_of(u);
         x[0] = x[1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        if (t.live) {
-            const float *src = p.src[t.kind] + s * p.src_ss[t.kind] + tok * p.src_st[t.kind] + t.head * HD + 4 * i;
+        if (u < last) {
+            const float *at[3];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) at[k] = p.src[k] + s * p.src_ss[k] + t * p.src_st[k];
+            const float *src = pick(kind, at[0], at[1], at[2]) + (u - pick(kind, 0, p.end[0], p.end[1])) * HD + 4 * i;
             x[0] = *reinterpret_cast<const v4f *>(src);
             x[1] = *reinterpret_cast<const v4f *>(src + H);
         }
     };
+    const bool turned = p.positions && lane < p.half;
+    const int32_t *place = p.positions + (int64_t)s * p.n * p.axes + (turned ? axis_of(p, lane) : 0);
+    double freq = 0.0;
+    int position = 0;
+    if (turned) {
+        freq = p.freqs[lane];
+        position = place[(int64_t)tok * p.axes];
+    }
     v4f next[2];
-    fetch(chunk * p.per, next);
-    if (p.positions) {
-        if (lane < p.half)
-            s_turn[wave][lane] = turn((double)p.positions[((int64_t)s * p.n + tok) * p.axes + axis_of(p, lane)] * p.freqs[lane]);
-        wave_lds_order();
-    }
-    // the turns of this lane's pairs: (4i + e, H + 4i + e), or adjacent ones
-    double2 t4[4];
-    bool turns[2] = {true, true};  // of each half of the lane's elements: are they turned at all
-    if (WHOLE && p.positions) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t4[e] = s_turn[wave][p.adjacent ? (e < 2 ? 2 * i + e : H / 2 + 2 * i + e - 2) : 4 * i + e];
-        if (p.adjacent) {
-            turns[0] = 2 * i < p.half;
-            turns[1] = H / 2 + 2 * i < p.half;
-        }
-    }
-    for (int u0 = chunk * p.per; u0 < last; u0 += U) {
-        const Unit t = unit(u0);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = next[e >> 2][e & 3];
-        if (u0 + U < last) fetch(u0 + U, next);
-        if (t.kind < 2) {
-            const float *w = p.norm[t.kind];
-            double y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[e];
-            if (w) {
-                double sum = 0.0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = fma(y[e], y[e], sum);
-                sum += xchg<XQ1>(sum);
-                sum += xchg<XQ2>(sum);
-                sum += xchg<XM8>(sum);
-                if (HD == 128) sum += xchg<XM16>(sum);
-                const double r = 1.0 / sqrt(sum * (1.0 / HD) + (double)p.eps);
-                const v4f w0 = *reinterpret_cast<const v4f *>(w + 4 * i), w1 = *reinterpret_cast<const v4f *>(w + H + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = y[e] * r * (double)(e < 4 ? w0 : w1)[e & 3];
+    fetch(tok, begin, next);
+    for (; tok < end; ++tok) {
+        double2 t4[4];  // the turns of this lane's pairs
+        bool turns[2] = {true, true};
+        if (p.positions) {
+            if (turned) {
+                s_turn[wave][lane] = turn((double)position * freq);
+                if (tok + 1 < end) position = place[(int64_t)(tok + 1) * p.axes];
             }
-            if (p.positions) {
-                if (WHOLE) {
+            wave_lds_order();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = PAIRS == kPairsAdjacent ? (e < 2 ? 2 * i + e : H / 2 + 2 * i + e - 2) : 4 * i + e;
+                if (PAIRS != kPairsPart) t4[e] = s_turn[wave][at];
+            }
+            if (PAIRS == kPairsAdjacent) {
+                turns[0] = 2 * i < p.half;
+                turns[1] = H / 2 + 2 * i < p.half;
+            }
+        }
+        for (int u0 = begin; u0 < last; u0 += U) {
+            const int u = u0 + lane / L, kind = kind_of(u), head = u - pick(kind, 0, p.end[0], p.end[1]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = next[e >> 2][e & 3];
+            if (u0 + U < last) fetch(tok, u0 + U, next);
+            else if (tok + 1 < end) fetch(tok + 1, begin, next);
+            const float *w = kind == 0 ? p.norm[0] : p.norm[1];
+            if (kind < 2 && (w || p.positions)) {
+                double y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[e];
+                if (w) {
+                    double sum = 0.0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = fma(y[e], y[e], sum);
+                    sum += xchg<XQ1>(sum);
+                    sum += xchg<XQ2>(sum);
+                    sum += xchg<XM8>(sum);
+                    if (HD == 128) sum += xchg<XM16>(sum);
+                    const double r = inverse_root(fma(sum, 1.0 / HD, (double)p.eps));
+                    const v4f w0 = *reinterpret_cast<const v4f *>(w + 4 * i), w1 = *reinterpret_cast<const v4f *>(w + H + 4 * i);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = y[e] * r * (double)(e < 4 ? w0 : w1)[e & 3];
+                }
+                if (!p.positions) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+                } else if (PAIRS == kPairsWhole) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        // one instruction stream for both orders: adjacent pairs are (0,1) (2,3) (4,5) (6,7)
-                        const double a = p.adjacent ? y[2 * e] : y[e], b = p.adjacent ? y[2 * e + 1] : y[e + 4];
-                        const bool on = turns[e >> 1];
-                        x[p.adjacent ? 2 * e : e] = (float)(on ? a * t4[e].x - b * t4[e].y : a);
-                        x[p.adjacent ? 2 * e + 1 : e + 4] = (float)(on ? b * t4[e].x + a * t4[e].y : b);
+                        x[e] = (float)(y[e] * t4[e].x - y[4 + e] * t4[e].y);
+                        x[4 + e] = (float)(y[4 + e] * t4[e].x + y[e] * t4[e].y);
+                    }
+                } else if (PAIRS == kPairsAdjacent) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const double a = y[2 * e], b = y[2 * e + 1];
+                        x[2 * e] = (float)(turns[e >> 1] ? a * t4[e].x - b * t4[e].y : a);
+                        x[2 * e + 1] = (float)(turns[e >> 1] ? b * t4[e].x + a * t4[e].y : b);
                     }
                 } else {
                     // elements d and d + half, half a multiple of 8: chunks of four `far` chunks apart
@@ -348,38 +402,35 @@ __global__ void __launch_bounds__(256) k_rows(RowsCall p) {
                     for (int h = 0; h < 2; ++h) {
                         const int q = h * L + i, mate = q < far ? q + far : q - far;
                         const int from = (lane & ~(L - 1)) + (mate & (L - 1));
-                        double z[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const double lower = __shfl(y[e], from & 63), upper = __shfl(y[4 + e], from & 63);
-                            z[e] = mate & L ? upper : lower;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const double own = y[4 * h + e];
-                            const int at = 4 * (q < far ? q : q - far) + e;
-                            const double2 tr = s_turn[wave][min(at, H - 1)];
-                            x[4 * h + e] = (float)(q < far ? own * tr.x - z[e] * tr.y : (q < 2 * far ? own * tr.x + z[e] * tr.y : own));
+                            const double own = y[4 * h + e], z = mate & L ? upper : lower;
+                            const double2 tr = s_turn[wave][min(4 * (q < far ? q : q - far) + e, H - 1)];
+                            x[4 * h + e] = (float)(q < far ? own * tr.x - z * tr.y : (q < 2 * far ? own * tr.x + z * tr.y : own));
                         }
                     }
                 }
+            }
+            if (u >= last) continue;
+            const int64_t row = row0 + tok;
+            if (BITS && kind) {
+                constexpr int B = BITS ? BITS : 4;
+                using F = QFormat<HD, B>;
+                const int64_t at = s * p.cache.seq_rows + (int64_t)head * p.cache.capacity + row;
+                const bool v = kind == 2;
+                q_store<HD, B>(x, (v ? p.cache.codes[1] : p.cache.codes[0]) + at * F::kCodes,
+                               (v ? p.cache.params[1] : p.cache.params[0]) + at * F::kParams, i, v);
             } else {
+                float *at[3];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+                for (int k = 0; k < 3; ++k) at[k] = p.dst[k] + s * p.dst_ss[k] + (k ? row : tok) * p.dst_st[k];
+                float *dst = pick(kind, at[0], at[1], at[2]) + head * HD + 4 * i;
+                *reinterpret_cast<v4f *>(dst) = (v4f){x[0], x[1], x[2], x[3]};
+                *reinterpret_cast<v4f *>(dst + H) = (v4f){x[4], x[5], x[6], x[7]};
             }
         }
-        if (!t.live) continue;
-        if (BITS && t.kind) {
-            constexpr int B = BITS ? BITS : 4;
-            using F = QFormat<HD, B>;
-            const int64_t at = s * p.cache.seq_rows + (int64_t)t.head * p.cache.capacity + row;
-            if (t.kind == 1) q_store<HD, B, false>(x, p.cache.codes[0] + at * F::kCodes, p.cache.params[0] + at * F::kParams, i);
-            else q_store<HD, B, true>(x, p.cache.codes[1] + at * F::kCodes, p.cache.params[1] + at * F::kParams, i);
-        } else {
-            float *dst = p.dst[t.kind] + s * p.dst_ss[t.kind] + (t.kind ? row : tok) * p.dst_st[t.kind] + t.head * HD + 4 * i;
-            *reinterpret_cast<v4f *>(dst) = (v4f){x[0], x[1], x[2], x[3]};
-            *reinterpret_cast<v4f *>(dst + H) = (v4f){x[4], x[5], x[6], x[7]};
-        }
+        if (p.positions) wave_lds_order();  // all lanes have read this token's turns
     }
 }
 
@@ -492,22 +543,31 @@ __device__ __forceinline__ QShare q_share(const QAttnPlan &pl, const QTile &t, i
     return h;
 }
 
-// Codes as fp16 numbers: 1024 + code is a bit pattern away, and the subtraction exact.
-__device__ __forceinline__ v2h code_pair(uint32_t bits, int half) {
-    return __builtin_bit_cast(v2h, bits | 0x64006400u) - (v2h){(_Float16)(1024 + half), (_Float16)(1024 + half)};
+// Codes as fp16 numbers: 1024 + n is a bit pattern away from n < 1024, and taking
+// 1024 off again exact.  `magic` holds the pattern in a vector register, where one
+// instruction can both mask and set bits (it may name a single scalar one).
+__device__ __forceinline__ uint32_t code_magic() {
+    uint32_t m = 0x64006400u;
+    asm("" : "+v"(m));
+    return m;
+}
+template <int LESS>  // 1024 + what the codes are stored with
+__device__ __forceinline__ v2h code_pair(uint32_t bits, uint32_t mask, uint32_t magic) {
+    return __builtin_bit_cast(v2h, (bits & mask) | magic) - (v2h){(_Float16)LESS, (_Float16)LESS};
 }
 
-// One block of 32 keys as a lane loads it.  Lane l = 16u + i.  K: codes of keys i
-// and 16 + i, elements 32c + 8u .. +7 of each 32 (a matrix instruction's operand);
-// V: keys 4u .. +3 and 16 + 4u .. +3, elements 4i .. +3 of each 64.  Parameters: a
-// word of the block's 32 keys' each, to be spread over the lanes through LDS.
+// Codes of 32 keys as a lane loads and uses them.  Lane l = 16u + i.  K: keys i and
+// 16 + i, elements 32c + 8u .. +7 of each 32 (a matrix instruction's operand); V: keys
+// 4u .. +3 and 16 + 4u .. +3, elements 4i .. +3 of each 64.  Of two codes of 4 bits
+// in a byte the upper one stays where it is, 16 times too large: the query row's
+// elements and the sums that meet it are that much smaller.
 template <int HD, int BITS>
-struct QBlockRegs {
+struct QCodes {
     using F = QFormat<HD, BITS>;
-    static constexpr int C = HD / 32, G = F::kGroups;
+    static constexpr int C = HD / 32;
     static constexpr int kKWords = C * BITS / 4;           // of a key's codes in a lane
     static constexpr int kVWords = HD == 64 && BITS == 4 ? 1 : HD * BITS / 512;  // (16 bits for heads of 64 in 4 bits)
-    uint32_t k[2][kKWords], v[8][kVWords], kp, vp;
+    uint32_t k[2][kKWords], v[8][kVWords];
 
     template <int W>
     __device__ __forceinline__ static void words(const uint8_t *at, uint32_t *to) {
@@ -528,52 +588,62 @@ struct QBlockRegs {
             to[0] = *reinterpret_cast<const uint32_t *>(at);
         }
     }
-    // rows from k0 on, those past `last` as that
-    __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *vc, const uint8_t *kpar, const uint8_t *vpar, int k0, int last, int lane) {
-        const int i = lane & 15, u = lane >> 4;
-        auto row = [&](int r) { return (int64_t)min(k0 + r, last); };
-        auto get = [&](auto row_of) {
+    // rows k0 .. k0 + 31 of a cache of `rows` rows, its last in place of those behind it
+    __device__ __forceinline__ void load_k(const uint8_t *codes, int k0, int rows, int lane) {
+        const uint8_t *at = codes + (int64_t)k0 * F::kCodes;
+        const uint32_t i = lane & 15, part = (lane >> 4) * (kKWords == 2 ? 8 : 16), last = rows - 1 - k0;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) words<kKWords>(kc + row_of(16 * t + i) * F::kCodes + 16 * u / (kKWords == 2 ? 2 : 1), k[t]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint8_t *at = vc + row_of(16 * (j >> 2) + 4 * u + (j & 3)) * F::kCodes;
-                if constexpr (HD == 64 && BITS == 4) v[j][0] = *reinterpret_cast<const uint16_t *>(at + 2 * i);
-                else words<kVWords>(at + 4 * kVWords * i, v[j]);
-            }
-            const int key = HD == 128 ? lane >> 1 : lane & 31, word = HD == 128 ? lane & 1 : 0;
-            kp = *reinterpret_cast<const uint32_t *>(kpar + row_of(key) * (4 * G) + 4 * word);
-            vp = *reinterpret_cast<const uint32_t *>(vpar + row_of(key) * (4 * G) + 4 * word);
-        };
-        get(row);
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t row = 16 * t + i;
+            words<kKWords>(at + ((k0 + kQBlock <= rows ? row : min(row, last)) * F::kCodes + part), k[t]);
+        }
     }
+    __device__ __forceinline__ void load_v(const uint8_t *codes, int k0, int rows, int lane) {
+        const uint8_t *at = codes + (int64_t)k0 * F::kCodes;
+        const uint32_t u = lane >> 4, part = (lane & 15) * (HD == 64 && BITS == 4 ? 2 : 4 * kVWords), last = rows - 1 - k0;
+        auto one = [&](int j, uint32_t row) {
+            if constexpr (HD == 64 && BITS == 4) v[j][0] = *reinterpret_cast<const uint16_t *>(at + (row * F::kCodes + part));
+            else words<kVWords>(at + (row * F::kCodes + part), v[j]);
+        };
+        if (k0 + kQBlock <= rows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) one(j, 16 * (j >> 2) + 4 * u + (j & 3));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) one(j, min(16 * (j >> 2) + 4 * u + (j & 3), last));
+        }
+    }
+    // what elements of key chunks are to be taken times: of eight, 0 .. 7
+    __device__ __forceinline__ static constexpr bool k_upper(int e) { return BITS == 4 && (e >> 1 & 1); }
+    __device__ __forceinline__ static constexpr bool v_upper(int t) { return BITS == 4 && (t & 1); }
     // K's operand of chunk c, key tile t
-    __device__ __forceinline__ v8h key(int t, int c) const {
+    __device__ __forceinline__ v8h key(int t, int c, uint32_t magic) const {
         v8h r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v2h x;
-            if constexpr (BITS == 4) x = code_pair(k[t][c] >> 4 * e & 0x000f000fu, 8);
-            else x = code_pair(__builtin_amdgcn_perm(0u, k[t][2 * c + e / 2], e & 1 ? 0x0c030c02u : 0x0c010c00u), 128);
+            if constexpr (BITS == 4) {
+                const uint32_t w = k[t][c] >> (e & 2 ? 8 : 0);
+                x = e & 1 ? code_pair<1024 + 128>(w, 0x00f000f0u, magic) : code_pair<1024 + 8>(w, 0x000f000fu, magic);
+            } else {
+                x = code_pair<1024 + 128>(__builtin_amdgcn_perm(magic, k[t][2 * c + e / 2], e & 1 ? 0x05030502u : 0x05010500u), ~0u, 0u);
+            }
             r[2 * e] = x[0];
             r[2 * e + 1] = x[1];
         }
         return r;
     }
     // V's operand of dim tile t: element 64 (t / 4) + 4i + t % 4 of eight keys
-    __device__ __forceinline__ v8h value(int t) const {
+    __device__ __forceinline__ v8h value(int t, uint32_t magic) const {
         v8h r;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
+            const uint32_t b = BITS == 4 ? t >> 1 : t & 3;  // the byte that holds it
+            const int w = BITS == 4 ? 0 : t >> 2;
+            const uint32_t two = __builtin_amdgcn_perm(v[j + 1][w], v[j][w], 0x0c040c00u + 0x00010001u * b);
             v2h x;
-            if constexpr (BITS == 4) {
-                const uint32_t b = t >> 1;  // the byte that holds it
-                const uint32_t two = __builtin_amdgcn_perm(v[j + 1][0], v[j][0], 0x0c040c00u + 0x00010001u * b);
-                x = code_pair(two >> 4 * (t & 1) & 0x000f000fu, 8);
-            } else {
-                const uint32_t b = t & 3;
-                x = code_pair(__builtin_amdgcn_perm(v[j + 1][t >> 2], v[j][t >> 2], 0x0c040c00u + 0x00010001u * b), 128);
-            }
+            if constexpr (BITS == 4) x = t & 1 ? code_pair<1024 + 128>(two, 0x00f000f0u, magic) : code_pair<1024 + 8>(two, 0x000f000fu, magic);
+            else x = code_pair<1024 + 128>(two, ~0u, magic);
             r[j] = x[0];
             r[j + 1] = x[1];
         }
@@ -601,12 +671,12 @@ __device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Floa
 // p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
 // exponent that brings V's largest step so far to 2^kQTop, so that the halves of p
 // step hold the products that count whatever V's size.  All rescales are by powers
-// of two.  NaN parameters of rows that a row does not see meet a select, never a
-// product.
+// of two.  A block's codes are requested as soon as the registers of the block
+// before are free.
 template <int HD, int BITS, int RT, bool SHAPED, bool KEYS>
-__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
+__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
-    using B = QBlockRegs<HD, BITS>;
+    using Codes = QCodes<HD, BITS>;
     constexpr int C = HD / 32, G = HD / 64, T = HD / 16;
     constexpr int kRows = 16 * RT * (KEYS ? 1 : 4);
     constexpr int kPar = 32 * 4 * G;  // bytes of a block's parameters of K or V
@@ -629,7 +699,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
     const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
-    const int last = p.cache.capacity - 1;
+    const int cap = p.cache.capacity;
     int block = share.from, end = share.to;
     if (KEYS) {
         block += wave;
@@ -638,8 +708,20 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
         end = min(end, (t.hi + kQBlock - 1) / kQBlock);
     }
     constexpr int kStep = KEYS ? 4 : 1;
-    B cur;
-    if (block < end) cur.load(kc, vc, kp, vp, block * kQBlock, last, lane);
+    // parameters: a word a lane, spread over the lanes through LDS
+    uint32_t kw = 0, vw = 0;
+    const uint32_t par_key = HD == 128 ? lane >> 1 : lane & 31, par_word = HD == 128 ? 4 * (lane & 1) : 0;
+    auto load_par = [&](int k0) {
+        const uint32_t row = min(par_key, (uint32_t)(cap - 1 - k0)) * (4 * G) + par_word;
+        kw = *reinterpret_cast<const uint32_t *>(kp + (int64_t)k0 * (4 * G) + row);
+        vw = *reinterpret_cast<const uint32_t *>(vp + (int64_t)k0 * (4 * G) + row);
+    };
+    Codes codes;
+    if (block < end) {
+        codes.load_k(kc, block * kQBlock, cap, lane);
+        load_par(block * kQBlock);
+        codes.load_v(vc, block * kQBlock, cap, lane);
+    }
 
     // query rows as halves below 2^kTop, their sums of each group
     v8h qh[RT][C], ql[RT][C];
@@ -667,7 +749,6 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[c][e]));
         const int e = row_exp(groups_umax(top));
-        split_row<C>(x, e, qh[rt], ql[rt]);
         const float up = pow2(kTop - e);
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
@@ -678,6 +759,12 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
                 for (int k = 0; k < 8; ++k) sum += x[c][k] * up;
             qs[rt][gr] = groups_sum(sum);
         }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (Codes::k_upper(k)) x[c][k] *= 0.0625f;
+        split_row<C>(x, e, qh[rt], ql[rt]);
         // score = product · f; with a cap: tanh(product · f) · cap
         const float size = pow2(e - kTop);
         f[rt] = SHAPED && p.cap > 0.0f ? fminf(p.scale * size * (1.0f / p.cap), 3.0e38f) : p.scale * kLog2e * size;
@@ -701,108 +788,130 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
     }
     uint32_t step_top = 0;  // bits of V's largest step so far
     int raise = kQTop + 14;  // exponent that brings it below 2^kQTop
+    const uint32_t magic = code_magic();
+    uint32_t *par = reinterpret_cast<uint32_t *>(s_par[wave]);
 
     for (; block < end; block += kStep) {
-        const int k0 = block * kQBlock;
+        const int k0 = block * kQBlock, next0 = k0 + kStep * kQBlock;
+        const bool more = block + kStep < end;
         const bool masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
-        // parameters of keys outside the tile's are zero
-        uint32_t kw = cur.kp, vw = cur.vp;
-        if (masked) {
-            const int key = k0 + (HD == 128 ? lane >> 1 : lane & 31);
+        if (masked) {  // parameters of keys outside the tile's are zero
+            const int key = k0 + (int)par_key;
             if (key < t.lo || key >= t.hi) kw = vw = 0;
         }
-        // V's largest step (NaN is none)
-        const uint32_t w = HD == 128 && (lane & 1) ? 0u : vw;
-        uint32_t s0 = w & 0xffffu, s1 = HD == 128 ? w >> 16 : 0u;
-        s0 = s0 > 0x7c00u ? 0u : s0;
-        s1 = s1 > 0x7c00u ? 0u : s1;
-        const uint32_t lane_top = max(s0, s1);
+        // V's largest step.  Numbers that are none stay out of products: they would
+        // meet the zero weights of rows that do not see them.  Rows that do get them below.
+        uint64_t bad[2] = {0, 0};
         bool moved = false;
-        if (__any(lane_top > step_top)) {
-            uint32_t y = groups_umax(lane_top);
+        {
+            const bool b0 = (vw & 0x7c00u) == 0x7c00u, b1 = (vw & 0x7c000000u) == 0x7c000000u;
+            const uint32_t s0 = vw & 0x7fffu, s1 = HD == 128 ? vw >> 16 : 0u;
+            const uint32_t lane_top = HD == 128 && (lane & 1) ? 0u : max(s0, s1);
+            if (__any((b0 || b1 || lane_top > step_top) && (HD == 128 || lane < 32))) {
+                if (b0) vw &= 0xffff0000u;
+                if (b1) vw &= 0x0000ffffu;
+                bad[0] = __ballot(HD == 128 ? b0 : b0 || b1);
+                bad[1] = __ballot(b1);
+                uint32_t y = HD == 128 && (lane & 1) ? 0u : max(vw & 0x7fffu, HD == 128 ? vw >> 16 : 0u);
+                y = groups_umax(y);
 #pragma unroll
-            for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
-            step_top = y;
-            // step < 2^(exponent - 14), subnormal ones < 2^-14
-            const int now = kQTop + 14 - (int)(y >> 10);
-            moved = now != raise;
-            raise = now;
+                for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
+                if (y > step_top) {
+                    step_top = y;
+                    // step < 2^(exponent - 14), subnormal ones < 2^-14
+                    const int now = kQTop + 14 - (int)(y >> 10);
+                    moved = now != raise;
+                    raise = now;
+                }
+            }
         }
-        uint32_t *par = reinterpret_cast<uint32_t *>(s_par[wave]);
         if (HD == 128 || lane < 32) {
             par[lane] = kw;
             par[kPar / 4 + lane] = vw;
         }
         wave_lds_order();
-        B next;
-        if (block + kStep < end) next.load(kc, vc, kp, vp, (block + kStep) * kQBlock, last, lane);
+        if (more) load_par(next0);
 
-        // scores of tile t, keys 4u .. +3
-        v8h kf[2][C];
+        // scores: row i, keys 16 · kt + 4u + k
+        float sc[RT][8];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt) {
+            v8h pars[G];
 #pragma unroll
-            for (int c = 0; c < C; ++c) kf[kt][c] = cur.key(kt, c);
-        v8h kpar[2][G], vpar[2][G];
+            for (int k = 0; k < G; ++k) pars[k] = *reinterpret_cast<const v8h *>(s_par[wave] + (16 * kt + 4 * u) * 4 * G + 16 * k);
+            v4f d[RT][G];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+            for (int c = 0; c < C; ++c) {
+                const v8h key = codes.key(kt, c, magic);
 #pragma unroll
-            for (int k = 0; k < G; ++k) {
-                kpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + (16 * kt + 4 * u) * 4 * G + 16 * k);
-                vpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + kPar + (16 * kt + 4 * u) * 4 * G + 16 * k);
-            }
-        auto step_of = [&](const v8h (&x)[2][G], int j, int gr) { const int at = (j & 3) * 2 * G + gr; return x[j >> 2][at >> 3][at & 7]; };
-        auto mid_of = [&](const v8h (&x)[2][G], int j, int gr) { const int at = (j & 3) * 2 * G + G + gr; return x[j >> 2][at >> 3][at & 7]; };
-        float w8[RT][8];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float sc[8];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                v4f d[G];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    d[gr] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 2 * gr; c < 2 * gr + 2; ++c) {
-                        d[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][c], qh[rt][c], d[gr], 0, 0, 0);
-                        d[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][c], ql[rt][c], d[gr], 0, 0, 0);
-                    }
+                for (int rt = 0; rt < RT; ++rt) {
+                    const v4f from = c % 2 ? d[rt][c / 2] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                    const v4f x = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qh[rt][c], from, 0, 0, 0);
+                    d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, ql[rt][c], x, 0, 0, 0);
                 }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int j = 4 * kt + k;
                     float x = 0.0f;
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        x = fmaf((float)mid_of(kpar, j, gr), qs[rt][gr], x);
-                        x = fmaf((float)step_of(kpar, j, gr), d[gr][k], x);
+                        const int at = k * 2 * G + gr;
+                        const float step = (float)pars[at >> 3][at & 7], mid = (float)pars[(at + G) >> 3][(at + G) & 7];
+                        x = gr ? fmaf(mid, qs[rt][gr], x) : mid * qs[rt][gr];
+                        x = fmaf(step, d[rt][gr][k], x);
                     }
-                    sc[j] = rounded(x * f[rt]);
+                    sc[rt][4 * kt + k] = rounded(x * f[rt]);
                 }
-            }
+        }
+        if (more) codes.load_k(kc, next0, cap, lane);
+
+        v8h wh[RT][G], wl[RT][G];
+        v8h vpar[2][G];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int k = 0; k < G; ++k) vpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + kPar + (16 * kt + 4 * u) * 4 * G + 16 * k);
+        auto v_par = [&](int j, int gr, int which) {  // step (which 0) or midpoint of the lane's key j
+            const int at = (j & 3) * 2 * G + which * G + gr;
+            return vpar[j >> 2][at >> 3][at & 7];
+        };
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float (&x)[8] = sc[rt];
             if (SHAPED) {
                 if (p.cap > 0.0f) {
-                    tanh_all<8>(sc);
+                    tanh_all<8>(x);
                     const float up = p.cap * kLog2e;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sc[j] *= up;
+                    for (int j = 0; j < 8; ++j) x[j] *= up;
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    sc[j] = rounded(fmaf(-slope[rt], (float)(pos[rt] - (k0 + 16 * (j >> 2) + 4 * u + (j & 3))), sc[j]));
+                    x[j] = rounded(fmaf(-slope[rt], (float)(pos[rt] - (k0 + 16 * (j >> 2) + 4 * u + (j & 3))), x[j]));
             }
             if (masked) {
                 const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = k0 + 16 * (j >> 2) + 4 * u + (j & 3);
-                    sc[j] = key >= from && key <= pos[rt] ? sc[j] : -INFINITY;
+                    const bool sees = key >= from && key <= pos[rt];
+                    x[j] = sees ? x[j] : -INFINITY;
                 }
             }
-            float top = sc[0];
+            if (bad[0] | bad[1]) {  // NaN for the rows that see it, in its group
+                const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
 #pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
+                for (int j = 0; j < 8; ++j) {
+                    const int at = 16 * (j >> 2) + 4 * u + (j & 3), key = k0 + at;
+                    const bool sees = key >= from && key <= pos[rt];
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr)
+                        if (sees && (bad[gr] >> (HD == 128 ? 2 * at : at) & (HD == 128 ? 3 : 1))) mids[rt][gr] = __builtin_nanf("");
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if (moved || __any(top > m[rt] + kQSlack)) {
                 top = groups_max(top);
                 if (top > m[rt]) m[rt] = fminf(ceilf(top), 3.0e38f);
@@ -817,50 +926,34 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w8[rt][j] = __builtin_amdgcn_exp2f(sc[j] - ref[rt]);
-                sum[rt] += w8[rt][j];
+                x[j] = __builtin_amdgcn_exp2f(x[j] - ref[rt]);
+                sum[rt] += x[j];
             }
-        }
-        // A NaN among V's parameters stays with the rows that see it: others' weights are zeros.
-        v8h wh[RT][G], wl[RT][G];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                    _Float16 sa = step_of(vpar, j, gr), sb = step_of(vpar, j + 1, gr);
-                    _Float16 ma = mid_of(vpar, j, gr), mb = mid_of(vpar, j + 1, gr);
-                    if (masked) {
-                        const int key = k0 + 16 * (j >> 2) + 4 * u + (j & 3);
-                        const bool a = key >= from && key <= pos[rt], b = key + 1 >= from && key + 1 <= pos[rt];
-                        sa = a ? sa : (_Float16)0;
-                        ma = a ? ma : (_Float16)0;
-                        sb = b ? sb : (_Float16)0;
-                        mb = b ? mb : (_Float16)0;
-                    }
                     v2h h, l;
-                    split_steps(w8[rt][j], sa, w8[rt][j + 1], sb, h, l);
+                    split_steps(x[j], v_par(j, gr, 0), x[j + 1], v_par(j + 1, gr, 0), h, l);
                     wh[rt][gr][j] = h[0];
                     wh[rt][gr][j + 1] = h[1];
                     wl[rt][gr][j] = l[0];
                     wl[rt][gr][j + 1] = l[1];
-                    mids[rt][gr] = fmaf((float)ma, w8[rt][j], mids[rt][gr]);
-                    mids[rt][gr] = fmaf((float)mb, w8[rt][j + 1], mids[rt][gr]);
+                    mids[rt][gr] = fmaf((float)v_par(j, gr, 1), x[j], mids[rt][gr]);
+                    mids[rt][gr] = fmaf((float)v_par(j + 1, gr, 1), x[j + 1], mids[rt][gr]);
                 }
         }
 #pragma unroll
         for (int k = 0; k < T; ++k) {
-            const v8h v = cur.value(k);
+            const v8h v = codes.value(k, magic);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh[rt][k / 4], acc[rt][k], 0, 0, 0);
                 acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl[rt][k / 4], acc[rt][k], 0, 0, 0);
             }
         }
+        if (more) codes.load_v(vc, next0, cap, lane);
         wave_lds_order();
-        cur = next;
     }
 
     // denominators and midpoints over a row's four lanes
@@ -871,7 +964,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_qcache_attn(QAttnCall 
         for (int gr = 0; gr < G; ++gr) {
             mids[rt][gr] = groups_sum(mids[rt][gr]);
 #pragma unroll
-            for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[rt][k] += mids[rt][gr];
+            for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[rt][k] = acc[rt][k] * (Codes::v_upper(k) ? 0.0625f : 1.0f) + mids[rt][gr];
         }
     }
     if (KEYS) {  // four waves' sums: 2 and 3 to 0 and 1, then 1 to 0
