@@ -219,48 +219,46 @@ int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const c
 
 // Row tiles and key shares of one attention call.
 struct QShape {
-    int rt;       // row tiles of 16 a wave
-    bool keys;    // a workgroup's waves share its rows
+    int rt;       // row tiles of 16 a workgroup
     int rows;     // of a workgroup
-    int tiles, splits, least;
+    int tiles, splits;
     int64_t slots, bytes;
 };
 QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     QShape q;
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
     q.rt = rows <= 16 ? 1 : 2;
-    q.keys = rows < 1024;
-    q.rows = 16 * q.rt * (q.keys ? 1 : 4);
+    q.rows = 16 * q.rt;
     q.tiles = round_up_div(rows, q.rows);
-    const int64_t work = q.tiles * groups, blocks = round_up_div(a->max_rows, kQBlock);
-    q.least = q.keys ? 4 : 8;
-    q.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 512 / work), 64, std::max<int64_t>(1, blocks / q.least)});
+    const int64_t work = q.tiles * groups;
+    const int64_t keys = a->window ? std::min<int64_t>(a->max_rows, (int64_t)a->window + q.rows) : a->max_rows;
+    const int64_t blocks = round_up_div(keys, kQBlock), waves = 4;
+    q.splits = blocks <= 3 * waves ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, 512 / work), 128, round_up_div(blocks, waves)});
     q.slots = q.splits > 1 ? work * q.splits : 0;
     q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
     return q;
 }
 
-template <int HD, int BITS, int RT, bool KEYS>
+template <int HD, int BITS, int RT>
 int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
     QAttnPlan pl{};
     pl.tiles = q.tiles;
     pl.splits = q.splits;
-    pl.least = q.least;
     pl.part = static_cast<float *>(work);
     pl.stat = reinterpret_cast<float2 *>(pl.part + q.slots * q.rows * HD);
     const dim3 grid(q.tiles * q.splits, p.cache.kvh, seqs);
-    if (p.cap > 0.0f || p.slopes) RC(launch(s, grid, 256, k_qcache_attn<HD, BITS, RT, true, KEYS>, p, pl));
-    else RC(launch(s, grid, 256, k_qcache_attn<HD, BITS, RT, false, KEYS>, p, pl));
+    const bool shaped = p.cap > 0.0f || p.slopes;
+    RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, RT, true> : k_qcache_attn<HD, BITS, RT, false>, p, pl));
     if (!q.slots) return POCR_OK;
-    constexpr int kRows = 16 * RT * (KEYS ? 1 : 4);
-    return launch(s, dim3(q.tiles * (kRows / (1024 / HD)), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows>, p, pl);
+    constexpr int kRows = 16 * RT, U = 1024 / HD;
+    if (q.splits >= 8) return launch(s, dim3(q.tiles * kRows / (U / 8), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 8>, p, pl);
+    return launch(s, dim3(q.tiles * kRows / (U / 2), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 2>, p, pl);
 }
 
 template <int HD, int BITS>
 int launch_qattn_t(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
-    if (q.rt == 1) return launch_qattn<HD, BITS, 1, true>(s, p, q, work, seqs);
-    if (q.keys) return launch_qattn<HD, BITS, 2, true>(s, p, q, work, seqs);
-    return launch_qattn<HD, BITS, 2, false>(s, p, q, work, seqs);
+    if (q.rt == 1) return launch_qattn<HD, BITS, 1>(s, p, q, work, seqs);
+    return launch_qattn<HD, BITS, 2>(s, p, q, work, seqs);
 }
 
 }  // namespace
@@ -369,6 +367,7 @@ extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *
     p.n = a->n;
     p.heads = a->heads;
     p.group = a->heads / c->kv_heads;
+    p.group_inv = p.group == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group);
     p.max_rows = a->max_rows;
     p.window = a->window;
     p.scale = default_scale(a->scale, c->head_dim);

@@ -490,13 +490,18 @@ struct QAttnCall {
     int64_t q_ss, q_st, o_ss, o_st;
     QRows cache;
     int n, heads, group, max_rows, window;
+    uint32_t group_inv;  // 2^32 / group, rounded up (group 1: 0)
     float scale, cap;
+    // the token of query row r < 2^24: the quotient, at most one too large before its correction
+    __device__ __forceinline__ int token(int r) const {
+        const uint32_t q = group == 1 ? (uint32_t)r : __umulhi((uint32_t)r, group_inv);
+        return (int)(q - (q * (uint32_t)group > (uint32_t)r));
+    }
 };
 
 // Row tiles and key shares of a call.
 struct QAttnPlan {
-    int tiles, splits;  // of a (sequence, KV head); shares a tile's keys may be cut into
-    int least;          // blocks of a share
+    int tiles, splits;  // of a (sequence, KV head); shares of a tile's keys
     float *part;        // [sequence][KV head][tile][split][rows][HD] sums
     float2 *stat;       // their rows' reference exponents and denominators
 };
@@ -522,25 +527,12 @@ __device__ __forceinline__ QTile q_tile(const QAttnCall &p, int s, int first, in
         t.count = 0;
         return t;
     }
-    const int tok0 = first / p.group, tok1 = (min(first + rows, all) - 1) / p.group, pos = t.len - t.count;
+    const int tok0 = p.token(first), tok1 = p.token(min(first + rows, all) - 1), pos = t.len - t.count;
     t.hi = max(0, pos + tok1 + 1);
     t.all_hi = max(0, pos + tok0 + 1);
     t.lo = p.window ? min(t.hi, max(0, pos + tok0 - p.window + 1)) : 0;
     t.all_lo = p.window ? max(0, pos + tok1 - p.window + 1) : 0;
     return t;
-}
-
-// the blocks of one share of a tile's keys
-struct QShare {
-    int parts, from, to;
-};
-__device__ __forceinline__ QShare q_share(const QAttnPlan &pl, const QTile &t, int part) {
-    const int first = t.lo / kQBlock, blocks = max(0, (t.hi + kQBlock - 1) / kQBlock - first);
-    QShare h;
-    h.parts = min(pl.splits, max(1, blocks / pl.least));
-    h.from = first + (int)((int64_t)blocks * part / h.parts);
-    h.to = first + (int)((int64_t)blocks * (part + 1) / h.parts);
-    return h;
 }
 
 // Codes as fp16 numbers: 1024 + n is a bit pattern away from n < 1024, and taking
@@ -657,10 +649,240 @@ __device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Floa
     lo = (v2h){(_Float16)__builtin_fmaf(a, (float)sa, -(float)hi[0]), (_Float16)__builtin_fmaf(b, (float)sb, -(float)hi[1])};
 }
 
-// Attention over codes.  Workgroup: a tile of query rows (token, head of the KV
-// head's group) of one sequence and KV head, and a share of its keys.  KEYS: 16 ·
-// RT rows, the four waves take its blocks of 32 keys in turn and join; otherwise
-// 16 · RT rows a wave, all of the share's blocks.
+// One query row's part of a score, in a lane of its tile.
+template <int HD>
+struct QQuery {
+    static constexpr int G = HD / 64;
+    float sum[G];   // of the row's elements of each group
+    float size;     // a power of two: score = size · product
+    float slope;
+    int from, pos;  // the keys it sees: [from, pos]
+};
+
+// A lane's share of query row r (token, head of the KV head's group), elements 32c +
+// 8u .. +7 of it.  Rows behind the last hold the last one's.
+template <int HD>
+__device__ __forceinline__ void q_fetch(const QAttnCall &p, int s, int g, int r, int u, v4f (&x)[HD / 16]) {
+    r = min(r, p.n * p.group - 1);
+    const int tok = p.token(r), head = g * p.group + r - tok * p.group;
+    const float *src = p.q + s * p.q_ss + tok * p.q_st + head * HD + 8 * u;
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[2 * c + e] = *reinterpret_cast<const v4f *>(src + 32 * c + 4 * e);
+}
+
+// The same times the scale, as halves below 2^kTop, smaller where they meet the
+// upper codes of bytes.
+template <int HD, int BITS, bool SHAPED>
+__device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int g, int r, const v4f (&y)[HD / 16], v8h (&hi)[HD / 32],
+                                        v8h (&lo)[HD / 32], QQuery<HD> &q) {
+    constexpr int C = HD / 32, G = HD / 64;
+    const bool live = r < t.count * p.group;
+    const int tok = p.token(live ? r : 0), head = g * p.group + (live ? r - tok * p.group : 0);
+    q.pos = live ? t.len - t.count + tok : -1;
+    q.from = p.window ? max(0, q.pos - p.window + 1) : 0;
+    const float scale = SHAPED && p.cap > 0.0f ? p.scale : p.scale * kLog2e;  // a cap takes scores as they are
+    float x[C][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[c][e] = live ? y[2 * c + e / 4][e & 3] * scale : 0.0f;
+            top = max(top, abs_bits(x[c][e]));
+        }
+    const int e = row_exp(groups_umax(top));
+    const float up = pow2(kTop - e);
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 2 * gr; c < 2 * gr + 2; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += x[c][k] * up;
+        q.sum[gr] = groups_sum(sum);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (QCodes<HD, BITS>::k_upper(k)) x[c][k] *= 0.0625f;
+    split_row<C>(x, e, hi, lo);
+    q.size = pow2(e - kTop);
+    q.slope = 0.0f;
+    if (SHAPED && p.slopes) {
+        const float y = p.slopes[head] * kLog2e;
+        q.slope = fabsf(y) == INFINITY ? copysignf(3.4028235e38f, y) : y;
+    }
+}
+
+// The parameters of a block's 32 keys: a word of K's and of V's a lane, spread over
+// the wave's lanes through LDS.
+template <int HD>
+struct QParams {
+    static constexpr int G = HD / 64, kBytes = 32 * 4 * G;  // of K or V
+    uint32_t k, v;
+    __device__ __forceinline__ static int key_of(int lane) { return HD == 128 ? lane >> 1 : lane & 31; }
+    __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, int k0, int rows, int lane) {
+        const uint32_t at = min((uint32_t)key_of(lane), (uint32_t)(rows - 1 - k0)) * (4 * G) + (HD == 128 ? 4 * (lane & 1) : 0);
+        k = *reinterpret_cast<const uint32_t *>(kp + (int64_t)k0 * (4 * G) + at);
+        v = *reinterpret_cast<const uint32_t *>(vp + (int64_t)k0 * (4 * G) + at);
+    }
+    // of the lane's keys 16 · kt + 4u .. +3
+    __device__ __forceinline__ static void get(const uint8_t *par, int kt, int u, v8h (&x)[G]) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) x[i] = *reinterpret_cast<const v8h *>(par + (16 * kt + 4 * u) * 4 * G + 16 * i);
+    }
+    // of the group gr of key k of those: the step (which 0) or the midpoint
+    __device__ __forceinline__ static _Float16 of(const v8h (&x)[G], int k, int gr, int which) {
+        const int at = k * 2 * G + which * G + gr;
+        return x[at >> 3][at & 7];
+    }
+};
+
+// V's largest step so far, the exponent that brings it below 2^kQTop, and the keys
+// of the present block with parameters that are no numbers.
+struct QScale {
+    uint32_t top = 0;  // its bits
+    int raise = kQTop + 14;
+    uint64_t bad[2] = {0, 0};
+    bool moved = false;
+    // `v`: a lane's word of V's parameters.  What is no number stays out of products,
+    // where it would meet the zero weights of rows that do not see it.
+    template <int HD>
+    __device__ __forceinline__ void look(uint32_t &v, int lane) {
+        const bool mine = HD == 128 || lane < 32, steps = HD == 64 || !(lane & 1);
+        const bool b0 = (v & 0x7c00u) == 0x7c00u, b1 = (v & 0x7c000000u) == 0x7c000000u;
+        const uint32_t most = max(v & 0x7fffu, HD == 128 ? v >> 16 : 0u);
+        bad[0] = bad[1] = 0;
+        moved = false;
+        if (!__any(mine && (b0 || b1 || (steps && most > top)))) return;
+        if (b0) v &= 0xffff0000u;
+        if (b1) v &= 0x0000ffffu;
+        bad[0] = __ballot(HD == 128 ? b0 : b0 || b1);
+        bad[1] = __ballot(b1);
+        uint32_t y = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 : 0u) : 0u);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
+        if (y <= top) return;
+        top = y;
+        const int now = kQTop + 14 - (int)(y >> 10);  // step < 2^(exponent - 14), subnormal ones < 2^-14
+        moved = now != raise;
+        raise = now;
+    }
+    // the group of the block's key is none
+    template <int HD>
+    __device__ __forceinline__ bool is_bad(int key, int gr) const { return bad[gr] >> (HD == 128 ? 2 * key : key) & (HD == 128 ? 3 : 1); }
+};
+
+// A row's running sums, in a lane of its tile.
+template <int HD>
+struct QSums {
+    static constexpr int G = HD / 64, T = HD / 16;
+    v4f acc[T];
+    float ref = kLowest, m = kLowest, total = 0.0f, mids[G];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < T; ++k) acc[k] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) mids[gr] = 0.0f;
+    }
+    // a block's products x (lane: keys 16 (j / 4) + 4u + j % 4 of its block) → weights times V's steps
+    template <bool SHAPED>
+    __device__ __forceinline__ void weigh(const QAttnCall &p, const QQuery<HD> &q, const QScale &scale, float (&x)[8], int k0, int u, bool masked,
+                                          const v8h (&v0)[G], const v8h (&v1)[G], v8h (&hi)[G], v8h (&lo)[G]) {
+        auto key_of = [&](int j) { return 16 * (j >> 2) + 4 * u + (j & 3); };
+        if (SHAPED) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= q.size;
+            if (p.cap > 0.0f) {
+                const float down = 1.0f / p.cap, up = p.cap * kLog2e;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= down;
+                tanh_all<8>(x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= up;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = rounded(fmaf(-q.slope, (float)(q.pos - k0 - key_of(j)), x[j]));
+        }
+        const float size = SHAPED ? 1.0f : q.size;  // exact, so a score may round with its reference
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = k0 + key_of(j);
+                x[j] = key >= q.from && key <= q.pos ? x[j] : -INFINITY;
+            }
+        }
+        if (scale.bad[0] | scale.bad[1]) {  // NaN for the rows that see one, in its group
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = k0 + key_of(j);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)
+                    if (key >= q.from && key <= q.pos && scale.is_bad<HD>(key_of(j), gr)) mids[gr] = __builtin_nanf("");
+            }
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * size;
+        if (scale.moved || __any(top > m + kQSlack)) {
+            top = groups_max(top);
+            if (top > m) m = fminf(ceilf(top), 3.0e38f);
+            const float now = fabsf(m) < kQFar ? m - (float)scale.raise : m, by = __builtin_amdgcn_exp2f(ref - now);
+            ref = now;
+            total *= by;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) mids[gr] *= by;
+#pragma unroll
+            for (int k = 0; k < T; ++k) acc[k] *= by;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], size, -ref));
+            total += x[j];
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const v8h(&par)[G] = j < 4 ? v0 : v1;
+                v2h h, l;
+                split_steps(x[j], QParams<HD>::of(par, j & 3, gr, 0), x[j + 1], QParams<HD>::of(par, (j & 3) + 1, gr, 0), h, l);
+                hi[gr][j] = h[0];
+                hi[gr][j + 1] = h[1];
+                lo[gr][j] = l[0];
+                lo[gr][j + 1] = l[1];
+                mids[gr] = fmaf((float)QParams<HD>::of(par, j & 3, gr, 1), x[j], mids[gr]);
+                mids[gr] = fmaf((float)QParams<HD>::of(par, (j & 3) + 1, gr, 1), x[j + 1], mids[gr]);
+            }
+    }
+    // the row's sums over its four lanes; acc in whole
+    template <int BITS>
+    __device__ __forceinline__ void finish() {
+        total = groups_sum(total);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            mids[gr] = groups_sum(mids[gr]);
+#pragma unroll
+            for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[k] = acc[k] * (QCodes<HD, BITS>::v_upper(k) ? 0.0625f : 1.0f) + mids[gr];
+        }
+        if (total == 0.0f) ref = kLowest;
+    }
+};
+
+// what a tile's row r leaves behind: its part of a share, or its result
+__device__ __forceinline__ float *q_out_row(const QAttnCall &p, int s, int g, int r, int hd) {
+    const int tok = p.token(r), head = g * p.group + r - tok * p.group;
+    return p.out + s * p.o_ss + tok * p.o_st + head * hd;
+}
+__device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int r, float ref, float total) {
+    const int tok = p.token(r), head = g * p.group + r - tok * p.group;
+    p.lse[((int64_t)s * p.n + tok) * p.heads + head] = total == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
+}
+
+// Attention over codes.  Workgroup: 16 · RT query rows (token, head of the KV head's
+// group) of one sequence and KV head; its W waves take the share's blocks of 32 keys
+// in turn and join.
 //
 // Codes go to the matrix instructions as they are, exact in fp16, and meet query
 // rows and weights as two fp16 halves each.  Scores come out transposed (lane l:
@@ -671,397 +893,257 @@ __device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Floa
 // p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
 // exponent that brings V's largest step so far to 2^kQTop, so that the halves of p
 // step hold the products that count whatever V's size.  All rescales are by powers
-// of two.  A block's codes are requested as soon as the registers of the block
-// before are free.
-template <int HD, int BITS, int RT, bool SHAPED, bool KEYS>
+// of two.  A wave's first blocks and its query rows do not depend on the sequence's
+// length, and are requested with it; later blocks two ahead, a block's codes as
+// soon as the registers of the one before are free.
+template <int HD, int BITS, int RT, bool SHAPED>
 __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
     using Codes = QCodes<HD, BITS>;
-    constexpr int C = HD / 32, G = HD / 64, T = HD / 16;
-    constexpr int kRows = 16 * RT * (KEYS ? 1 : 4);
-    constexpr int kPar = 32 * 4 * G;  // bytes of a block's parameters of K or V
-    __shared__ __attribute__((aligned(16))) uint8_t s_par[4][2 * kPar];
-    __shared__ v4f s_acc[KEYS ? 2 : 1][KEYS ? RT * T : 1][64];
-    __shared__ float s_ref[KEYS ? 4 : 1][16 * RT], s_sum[KEYS ? 4 : 1][16 * RT];
+    using Params = QParams<HD>;
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, W = 4, kRows = 16 * RT;
+    constexpr int kAhead = HD == 64 || (BITS == 4 && RT == 1) ? 2 : 1;  // blocks in flight; more would leave the registers
+    union Shared {
+        struct {
+            v8h q[RT][C][2][64];
+            uint8_t par[W][2 * Params::kBytes];
+        } in;
+        v4f acc[W][RT][T][64];
+    };
+    __shared__ Shared sh;
+    __shared__ QQuery<HD> s_query[RT][16];
+    __shared__ float s_ref[W][kRows], s_sum[W][kRows];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
     const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
-    const QTile wt = q_tile(p, s, tile * kRows, kRows);
-    if (!wt.count) return;
-    const QShare share = q_share(pl, wt, part);
-    if (part >= share.parts) return;
-    const int first = tile * kRows + (KEYS ? 0 : wave * 16 * RT), all = wt.count * p.group;
-    if (first >= all) return;  // no barriers without KEYS
-    const QTile t = KEYS ? wt : q_tile(p, s, first, 16 * RT);
-
     const int64_t base = s * p.cache.seq_rows + (int64_t)g * p.cache.capacity;
     const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
-    const int cap = p.cache.capacity;
-    int block = share.from, end = share.to;
-    if (KEYS) {
-        block += wave;
-    } else {
-        block = max(block, t.lo / kQBlock);
-        end = min(end, (t.hi + kQBlock - 1) / kQBlock);
-    }
-    constexpr int kStep = KEYS ? 4 : 1;
-    // parameters: a word a lane, spread over the lanes through LDS
-    uint32_t kw = 0, vw = 0;
-    const uint32_t par_key = HD == 128 ? lane >> 1 : lane & 31, par_word = HD == 128 ? 4 * (lane & 1) : 0;
-    auto load_par = [&](int k0) {
-        const uint32_t row = min(par_key, (uint32_t)(cap - 1 - k0)) * (4 * G) + par_word;
-        kw = *reinterpret_cast<const uint32_t *>(kp + (int64_t)k0 * (4 * G) + row);
-        vw = *reinterpret_cast<const uint32_t *>(vp + (int64_t)k0 * (4 * G) + row);
+    const int cap = p.cache.capacity, step = pl.splits * W, first = tile * kRows;
+    int block = part * W + wave;
+    struct Block {
+        Codes codes;
+        Params par;
+    } b0, b1;
+    auto load = [&](Block &b, int at) {
+        b.codes.load_k(kc, at * kQBlock, cap, lane);
+        b.par.load(kp, vp, at * kQBlock, cap, lane);
+        b.codes.load_v(vc, at * kQBlock, cap, lane);
     };
-    Codes codes;
-    if (block < end) {
-        codes.load_k(kc, block * kQBlock, cap, lane);
-        load_par(block * kQBlock);
-        codes.load_v(vc, block * kQBlock, cap, lane);
+    const int last = (cap - 1) / kQBlock;
+    if (!p.window && block <= last) load(b0, block);
+    v4f y[HD / 16];
+    if (wave < RT) q_fetch<HD>(p, s, g, first + 16 * wave + i, u, y);
+    if (kAhead == 2 && !p.window && block + step <= last) load(b1, block + step);
+    const QTile t = q_tile(p, s, first, kRows);
+    if (!t.count) return;
+    const int end = (t.hi + kQBlock - 1) / kQBlock, all = t.count * p.group;
+    if (p.window) {
+        block += t.lo / kQBlock;
+        if (block < end) load(b0, block);
+        if (kAhead == 2 && block + step < end) load(b1, block + step);
     }
-
-    // query rows as halves below 2^kTop, their sums of each group
-    v8h qh[RT][C], ql[RT][C];
-    float qs[RT][G], f[RT], slope[RT];
-    int pos[RT];
+    if (wave < RT) {
+        v8h hi[C], lo[C];
+        QQuery<HD> q;
+        q_query<HD, BITS, SHAPED>(p, t, g, first + 16 * wave + i, y, hi, lo, q);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            sh.in.q[wave][c][0][lane] = hi[c];
+            sh.in.q[wave][c][1][lane] = lo[c];
+        }
+        if (u == 0) s_query[wave][i] = q;
+    }
+    __syncthreads();
+    QQuery<HD> query[RT];
+    QSums<HD> sums[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = first + 16 * rt + i;
-        const bool live = r < all;
-        const int tok = live ? r / p.group : 0, head = g * p.group + (live ? r - tok * p.group : 0);
-        pos[rt] = live ? wt.len - wt.count + tok : -1;
-        float x[C][8];
-        const float *src = p.q + s * p.q_ss + tok * p.q_st + head * HD + 8 * u;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const v4f y = *reinterpret_cast<const v4f *>(src + 32 * c + e);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[c][e + k] = live ? y[k] : 0.0f;
-            }
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[c][e]));
-        const int e = row_exp(groups_umax(top));
-        const float up = pow2(kTop - e);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int c = 2 * gr; c < 2 * gr + 2; ++c)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum += x[c][k] * up;
-            qs[rt][gr] = groups_sum(sum);
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (Codes::k_upper(k)) x[c][k] *= 0.0625f;
-        split_row<C>(x, e, qh[rt], ql[rt]);
-        // score = product · f; with a cap: tanh(product · f) · cap
-        const float size = pow2(e - kTop);
-        f[rt] = SHAPED && p.cap > 0.0f ? fminf(p.scale * size * (1.0f / p.cap), 3.0e38f) : p.scale * kLog2e * size;
-        slope[rt] = 0.0f;
-        if (SHAPED && p.slopes) {
-            const float y = p.slopes[head] * kLog2e;
-            slope[rt] = fabsf(y) == INFINITY ? copysignf(3.4028235e38f, y) : y;
-        }
+        query[rt] = s_query[rt][i];
+        sums[rt].clear();
     }
-
-    v4f acc[RT][T];
-    float ref[RT], m[RT], sum[RT], mids[RT][G];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int k = 0; k < T; ++k) acc[rt][k] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        m[rt] = ref[rt] = kLowest;
-        sum[rt] = 0.0f;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) mids[rt][gr] = 0.0f;
-    }
-    uint32_t step_top = 0;  // bits of V's largest step so far
-    int raise = kQTop + 14;  // exponent that brings it below 2^kQTop
+    QScale scale;
     const uint32_t magic = code_magic();
-    uint32_t *par = reinterpret_cast<uint32_t *>(s_par[wave]);
+    uint8_t *mine = sh.in.par[wave];
 
-    for (; block < end; block += kStep) {
-        const int k0 = block * kQBlock, next0 = k0 + kStep * kQBlock;
-        const bool more = block + kStep < end;
-        const bool masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
+    auto work = [&](Block &b) {
+        const int k0 = block * kQBlock, next0 = k0 + kAhead * step * kQBlock;
+        const bool more = block + kAhead * step < end, masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
         if (masked) {  // parameters of keys outside the tile's are zero
-            const int key = k0 + (int)par_key;
-            if (key < t.lo || key >= t.hi) kw = vw = 0;
+            const int key = k0 + Params::key_of(lane);
+            if (key < t.lo || key >= t.hi) b.par.k = b.par.v = 0;
         }
-        // V's largest step.  Numbers that are none stay out of products: they would
-        // meet the zero weights of rows that do not see them.  Rows that do get them below.
-        uint64_t bad[2] = {0, 0};
-        bool moved = false;
-        {
-            const bool b0 = (vw & 0x7c00u) == 0x7c00u, b1 = (vw & 0x7c000000u) == 0x7c000000u;
-            const uint32_t s0 = vw & 0x7fffu, s1 = HD == 128 ? vw >> 16 : 0u;
-            const uint32_t lane_top = HD == 128 && (lane & 1) ? 0u : max(s0, s1);
-            if (__any((b0 || b1 || lane_top > step_top) && (HD == 128 || lane < 32))) {
-                if (b0) vw &= 0xffff0000u;
-                if (b1) vw &= 0x0000ffffu;
-                bad[0] = __ballot(HD == 128 ? b0 : b0 || b1);
-                bad[1] = __ballot(b1);
-                uint32_t y = HD == 128 && (lane & 1) ? 0u : max(vw & 0x7fffu, HD == 128 ? vw >> 16 : 0u);
-                y = groups_umax(y);
-#pragma unroll
-                for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
-                if (y > step_top) {
-                    step_top = y;
-                    // step < 2^(exponent - 14), subnormal ones < 2^-14
-                    const int now = kQTop + 14 - (int)(y >> 10);
-                    moved = now != raise;
-                    raise = now;
-                }
-            }
-        }
+        scale.look<HD>(b.par.v, lane);
         if (HD == 128 || lane < 32) {
-            par[lane] = kw;
-            par[kPar / 4 + lane] = vw;
+            reinterpret_cast<uint32_t *>(mine)[lane] = b.par.k;
+            reinterpret_cast<uint32_t *>(mine + Params::kBytes)[lane] = b.par.v;
         }
         wave_lds_order();
-        if (more) load_par(next0);
+        if (more) b.par.load(kp, vp, next0, cap, lane);
 
-        // scores: row i, keys 16 · kt + 4u + k
-        float sc[RT][8];
+        float x[RT][8];  // row i, keys 16 · kt + 4u + k
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            v8h pars[G];
-#pragma unroll
-            for (int k = 0; k < G; ++k) pars[k] = *reinterpret_cast<const v8h *>(s_par[wave] + (16 * kt + 4 * u) * 4 * G + 16 * k);
             v4f d[RT][G];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const v8h key = codes.key(kt, c, magic);
+                const v8h key = b.codes.key(kt, c, magic);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     const v4f from = c % 2 ? d[rt][c / 2] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                    const v4f x = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qh[rt][c], from, 0, 0, 0);
-                    d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, ql[rt][c], x, 0, 0, 0);
+                    const v4f y = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, sh.in.q[rt][c][0][lane], from, 0, 0, 0);
+                    d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, sh.in.q[rt][c][1][lane], y, 0, 0, 0);
                 }
             }
+            v8h pk[G];
+            Params::get(mine, kt, u, pk);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float x = 0.0f;
+                    float y = 0.0f;
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        const int at = k * 2 * G + gr;
-                        const float step = (float)pars[at >> 3][at & 7], mid = (float)pars[(at + G) >> 3][(at + G) & 7];
-                        x = gr ? fmaf(mid, qs[rt][gr], x) : mid * qs[rt][gr];
-                        x = fmaf(step, d[rt][gr][k], x);
+                        const float mid = (float)Params::of(pk, k, gr, 1);
+                        y = gr ? fmaf(mid, query[rt].sum[gr], y) : mid * query[rt].sum[gr];
+                        y = fmaf((float)Params::of(pk, k, gr, 0), d[rt][gr][k], y);
                     }
-                    sc[rt][4 * kt + k] = rounded(x * f[rt]);
+                    x[rt][4 * kt + k] = y;
                 }
         }
-        if (more) codes.load_k(kc, next0, cap, lane);
-
-        v8h wh[RT][G], wl[RT][G];
-        v8h vpar[2][G];
+        if (more) b.codes.load_k(kc, next0, cap, lane);
+        v8h pv0[G], pv1[G], hi[RT][G], lo[RT][G];
+        Params::get(mine + Params::kBytes, 0, u, pv0);
+        Params::get(mine + Params::kBytes, 1, u, pv1);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int k = 0; k < G; ++k) vpar[kt][k] = *reinterpret_cast<const v8h *>(s_par[wave] + kPar + (16 * kt + 4 * u) * 4 * G + 16 * k);
-        auto v_par = [&](int j, int gr, int which) {  // step (which 0) or midpoint of the lane's key j
-            const int at = (j & 3) * 2 * G + which * G + gr;
-            return vpar[j >> 2][at >> 3][at & 7];
-        };
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float (&x)[8] = sc[rt];
-            if (SHAPED) {
-                if (p.cap > 0.0f) {
-                    tanh_all<8>(x);
-                    const float up = p.cap * kLog2e;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] *= up;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    x[j] = rounded(fmaf(-slope[rt], (float)(pos[rt] - (k0 + 16 * (j >> 2) + 4 * u + (j & 3))), x[j]));
-            }
-            if (masked) {
-                const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int key = k0 + 16 * (j >> 2) + 4 * u + (j & 3);
-                    const bool sees = key >= from && key <= pos[rt];
-                    x[j] = sees ? x[j] : -INFINITY;
-                }
-            }
-            if (bad[0] | bad[1]) {  // NaN for the rows that see it, in its group
-                const int from = p.window ? max(0, pos[rt] - p.window + 1) : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int at = 16 * (j >> 2) + 4 * u + (j & 3), key = k0 + at;
-                    const bool sees = key >= from && key <= pos[rt];
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr)
-                        if (sees && (bad[gr] >> (HD == 128 ? 2 * at : at) & (HD == 128 ? 3 : 1))) mids[rt][gr] = __builtin_nanf("");
-                }
-            }
-            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            if (moved || __any(top > m[rt] + kQSlack)) {
-                top = groups_max(top);
-                if (top > m[rt]) m[rt] = fminf(ceilf(top), 3.0e38f);
-                const float now = fabsf(m[rt]) < kQFar ? m[rt] - (float)raise : m[rt];
-                const float by = __builtin_amdgcn_exp2f(ref[rt] - now);
-                ref[rt] = now;
-                sum[rt] *= by;
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) mids[rt][gr] *= by;
-#pragma unroll
-                for (int k = 0; k < T; ++k) acc[rt][k] *= by;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(x[j] - ref[rt]);
-                sum[rt] += x[j];
-            }
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    v2h h, l;
-                    split_steps(x[j], v_par(j, gr, 0), x[j + 1], v_par(j + 1, gr, 0), h, l);
-                    wh[rt][gr][j] = h[0];
-                    wh[rt][gr][j + 1] = h[1];
-                    wl[rt][gr][j] = l[0];
-                    wl[rt][gr][j + 1] = l[1];
-                    mids[rt][gr] = fmaf((float)v_par(j, gr, 1), x[j], mids[rt][gr]);
-                    mids[rt][gr] = fmaf((float)v_par(j + 1, gr, 1), x[j + 1], mids[rt][gr]);
-                }
-        }
+        for (int rt = 0; rt < RT; ++rt)
+            sums[rt].template weigh<SHAPED>(p, query[rt], scale, x[rt], k0, u, masked, pv0, pv1, hi[rt], lo[rt]);
 #pragma unroll
         for (int k = 0; k < T; ++k) {
-            const v8h v = codes.value(k, magic);
+            const v8h v = b.codes.value(k, magic);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh[rt][k / 4], acc[rt][k], 0, 0, 0);
-                acc[rt][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl[rt][k / 4], acc[rt][k], 0, 0, 0);
+                v4f &a = sums[rt].acc[k];
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[rt][k / 4], a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[rt][k / 4], a, 0, 0, 0);
             }
         }
-        if (more) codes.load_v(vc, next0, cap, lane);
+        if (more) b.codes.load_v(vc, next0, cap, lane);
         wave_lds_order();
+        block += step;
+    };
+    while (block < end) {
+        work(b0);
+        if (kAhead == 1) continue;
+        if (block >= end) break;
+        work(b1);
     }
 
-    // denominators and midpoints over a row's four lanes
+    // The waves' sums, to the rows' largest reference.  A lane's four numbers of LDS are
+    // neighbours: elements 64 (k / 4) + 16u + 4r + k % 4 of dim tiles k, registers r.
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        sum[rt] = groups_sum(sum[rt]);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            mids[rt][gr] = groups_sum(mids[rt][gr]);
-#pragma unroll
-            for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[rt][k] = acc[rt][k] * (Codes::v_upper(k) ? 0.0625f : 1.0f) + mids[rt][gr];
+        sums[rt].template finish<BITS>();
+        if (u == 0) {
+            s_ref[wave][16 * rt + i] = sums[rt].ref;
+            s_sum[wave][16 * rt + i] = sums[rt].total;
         }
     }
-    if (KEYS) {  // four waves' sums: 2 and 3 to 0 and 1, then 1 to 0
-        if (u == 0)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                s_ref[wave][16 * rt + i] = sum[rt] == 0.0f ? kLowest : ref[rt];
-                s_sum[wave][16 * rt + i] = sum[rt];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float top = kLowest, total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ref[w][16 * rt + i]);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) total += s_sum[w][16 * rt + i] * __builtin_amdgcn_exp2f(s_ref[w][16 * rt + i] - top);
-            const float by = __builtin_amdgcn_exp2f((sum[rt] == 0.0f ? kLowest : ref[rt]) - top);
-#pragma unroll
-            for (int k = 0; k < T; ++k) acc[rt][k] *= by;
-            sum[rt] = total;
-            ref[rt] = top;
-        }
-#pragma unroll
-        for (int half = 2; half; half >>= 1) {
-            if (wave >= half && wave < 2 * half)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int k = 0; k < T; ++k) s_acc[wave - half][rt * T + k][lane] = acc[rt][k];
-            __syncthreads();
-            if (wave < half)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int k = 0; k < T; ++k) acc[rt][k] += s_acc[wave][rt * T + k][lane];
-            __syncthreads();
-        }
-        if (wave) return;
-    }
-    const int64_t slot = (((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part;
+    __syncthreads();
+    float ref[RT], total[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = first + 16 * rt + i;
+        ref[rt] = kLowest;
+        total[rt] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) ref[rt] = fmaxf(ref[rt], s_ref[w][16 * rt + i]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) total[rt] += s_sum[w][16 * rt + i] * __builtin_amdgcn_exp2f(s_ref[w][16 * rt + i] - ref[rt]);
+    }
+    const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float by = __builtin_amdgcn_exp2f(sums[rt].ref - ref[rt]);
+#pragma unroll
+        for (int k = 0; k < T; ++k) {
+            const int gr = k / 4, r = k % 4;
+            sh.acc[wave][rt][k][lane] = (v4f){sums[rt].acc[4 * gr][r], sums[rt].acc[4 * gr + 1][r], sums[rt].acc[4 * gr + 2][r], sums[rt].acc[4 * gr + 3][r]} * by;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = 16 * rt + i, r = first + row;
         if (r >= all) continue;
-        float *dst;
-        float by = 1.0f;
-        if (share.parts > 1) {
-            const int64_t at = slot * kRows + (r - tile * kRows);
-            dst = pl.part + at * HD;
-            if (u == 0) pl.stat[at] = make_float2(sum[rt] == 0.0f ? kLowest : ref[rt], sum[rt]);
-        } else {
-            const int tok = r / p.group, head = g * p.group + r - tok * p.group;
-            dst = p.out + s * p.o_ss + tok * p.o_st + head * HD;
-            by = sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
-            if (p.lse && u == 0)
-                p.lse[((int64_t)s * p.n + tok) * p.heads + head] =
-                    sum[rt] == 0.0f ? -INFINITY : (ref[rt] + __builtin_amdgcn_logf(sum[rt])) * 0.69314718055994531f;
+        float *dst = pl.splits > 1 ? pl.part + (slot + row) * HD : q_out_row(p, s, g, r, HD);
+        const float by = pl.splits > 1 ? 1.0f : (total[rt] == 0.0f ? 0.0f : 1.0f / total[rt]);
+#pragma unroll
+        for (int k = wave; k < T; k += W) {
+            v4f sum = sh.acc[0][rt][k][lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) sum += sh.acc[w][rt][k][lane];
+            *reinterpret_cast<v4f *>(dst + 64 * (k / 4) + 16 * u + 4 * (k % 4)) = sum * by;
         }
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<v4f *>(dst + 64 * gr + 16 * u + 4 * k) =
-                    (v4f){acc[rt][4 * gr][k] * by, acc[rt][4 * gr + 1][k] * by, acc[rt][4 * gr + 2][k] * by, acc[rt][4 * gr + 3][k] * by};
+        if (wave == 0 && u == 0) {
+            if (pl.splits > 1) pl.stat[slot + row] = make_float2(ref[rt], total[rt]);
+            else if (p.lse) q_out_lse(p, s, g, r, ref[rt], total[rt]);
+        }
     }
 }
 
-// A tile's shares joined: HD / 4 lanes a row.
-template <int HD, int ROWS>
+// A tile's shares joined: HD / 4 lanes a row and share, N shares at a time (all of
+// them where there are no more: one round of loads behind the launch).
+template <int HD, int ROWS, int N>
 __global__ void __launch_bounds__(256) k_qcache_join(QAttnCall p, QAttnPlan pl) {
-    constexpr int L = HD / 4, U = 256 / L;
-    const int i = threadIdx.x % L, g = blockIdx.y, s = blockIdx.z;
-    const int tile = blockIdx.x / (ROWS / U), row = (int)(blockIdx.x % (ROWS / U)) * U + (int)threadIdx.x / L;
-    const QTile t = q_tile(p, s, tile * ROWS, ROWS);
+    constexpr int L = HD / 4, U = 256 / L, R = U / N;  // rows of a workgroup
+    __shared__ float s_ref[U], s_sum[U];
+    __shared__ v4f s_acc[U][L];
+    const int i = threadIdx.x % L, unit = threadIdx.x / L, g = blockIdx.y, s = blockIdx.z;
+    const int tile = blockIdx.x / (ROWS / R), row = (int)(blockIdx.x % (ROWS / R)) * R + unit / N, from = unit % N;
     const int r = tile * ROWS + row;
-    if (r >= t.count * p.group) return;
-    const int parts = q_share(pl, t, 0).parts;
-    if (parts == 1) return;
     const int64_t at = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits) * ROWS + row;
-    const float2 *stat = pl.stat + at;
-    const float *part = pl.part + at * HD + 4 * i;
-    float top = kLowest, total = 0.0f;
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, stat[(int64_t)k * ROWS].x);
+    const int count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
+    const bool live = r < count * p.group;  // other rows' slots hold nothing
+    float ref = kLowest, total = 0.0f;
     v4f sum = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
 #pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-        const float2 st = stat[(int64_t)k * ROWS];
-        const float by = __builtin_amdgcn_exp2f(st.x - top);
-        total += st.y * by;
-        sum += *reinterpret_cast<const v4f *>(part + (int64_t)k * ROWS * HD) * by;
+        for (int k = from; k < pl.splits; k += N) {
+            const float2 st = pl.stat[at + (int64_t)k * ROWS];
+            const v4f x = *reinterpret_cast<const v4f *>(pl.part + (at + (int64_t)k * ROWS) * HD + 4 * i);
+            const float top = fmaxf(ref, st.x), a = __builtin_amdgcn_exp2f(ref - top), b = __builtin_amdgcn_exp2f(st.x - top);
+            sum = sum * a + x * b;
+            total = total * a + st.y * b;
+            ref = top;
+        }
     }
-    const int tok = r / p.group, head = g * p.group + r - tok * p.group;
-    *reinterpret_cast<v4f *>(p.out + s * p.o_ss + tok * p.o_st + head * HD + 4 * i) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
-    if (p.lse && i == 0)
-        p.lse[((int64_t)s * p.n + tok) * p.heads + head] =
-            total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
+    if (N > 1) {
+        if (i == 0) {
+            s_ref[unit] = ref;
+            s_sum[unit] = total;
+        }
+        s_acc[unit][i] = sum;
+        __syncthreads();
+        if (from) return;
+        float top = ref;
+#pragma unroll
+        for (int k = 1; k < N; ++k) top = fmaxf(top, s_ref[unit + k]);
+        const float a = __builtin_amdgcn_exp2f(ref - top);
+        sum *= a;
+        total *= a;
+#pragma unroll
+        for (int k = 1; k < N; ++k) {
+            const float b = __builtin_amdgcn_exp2f(s_ref[unit + k] - top);
+            sum += s_acc[unit + k][i] * b;
+            total += s_sum[unit + k] * b;
+        }
+        ref = top;
+    }
+    if (!live) return;
+    *reinterpret_cast<v4f *>(q_out_row(p, s, g, r, HD) + 4 * i) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
+    if (p.lse && i == 0) q_out_lse(p, s, g, r, ref, total);
 }
 
 }  // namespace pocr
