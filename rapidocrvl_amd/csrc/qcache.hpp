@@ -609,16 +609,17 @@ struct QCodes {
     __device__ __forceinline__ static constexpr bool k_upper(int e) { return BITS == 4 && (e >> 1 & 1); }
     __device__ __forceinline__ static constexpr bool v_upper(int t) { return BITS == 4 && (t & 1); }
     // K's operand of chunk c, key tile t
-    __device__ __forceinline__ v8h key(int t, int c, uint32_t magic) const {
+    __device__ __forceinline__ v8h key(int t, int c, uint32_t magic) const { return key_of(k[t], c, magic); }
+    __device__ __forceinline__ static v8h key_of(const uint32_t *k, int c, uint32_t magic) {
         v8h r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v2h x;
             if constexpr (BITS == 4) {
-                const uint32_t w = k[t][c] >> (e & 2 ? 8 : 0);
+                const uint32_t w = k[c] >> (e & 2 ? 8 : 0);
                 x = e & 1 ? code_pair<1024 + 128>(w, 0x00f000f0u, magic) : code_pair<1024 + 8>(w, 0x000f000fu, magic);
             } else {
-                x = code_pair<1024 + 128>(__builtin_amdgcn_perm(magic, k[t][2 * c + e / 2], e & 1 ? 0x05030502u : 0x05010500u), ~0u, 0u);
+                x = code_pair<1024 + 128>(__builtin_amdgcn_perm(magic, k[2 * c + e / 2], e & 1 ? 0x05030502u : 0x05010500u), ~0u, 0u);
             }
             r[2 * e] = x[0];
             r[2 * e + 1] = x[1];
@@ -741,28 +742,53 @@ struct QParams {
     }
 };
 
-// V's largest step so far, the exponent that brings it below 2^kQTop, and the keys
-// of the present block with parameters that are no numbers.
+// products of a row's halves with keys' codes, d of each group → of the row with the
+// four keys, by the keys' parameters
+template <int HD>
+__device__ __forceinline__ void q_scores(const QQuery<HD> &q, const v8h (&par)[HD / 64], const v4f (&d)[HD / 64], float *x) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float y = 0.0f;
+#pragma unroll
+        for (int gr = 0; gr < HD / 64; ++gr) {
+            const float mid = (float)QParams<HD>::of(par, k, gr, 1);
+            y = gr ? fmaf(mid, q.sum[gr], y) : mid * q.sum[gr];
+            y = fmaf((float)QParams<HD>::of(par, k, gr, 0), d[gr][k], y);
+        }
+        x[k] = y;
+    }
+}
+
+// V's largest step so far, the exponent that brings it below 2^kQTop, and whether
+// the present block has parameters that are no numbers.
+constexpr uint16_t kQBad = 0x8000;  // in place of such a group's step: no step is a negative zero
 struct QScale {
     uint32_t top = 0;  // its bits
     int raise = kQTop + 14;
-    uint64_t bad[2] = {0, 0};
-    bool moved = false;
+    bool moved = false, bad = false;
     // `v`: a lane's word of V's parameters.  What is no number stays out of products,
     // where it would meet the zero weights of rows that do not see it.
     template <int HD>
     __device__ __forceinline__ void look(uint32_t &v, int lane) {
         const bool mine = HD == 128 || lane < 32, steps = HD == 64 || !(lane & 1);
-        const bool b0 = (v & 0x7c00u) == 0x7c00u, b1 = (v & 0x7c000000u) == 0x7c000000u;
+        bool b0 = (v & 0x7c00u) == 0x7c00u, b1 = (v & 0x7c000000u) == 0x7c000000u;
         const uint32_t most = max(v & 0x7fffu, HD == 128 ? v >> 16 : 0u);
-        bad[0] = bad[1] = 0;
-        moved = false;
+        moved = bad = false;
         if (!__any(mine && (b0 || b1 || (steps && most > top)))) return;
-        if (b0) v &= 0xffff0000u;
-        if (b1) v &= 0x0000ffffu;
-        bad[0] = __ballot(HD == 128 ? b0 : b0 || b1);
-        bad[1] = __ballot(b1);
-        uint32_t y = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 : 0u) : 0u);
+        bad = __any(mine && (b0 || b1));
+        if (bad) {
+            if constexpr (HD == 128) {  // the steps of both groups, the midpoints of both: two lanes
+                const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);
+                b0 = b0 || (other & 0x7c00u) == 0x7c00u;
+                b1 = b1 || (other & 0x7c000000u) == 0x7c000000u;
+                const uint32_t mark = steps ? kQBad : 0u;
+                if (b0) v = (v & 0xffff0000u) | mark;
+                if (b1) v = (v & 0x0000ffffu) | mark << 16;
+            } else {
+                if (b0 || b1) v = kQBad;
+            }
+        }
+        uint32_t y = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 & 0x7fffu : 0u) : 0u);
 #pragma unroll
         for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
         if (y <= top) return;
@@ -771,9 +797,6 @@ struct QScale {
         moved = now != raise;
         raise = now;
     }
-    // the group of the block's key is none
-    template <int HD>
-    __device__ __forceinline__ bool is_bad(int key, int gr) const { return bad[gr] >> (HD == 128 ? 2 * key : key) & (HD == 128 ? 3 : 1); }
 };
 
 // A row's running sums, in a lane of its tile.
@@ -815,13 +838,15 @@ struct QSums {
                 x[j] = key >= q.from && key <= q.pos ? x[j] : -INFINITY;
             }
         }
-        if (scale.bad[0] | scale.bad[1]) {  // NaN for the rows that see one, in its group
+        if (scale.bad) {  // NaN for the rows that see one, in its group
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = k0 + key_of(j);
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr)
-                    if (key >= q.from && key <= q.pos && scale.is_bad<HD>(key_of(j), gr)) mids[gr] = __builtin_nanf("");
+                for (int gr = 0; gr < G; ++gr) {
+                    const _Float16 step = QParams<HD>::of(j < 4 ? v0 : v1, j & 3, gr, 0);
+                    if (key >= q.from && key <= q.pos && __builtin_bit_cast(uint16_t, step) == kQBad) mids[gr] = __builtin_nanf("");
+                }
             }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * size;
@@ -1000,18 +1025,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
             v8h pk[G];
             Params::get(mine, kt, u, pk);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float y = 0.0f;
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        const float mid = (float)Params::of(pk, k, gr, 1);
-                        y = gr ? fmaf(mid, query[rt].sum[gr], y) : mid * query[rt].sum[gr];
-                        y = fmaf((float)Params::of(pk, k, gr, 0), d[rt][gr][k], y);
-                    }
-                    x[rt][4 * kt + k] = y;
-                }
+            for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt], pk, d[rt], x[rt] + 4 * kt);
         }
         if (more) b.codes.load_k(kc, next0, cap, lane);
         v8h pv0[G], pv1[G], hi[RT][G], lo[RT][G];
@@ -1089,6 +1103,199 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
         if (wave == 0 && u == 0) {
             if (pl.splits > 1) pl.stat[slot + row] = make_float2(ref[rt], total[rt]);
             else if (p.lse) q_out_lse(p, s, g, r, ref[rt], total[rt]);
+        }
+    }
+}
+
+// One wave's part of a block's codes on their way into LDS, as the matrix
+// instructions take them, for the four waves of a workgroup.  Chunks of 16 bytes a
+// lane: K's [key tile][chunk], wave w those of key tile w / 2 with c / (C / 2) = w % 2;
+// V's [dim tile], wave w those with t / (T / 4) = w.
+template <int HD, int BITS>
+struct QLayer {
+    using F = QFormat<HD, BITS>;
+    static constexpr int C = HD / 32, T = HD / 16, kK = C / 2, kV = T / 4;  // of a wave
+    static constexpr int kBytes = (2 * C + T) * 1024;
+    uint32_t k[kK * BITS / 4];
+    uint32_t v[8];
+    __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *vc, int k0, int rows, int wave, int lane) {
+        const uint32_t i = lane & 15, u = lane >> 4, last = rows - 1 - k0;
+        const bool whole = k0 + kQBlock <= rows;
+        const uint32_t key = 16 * (wave >> 1) + i, half = wave & 1;
+        const uint32_t at = HD == 128 ? (BITS == 4 ? 16 * u + 8 * half : 64 * half + 16 * u) : (BITS == 4 ? 8 * u + 4 * half : 16 * u + 8 * half);
+        QCodes<HD, BITS>::template words<kK * BITS / 4>(kc + (int64_t)k0 * F::kCodes + ((whole ? key : min(key, last)) * F::kCodes + at), k);
+        // codes of dim tiles kV · wave ..: a byte's two, a byte, or two bytes
+        const uint8_t *vb = vc + (int64_t)k0 * F::kCodes;
+        const uint32_t place = HD == 128 ? (BITS == 4 ? 4 * i + wave : 8 * i + 2 * wave) : (BITS == 4 ? 2 * i + (wave >> 1) : 4 * i + wave);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t r = 16 * (j >> 2) + 4 * u + (j & 3), off = (whole ? r : min(r, last)) * F::kCodes + place;
+            if constexpr (HD == 128 && BITS == 8) v[j] = *reinterpret_cast<const uint16_t *>(vb + off);
+            else v[j] = vb[off];
+        }
+    }
+    __device__ __forceinline__ void put(uint8_t *to, int wave, int lane, uint32_t magic) const {
+        v8h *kf = reinterpret_cast<v8h *>(to) + ((wave >> 1) * C + (wave & 1) * kK) * 64 + lane;
+#pragma unroll
+        for (int c = 0; c < kK; ++c) kf[64 * c] = QCodes<HD, BITS>::key_of(k, c, magic);
+        v8h *vf = reinterpret_cast<v8h *>(to) + (2 * C + wave * kV) * 64 + lane;
+        v8h r[kV];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t two = v[j] | v[j + 1] << 16;
+            v2h x[2];
+            if constexpr (BITS == 4) {
+                const v2h lower = code_pair<1024 + 8>(two, 0x000f000fu, magic), upper = code_pair<1024 + 128>(two, 0x00f000f0u, magic);
+                if constexpr (kV == 2) {
+                    x[0] = lower;
+                    x[1] = upper;
+                } else {
+                    x[0] = wave & 1 ? upper : lower;
+                }
+            } else {
+                x[0] = code_pair<1024 + 128>(two, 0x00ff00ffu, magic);
+                if constexpr (kV == 2) x[1] = code_pair<1024 + 128>(two >> 8, 0x00ff00ffu, magic);
+            }
+#pragma unroll
+            for (int t = 0; t < kV; ++t) {
+                r[t][j] = x[t][0];
+                r[t][j + 1] = x[t][1];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kV; ++t) vf[64 * t] = r[t];
+    }
+};
+
+// The same attention for many query rows: 16 · RT rows a wave, four waves that take
+// the share's blocks together, each unpacking a quarter of a block's codes into LDS
+// for all of them while the block before is multiplied (two buffers, one barrier a
+// block).
+template <int HD, int BITS, int RT, bool SHAPED>
+__global__ void __launch_bounds__(256, 2) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
+    using F = QFormat<HD, BITS>;
+    using Layer = QLayer<HD, BITS>;
+    using Params = QParams<HD>;
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 64 * RT;
+    __shared__ struct {
+        __attribute__((aligned(16))) uint8_t codes[Layer::kBytes], par[2 * Params::kBytes];
+    } sh[2];
+    __shared__ v8h s_low[4][RT][C][64];  // the query rows' lower halves
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
+    const int g = blockIdx.y, s = blockIdx.z;
+    const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
+    const QTile wt = q_tile(p, s, tile * kRows, kRows);
+    if (!wt.count) return;
+    const int64_t base = s * p.cache.seq_rows + (int64_t)g * p.cache.capacity;
+    const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
+    const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
+    const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
+    const int cap = p.cache.capacity, step = pl.splits, first = tile * kRows + 16 * RT * wave, all = wt.count * p.group;
+    const int end = (wt.hi + kQBlock - 1) / kQBlock;
+    int block = wt.lo / kQBlock + part;
+
+    Layer layer;
+    Params par;
+    if (block < end) {
+        layer.load(kc, vc, block * kQBlock, cap, wave, lane);
+        par.load(kp, vp, block * kQBlock, cap, lane);
+    }
+    const QTile t = q_tile(p, s, first, 16 * RT);  // this wave's rows; none: nothing is seen
+    v8h qh[RT][C];
+    QQuery<HD> query[RT];
+    QSums<HD> sums[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        v4f y[HD / 16];
+        v8h ql[C];
+        q_fetch<HD>(p, s, g, first + 16 * rt + i, u, y);
+        q_query<HD, BITS, SHAPED>(p, wt, g, first + 16 * rt + i, y, qh[rt], ql, query[rt]);
+        sums[rt].clear();
+#pragma unroll
+        for (int c = 0; c < C; ++c) s_low[wave][rt][c][lane] = ql[c];
+    }
+    QScale next_scale;
+    const uint32_t magic = code_magic();
+    // a block's codes and parameters into a buffer; the block after it is then requested
+    auto put = [&](int at, int b) {
+        const int k0 = at * kQBlock;
+        if (k0 < wt.all_lo || k0 + kQBlock > wt.all_hi) {  // parameters of keys outside the tile's are zero
+            const int key = k0 + Params::key_of(lane);
+            if (key < wt.lo || key >= wt.hi) par.k = par.v = 0;
+        }
+        next_scale.look<HD>(par.v, lane);
+        if (wave < 2 && (HD == 128 || lane < 32)) reinterpret_cast<uint32_t *>(sh[b].par + wave * Params::kBytes)[lane] = wave ? par.v : par.k;
+        layer.put(sh[b].codes, wave, lane, magic);
+        if (at + step < end) {
+            layer.load(kc, vc, (at + step) * kQBlock, cap, wave, lane);
+            par.load(kp, vp, (at + step) * kQBlock, cap, lane);
+        }
+    };
+    if (block < end) put(block, 0);
+    __syncthreads();
+    for (int b = 0; block < end; block += step, b ^= 1) {
+        const QScale scale = next_scale;
+        if (block + step < end) put(block + step, b ^ 1);
+        const int k0 = block * kQBlock;
+        if (k0 < t.hi && k0 + kQBlock > t.lo) {
+            const bool masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
+            const v8h *kf = reinterpret_cast<const v8h *>(sh[b].codes) + lane, *vf = kf + 2 * C * 64;
+            float x[RT][8];  // row i, keys 16 · kt + 4u + k
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                v4f d[RT][G];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const v8h key = kf[(kt * C + c) * 64];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const v4f from = c % 2 ? d[rt][c / 2] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                        const v4f y = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qh[rt][c], from, 0, 0, 0);
+                        d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, s_low[wave][rt][c][lane], y, 0, 0, 0);
+                    }
+                }
+                v8h pk[G];
+                Params::get(sh[b].par, kt, u, pk);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt], pk, d[rt], x[rt] + 4 * kt);
+            }
+            v8h pv0[G], pv1[G], hi[RT][G], lo[RT][G];
+            Params::get(sh[b].par + Params::kBytes, 0, u, pv0);
+            Params::get(sh[b].par + Params::kBytes, 1, u, pv1);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                sums[rt].template weigh<SHAPED>(p, query[rt], scale, x[rt], k0, u, masked, pv0, pv1, hi[rt], lo[rt]);
+#pragma unroll
+            for (int k = 0; k < T; ++k) {
+                const v8h v = vf[k * 64];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    v4f &a = sums[rt].acc[k];
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[rt][k / 4], a, 0, 0, 0);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[rt][k / 4], a, 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        sums[rt].template finish<BITS>();
+        const int r = first + 16 * rt + i, row = r - tile * kRows;
+        if (r >= all) continue;
+        float *dst = pl.splits > 1 ? pl.part + (slot + row) * HD : q_out_row(p, s, g, r, HD);
+        const float by = pl.splits > 1 ? 1.0f : (sums[rt].total == 0.0f ? 0.0f : 1.0f / sums[rt].total);
+#pragma unroll
+        for (int k = 0; k < T; ++k) {
+            const int gr = k / 4, e = k % 4;
+            *reinterpret_cast<v4f *>(dst + 64 * gr + 16 * u + 4 * e) =
+                (v4f){sums[rt].acc[4 * gr][e], sums[rt].acc[4 * gr + 1][e], sums[rt].acc[4 * gr + 2][e], sums[rt].acc[4 * gr + 3][e]} * by;
+        }
+        if (u == 0) {
+            if (pl.splits > 1) pl.stat[slot + row] = make_float2(sums[rt].ref, sums[rt].total);
+            else if (p.lse) q_out_lse(p, s, g, r, sums[rt].ref, sums[rt].total);
         }
     }
 }
