@@ -219,8 +219,8 @@ int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const c
 
 // Row tiles and key shares of one attention call.
 struct QShape {
-    int rt;      // row tiles of 16 a wave
-    bool many;   // four waves of rows of their own
+    int rt;      // row tiles of 16 a workgroup (many: waves of one each)
+    bool many;
     int rows;    // of a workgroup
     int tiles, splits;
     int64_t slots, bytes;
@@ -230,14 +230,15 @@ QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
     const char *e1 = getenv("Q_MANY"), *e2 = getenv("Q_WANT"), *e3 = getenv("Q_TWO");
     q.many = rows > (e1 ? atoi(e1) : 32);
-    q.rt = q.many ? (rows <= (e3 ? atoi(e3) : 64) ? 1 : 2) : (rows <= 16 ? 1 : 2);
-    q.rows = 16 * q.rt * (q.many ? 4 : 1);
+    q.rt = q.many ? (c->head_dim == 64 || rows <= (e3 ? atoi(e3) : 64) ? 4 : 8) : (rows <= 16 ? 1 : 2);
+    q.rows = 16 * q.rt;
     q.tiles = round_up_div(rows, q.rows);
     const int64_t work = q.tiles * groups;
     const int64_t keys = a->window ? std::min<int64_t>(a->max_rows, (int64_t)a->window + q.rows) : a->max_rows;
     const int64_t blocks = round_up_div(keys, kQBlock), least = q.many ? 2 : 4;
-    const int want = e2 ? atoi(e2) : 512;
-    q.splits = blocks <= 12 ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, want / work), 128, round_up_div(blocks, least)});
+    const int want = e2 ? atoi(e2) : (q.many && q.rt == 8 ? 256 : 512);
+    const char *e4 = getenv("Q_ONE");
+    q.splits = blocks <= (q.many || q.rt == 2 ? 12 : (e4 ? atoi(e4) : 32)) ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, want / work), 128, round_up_div(blocks, least)});
     q.slots = q.splits > 1 ? work * q.splits : 0;
     q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
     return q;
@@ -252,18 +253,21 @@ int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work,
     pl.stat = reinterpret_cast<float2 *>(pl.part + q.slots * q.rows * HD);
     const dim3 grid(q.tiles * q.splits, p.cache.kvh, seqs);
     const bool shaped = p.cap > 0.0f || p.slopes;
-    if constexpr (MANY) RC(launch(s, grid, 256, shaped ? k_qcache_attn_rows<HD, BITS, RT, true> : k_qcache_attn_rows<HD, BITS, RT, false>, p, pl));
-    else RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, RT, true> : k_qcache_attn<HD, BITS, RT, false>, p, pl));
+    if constexpr (MANY) RC(launch(s, grid, 64 * RT, shaped ? k_qcache_attn_rows<HD, BITS, RT, true> : k_qcache_attn_rows<HD, BITS, RT, false>, p, pl));
+    else if (RT == 1 && q.splits == 1) RC(launch(s, grid, 512, shaped ? k_qcache_attn<HD, BITS, 1, 8, true> : k_qcache_attn<HD, BITS, 1, 8, false>, p, pl));
+    else RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, RT, 4, true> : k_qcache_attn<HD, BITS, RT, 4, false>, p, pl));
     if (!q.slots) return POCR_OK;
-    constexpr int kRows = 16 * RT * (MANY ? 4 : 1), U = 1024 / HD;
+    constexpr int kRows = 16 * RT, U = 1024 / HD;
     if (q.splits >= 8) return launch(s, dim3(q.tiles * kRows / (U / 8), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 8>, p, pl);
     return launch(s, dim3(q.tiles * kRows / (U / 2), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 2>, p, pl);
 }
 
 template <int HD, int BITS>
 int launch_qattn_t(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
-    if (q.many) return q.rt == 1 ? launch_qattn<HD, BITS, 1, true>(s, p, q, work, seqs) : launch_qattn<HD, BITS, 2, true>(s, p, q, work, seqs);
-    return q.rt == 1 ? launch_qattn<HD, BITS, 1, false>(s, p, q, work, seqs) : launch_qattn<HD, BITS, 2, false>(s, p, q, work, seqs);
+    if (!q.many) return q.rt == 1 ? launch_qattn<HD, BITS, 1, false>(s, p, q, work, seqs) : launch_qattn<HD, BITS, 2, false>(s, p, q, work, seqs);
+    if constexpr (HD == 128)
+        if (q.rt == 8) return launch_qattn<HD, BITS, 8, true>(s, p, q, work, seqs);
+    return launch_qattn<HD, BITS, 4, true>(s, p, q, work, seqs);
 }
 
 }  // namespace

@@ -507,8 +507,8 @@ struct QAttnPlan {
 };
 
 constexpr int kQBlock = 32;      // keys per step of a wave
-constexpr int kQTop = 13;        // weights times steps stay below 2^(kQTop + kQSlack)
-constexpr int kQSlack = 2;       // a score may pass its row's reference by this before that moves
+constexpr int kQTop = 9;         // weights times steps stay below 2^(kQTop + kQSlack)
+constexpr int kQSlack = 6;       // a score may pass its row's reference by this before that moves
 constexpr float kQFar = 4194304.0f;  // up to here whole numbers and their differences are exact
 
 // the query rows of a tile: [first, last] and what they see
@@ -631,16 +631,19 @@ struct QCodes {
         v8h r;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const uint32_t b = BITS == 4 ? t >> 1 : t & 3;  // the byte that holds it
-            const int w = BITS == 4 ? 0 : t >> 2;
-            const uint32_t two = __builtin_amdgcn_perm(v[j + 1][w], v[j][w], 0x0c040c00u + 0x00010001u * b);
-            v2h x;
-            if constexpr (BITS == 4) x = t & 1 ? code_pair<1024 + 128>(two, 0x00f000f0u, magic) : code_pair<1024 + 8>(two, 0x000f000fu, magic);
-            else x = code_pair<1024 + 128>(two, ~0u, magic);
+            const v2h x = value_pair(v[j], v[j + 1], t, magic);
             r[j] = x[0];
             r[j + 1] = x[1];
         }
         return r;
+    }
+    // code t of two keys' words
+    __device__ __forceinline__ static v2h value_pair(const uint32_t *a, const uint32_t *b, int t, uint32_t magic) {
+        const uint32_t at = BITS == 4 ? t >> 1 : t & 3;  // the byte that holds it
+        const int w = BITS == 4 ? 0 : t >> 2;
+        const uint32_t two = __builtin_amdgcn_perm(b[w], a[w], 0x0c040c00u + 0x00010001u * at);
+        if constexpr (BITS == 4) return t & 1 ? code_pair<1024 + 128>(two, 0x00f000f0u, magic) : code_pair<1024 + 8>(two, 0x000f000fu, magic);
+        else return code_pair<1024 + 128>(two, ~0u, magic);
     }
 };
 
@@ -771,16 +774,20 @@ struct QScale {
     template <int HD>
     __device__ __forceinline__ void look(uint32_t &v, int lane) {
         const bool mine = HD == 128 || lane < 32, steps = HD == 64 || !(lane & 1);
-        bool b0 = (v & 0x7c00u) == 0x7c00u, b1 = (v & 0x7c000000u) == 0x7c000000u;
-        const uint32_t most = max(v & 0x7fffu, HD == 128 ? v >> 16 : 0u);
+        const uint32_t low = v & 0x7fffu, high = v >> 16 & 0x7fffu, none = 0x7bffu;  // none: the largest number
         moved = bad = false;
-        if (!__any(mine && (b0 || b1 || (steps && most > top)))) return;
+        if constexpr (HD == 128) {
+            if (!__any(max(low, high) > (steps ? top : none))) return;
+        } else {
+            if (!__any(mine && (low > top || high > none))) return;
+        }
+        bool b0 = low > none, b1 = high > none;
         bad = __any(mine && (b0 || b1));
         if (bad) {
             if constexpr (HD == 128) {  // the steps of both groups, the midpoints of both: two lanes
                 const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);
-                b0 = b0 || (other & 0x7c00u) == 0x7c00u;
-                b1 = b1 || (other & 0x7c000000u) == 0x7c000000u;
+                b0 = b0 || (other & 0x7fffu) > none;
+                b1 = b1 || (other >> 16 & 0x7fffu) > none;
                 const uint32_t mark = steps ? kQBad : 0u;
                 if (b0) v = (v & 0xffff0000u) | mark;
                 if (b1) v = (v & 0x0000ffffu) | mark << 16;
@@ -788,12 +795,12 @@ struct QScale {
                 if (b0 || b1) v = kQBad;
             }
         }
-        uint32_t y = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 & 0x7fffu : 0u) : 0u);
+        uint32_t most = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 & 0x7fffu : 0u) : 0u);
 #pragma unroll
-        for (int o = 8; o; o >>= 1) y = max(y, (uint32_t)__shfl_xor((int)y, o));
-        if (y <= top) return;
-        top = y;
-        const int now = kQTop + 14 - (int)(y >> 10);  // step < 2^(exponent - 14), subnormal ones < 2^-14
+        for (int o = 8; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+        if (most <= top) return;
+        top = most;
+        const int now = kQTop + 14 - (int)(most >> 10);  // step < 2^(exponent - 14), subnormal ones < 2^-14
         moved = now != raise;
         raise = now;
     }
@@ -811,11 +818,14 @@ struct QSums {
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) mids[gr] = 0.0f;
     }
-    // a block's products x (lane: keys 16 (j / 4) + 4u + j % 4 of its block) → weights times V's steps
+    // products x of a block from key k0 on (lane: keys 16 (j / 4) + 4u + j % 4) → scores,
+    // but for q.size, and the row's reference.  rare: some row does not see all keys, or
+    // some of V's parameters are no numbers.
     template <bool SHAPED>
-    __device__ __forceinline__ void weigh(const QAttnCall &p, const QQuery<HD> &q, const QScale &scale, float (&x)[8], int k0, int u, bool masked,
-                                          const v8h (&v0)[G], const v8h (&v1)[G], v8h (&hi)[G], v8h (&lo)[G]) {
-        auto key_of = [&](int j) { return 16 * (j >> 2) + 4 * u + (j & 3); };
+    __device__ __forceinline__ void shape(const QAttnCall &p, const QQuery<HD> &q, int raise, bool moved, float (&x)[8], int k0, int u, bool rare,
+                                          const v8h (&v)[2][G]) {
+        auto key_of = [&](int j) { return k0 + 16 * (j >> 2) + 4 * u + (j & 3); };
+        const float size = SHAPED ? 1.0f : q.size;  // exact, so a score may round with its reference
         if (SHAPED) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= q.size;
@@ -828,32 +838,26 @@ struct QSums {
                 for (int j = 0; j < 8; ++j) x[j] *= up;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = rounded(fmaf(-q.slope, (float)(q.pos - k0 - key_of(j)), x[j]));
+            for (int j = 0; j < 8; ++j) x[j] = rounded(fmaf(-q.slope, (float)(q.pos - key_of(j)), x[j]));
         }
-        const float size = SHAPED ? 1.0f : q.size;  // exact, so a score may round with its reference
-        if (masked) {
+        if (rare) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int key = k0 + key_of(j);
-                x[j] = key >= q.from && key <= q.pos ? x[j] : -INFINITY;
-            }
-        }
-        if (scale.bad) {  // NaN for the rows that see one, in its group
+                const int key = key_of(j);
+                const bool sees = key >= q.from && key <= q.pos;
+                x[j] = sees ? x[j] : -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = k0 + key_of(j);
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    const _Float16 step = QParams<HD>::of(j < 4 ? v0 : v1, j & 3, gr, 0);
-                    if (key >= q.from && key <= q.pos && __builtin_bit_cast(uint16_t, step) == kQBad) mids[gr] = __builtin_nanf("");
+                for (int gr = 0; gr < G; ++gr) {  // NaN for the rows that see one, in its group
+                    const _Float16 step = QParams<HD>::of(v[j >> 2], j & 3, gr, 0);
+                    if (sees && __builtin_bit_cast(uint16_t, step) == kQBad) mids[gr] = __builtin_nanf("");
                 }
             }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * size;
-        if (scale.moved || __any(top > m + kQSlack)) {
+        if (__any(moved || top > m + kQSlack)) {
             top = groups_max(top);
             if (top > m) m = fminf(ceilf(top), 3.0e38f);
-            const float now = fabsf(m) < kQFar ? m - (float)scale.raise : m, by = __builtin_amdgcn_exp2f(ref - now);
+            const float now = fabsf(m) < kQFar ? m - (float)raise : m, by = __builtin_amdgcn_exp2f(ref - now);
             ref = now;
             total *= by;
 #pragma unroll
@@ -861,6 +865,11 @@ struct QSums {
 #pragma unroll
             for (int k = 0; k < T; ++k) acc[k] *= by;
         }
+    }
+    // scores → weights times V's steps, as halves
+    template <bool SHAPED>
+    __device__ __forceinline__ void split(const QQuery<HD> &q, float (&x)[8], const v8h (&v)[2][G], v8h (&hi)[G], v8h (&lo)[G]) {
+        const float size = SHAPED ? 1.0f : q.size;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], size, -ref));
@@ -870,7 +879,7 @@ struct QSums {
         for (int gr = 0; gr < G; ++gr)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const v8h(&par)[G] = j < 4 ? v0 : v1;
+                const v8h(&par)[G] = v[j >> 2];
                 v2h h, l;
                 split_steps(x[j], QParams<HD>::of(par, j & 3, gr, 0), x[j + 1], QParams<HD>::of(par, (j & 3) + 1, gr, 0), h, l);
                 hi[gr][j] = h[0];
@@ -918,20 +927,19 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 // p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
 // exponent that brings V's largest step so far to 2^kQTop, so that the halves of p
 // step hold the products that count whatever V's size.  All rescales are by powers
-// of two.  A wave's first blocks and its query rows do not depend on the sequence's
-// length, and are requested with it; later blocks two ahead, a block's codes as
-// soon as the registers of the one before are free.
-template <int HD, int BITS, int RT, bool SHAPED>
-__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
+// of two.  A wave's first block and its query rows do not depend on the sequence's
+// length, and are requested with it; a later block's codes as soon as the registers
+// of the one before are free.
+template <int HD, int BITS, int RT, int W, bool SHAPED>
+__global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
     using Codes = QCodes<HD, BITS>;
     using Params = QParams<HD>;
-    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, W = 4, kRows = 16 * RT;
-    constexpr int kAhead = HD == 64 || (BITS == 4 && RT == 1) ? 2 : 1;  // blocks in flight; more would leave the registers
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 16 * RT;
     union Shared {
         struct {
             v8h q[RT][C][2][64];
-            uint8_t par[W][2 * Params::kBytes];
+            uint8_t par[W][2][Params::kBytes];
         } in;
         v4f acc[W][RT][T][64];
     };
@@ -948,27 +956,22 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
     const int cap = p.cache.capacity, step = pl.splits * W, first = tile * kRows;
     int block = part * W + wave;
-    struct Block {
-        Codes codes;
-        Params par;
-    } b0, b1;
-    auto load = [&](Block &b, int at) {
-        b.codes.load_k(kc, at * kQBlock, cap, lane);
-        b.par.load(kp, vp, at * kQBlock, cap, lane);
-        b.codes.load_v(vc, at * kQBlock, cap, lane);
+    Codes codes;
+    Params par;
+    auto load = [&](int at) {
+        codes.load_k(kc, at * kQBlock, cap, lane);
+        par.load(kp, vp, at * kQBlock, cap, lane);
+        codes.load_v(vc, at * kQBlock, cap, lane);
     };
-    const int last = (cap - 1) / kQBlock;
-    if (!p.window && block <= last) load(b0, block);
+    if (!p.window && block <= (cap - 1) / kQBlock) load(block);
     v4f y[HD / 16];
     if (wave < RT) q_fetch<HD>(p, s, g, first + 16 * wave + i, u, y);
-    if (kAhead == 2 && !p.window && block + step <= last) load(b1, block + step);
     const QTile t = q_tile(p, s, first, kRows);
     if (!t.count) return;
     const int end = (t.hi + kQBlock - 1) / kQBlock, all = t.count * p.group;
     if (p.window) {
         block += t.lo / kQBlock;
-        if (block < end) load(b0, block);
-        if (kAhead == 2 && block + step < end) load(b1, block + step);
+        if (block < end) load(block);
     }
     if (wave < RT) {
         v8h hi[C], lo[C];
@@ -985,28 +988,27 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
     QQuery<HD> query[RT];
     QSums<HD> sums[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        query[rt] = s_query[rt][i];
-        sums[rt].clear();
-    }
+    for (int rt = 0; rt < RT; ++rt) query[rt] = s_query[rt][i];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) sums[rt].clear();
     QScale scale;
     const uint32_t magic = code_magic();
-    uint8_t *mine = sh.in.par[wave];
+    uint8_t *kpar = sh.in.par[wave][0], *vpar = sh.in.par[wave][1];
 
-    auto work = [&](Block &b) {
-        const int k0 = block * kQBlock, next0 = k0 + kAhead * step * kQBlock;
-        const bool more = block + kAhead * step < end, masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
+    for (; block < end; block += step) {
+        const int k0 = block * kQBlock, next0 = k0 + step * kQBlock;
+        const bool more = block + step < end, masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
         if (masked) {  // parameters of keys outside the tile's are zero
             const int key = k0 + Params::key_of(lane);
-            if (key < t.lo || key >= t.hi) b.par.k = b.par.v = 0;
+            if (key < t.lo || key >= t.hi) par.k = par.v = 0;
         }
-        scale.look<HD>(b.par.v, lane);
+        scale.look<HD>(par.v, lane);
         if (HD == 128 || lane < 32) {
-            reinterpret_cast<uint32_t *>(mine)[lane] = b.par.k;
-            reinterpret_cast<uint32_t *>(mine + Params::kBytes)[lane] = b.par.v;
+            reinterpret_cast<uint32_t *>(kpar)[lane] = par.k;
+            reinterpret_cast<uint32_t *>(vpar)[lane] = par.v;
         }
         wave_lds_order();
-        if (more) b.par.load(kp, vp, next0, cap, lane);
+        if (more) par.load(kp, vp, next0, cap, lane);
 
         float x[RT][8];  // row i, keys 16 · kt + 4u + k
 #pragma unroll
@@ -1014,7 +1016,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
             v4f d[RT][G];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const v8h key = b.codes.key(kt, c, magic);
+                const v8h key = codes.key(kt, c, magic);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     const v4f from = c % 2 ? d[rt][c / 2] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
@@ -1023,20 +1025,22 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
                 }
             }
             v8h pk[G];
-            Params::get(mine, kt, u, pk);
+            Params::get(kpar, kt, u, pk);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt], pk, d[rt], x[rt] + 4 * kt);
         }
-        if (more) b.codes.load_k(kc, next0, cap, lane);
-        v8h pv0[G], pv1[G], hi[RT][G], lo[RT][G];
-        Params::get(mine + Params::kBytes, 0, u, pv0);
-        Params::get(mine + Params::kBytes, 1, u, pv1);
+        if (more) codes.load_k(kc, next0, cap, lane);
+        v8h pv[2][G], hi[RT][G], lo[RT][G];
+        Params::get(vpar, 0, u, pv[0]);
+        Params::get(vpar, 1, u, pv[1]);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            sums[rt].template weigh<SHAPED>(p, query[rt], scale, x[rt], k0, u, masked, pv0, pv1, hi[rt], lo[rt]);
+        for (int rt = 0; rt < RT; ++rt) {
+            sums[rt].template shape<SHAPED>(p, query[rt], scale.raise, scale.moved, x[rt], k0, u, masked || scale.bad, pv);
+            sums[rt].template split<SHAPED>(query[rt], x[rt], pv, hi[rt], lo[rt]);
+        }
 #pragma unroll
         for (int k = 0; k < T; ++k) {
-            const v8h v = b.codes.value(k, magic);
+            const v8h v = codes.value(k, magic);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 v4f &a = sums[rt].acc[k];
@@ -1044,15 +1048,8 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
                 a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[rt][k / 4], a, 0, 0, 0);
             }
         }
-        if (more) b.codes.load_v(vc, next0, cap, lane);
+        if (more) codes.load_v(vc, next0, cap, lane);
         wave_lds_order();
-        block += step;
-    };
-    while (block < end) {
-        work(b0);
-        if (kAhead == 1) continue;
-        if (block >= end) break;
-        work(b1);
     }
 
     // The waves' sums, to the rows' largest reference.  A lane's four numbers of LDS are
@@ -1108,79 +1105,64 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_qcache_attn(QAttnCall 
 }
 
 // One wave's part of a block's codes on their way into LDS, as the matrix
-// instructions take them, for the four waves of a workgroup.  Chunks of 16 bytes a
-// lane: K's [key tile][chunk], wave w those of key tile w / 2 with c / (C / 2) = w % 2;
-// V's [dim tile], wave w those with t / (T / 4) = w.
-template <int HD, int BITS>
+// instructions take them, for the W waves of a workgroup: 16 bytes a lane for each of
+// K's [key tile][chunk] and V's [dim tile].  Of K a wave has whole pieces, of V a
+// lane's pair of keys (four waves: all dim tiles of it, eight: half of them), so
+// that its loads are words of codes and not their bytes.
+template <int HD, int BITS, int W>
 struct QLayer {
     using F = QFormat<HD, BITS>;
-    static constexpr int C = HD / 32, T = HD / 16, kK = C / 2, kV = T / 4;  // of a wave
-    static constexpr int kBytes = (2 * C + T) * 1024;
-    uint32_t k[kK * BITS / 4];
-    uint32_t v[8];
-    __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *vc, int k0, int rows, int wave, int lane) {
-        const uint32_t i = lane & 15, u = lane >> 4, last = rows - 1 - k0;
-        const bool whole = k0 + kQBlock <= rows;
-        const uint32_t key = 16 * (wave >> 1) + i, half = wave & 1;
-        const uint32_t at = HD == 128 ? (BITS == 4 ? 16 * u + 8 * half : 64 * half + 16 * u) : (BITS == 4 ? 8 * u + 4 * half : 16 * u + 8 * half);
-        QCodes<HD, BITS>::template words<kK * BITS / 4>(kc + (int64_t)k0 * F::kCodes + ((whole ? key : min(key, last)) * F::kCodes + at), k);
-        // codes of dim tiles kV · wave ..: a byte's two, a byte, or two bytes
-        const uint8_t *vb = vc + (int64_t)k0 * F::kCodes;
-        const uint32_t place = HD == 128 ? (BITS == 4 ? 4 * i + wave : 8 * i + 2 * wave) : (BITS == 4 ? 2 * i + (wave >> 1) : 4 * i + wave);
+    static constexpr int C = HD / 32, T = HD / 16, kK = 2 * C / W, kV = 4 * T / W;  // of a wave: K's pieces, V's dim tiles
+    static constexpr int kKBytes = 2 * C * 1024, kVBytes = T * 1024, kWords = BITS / 4;
+    static constexpr int kVWords = (kV * BITS + 31) / 32;  // of a key's codes in a lane
+    uint32_t k[kK * kWords], v[2][kVWords];
+    // rows k0 .. k0 + 31 of a cache of `rows` rows, its last in place of those behind it
+    __device__ __forceinline__ void load_k(const uint8_t *codes, int k0, int rows, int wave, int lane) {
+        const uint32_t i = lane & 15, u = lane >> 4, f = wave * kK, c = f % C;  // pieces f, f + 1: neighbours
+        k0 = min(k0, rows - 1);  // behind the last block: nothing uses it
+        const uint32_t part = BITS == 4 ? 4 * (u * C + c) : 64 * (c >> 1) + 16 * u + 8 * (c & 1);
+        QCodes<HD, BITS>::template words<kK * kWords>(
+            codes + (int64_t)k0 * F::kCodes + (min(16 * (f / C) + i, (uint32_t)(rows - 1 - k0)) * F::kCodes + part), k);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *codes, int k0, int rows, int wave, int lane) {
+        const uint32_t i = lane & 15, u = lane >> 4, j = 2 * (wave & 3);  // keys of slots j and j + 1
+        k0 = min(k0, rows - 1);
+        const uint32_t part = T * BITS / 8 * i + (W == 8 ? (wave >> 2) * (kV * BITS / 8) : 0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t r = 16 * (j >> 2) + 4 * u + (j & 3), off = (whole ? r : min(r, last)) * F::kCodes + place;
-            if constexpr (HD == 128 && BITS == 8) v[j] = *reinterpret_cast<const uint16_t *>(vb + off);
-            else v[j] = vb[off];
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t row = 16 * (j >> 2) + 4 * u + (j & 3) + n;
+            const uint8_t *at = codes + (int64_t)k0 * F::kCodes + (min(row, (uint32_t)(rows - 1 - k0)) * F::kCodes + part);
+            if constexpr (kV * BITS == 16) v[n][0] = *reinterpret_cast<const uint16_t *>(at);
+            else QCodes<HD, BITS>::template words<kVWords>(at, v[n]);
         }
     }
-    __device__ __forceinline__ void put(uint8_t *to, int wave, int lane, uint32_t magic) const {
-        v8h *kf = reinterpret_cast<v8h *>(to) + ((wave >> 1) * C + (wave & 1) * kK) * 64 + lane;
+    __device__ __forceinline__ void put_k(uint8_t *to, int wave, int lane, uint32_t magic) const {
 #pragma unroll
-        for (int c = 0; c < kK; ++c) kf[64 * c] = QCodes<HD, BITS>::key_of(k, c, magic);
-        v8h *vf = reinterpret_cast<v8h *>(to) + (2 * C + wave * kV) * 64 + lane;
-        v8h r[kV];
+        for (int n = 0; n < kK; ++n) reinterpret_cast<v8h *>(to)[(wave * kK + n) * 64 + lane] = QCodes<HD, BITS>::key_of(k, n, magic);
+    }
+    __device__ __forceinline__ void put_v(uint8_t *to, int wave, int lane, uint32_t magic) const {
+        v2h *at = reinterpret_cast<v2h *>(to) + ((W == 8 ? (wave >> 2) * kV : 0) * 64 + lane) * 4 + (wave & 3);
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const uint32_t two = v[j] | v[j + 1] << 16;
-            v2h x[2];
-            if constexpr (BITS == 4) {
-                const v2h lower = code_pair<1024 + 8>(two, 0x000f000fu, magic), upper = code_pair<1024 + 128>(two, 0x00f000f0u, magic);
-                if constexpr (kV == 2) {
-                    x[0] = lower;
-                    x[1] = upper;
-                } else {
-                    x[0] = wave & 1 ? upper : lower;
-                }
-            } else {
-                x[0] = code_pair<1024 + 128>(two, 0x00ff00ffu, magic);
-                if constexpr (kV == 2) x[1] = code_pair<1024 + 128>(two >> 8, 0x00ff00ffu, magic);
-            }
-#pragma unroll
-            for (int t = 0; t < kV; ++t) {
-                r[t][j] = x[t][0];
-                r[t][j + 1] = x[t][1];
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < kV; ++t) vf[64 * t] = r[t];
+        for (int t = 0; t < kV; ++t) at[256 * t] = QCodes<HD, BITS>::value_pair(v[0], v[1], t, magic);
     }
 };
 
-// The same attention for many query rows: 16 · RT rows a wave, four waves that take
-// the share's blocks together, each unpacking a quarter of a block's codes into LDS
-// for all of them while the block before is multiplied (two buffers, one barrier a
-// block).
-template <int HD, int BITS, int RT, bool SHAPED>
-__global__ void __launch_bounds__(256, 2) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
+// The same attention for many query rows: W waves of 16 rows take the share's blocks
+// together, each unpacking its part of a block's codes into LDS for all of them.
+// A wave's vector instructions take longer than its matrix instructions, and run
+// beside them only where they lie between them: the next block's scores are
+// multiplied among this block's exponentials, this block's sums among the unpacking
+// of later codes.  So a round needs the next block's keys and this block's values;
+// both have two buffers, their parameters three, and a round one barrier.
+template <int HD, int BITS, int W, bool SHAPED>
+__global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
-    using Layer = QLayer<HD, BITS>;
+    using Layer = QLayer<HD, BITS, W>;
     using Params = QParams<HD>;
-    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 64 * RT;
-    __shared__ struct {
-        __attribute__((aligned(16))) uint8_t codes[Layer::kBytes], par[2 * Params::kBytes];
-    } sh[2];
-    __shared__ v8h s_low[4][RT][C][64];  // the query rows' lower halves
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 16 * W;
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][Layer::kKBytes], s_v[2][Layer::kVBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t s_kpar[3][Params::kBytes], s_vpar[2][Params::kBytes];
+    __shared__ int2 s_raise[2];  // what V's parameters ask for: QScale's raise and bad
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
@@ -1191,112 +1173,132 @@ __global__ void __launch_bounds__(256, 2) k_qcache_attn_rows(QAttnCall p, QAttnP
     const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
-    const int cap = p.cache.capacity, step = pl.splits, first = tile * kRows + 16 * RT * wave, all = wt.count * p.group;
-    const int end = (wt.hi + kQBlock - 1) / kQBlock;
-    int block = wt.lo / kQBlock + part;
+    const int cap = p.cache.capacity, step = pl.splits * kQBlock, first = tile * kRows + 16 * wave, all = wt.count * p.group;
+    int k0 = (wt.lo / kQBlock + part) * kQBlock;  // of this round's block
 
     Layer layer;
-    Params par;
-    if (block < end) {
-        layer.load(kc, vc, block * kQBlock, cap, wave, lane);
-        par.load(kp, vp, block * kQBlock, cap, lane);
-    }
-    const QTile t = q_tile(p, s, first, 16 * RT);  // this wave's rows; none: nothing is seen
-    v8h qh[RT][C];
-    QQuery<HD> query[RT];
-    QSums<HD> sums[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        v4f y[HD / 16];
-        v8h ql[C];
-        q_fetch<HD>(p, s, g, first + 16 * rt + i, u, y);
-        q_query<HD, BITS, SHAPED>(p, wt, g, first + 16 * rt + i, y, qh[rt], ql, query[rt]);
-        sums[rt].clear();
-#pragma unroll
-        for (int c = 0; c < C; ++c) s_low[wave][rt][c][lane] = ql[c];
-    }
-    QScale next_scale;
     const uint32_t magic = code_magic();
-    // a block's codes and parameters into a buffer; the block after it is then requested
-    auto put = [&](int at, int b) {
-        const int k0 = at * kQBlock;
-        if (k0 < wt.all_lo || k0 + kQBlock > wt.all_hi) {  // parameters of keys outside the tile's are zero
-            const int key = k0 + Params::key_of(lane);
-            if (key < wt.lo || key >= wt.hi) par.k = par.v = 0;
-        }
-        next_scale.look<HD>(par.v, lane);
-        if (wave < 2 && (HD == 128 || lane < 32)) reinterpret_cast<uint32_t *>(sh[b].par + wave * Params::kBytes)[lane] = wave ? par.v : par.k;
-        layer.put(sh[b].codes, wave, lane, magic);
-        if (at + step < end) {
-            layer.load(kc, vc, (at + step) * kQBlock, cap, wave, lane);
-            par.load(kp, vp, (at + step) * kQBlock, cap, lane);
+    uint32_t kw, vw;  // a word of parameters: the next block's keys', this block's values'
+    auto load_par = [&](const uint8_t *at, int from) {
+        const int k = min(from, cap - 1);
+        return *reinterpret_cast<const uint32_t *>(at + (int64_t)k * (4 * G) + min((uint32_t)Params::key_of(lane), (uint32_t)(cap - 1 - k)) * (4 * G) +
+                                                   (HD == 128 ? 4 * (lane & 1) : 0));
+    };
+    // parameters of keys outside the tile's are zero
+    auto outside = [&](int from) {
+        const int key = from + Params::key_of(lane);
+        return (from < wt.all_lo || from + kQBlock > wt.all_hi) && (key < wt.lo || key >= wt.hi);
+    };
+    auto put_par = [&](uint8_t *to, uint32_t w) {
+        if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(to)[lane] = w;
+    };
+    layer.load_k(kc, k0, cap, wave, lane);
+    kw = load_par(kp, k0);
+    v8h qh[C], ql[C];
+    QQuery<HD> query;
+    QSums<HD> sums;
+    {
+        v4f y[HD / 16];
+        q_fetch<HD>(p, s, g, first + i, u, y);
+        layer.load_v(vc, k0, cap, wave, lane);
+        vw = load_par(vp, k0);
+        q_query<HD, BITS, SHAPED>(p, wt, g, first + i, y, qh, ql, query);
+        sums.clear();
+    }
+    layer.put_k(s_k[0], wave, lane, magic);
+    if (wave == 0) put_par(s_kpar[0], outside(k0) ? 0u : kw);
+    layer.load_k(kc, k0 + step, cap, wave, lane);
+    kw = load_par(kp, k0 + step);
+    __syncthreads();
+    v4f d[2][G];
+    // four sums at a time, so that no product waits for the one before
+    auto multiply = [&](const uint8_t *codes) {
+        const v8h *kf = reinterpret_cast<const v8h *>(codes) + lane;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            v8h key[2][G];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        if (half == 0) key[kt][gr] = kf[(kt * C + 2 * gr + c) * 64];
+                        const v4f from = c || half ? d[kt][gr] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                        d[kt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[kt][gr], half ? ql[2 * gr + c] : qh[2 * gr + c], from, 0, 0, 0);
+                    }
         }
     };
-    if (block < end) put(block, 0);
-    __syncthreads();
-    for (int b = 0; block < end; block += step, b ^= 1) {
-        const QScale scale = next_scale;
-        if (block + step < end) put(block + step, b ^ 1);
-        const int k0 = block * kQBlock;
-        if (k0 < t.hi && k0 + kQBlock > t.lo) {
-            const bool masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
-            const v8h *kf = reinterpret_cast<const v8h *>(sh[b].codes) + lane, *vf = kf + 2 * C * 64;
-            float x[RT][8];  // row i, keys 16 · kt + 4u + k
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                v4f d[RT][G];
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const v8h key = kf[(kt * C + c) * 64];
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        const v4f from = c % 2 ? d[rt][c / 2] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                        const v4f y = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qh[rt][c], from, 0, 0, 0);
-                        d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, s_low[wave][rt][c][lane], y, 0, 0, 0);
-                    }
-                }
-                v8h pk[G];
-                Params::get(sh[b].par, kt, u, pk);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt], pk, d[rt], x[rt] + 4 * kt);
-            }
-            v8h pv0[G], pv1[G], hi[RT][G], lo[RT][G];
-            Params::get(sh[b].par + Params::kBytes, 0, u, pv0);
-            Params::get(sh[b].par + Params::kBytes, 1, u, pv1);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                sums[rt].template weigh<SHAPED>(p, query[rt], scale, x[rt], k0, u, masked, pv0, pv1, hi[rt], lo[rt]);
-#pragma unroll
-            for (int k = 0; k < T; ++k) {
-                const v8h v = vf[k * 64];
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    v4f &a = sums[rt].acc[k];
-                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[rt][k / 4], a, 0, 0, 0);
-                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[rt][k / 4], a, 0, 0, 0);
-                }
-            }
+    multiply(s_k[0]);
+    layer.put_k(s_k[1], wave, lane, magic);
+    layer.put_v(s_v[0], wave, lane, magic);
+    layer.load_k(kc, k0 + 2 * step, cap, wave, lane);
+    layer.load_v(vc, k0 + step, cap, wave, lane);
+    QScale scale;  // wave 1's
+    int raise = scale.raise;
+    int b = 0, b3 = 0;  // round number mod 2 and 3
+    for (; k0 < wt.hi; k0 += step) {
+        const int b3next = b3 == 2 ? 0 : b3 + 1;
+        if (wave == 0) put_par(s_kpar[b3next], outside(k0 + step) ? 0u : kw);
+        if (wave == 1) {
+            vw = outside(k0) ? 0u : vw;
+            scale.look<HD>(vw, lane);
+            put_par(s_vpar[b], vw);
+            if (lane == 0) s_raise[b] = make_int2(scale.raise, scale.bad);
         }
+        kw = load_par(kp, k0 + 2 * step);
+        vw = load_par(vp, k0 + step);
         __syncthreads();
+        const int2 ask = s_raise[b];
+        float x[8];  // row i, keys 16 · kt + 4u + k
+        v8h pv[2][G];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            v8h pk[G];
+            Params::get(s_kpar[b3], kt, u, pk);
+            q_scores<HD>(query, pk, d[kt], x + 4 * kt);
+            Params::get(s_vpar[b], kt, u, pv[kt]);
+        }
+        const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
+        sums.template shape<SHAPED>(p, query, ask.x, ask.x != raise, x, k0, u, rare, pv);
+        raise = ask.x;
+        v8h hi[G], lo[G];
+        multiply(s_k[b ^ 1]);
+        sums.template split<SHAPED>(query, x, pv, hi, lo);
+        const v8h *vf = reinterpret_cast<const v8h *>(s_v[b]) + lane;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            v8h v[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (half == 0) v[k] = vf[(4 * gr + k) * 64];
+                    sums.acc[4 * gr + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], half ? lo[gr] : hi[gr], sums.acc[4 * gr + k], 0, 0, 0);
+                }
+        }
+        layer.put_k(s_k[b], wave, lane, magic);
+        layer.put_v(s_v[b ^ 1], wave, lane, magic);
+        layer.load_k(kc, k0 + 3 * step, cap, wave, lane);
+        layer.load_v(vc, k0 + 2 * step, cap, wave, lane);
+        b ^= 1;
+        b3 = b3next;
     }
+    sums.template finish<BITS>();
+    const int r = first + i, row = r - tile * kRows;
+    if (r >= all) return;
     const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
+    float *dst = pl.splits > 1 ? pl.part + (slot + row) * HD : q_out_row(p, s, g, r, HD);
+    const float by = pl.splits > 1 ? 1.0f : (sums.total == 0.0f ? 0.0f : 1.0f / sums.total);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        sums[rt].template finish<BITS>();
-        const int r = first + 16 * rt + i, row = r - tile * kRows;
-        if (r >= all) continue;
-        float *dst = pl.splits > 1 ? pl.part + (slot + row) * HD : q_out_row(p, s, g, r, HD);
-        const float by = pl.splits > 1 ? 1.0f : (sums[rt].total == 0.0f ? 0.0f : 1.0f / sums[rt].total);
-#pragma unroll
-        for (int k = 0; k < T; ++k) {
-            const int gr = k / 4, e = k % 4;
-            *reinterpret_cast<v4f *>(dst + 64 * gr + 16 * u + 4 * e) =
-                (v4f){sums[rt].acc[4 * gr][e], sums[rt].acc[4 * gr + 1][e], sums[rt].acc[4 * gr + 2][e], sums[rt].acc[4 * gr + 3][e]} * by;
-        }
-        if (u == 0) {
-            if (pl.splits > 1) pl.stat[slot + row] = make_float2(sums[rt].ref, sums[rt].total);
-            else if (p.lse) q_out_lse(p, s, g, r, sums[rt].ref, sums[rt].total);
-        }
+    for (int k = 0; k < T; ++k) {
+        const int gr = k / 4, e = k % 4;
+        *reinterpret_cast<v4f *>(dst + 64 * gr + 16 * u + 4 * e) =
+            (v4f){sums.acc[4 * gr][e], sums.acc[4 * gr + 1][e], sums.acc[4 * gr + 2][e], sums.acc[4 * gr + 3][e]} * by;
+    }
+    if (u == 0) {
+        if (pl.splits > 1) pl.stat[slot + row] = make_float2(sums.ref, sums.total);
+        else if (p.lse) q_out_lse(p, s, g, r, sums.ref, sums.total);
     }
 }
 

@@ -9,7 +9,8 @@ Attention.  A score is sum over groups of step * (q . c) + mid * (sum of q): wit
 A = sum |q| (step |c| + |mid|), q keeps 22 bits (2^-21 with truncated remainders)
 and its sums add at most 17u of A.  The scale, the shift, a cap, a bias and the
 exponential add what cache_ops_f64.attention states.  A weight times a step keeps 22
-bits, or 2^-36 of the largest step its row sees; numerator and denominator
+bits, or 2^-32 of the largest step its row sees (halves down to 2^-25 in fp16,
+steps brought to 2^8 and more, sums of weights of 1/2 and more); numerator and denominator
 each carry (N/16 + 32)u of their sums.
 """
 import numpy as np
@@ -128,5 +129,5 @@ def attention(q, k, v, seen, scale, cap=0.0, slope=None, dist=None):
     lse_err = rows + np.abs(np.where(np.isfinite(lse), lse, 0.0)) * 2 * U + 2 * U
     size = np.abs(va) + np.abs(vb)
     out_err = (p * (d + rows[:, None])) @ size + (p @ size) * (2.0 ** -21 + steps[:, None] + 2 * U) + 1e-38
-    out_err += (np.where(seen, size.max(1), 0.0).max(1, initial=0.0) * seen.sum(1))[:, None] * 2.0 ** -36
+    out_err += (np.where(seen, size.max(1), 0.0).max(1, initial=0.0) * seen.sum(1))[:, None] * 2.0 ** -32
     return p @ (va + vb), lse, out_err, lse_err
