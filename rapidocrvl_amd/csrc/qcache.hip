@@ -219,8 +219,8 @@ int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const c
 
 // Row tiles and key shares of one attention call.
 struct QShape {
-    int rt;      // row tiles of 16 a workgroup (many: waves of one each)
-    bool many;
+    bool many;   // k_qcache_attn_rows
+    int rt;      // else: row tiles of 16 a workgroup
     int rows;    // of a workgroup
     int tiles, splits;
     int64_t slots, bytes;
@@ -228,46 +228,45 @@ struct QShape {
 QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     QShape q;
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
-    const char *e1 = getenv("Q_MANY"), *e2 = getenv("Q_WANT"), *e3 = getenv("Q_TWO");
-    q.many = rows > (e1 ? atoi(e1) : 32);
-    q.rt = q.many ? (c->head_dim == 64 || rows <= (e3 ? atoi(e3) : 64) ? 4 : 8) : (rows <= 16 ? 1 : 2);
-    q.rows = 16 * q.rt;
+    q.many = rows > 32;
+    q.rt = rows <= 16 ? 1 : 2;
+    q.rows = q.many ? 64 : 16 * q.rt;
     q.tiles = round_up_div(rows, q.rows);
     const int64_t work = q.tiles * groups;
     const int64_t keys = a->window ? std::min<int64_t>(a->max_rows, (int64_t)a->window + q.rows) : a->max_rows;
-    const int64_t blocks = round_up_div(keys, kQBlock), least = q.many ? 2 : 4;
-    const int want = e2 ? atoi(e2) : (q.many && q.rt == 8 ? 256 : 512);
-    const char *e4 = getenv("Q_ONE");
-    q.splits = blocks <= (q.many || q.rt == 2 ? 12 : (e4 ? atoi(e4) : 32)) ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, want / work), 128, round_up_div(blocks, least)});
+    const int64_t blocks = round_up_div(keys, kQBlock), whole = q.many || q.rt == 2 ? 12 : 32, least = q.many ? 3 : 4;
+    const int want = q.many ? 768 : 512;
+    q.splits = blocks <= whole ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, want / work), 128, round_up_div(blocks, least)});
     q.slots = q.splits > 1 ? work * q.splits : 0;
     q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
     return q;
 }
 
-template <int HD, int BITS, int RT, bool MANY>
+template <int HD, int BITS, int ROWS>  // rows of a workgroup
 int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
     QAttnPlan pl{};
     pl.tiles = q.tiles;
     pl.splits = q.splits;
     pl.part = static_cast<float *>(work);
-    pl.stat = reinterpret_cast<float2 *>(pl.part + q.slots * q.rows * HD);
+    pl.stat = reinterpret_cast<float2 *>(pl.part + q.slots * ROWS * HD);
     const dim3 grid(q.tiles * q.splits, p.cache.kvh, seqs);
     const bool shaped = p.cap > 0.0f || p.slopes;
-    if constexpr (MANY) RC(launch(s, grid, 64 * RT, shaped ? k_qcache_attn_rows<HD, BITS, RT, true> : k_qcache_attn_rows<HD, BITS, RT, false>, p, pl));
-    else if (RT == 1 && q.splits == 1) RC(launch(s, grid, 512, shaped ? k_qcache_attn<HD, BITS, 1, 8, true> : k_qcache_attn<HD, BITS, 1, 8, false>, p, pl));
-    else RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, RT, 4, true> : k_qcache_attn<HD, BITS, RT, 4, false>, p, pl));
-    if (!q.slots) return POCR_OK;
-    constexpr int kRows = 16 * RT, U = 1024 / HD;
-    if (q.splits >= 8) return launch(s, dim3(q.tiles * kRows / (U / 8), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 8>, p, pl);
-    return launch(s, dim3(q.tiles * kRows / (U / 2), p.cache.kvh, seqs), 256, k_qcache_join<HD, kRows, 2>, p, pl);
+    if constexpr (ROWS == 64) {
+        RC(launch(s, grid, 256, shaped ? k_qcache_attn_rows<HD, BITS, true> : k_qcache_attn_rows<HD, BITS, false>, p, pl));
+    } else {
+        if (ROWS == 16 && q.splits == 1) return launch(s, grid, 512, shaped ? k_qcache_attn<HD, BITS, 1, 8, true> : k_qcache_attn<HD, BITS, 1, 8, false>, p, pl);
+        RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, ROWS / 16, 4, true> : k_qcache_attn<HD, BITS, ROWS / 16, 4, false>, p, pl));
+    }
+    if (q.splits == 1) return POCR_OK;
+    constexpr int U = 1024 / HD;
+    if (q.splits >= 8) return launch(s, dim3(q.tiles * ROWS / (U / 8), p.cache.kvh, seqs), 256, k_qcache_join<HD, ROWS, 8>, p, pl);
+    return launch(s, dim3(q.tiles * ROWS / (U / 2), p.cache.kvh, seqs), 256, k_qcache_join<HD, ROWS, 2>, p, pl);
 }
 
 template <int HD, int BITS>
 int launch_qattn_t(hipStream_t s, const QAttnCall &p, const QShape &q, void *work, int seqs) {
-    if (!q.many) return q.rt == 1 ? launch_qattn<HD, BITS, 1, false>(s, p, q, work, seqs) : launch_qattn<HD, BITS, 2, false>(s, p, q, work, seqs);
-    if constexpr (HD == 128)
-        if (q.rt == 8) return launch_qattn<HD, BITS, 8, true>(s, p, q, work, seqs);
-    return launch_qattn<HD, BITS, 4, true>(s, p, q, work, seqs);
+    if (q.many) return launch_qattn<HD, BITS, 64>(s, p, q, work, seqs);
+    return q.rt == 1 ? launch_qattn<HD, BITS, 16>(s, p, q, work, seqs) : launch_qattn<HD, BITS, 32>(s, p, q, work, seqs);
 }
 
 }  // namespace

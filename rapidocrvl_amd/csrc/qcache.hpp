@@ -548,6 +548,33 @@ __device__ __forceinline__ v2h code_pair(uint32_t bits, uint32_t mask, uint32_t 
     return __builtin_bit_cast(v2h, (bits & mask) | magic) - (v2h){(_Float16)LESS, (_Float16)LESS};
 }
 
+// Rows k0 .. k0 + 31, W bytes each, of a cache of `rows` rows: what lies behind its
+// last row is not read, and comes as zeros.
+template <int W>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t q_block(const uint8_t *at, int k0, int rows) {
+    const int count = min(rows - min(k0, rows), kQBlock);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(at) + (int64_t)k0 * W, 0, count * W, 0x00027000);
+}
+template <int N>
+__device__ __forceinline__ void q_words(__amdgpu_buffer_rsrc_t from, uint32_t at, uint32_t *to) {
+    if constexpr (N == 8) {
+        q_words<4>(from, at, to);
+        q_words<4>(from, at + 64, to + 4);
+    } else if constexpr (N == 4) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+        to[0] = x[0];
+        to[1] = x[1];
+        to[2] = x[2];
+        to[3] = x[3];
+    } else if constexpr (N == 2) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0);
+        to[0] = x[0];
+        to[1] = x[1];
+    } else {
+        to[0] = __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
+    }
+}
+
 // Codes of 32 keys as a lane loads and uses them.  Lane l = 16u + i.  K: keys i and
 // 16 + i, elements 32c + 8u .. +7 of each 32 (a matrix instruction's operand); V: keys
 // 4u .. +3 and 16 + 4u .. +3, elements 4i .. +3 of each 64.  Of two codes of 4 bits
@@ -561,48 +588,21 @@ struct QCodes {
     static constexpr int kVWords = HD == 64 && BITS == 4 ? 1 : HD * BITS / 512;  // (16 bits for heads of 64 in 4 bits)
     uint32_t k[2][kKWords], v[8][kVWords];
 
-    template <int W>
-    __device__ __forceinline__ static void words(const uint8_t *at, uint32_t *to) {
-        if constexpr (W == 8) {
-            words<4>(at, to);
-            words<4>(at + 64, to + 4);
-        } else if constexpr (W == 4) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(at);
-            to[0] = x.x;
-            to[1] = x.y;
-            to[2] = x.z;
-            to[3] = x.w;
-        } else if constexpr (W == 2) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(at);
-            to[0] = x.x;
-            to[1] = x.y;
-        } else {
-            to[0] = *reinterpret_cast<const uint32_t *>(at);
-        }
-    }
-    // rows k0 .. k0 + 31 of a cache of `rows` rows, its last in place of those behind it
+    // rows k0 .. k0 + 31 of a cache of `rows` rows
     __device__ __forceinline__ void load_k(const uint8_t *codes, int k0, int rows, int lane) {
-        const uint8_t *at = codes + (int64_t)k0 * F::kCodes;
-        const uint32_t i = lane & 15, part = (lane >> 4) * (kKWords == 2 ? 8 : 16), last = rows - 1 - k0;
+        const auto from = q_block<F::kCodes>(codes, k0, rows);
+        const uint32_t at = (lane & 15) * F::kCodes + (lane >> 4) * (kKWords == 2 ? 8 : 16);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint32_t row = 16 * t + i;
-            words<kKWords>(at + ((k0 + kQBlock <= rows ? row : min(row, last)) * F::kCodes + part), k[t]);
-        }
+        for (int t = 0; t < 2; ++t) q_words<kKWords>(from, at + 16 * t * F::kCodes, k[t]);
     }
     __device__ __forceinline__ void load_v(const uint8_t *codes, int k0, int rows, int lane) {
-        const uint8_t *at = codes + (int64_t)k0 * F::kCodes;
-        const uint32_t u = lane >> 4, part = (lane & 15) * (HD == 64 && BITS == 4 ? 2 : 4 * kVWords), last = rows - 1 - k0;
-        auto one = [&](int j, uint32_t row) {
-            if constexpr (HD == 64 && BITS == 4) v[j][0] = *reinterpret_cast<const uint16_t *>(at + (row * F::kCodes + part));
-            else words<kVWords>(at + (row * F::kCodes + part), v[j]);
-        };
-        if (k0 + kQBlock <= rows) {
+        const auto from = q_block<F::kCodes>(codes, k0, rows);
+        const uint32_t at = (lane >> 4) * 4 * F::kCodes + (lane & 15) * (HD == 64 && BITS == 4 ? 2 : 4 * kVWords);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) one(j, 16 * (j >> 2) + 4 * u + (j & 3));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) one(j, min(16 * (j >> 2) + 4 * u + (j & 3), last));
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t row = at + (16 * (j >> 2) + (j & 3)) * F::kCodes;
+            if constexpr (HD == 64 && BITS == 4) v[j][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, row, 0, 0);
+            else q_words<kVWords>(from, row, v[j]);
         }
     }
     // what elements of key chunks are to be taken times: of eight, 0 .. 7
@@ -657,7 +657,7 @@ __device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Floa
 template <int HD>
 struct QQuery {
     static constexpr int G = HD / 64;
-    float sum[G];   // of the row's elements of each group
+    float sum;      // of the row's elements of group u, in lane 16u + i (zero where there is none)
     float size;     // a power of two: score = size · product
     float slope;
     int from, pos;  // the keys it sees: [from, pos]
@@ -679,7 +679,7 @@ __device__ __forceinline__ void q_fetch(const QAttnCall &p, int s, int g, int r,
 // The same times the scale, as halves below 2^kTop, smaller where they meet the
 // upper codes of bytes.
 template <int HD, int BITS, bool SHAPED>
-__device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int g, int r, const v4f (&y)[HD / 16], v8h (&hi)[HD / 32],
+__device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int g, int r, int u, const v4f (&y)[HD / 16], v8h (&hi)[HD / 32],
                                         v8h (&lo)[HD / 32], QQuery<HD> &q) {
     constexpr int C = HD / 32, G = HD / 64;
     const bool live = r < t.count * p.group;
@@ -698,6 +698,7 @@ __device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int 
         }
     const int e = row_exp(groups_umax(top));
     const float up = pow2(kTop - e);
+    q.sum = 0.0f;
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
         float sum = 0.0f;
@@ -705,7 +706,8 @@ __device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int 
         for (int c = 2 * gr; c < 2 * gr + 2; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) sum += x[c][k] * up;
-        q.sum[gr] = groups_sum(sum);
+        sum = groups_sum(sum);
+        if (u == gr) q.sum = sum;
     }
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -728,10 +730,12 @@ struct QParams {
     static constexpr int G = HD / 64, kBytes = 32 * 4 * G;  // of K or V
     uint32_t k, v;
     __device__ __forceinline__ static int key_of(int lane) { return HD == 128 ? lane >> 1 : lane & 31; }
+    __device__ __forceinline__ static uint32_t word(const uint8_t *par, int k0, int rows, int lane) {
+        return __builtin_amdgcn_raw_buffer_load_b32(q_block<4 * G>(par, k0, rows), HD == 128 ? 4 * lane : 4 * (lane & 31), 0, 0);
+    }
     __device__ __forceinline__ void load(const uint8_t *kp, const uint8_t *vp, int k0, int rows, int lane) {
-        const uint32_t at = min((uint32_t)key_of(lane), (uint32_t)(rows - 1 - k0)) * (4 * G) + (HD == 128 ? 4 * (lane & 1) : 0);
-        k = *reinterpret_cast<const uint32_t *>(kp + (int64_t)k0 * (4 * G) + at);
-        v = *reinterpret_cast<const uint32_t *>(vp + (int64_t)k0 * (4 * G) + at);
+        k = word(kp, k0, rows, lane);
+        v = word(vp, k0, rows, lane);
     }
     // of the lane's keys 16 · kt + 4u .. +3
     __device__ __forceinline__ static void get(const uint8_t *par, int kt, int u, v8h (&x)[G]) {
@@ -745,20 +749,21 @@ struct QParams {
     }
 };
 
-// products of a row's halves with keys' codes, d of each group → of the row with the
-// four keys, by the keys' parameters
+// Products of a row's halves with keys' codes, d of each group → of the row with the
+// keys 16 · kt + 4u .. +3, by the keys' parameters: step · d, and midpoint · sum of the
+// row's elements, a matrix product in 32 bits that leaves half of the multiply-adds.
 template <int HD>
-__device__ __forceinline__ void q_scores(const QQuery<HD> &q, const v8h (&par)[HD / 64], const v4f (&d)[HD / 64], float *x) {
+__device__ __forceinline__ void q_scores(float sum, const uint8_t *par, int kt, int i, int u, const v4f (&d)[HD / 64], float *x) {
+    constexpr int G = HD / 64;
+    const float mid = (float)reinterpret_cast<const _Float16 *>(par)[(16 * kt + i) * 2 * G + G + (u & (G - 1))];
+    const v4f y = __builtin_amdgcn_mfma_f32_16x16x4f32(mid, sum, (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+    v8h steps[G];
+    QParams<HD>::get(par, kt, u, steps);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        float y = 0.0f;
+        x[k] = y[k];
 #pragma unroll
-        for (int gr = 0; gr < HD / 64; ++gr) {
-            const float mid = (float)QParams<HD>::of(par, k, gr, 1);
-            y = gr ? fmaf(mid, q.sum[gr], y) : mid * q.sum[gr];
-            y = fmaf((float)QParams<HD>::of(par, k, gr, 0), d[gr][k], y);
-        }
-        x[k] = y;
+        for (int gr = 0; gr < G; ++gr) x[k] = fmaf((float)QParams<HD>::of(steps, k, gr, 0), d[gr][k], x[k]);
     }
 }
 
@@ -945,6 +950,7 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
     };
     __shared__ Shared sh;
     __shared__ QQuery<HD> s_query[RT][16];
+    __shared__ float s_qsum[RT][64];
     __shared__ float s_ref[W][kRows], s_sum[W][kRows];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
@@ -976,19 +982,23 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
     if (wave < RT) {
         v8h hi[C], lo[C];
         QQuery<HD> q;
-        q_query<HD, BITS, SHAPED>(p, t, g, first + 16 * wave + i, y, hi, lo, q);
+        q_query<HD, BITS, SHAPED>(p, t, g, first + 16 * wave + i, u, y, hi, lo, q);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             sh.in.q[wave][c][0][lane] = hi[c];
             sh.in.q[wave][c][1][lane] = lo[c];
         }
         if (u == 0) s_query[wave][i] = q;
+        s_qsum[wave][lane] = q.sum;
     }
     __syncthreads();
     QQuery<HD> query[RT];
     QSums<HD> sums[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) query[rt] = s_query[rt][i];
+    for (int rt = 0; rt < RT; ++rt) {
+        query[rt] = s_query[rt][i];
+        query[rt].sum = s_qsum[rt][lane];
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) sums[rt].clear();
     QScale scale;
@@ -1024,10 +1034,8 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
                     d[rt][c / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, sh.in.q[rt][c][1][lane], y, 0, 0, 0);
                 }
             }
-            v8h pk[G];
-            Params::get(kpar, kt, u, pk);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt], pk, d[rt], x[rt] + 4 * kt);
+            for (int rt = 0; rt < RT; ++rt) q_scores<HD>(query[rt].sum, kpar, kt, i, u, d[rt], x[rt] + 4 * kt);
         }
         if (more) codes.load_k(kc, next0, cap, lane);
         v8h pv[2][G], hi[RT][G], lo[RT][G];
@@ -1105,35 +1113,31 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
 }
 
 // One wave's part of a block's codes on their way into LDS, as the matrix
-// instructions take them, for the W waves of a workgroup: 16 bytes a lane for each of
-// K's [key tile][chunk] and V's [dim tile].  Of K a wave has whole pieces, of V a
-// lane's pair of keys (four waves: all dim tiles of it, eight: half of them), so
-// that its loads are words of codes and not their bytes.
-template <int HD, int BITS, int W>
+// instructions take them, for the four waves of a workgroup: 16 bytes a lane for each
+// of K's [key tile][chunk] and V's [dim tile].  Of K a wave has whole pieces, of V a
+// pair of keys in all dim tiles, so that its loads are words of codes and not their
+// bytes.
+template <int HD, int BITS>
 struct QLayer {
     using F = QFormat<HD, BITS>;
-    static constexpr int C = HD / 32, T = HD / 16, kK = 2 * C / W, kV = 4 * T / W;  // of a wave: K's pieces, V's dim tiles
+    static constexpr int C = HD / 32, T = HD / 16, kK = C / 2;  // K's pieces of a wave
     static constexpr int kKBytes = 2 * C * 1024, kVBytes = T * 1024, kWords = BITS / 4;
-    static constexpr int kVWords = (kV * BITS + 31) / 32;  // of a key's codes in a lane
+    static constexpr int kVWords = (T * BITS + 31) / 32;  // of a key's codes in a lane
     uint32_t k[kK * kWords], v[2][kVWords];
-    // rows k0 .. k0 + 31 of a cache of `rows` rows, its last in place of those behind it
+    // rows k0 .. k0 + 31 of a cache of `rows` rows
     __device__ __forceinline__ void load_k(const uint8_t *codes, int k0, int rows, int wave, int lane) {
         const uint32_t i = lane & 15, u = lane >> 4, f = wave * kK, c = f % C;  // pieces f, f + 1: neighbours
-        k0 = min(k0, rows - 1);  // behind the last block: nothing uses it
         const uint32_t part = BITS == 4 ? 4 * (u * C + c) : 64 * (c >> 1) + 16 * u + 8 * (c & 1);
-        QCodes<HD, BITS>::template words<kK * kWords>(
-            codes + (int64_t)k0 * F::kCodes + (min(16 * (f / C) + i, (uint32_t)(rows - 1 - k0)) * F::kCodes + part), k);
+        q_words<kK * kWords>(q_block<F::kCodes>(codes, k0, rows), (16 * (f / C) + i) * F::kCodes + part, k);
     }
     __device__ __forceinline__ void load_v(const uint8_t *codes, int k0, int rows, int wave, int lane) {
-        const uint32_t i = lane & 15, u = lane >> 4, j = 2 * (wave & 3);  // keys of slots j and j + 1
-        k0 = min(k0, rows - 1);
-        const uint32_t part = T * BITS / 8 * i + (W == 8 ? (wave >> 2) * (kV * BITS / 8) : 0);
+        const auto from = q_block<F::kCodes>(codes, k0, rows);
+        const uint32_t i = lane & 15, u = lane >> 4, j = 2 * wave;  // keys of slots j and j + 1
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const uint32_t row = 16 * (j >> 2) + 4 * u + (j & 3) + n;
-            const uint8_t *at = codes + (int64_t)k0 * F::kCodes + (min(row, (uint32_t)(rows - 1 - k0)) * F::kCodes + part);
-            if constexpr (kV * BITS == 16) v[n][0] = *reinterpret_cast<const uint16_t *>(at);
-            else QCodes<HD, BITS>::template words<kVWords>(at, v[n]);
+            const uint32_t at = (16 * (j >> 2) + 4 * u + (j & 3) + n) * F::kCodes + T * BITS / 8 * i;
+            if constexpr (T * BITS == 16) v[n][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0);
+            else q_words<kVWords>(from, at, v[n]);
         }
     }
     __device__ __forceinline__ void put_k(uint8_t *to, int wave, int lane, uint32_t magic) const {
@@ -1141,9 +1145,9 @@ struct QLayer {
         for (int n = 0; n < kK; ++n) reinterpret_cast<v8h *>(to)[(wave * kK + n) * 64 + lane] = QCodes<HD, BITS>::key_of(k, n, magic);
     }
     __device__ __forceinline__ void put_v(uint8_t *to, int wave, int lane, uint32_t magic) const {
-        v2h *at = reinterpret_cast<v2h *>(to) + ((W == 8 ? (wave >> 2) * kV : 0) * 64 + lane) * 4 + (wave & 3);
+        v2h *at = reinterpret_cast<v2h *>(to) + 4 * lane + wave;
 #pragma unroll
-        for (int t = 0; t < kV; ++t) at[256 * t] = QCodes<HD, BITS>::value_pair(v[0], v[1], t, magic);
+        for (int t = 0; t < T; ++t) at[256 * t] = QCodes<HD, BITS>::value_pair(v[0], v[1], t, magic);
     }
 };
 
@@ -1154,12 +1158,12 @@ struct QLayer {
 // multiplied among this block's exponentials, this block's sums among the unpacking
 // of later codes.  So a round needs the next block's keys and this block's values;
 // both have two buffers, their parameters three, and a round one barrier.
-template <int HD, int BITS, int W, bool SHAPED>
-__global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
+template <int HD, int BITS, bool SHAPED>
+__global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
-    using Layer = QLayer<HD, BITS, W>;
+    using Layer = QLayer<HD, BITS>;
     using Params = QParams<HD>;
-    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 16 * W;
+    constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 64;
     __shared__ __attribute__((aligned(16))) uint8_t s_k[2][Layer::kKBytes], s_v[2][Layer::kVBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_kpar[3][Params::kBytes], s_vpar[2][Params::kBytes];
     __shared__ int2 s_raise[2];  // what V's parameters ask for: QScale's raise and bad
@@ -1167,67 +1171,69 @@ __global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
     const int g = blockIdx.y, s = blockIdx.z;
     const int tile = pl.tiles - 1 - (int)(blockIdx.x / pl.splits), part = blockIdx.x % pl.splits;  // long rows first
-    const QTile wt = q_tile(p, s, tile * kRows, kRows);
-    if (!wt.count) return;
     const int64_t base = s * p.cache.seq_rows + (int64_t)g * p.cache.capacity;
     const uint8_t *kc = p.cache.codes[0] + base * F::kCodes, *vc = p.cache.codes[1] + base * F::kCodes;
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.cache.params[0] + base * F::kParams);
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.cache.params[1] + base * F::kParams);
-    const int cap = p.cache.capacity, step = pl.splits * kQBlock, first = tile * kRows + 16 * wave, all = wt.count * p.group;
-    int k0 = (wt.lo / kQBlock + part) * kQBlock;  // of this round's block
+    const int cap = p.cache.capacity, step = pl.splits * kQBlock, first = tile * kRows + 16 * wave;
+    int k0 = part * kQBlock;  // of this round's block
 
     Layer layer;
     const uint32_t magic = code_magic();
     uint32_t kw, vw;  // a word of parameters: the next block's keys', this block's values'
-    auto load_par = [&](const uint8_t *at, int from) {
-        const int k = min(from, cap - 1);
-        return *reinterpret_cast<const uint32_t *>(at + (int64_t)k * (4 * G) + min((uint32_t)Params::key_of(lane), (uint32_t)(cap - 1 - k)) * (4 * G) +
-                                                   (HD == 128 ? 4 * (lane & 1) : 0));
+    auto load_par = [&](const uint8_t *at, int from) { return Params::word(at, from, cap, lane); };
+    auto put_par = [&](uint8_t *to, uint32_t w) {
+        if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(to)[lane] = w;
     };
+    auto load_first = [&] {
+        layer.load_k(kc, k0, cap, wave, lane);
+        kw = load_par(kp, k0);
+        layer.load_v(vc, k0, cap, wave, lane);
+        vw = load_par(vp, k0);
+    };
+    if (!p.window) load_first();
+    v4f y[HD / 16];
+    q_fetch<HD>(p, s, g, first + i, u, y);
+    const QTile wt = q_tile(p, s, tile * kRows, kRows);
+    if (!wt.count) return;
+    const int all = wt.count * p.group;
+    if (p.window) {
+        k0 += wt.lo / kQBlock * kQBlock;
+        load_first();
+    }
     // parameters of keys outside the tile's are zero
     auto outside = [&](int from) {
         const int key = from + Params::key_of(lane);
         return (from < wt.all_lo || from + kQBlock > wt.all_hi) && (key < wt.lo || key >= wt.hi);
     };
-    auto put_par = [&](uint8_t *to, uint32_t w) {
-        if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(to)[lane] = w;
-    };
-    layer.load_k(kc, k0, cap, wave, lane);
-    kw = load_par(kp, k0);
     v8h qh[C], ql[C];
     QQuery<HD> query;
     QSums<HD> sums;
-    {
-        v4f y[HD / 16];
-        q_fetch<HD>(p, s, g, first + i, u, y);
-        layer.load_v(vc, k0, cap, wave, lane);
-        vw = load_par(vp, k0);
-        q_query<HD, BITS, SHAPED>(p, wt, g, first + i, y, qh, ql, query);
-        sums.clear();
-    }
+    q_query<HD, BITS, SHAPED>(p, wt, g, first + i, u, y, qh, ql, query);
+    sums.clear();
     layer.put_k(s_k[0], wave, lane, magic);
     if (wave == 0) put_par(s_kpar[0], outside(k0) ? 0u : kw);
     layer.load_k(kc, k0 + step, cap, wave, lane);
     kw = load_par(kp, k0 + step);
     __syncthreads();
     v4f d[2][G];
-    // four sums at a time, so that no product waits for the one before
+    // two sums at a time: one product does not wait for the one before
     auto multiply = [&](const uint8_t *codes) {
         const v8h *kf = reinterpret_cast<const v8h *>(codes) + lane;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            v8h key[2][G];
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int c = 0; c < 2; ++c) {
+                v8h key[G];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        if (half == 0) key[kt][gr] = kf[(kt * C + 2 * gr + c) * 64];
+                        if (half == 0) key[gr] = kf[(kt * C + 2 * gr + c) * 64];
                         const v4f from = c || half ? d[kt][gr] : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                        d[kt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[kt][gr], half ? ql[2 * gr + c] : qh[2 * gr + c], from, 0, 0, 0);
+                        d[kt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[gr], half ? ql[2 * gr + c] : qh[2 * gr + c], from, 0, 0, 0);
                     }
-        }
+            }
     };
     multiply(s_k[0]);
     layer.put_k(s_k[1], wave, lane, magic);
@@ -1254,9 +1260,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_
         v8h pv[2][G];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            v8h pk[G];
-            Params::get(s_kpar[b3], kt, u, pk);
-            q_scores<HD>(query, pk, d[kt], x + 4 * kt);
+            q_scores<HD>(query.sum, s_kpar[b3], kt, i, u, d[kt], x + 4 * kt);
             Params::get(s_vpar[b], kt, u, pv[kt]);
         }
         const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
@@ -1274,7 +1278,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (half == 0) v[k] = vf[(4 * gr + k) * 64];
-                    sums.acc[4 * gr + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], half ? lo[gr] : hi[gr], sums.acc[4 * gr + k], 0, 0, 0);
+                    v4f &a = sums.acc[4 * gr + k];
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], half ? lo[gr] : hi[gr], a, 0, 0, 0);
                 }
         }
         layer.put_k(s_k[b], wave, lane, magic);
@@ -1284,10 +1289,10 @@ __global__ void __launch_bounds__(64 * W, W == 8 || BITS == 8 ? 2 : 3) k_qcache_
         b ^= 1;
         b3 = b3next;
     }
+    const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
     sums.template finish<BITS>();
     const int r = first + i, row = r - tile * kRows;
     if (r >= all) return;
-    const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
     float *dst = pl.splits > 1 ? pl.part + (slot + row) * HD : q_out_row(p, s, g, r, HD);
     const float by = pl.splits > 1 ? 1.0f : (sums.total == 0.0f ? 0.0f : 1.0f / sums.total);
 #pragma unroll
