@@ -1165,7 +1165,7 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     using Params = QParams<HD>;
     constexpr int C = HD / 32, G = HD / 64, T = HD / 16, kRows = 64;
     __shared__ __attribute__((aligned(16))) uint8_t s_k[2][Layer::kKBytes], s_v[2][Layer::kVBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t s_kpar[3][Params::kBytes], s_vpar[2][Params::kBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t s_kpar[2][Params::kBytes], s_vpar[2][Params::kBytes];
     __shared__ int2 s_raise[2];  // what V's parameters ask for: QScale's raise and bad
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, u = lane >> 4;
@@ -1178,18 +1178,21 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     const int cap = p.cache.capacity, step = pl.splits * kQBlock, first = tile * kRows + 16 * wave;
     int k0 = part * kQBlock;  // of this round's block
 
-    Layer layer;
+    Layer layer[2];  // of blocks of even and of odd number
     const uint32_t magic = code_magic();
-    uint32_t kw, vw;  // a word of parameters: the next block's keys', this block's values'
+    uint32_t kw[2], vw[2];  // a word of their parameters
     auto load_par = [&](const uint8_t *at, int from) { return Params::word(at, from, cap, lane); };
     auto put_par = [&](uint8_t *to, uint32_t w) {
         if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(to)[lane] = w;
     };
     auto load_first = [&] {
-        layer.load_k(kc, k0, cap, wave, lane);
-        kw = load_par(kp, k0);
-        layer.load_v(vc, k0, cap, wave, lane);
-        vw = load_par(vp, k0);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            layer[n].load_k(kc, k0 + n * step, cap, wave, lane);
+            kw[n] = load_par(kp, k0 + n * step);
+            layer[n].load_v(vc, k0 + n * step, cap, wave, lane);
+            vw[n] = load_par(vp, k0 + n * step);
+        }
     };
     if (!p.window) load_first();
     v4f y[HD / 16];
@@ -1211,10 +1214,10 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     QSums<HD> sums;
     q_query<HD, BITS, SHAPED>(p, wt, g, first + i, u, y, qh, ql, query);
     sums.clear();
-    layer.put_k(s_k[0], wave, lane, magic);
-    if (wave == 0) put_par(s_kpar[0], outside(k0) ? 0u : kw);
-    layer.load_k(kc, k0 + step, cap, wave, lane);
-    kw = load_par(kp, k0 + step);
+    layer[0].put_k(s_k[0], wave, lane, magic);
+    if (wave == 0) put_par(s_kpar[0], outside(k0) ? 0u : kw[0]);
+    layer[0].load_k(kc, k0 + 2 * step, cap, wave, lane);
+    kw[0] = load_par(kp, k0 + 2 * step);
     __syncthreads();
     v4f d[2][G];
     // two sums at a time: one product does not wait for the one before
@@ -1236,40 +1239,40 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
             }
     };
     multiply(s_k[0]);
-    layer.put_k(s_k[1], wave, lane, magic);
-    layer.put_v(s_v[0], wave, lane, magic);
-    layer.load_k(kc, k0 + 2 * step, cap, wave, lane);
-    layer.load_v(vc, k0 + step, cap, wave, lane);
+    layer[1].put_k(s_k[1], wave, lane, magic);
+    layer[0].put_v(s_v[0], wave, lane, magic);
+    layer[1].load_k(kc, k0 + 3 * step, cap, wave, lane);
+    layer[0].load_v(vc, k0 + 2 * step, cap, wave, lane);
     QScale scale;  // wave 1's
     int raise = scale.raise;
-    int b = 0, b3 = 0;  // round number mod 2 and 3
-    for (; k0 < wt.hi; k0 += step) {
-        const int b3next = b3 == 2 ? 0 : b3 + 1;
-        if (wave == 0) put_par(s_kpar[b3next], outside(k0 + step) ? 0u : kw);
+    // the round of a block of even (N 0) or odd number; k0 moves on
+    auto round = [&](auto number) {
+        constexpr int N = decltype(number)::value;
         if (wave == 1) {
-            vw = outside(k0) ? 0u : vw;
-            scale.look<HD>(vw, lane);
-            put_par(s_vpar[b], vw);
-            if (lane == 0) s_raise[b] = make_int2(scale.raise, scale.bad);
+            vw[N] = outside(k0) ? 0u : vw[N];
+            scale.look<HD>(vw[N], lane);
+            put_par(s_vpar[N], vw[N]);
+            if (lane == 0) s_raise[N] = make_int2(scale.raise, scale.bad);
         }
-        kw = load_par(kp, k0 + 2 * step);
-        vw = load_par(vp, k0 + step);
+        vw[N] = load_par(vp, k0 + 2 * step);
         __syncthreads();
-        const int2 ask = s_raise[b];
+        if (wave == 0) put_par(s_kpar[1 - N], outside(k0 + step) ? 0u : kw[1 - N]);
+        kw[1 - N] = load_par(kp, k0 + 3 * step);
+        const int2 ask = s_raise[N];
         float x[8];  // row i, keys 16 · kt + 4u + k
         v8h pv[2][G];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            q_scores<HD>(query.sum, s_kpar[b3], kt, i, u, d[kt], x + 4 * kt);
-            Params::get(s_vpar[b], kt, u, pv[kt]);
+            q_scores<HD>(query.sum, s_kpar[N], kt, i, u, d[kt], x + 4 * kt);
+            Params::get(s_vpar[N], kt, u, pv[kt]);
         }
         const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
         sums.template shape<SHAPED>(p, query, ask.x, ask.x != raise, x, k0, u, rare, pv);
         raise = ask.x;
         v8h hi[G], lo[G];
-        multiply(s_k[b ^ 1]);
+        multiply(s_k[1 - N]);
         sums.template split<SHAPED>(query, x, pv, hi, lo);
-        const v8h *vf = reinterpret_cast<const v8h *>(s_v[b]) + lane;
+        const v8h *vf = reinterpret_cast<const v8h *>(s_v[N]) + lane;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
             v8h v[4];
@@ -1282,12 +1285,16 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
                     a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], half ? lo[gr] : hi[gr], a, 0, 0, 0);
                 }
         }
-        layer.put_k(s_k[b], wave, lane, magic);
-        layer.put_v(s_v[b ^ 1], wave, lane, magic);
-        layer.load_k(kc, k0 + 3 * step, cap, wave, lane);
-        layer.load_v(vc, k0 + 2 * step, cap, wave, lane);
-        b ^= 1;
-        b3 = b3next;
+        layer[N].put_k(s_k[N], wave, lane, magic);
+        layer[1 - N].put_v(s_v[1 - N], wave, lane, magic);
+        layer[N].load_k(kc, k0 + 4 * step, cap, wave, lane);
+        layer[1 - N].load_v(vc, k0 + 3 * step, cap, wave, lane);
+        k0 += step;
+    };
+    while (k0 < wt.hi) {
+        round(std::integral_constant<int, 0>{});
+        if (k0 >= wt.hi) break;
+        round(std::integral_constant<int, 1>{});
     }
     const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
     sums.template finish<BITS>();
