@@ -225,18 +225,39 @@ struct QShape {
     int tiles, splits;
     int64_t slots, bytes;
 };
+// The choices were measured at heads of 128 in 4 bits unless stated, 16 heads on 2 KV
+// heads, both sides in us.
+// Rows of a (sequence, KV head).  Up to 32 a wave takes blocks of its own for all of
+// them, more come in tiles of 64 whose waves take blocks together: 24 rows behind 500
+// keys 10.7 : 11.9, of 16 sequences behind 8,192 keys 26.3 : 36.8, 32 rows 26.5 : 37.5.
+// 48 rows in three row tiles of a wave spilled registers.
+// One launch without a join, up to the keys where shares and their join take no longer:
+// 16 rows 512 keys 8.7 : 9.1, 768 keys 10.5 : 9.2; 32 rows 256 keys 9.8 : 10.3, 384 keys
+// 11.4 : 10.7; 48 rows 128 keys 10.1 : 10.5, 160 keys 11.3 : 10.9.  Heads of 64: 16 rows
+// 1,024 keys 8.8 : 9.0, 1,280 keys 9.9 : 9.0; 32 rows 512 keys 9.5 : 9.3; 48 rows 192 keys
+// 8.8 : 9.8, 256 keys 10.2 : 9.1.
+// Shares: few rows 512 workgroups (16 sequences of 8 rows, 8,192 keys, in 256, 512 and
+// 768: 19.7, 18.3, 18.9) of 4 blocks or more, one for each wave (8 rows, 8,192 keys, 2, 4
+// and 8: 10.4, 9.3, 10.0).  Many rows: one workgroup a CU first, of 2 blocks or more (64
+// rows, 2,048 keys, 2, 3 and 6: 12.0, 13.2, 15.7), then three, of 6 or more (64 rows of 16
+// sequences, 2,048 keys, 2, 3 and 6: 27.5, 27.2, 24.4; 4,800 rows, 8,192 keys, 3 and 5
+// shares: 169, 136).
 QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     QShape q;
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
+    const bool small = c->head_dim == 64;
     q.many = rows > 32;
     q.rt = rows <= 16 ? 1 : 2;
     q.rows = q.many ? 64 : 16 * q.rt;
     q.tiles = round_up_div(rows, q.rows);
     const int64_t work = q.tiles * groups;
     const int64_t keys = a->window ? std::min<int64_t>(a->max_rows, (int64_t)a->window + q.rows) : a->max_rows;
-    const int64_t blocks = round_up_div(keys, kQBlock), whole = q.many || q.rt == 2 ? 12 : 32, least = q.many ? 3 : 4;
-    const int want = q.many ? 768 : 512;
-    q.splits = blocks <= whole ? 1 : (int)std::min<int64_t>({std::max<int64_t>(1, want / work), 128, round_up_div(blocks, least)});
+    const int64_t blocks = round_up_div(keys, kQBlock);
+    const int whole = q.many ? (small ? 6 : 4) : (q.rt == 2 ? 8 : 16) * (small ? 2 : 1);
+    // so many shares that at most `wgs` workgroups result, of `least` blocks or more
+    auto shares = [&](int64_t wgs, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>(wgs / work, round_up_div(blocks, least))); };
+    const int64_t most = q.many ? std::max(shares(256, 2), shares(768, 6)) : shares(512, 4);
+    q.splits = blocks <= whole ? 1 : (int)std::min<int64_t>(most, 128);
     q.slots = q.splits > 1 ? work * q.splits : 0;
     q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
     return q;
