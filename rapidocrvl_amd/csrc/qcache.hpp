@@ -1151,13 +1151,23 @@ struct QLayer {
     }
 };
 
-// The same attention for many query rows: W waves of 16 rows take the share's blocks
+// The same attention for many query rows: four waves of 16 rows take the share's blocks
 // together, each unpacking its part of a block's codes into LDS for all of them.
-// A wave's vector instructions take longer than its matrix instructions, and run
-// beside them only where they lie between them: the next block's scores are
-// multiplied among this block's exponentials, this block's sums among the unpacking
-// of later codes.  So a round needs the next block's keys and this block's values;
-// both have two buffers, their parameters three, and a round one barrier.
+//
+// A round of a wave (32 keys, heads of 128) has 32 matrix instructions of 16 cycles and
+// about 170 vector instructions of 4, which run beside them only where they lie between
+// them: the next block's scores are multiplied among this block's exponentials, this
+// block's sums among the unpacking of later codes.  So a round needs the next block's
+// keys and this block's values, both in two buffers, and one barrier; codes are
+// requested two blocks ahead.  Rounds come in pairs, so that buffers and registers are
+// fixed numbers of the code.
+//
+// 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 120 to 129 us,
+// 0.35 PFLOP/s (1.16 for a large fp16 product).  Vector instructions bound it (46 % of
+// the cycles, with their matrix instructions 80 %).  Eight waves of one workgroup: 143;
+// four waves with a block's codes one round ahead: 126 where this took 120; 32 rows a
+// wave spilled 22 registers: 177; four sums of scores at a time in place of two: 143,
+// spilled too.
 template <int HD, int BITS, bool SHAPED>
 __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
@@ -1180,18 +1190,14 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
 
     Layer layer[2];  // of blocks of even and of odd number
     const uint32_t magic = code_magic();
-    uint32_t kw[2], vw[2];  // a word of their parameters
-    auto load_par = [&](const uint8_t *at, int from) { return Params::word(at, from, cap, lane); };
-    auto put_par = [&](uint8_t *to, uint32_t w) {
-        if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(to)[lane] = w;
-    };
+    uint32_t par[2];  // a word of their parameters: wave 0 K's, the others V's
+    auto load_par = [&](int from) { return Params::word(wave ? vp : kp, from, cap, lane); };
     auto load_first = [&] {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             layer[n].load_k(kc, k0 + n * step, cap, wave, lane);
-            kw[n] = load_par(kp, k0 + n * step);
+            par[n] = load_par(k0 + n * step);
             layer[n].load_v(vc, k0 + n * step, cap, wave, lane);
-            vw[n] = load_par(vp, k0 + n * step);
         }
     };
     if (!p.window) load_first();
@@ -1204,20 +1210,31 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         k0 += wt.lo / kQBlock * kQBlock;
         load_first();
     }
-    // parameters of keys outside the tile's are zero
-    auto outside = [&](int from) {
-        const int key = from + Params::key_of(lane);
-        return (from < wt.all_lo || from + kQBlock > wt.all_hi) && (key < wt.lo || key >= wt.hi);
-    };
     v8h qh[C], ql[C];
     QQuery<HD> query;
     QSums<HD> sums;
     q_query<HD, BITS, SHAPED>(p, wt, g, first + i, u, y, qh, ql, query);
     sums.clear();
+    // parameters of the block from key `from` on for the waves, those of keys outside
+    // the tile's as zeros, and the load of those two blocks later
+    QScale scale;  // wave 1's
+    auto put_par = [&](auto number, int from) {
+        constexpr int N = decltype(number)::value;
+        if (wave < 2) {
+            const int key = from + Params::key_of(lane);
+            uint32_t w = par[N];
+            if ((from < wt.all_lo || from + kQBlock > wt.all_hi) && (key < wt.lo || key >= wt.hi)) w = 0;
+            if (wave) {
+                scale.look<HD>(w, lane);
+                if (lane == 0) s_raise[N] = make_int2(scale.raise, scale.bad);
+            }
+            if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(wave ? s_vpar[N] : s_kpar[N])[lane] = w;
+        }
+        par[N] = load_par(from + 2 * step);
+    };
     layer[0].put_k(s_k[0], wave, lane, magic);
-    if (wave == 0) put_par(s_kpar[0], outside(k0) ? 0u : kw[0]);
+    put_par(std::integral_constant<int, 0>{}, k0);
     layer[0].load_k(kc, k0 + 2 * step, cap, wave, lane);
-    kw[0] = load_par(kp, k0 + 2 * step);
     __syncthreads();
     v4f d[2][G];
     // two sums at a time: one product does not wait for the one before
@@ -1243,21 +1260,12 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     layer[0].put_v(s_v[0], wave, lane, magic);
     layer[1].load_k(kc, k0 + 3 * step, cap, wave, lane);
     layer[0].load_v(vc, k0 + 2 * step, cap, wave, lane);
-    QScale scale;  // wave 1's
-    int raise = scale.raise;
+    int raise = kQTop + 14;  // as QScale begins
     // the round of a block of even (N 0) or odd number; k0 moves on
     auto round = [&](auto number) {
         constexpr int N = decltype(number)::value;
-        if (wave == 1) {
-            vw[N] = outside(k0) ? 0u : vw[N];
-            scale.look<HD>(vw[N], lane);
-            put_par(s_vpar[N], vw[N]);
-            if (lane == 0) s_raise[N] = make_int2(scale.raise, scale.bad);
-        }
-        vw[N] = load_par(vp, k0 + 2 * step);
         __syncthreads();
-        if (wave == 0) put_par(s_kpar[1 - N], outside(k0 + step) ? 0u : kw[1 - N]);
-        kw[1 - N] = load_par(kp, k0 + 3 * step);
+        put_par(std::integral_constant<int, 1 - N>{}, k0 + step);
         const int2 ask = s_raise[N];
         float x[8];  // row i, keys 16 · kt + 4u + k
         v8h pv[2][G];
@@ -1291,10 +1299,9 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         layer[1 - N].load_v(vc, k0 + 3 * step, cap, wave, lane);
         k0 += step;
     };
-    while (k0 < wt.hi) {
+    for (int left = (wt.hi - k0 + step - 1) / step; left > 0; left -= 2) {
         round(std::integral_constant<int, 0>{});
-        if (k0 >= wt.hi) break;
-        round(std::integral_constant<int, 1>{});
+        if (left > 1) round(std::integral_constant<int, 1>{});
     }
     const int64_t slot = ((((int64_t)s * p.cache.kvh + g) * pl.tiles + tile) * pl.splits + part) * kRows;
     sums.template finish<BITS>();
