@@ -537,9 +537,12 @@ int pocr_qcache_read(pocr_ctx *ctx, const pocr_qread_args *args, const pocr_qcac
  * its own, with a window the last `window` of those.  Scores as in the section
  * above, |position(i) - position(j)| the distance in rows.  A token that sees
  * nothing (its position is negative) has an out row of zeros and -inf for its
- * lse.  Rows of out and lse behind a sequence's last token are left as they were.
+ * lse.  Rows of out and lse behind a sequence's last token are left as they were;
+ * rows of q behind it may be read, but count for nothing.
  * A row that sees a group of NaN comes out not finite: the whole of it for a
- * key's group, with its lse, that group's elements for a value's. */
+ * key's group, with its lse, that group's elements for a value's.  Statistics and
+ * sums are fp32; query elements have 22 bits, and so has a weight times a value's
+ * step, down to 2^-32 of the largest step that its row sees. */
 typedef struct {
     const float *q;           /* sequence s, token t, head h: q + s*q_seq_stride + t*q_stride + h*head_dim */
     float *out;               /* likewise, no two rows overlap */

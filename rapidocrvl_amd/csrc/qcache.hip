@@ -217,6 +217,9 @@ int attention_shape(const pocr_qattention_args *a, const pocr_qcache *c, const c
     return POCR_OK;
 }
 
+// A window that holds every row is none, which keeps positions less it in 32 bits.
+int window_of(const pocr_qattention_args *a) { return a->window < a->max_rows ? a->window : 0; }
+
 // Row tiles and key shares of one attention call.
 struct QShape {
     bool many;   // k_qcache_attn_rows
@@ -251,7 +254,8 @@ QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     q.rows = q.many ? 64 : 16 * q.rt;
     q.tiles = round_up_div(rows, q.rows);
     const int64_t work = q.tiles * groups;
-    const int64_t keys = a->window ? std::min<int64_t>(a->max_rows, (int64_t)a->window + q.rows) : a->max_rows;
+    const int window = window_of(a);
+    const int64_t keys = window ? std::min<int64_t>(a->max_rows, (int64_t)window + q.rows) : a->max_rows;
     const int64_t blocks = round_up_div(keys, kQBlock);
     const int whole = q.many ? (small ? 6 : 4) : (q.rt == 2 ? 8 : 16) * (small ? 2 : 1);
     // so many shares that at most `wgs` workgroups result, of `least` blocks or more
@@ -279,6 +283,7 @@ int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work,
         RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, ROWS / 16, 4, true> : k_qcache_attn<HD, BITS, ROWS / 16, 4, false>, p, pl));
     }
     if (q.splits == 1) return POCR_OK;
+    // 13 shares of 8 rows, eight at a time and two: 8.9, 9.5 us; 5 shares of 4,800 rows: 117, 115.
     constexpr int U = 1024 / HD;
     if (q.splits >= 8) return launch(s, dim3(q.tiles * ROWS / (U / 8), p.cache.kvh, seqs), 256, k_qcache_join<HD, ROWS, 8>, p, pl);
     return launch(s, dim3(q.tiles * ROWS / (U / 2), p.cache.kvh, seqs), 256, k_qcache_join<HD, ROWS, 2>, p, pl);
@@ -398,7 +403,7 @@ extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *
     p.group = a->heads / c->kv_heads;
     p.group_inv = p.group == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group);
     p.max_rows = a->max_rows;
-    p.window = a->window;
+    p.window = window_of(a);
     p.scale = default_scale(a->scale, c->head_dim);
     p.cap = a->cap;
     hipStream_t s = (hipStream_t)stream;

@@ -297,7 +297,17 @@ enum : int { kPairsWhole = 0, kPairsAdjacent = 1, kPairsPart = 2 };
 
 // Wave: `tokens` tokens one after the other, `per` heads of each, HD / 8 lanes a
 // head; the next heads are on their way meanwhile.  A token's angles are computed
-// once, one a lane, and go through LDS to the lanes of every head.
+// once, one a lane, and go through LDS to the lanes of every head; an angle's product,
+// its turn and the norm's sum are in 64 bits, so that a row is the same to its last
+// bit, and its code with it, whichever call makes it.
+//
+// Memory bounds it: 8,192 normed tokens of 16 + 2 + 2 heads of 128 rotated 37 us (168 MB,
+// 4.5 TB/s), with K and V into 4 bits 37 too (151 MB: the quantising shows), 18 layers of
+// 1,345 K and V rows of 2 heads into 8 bits 18.4 (62 MB).  1,345 tokens of 16 + 2 heads
+// take 8.5 us (27 MB), where the launch and the first loads' way count.  The simplest
+// form, a lane with eight neighbouring elements and a wave a head, took 118 us for the
+// first: its loads and stores were halves of lines, and a rotation fetched its other
+// half from eight lanes away.
 template <int HD, int BITS, int PAIRS>  // BITS 0: fp32 destinations
 __global__ void __launch_bounds__(256) k_rows(RowsCall p) {
     constexpr int L = HD / 8, U = 64 / L, H = HD / 2;
@@ -447,7 +457,11 @@ struct QReadCall {
     int row0;  // first row of the grid
 };
 
-// HD / 8 lanes a row of a head, K and V one after the other
+// HD / 8 lanes a row of a head, K and V one after the other: mid + step * code, a
+// multiply-add.  Stores bound it: 18 caches of 1,609 rows of 2 heads of 128 in 4 bits
+// (60 MB) 11.4 to 12.3 us, 4.8 to 5.2 TB/s; 2,048 listed rows of each in 8 bits (84 MB)
+// 19.7, 4.3 TB/s.  Loads of codes and parameters are short pieces of lines, which the
+// neighbours' loads find in the cache.
 template <int HD, int BITS>
 __global__ void __launch_bounds__(256) k_qcache_read(QReadCall p) {
     using F = QFormat<HD, BITS>;
@@ -924,9 +938,10 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 // in turn and join.
 //
 // Codes go to the matrix instructions as they are, exact in fp16, and meet query
-// rows and weights as two fp16 halves each.  Scores come out transposed (lane l:
-// query row l % 16, keys 4 (l / 16) + r of each 16), so a row's statistics stay
-// with its four lanes and its weights are the second product's operand:
+// rows and weights as two fp16 halves each, 22 bits together.  Scores come out
+// transposed (lane l: query row l % 16, keys 4 (l / 16) + r of each 16), so a row's
+// statistics stay with its four lanes, in 32 bits, and its weights are the second
+// product's operand:
 //   q . k = sum over groups of step (q . c) + mid (sum of q),
 //   out = sum over keys of (p step) . c + sum of p mid.
 // p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
@@ -935,6 +950,14 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 // of two.  A wave's first block and its query rows do not depend on the sequence's
 // length, and are requested with it; a later block's codes as soon as the registers
 // of the one before are free.
+//
+// Few rows are bound by the chain of one wave: launch, lengths and first codes (5 us),
+// then 0.7 us a block, sums joined in LDS.  One token of 16 heads on 2 KV heads of 128 in
+// 4 bits behind 1,609 rows 9.3 us with the join (two launches alone are 6.2 for the host);
+// 16 of them behind up to 8,192 rows (33 MB) 17.1, of which loads without arithmetic
+// 12.8.  Two blocks of a wave on their way: 18.0, registers for two workgroups a CU in
+// place of three; two blocks a round: one token 10.7.  Eight waves where one launch
+// does it all: 8 tokens of 4 heads of 64 behind 700 rows 7.9 us, with four 9.6.
 template <int HD, int BITS, int RT, int W, bool SHAPED>
 __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
@@ -1321,8 +1344,8 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     }
 }
 
-// A tile's shares joined: HD / 4 lanes a row and share, N shares at a time (all of
-// them where there are no more: one round of loads behind the launch).
+// A tile's shares joined: HD / 4 lanes a row and share, N shares at a time, the sums of
+// each to the largest reference.  3 to 4 us under a trace, launch and one round of loads.
 template <int HD, int ROWS, int N>
 __global__ void __launch_bounds__(256) k_qcache_join(QAttnCall p, QAttnPlan pl) {
     constexpr int L = HD / 4, U = 256 / L, R = U / N;  // rows of a workgroup

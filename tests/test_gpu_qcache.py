@@ -504,6 +504,14 @@ def test_attention_windows(ctx, rng, n, window, cap, bias):
                counts=[n, n + 5, n, 1, 1, n, max(0, n - 2)], window=window, cap=cap, slopes=slopes).run(ctx).check()
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 150, 149])
+@pytest.mark.parametrize("n", [10, 70])
+def test_attention_windows_of_any_size(ctx, rng, n, window):
+    """The largest windows with tokens before the cache's first row: positions less the window do not wrap."""
+    with base.Hip() as hip:
+        Attend(hip, rng, 4, n, 150, 4, 2, 128, 4, lens=[150, 5, 1, 0], window=window).run(ctx).check()
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("seqs,n,rows", [(1, 1, 9000), (5, 1, 2100), (1, 12, 3000), (1, 200, 1500), (2, 65, 700)])
 def test_attention_long(ctx, rng, bits, seqs, n, rows):
