@@ -28,7 +28,6 @@ struct QFormat {
     static constexpr int kCodes = HD * BITS / 8;      // bytes of a row's codes
     static constexpr int kParams = 2 * kGroups;       // fp16 numbers: steps, midpoints
     static constexpr int kHalf = 1 << (BITS - 1);     // codes from -kHalf to kHalf - 1, stored as code + kHalf
-    static constexpr int kLanes = HD / 8;             // lanes of 8 neighbouring elements
 };
 
 // A lane's elements: HD / 8 lanes hold a row of a head, lane i elements 4i .. +3 and
@@ -668,9 +667,7 @@ __device__ __forceinline__ void split_steps(float a, _Float16 sa, float b, _Floa
 }
 
 // One query row's part of a score, in a lane of its tile.
-template <int HD>
 struct QQuery {
-    static constexpr int G = HD / 64;
     float sum;      // of the row's elements of group u, in lane 16u + i (zero where there is none)
     float size;     // a power of two: score = size · product
     float slope;
@@ -694,7 +691,7 @@ __device__ __forceinline__ void q_fetch(const QAttnCall &p, int s, int g, int r,
 // upper codes of bytes.
 template <int HD, int BITS, bool SHAPED>
 __device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int g, int r, int u, const v4f (&y)[HD / 16], v8h (&hi)[HD / 32],
-                                        v8h (&lo)[HD / 32], QQuery<HD> &q) {
+                                        v8h (&lo)[HD / 32], QQuery &q) {
     constexpr int C = HD / 32, G = HD / 64;
     const bool live = r < t.count * p.group;
     const int tok = p.token(live ? r : 0), head = g * p.group + (live ? r - tok * p.group : 0);
@@ -841,7 +838,7 @@ struct QSums {
     // but for q.size, and the row's reference.  rare: some row does not see all keys, or
     // some of V's parameters are no numbers.
     template <bool SHAPED>
-    __device__ __forceinline__ void shape(const QAttnCall &p, const QQuery<HD> &q, int raise, bool moved, float (&x)[8], int k0, int u, bool rare,
+    __device__ __forceinline__ void shape(const QAttnCall &p, const QQuery &q, int raise, bool moved, float (&x)[8], int k0, int u, bool rare,
                                           const v8h (&v)[2][G]) {
         auto key_of = [&](int j) { return k0 + 16 * (j >> 2) + 4 * u + (j & 3); };
         const float size = SHAPED ? 1.0f : q.size;  // exact, so a score may round with its reference
@@ -887,7 +884,7 @@ struct QSums {
     }
     // scores → weights times V's steps, as halves
     template <bool SHAPED>
-    __device__ __forceinline__ void split(const QQuery<HD> &q, float (&x)[8], const v8h (&v)[2][G], v8h (&hi)[G], v8h (&lo)[G]) {
+    __device__ __forceinline__ void split(const QQuery &q, float (&x)[8], const v8h (&v)[2][G], v8h (&hi)[G], v8h (&lo)[G]) {
         const float size = SHAPED ? 1.0f : q.size;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -972,7 +969,7 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
         v4f acc[W][RT][T][64];
     };
     __shared__ Shared sh;
-    __shared__ QQuery<HD> s_query[RT][16];
+    __shared__ QQuery s_query[RT][16];
     __shared__ float s_qsum[RT][64];
     __shared__ float s_ref[W][kRows], s_sum[W][kRows];
 
@@ -1004,7 +1001,7 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
     }
     if (wave < RT) {
         v8h hi[C], lo[C];
-        QQuery<HD> q;
+        QQuery q;
         q_query<HD, BITS, SHAPED>(p, t, g, first + 16 * wave + i, u, y, hi, lo, q);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -1015,7 +1012,7 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
         s_qsum[wave][lane] = q.sum;
     }
     __syncthreads();
-    QQuery<HD> query[RT];
+    QQuery query[RT];
     QSums<HD> sums[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -1177,20 +1174,21 @@ struct QLayer {
 // The same attention for many query rows: four waves of 16 rows take the share's blocks
 // together, each unpacking its part of a block's codes into LDS for all of them.
 //
-// A round of a wave (32 keys, heads of 128) has 32 matrix instructions of 16 cycles and
-// about 170 vector instructions of 4, which run beside them only where they lie between
-// them: the next block's scores are multiplied among this block's exponentials, this
-// block's sums among the unpacking of later codes.  So a round needs the next block's
-// keys and this block's values, both in two buffers, and one barrier; codes are
+// A round of a wave (32 keys, heads of 128) has 34 matrix instructions of 16 cycles or 32
+// and about 150 vector instructions of 4, which run beside them only where they lie
+// between them: the next block's scores are multiplied among this block's exponentials,
+// this block's sums among the unpacking of later codes.  So a round needs the next
+// block's keys and this block's values, both in two buffers, and one barrier; codes are
 // requested two blocks ahead.  Rounds come in pairs, so that buffers and registers are
 // fixed numbers of the code.
 //
-// 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 120 to 129 us,
-// 0.35 PFLOP/s (1.16 for a large fp16 product).  Vector instructions bound it (46 % of
-// the cycles, with their matrix instructions 80 %).  Eight waves of one workgroup: 143;
-// four waves with a block's codes one round ahead: 126 where this took 120; 32 rows a
-// wave spilled 22 registers: 177; four sums of scores at a time in place of two: 143,
-// spilled too.
+// 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 117 to 129 us
+// with the join, 0.32 to 0.36 PFLOP/s (1.16 for a large fp16 product).  A round's chain
+// of LDS reads, products, exponentials and products bounds it, three waves to a SIMD:
+// vector instructions take 40 % of the cycles, matrix instructions a third, LDS 40 %.
+// Eight waves a workgroup took 143 us where four took 138; codes one round ahead 135
+// where this takes 129; 32 rows a wave spilled 22 registers and took 177 where 16 took
+// 136; four sums of scores at a time in place of two, spilled too, 143 where two took 126.
 template <int HD, int BITS, bool SHAPED>
 __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
@@ -1234,7 +1232,7 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         load_first();
     }
     v8h qh[C], ql[C];
-    QQuery<HD> query;
+    QQuery query;
     QSums<HD> sums;
     q_query<HD, BITS, SHAPED>(p, wt, g, first + i, u, y, qh, ql, query);
     sums.clear();
