@@ -1136,7 +1136,8 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
 // instructions take them, for the four waves of a workgroup: 16 bytes a lane for each
 // of K's [key tile][chunk] and V's [dim tile].  Of K a wave has whole pieces, of V a
 // pair of keys in all dim tiles, so that its loads are words of codes and not their
-// bytes.
+// bytes; another pair in each of its lane groups, so that its words lie in different
+// banks.
 template <int HD, int BITS>
 struct QLayer {
     using F = QFormat<HD, BITS>;
@@ -1152,7 +1153,7 @@ struct QLayer {
     }
     __device__ __forceinline__ void load_v(const uint8_t *codes, int k0, int rows, int wave, int lane) {
         const auto from = q_block<F::kCodes>(codes, k0, rows);
-        const uint32_t i = lane & 15, u = lane >> 4, j = 2 * wave;  // keys of slots j and j + 1
+        const uint32_t i = lane & 15, u = lane >> 4, j = 2 * (wave ^ u);  // keys of slots j and j + 1
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const uint32_t at = (16 * (j >> 2) + 4 * u + (j & 3) + n) * F::kCodes + T * BITS / 8 * i;
@@ -1165,7 +1166,7 @@ struct QLayer {
         for (int n = 0; n < kK; ++n) reinterpret_cast<v8h *>(to)[(wave * kK + n) * 64 + lane] = QCodes<HD, BITS>::key_of(k, n, magic);
     }
     __device__ __forceinline__ void put_v(uint8_t *to, int wave, int lane, uint32_t magic) const {
-        v2h *at = reinterpret_cast<v2h *>(to) + 4 * lane + wave;
+        v2h *at = reinterpret_cast<v2h *>(to) + 4 * lane + (wave ^ lane >> 4);
 #pragma unroll
         for (int t = 0; t < T; ++t) at[256 * t] = QCodes<HD, BITS>::value_pair(v[0], v[1], t, magic);
     }
