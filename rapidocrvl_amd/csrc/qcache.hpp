@@ -1181,15 +1181,17 @@ struct QLayer {
 // this block's sums among the unpacking of later codes.  So a round needs the next
 // block's keys and this block's values, both in two buffers, and one barrier; codes are
 // requested two blocks ahead.  Rounds come in pairs, so that buffers and registers are
-// fixed numbers of the code.
+// fixed numbers of the code.  From its scores to its sums a wave goes before those of
+// other workgroups that unpack or wait, which keeps them apart in their rounds.
 //
-// 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 117 to 129 us
-// with the join, 0.32 to 0.36 PFLOP/s (1.16 for a large fp16 product).  A round's chain
+// 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 112 to 125 us
+// with the join, 0.33 to 0.37 PFLOP/s (1.16 for a large fp16 product).  A round's chain
 // of LDS reads, products, exponentials and products bounds it, three waves to a SIMD:
 // vector instructions take 40 % of the cycles, matrix instructions a third, LDS 40 %.
 // Eight waves a workgroup took 143 us where four took 138; codes one round ahead 135
 // where this takes 129; 32 rows a wave spilled 22 registers and took 177 where 16 took
-// 136; four sums of scores at a time in place of two, spilled too, 143 where two took 126.
+// 136; four sums of scores at a time in place of two, spilled too, 143 where two took
+// 126; without the priorities 117 where this takes 112.
 template <int HD, int BITS, bool SHAPED>
 __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
@@ -1296,6 +1298,7 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
             q_scores<HD>(query.sum, s_kpar[N], kt, i, u, d[kt], x + 4 * kt);
             Params::get(s_vpar[N], kt, u, pv[kt]);
         }
+        __builtin_amdgcn_s_setprio(1);
         const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
         sums.template shape<SHAPED>(p, query, ask.x, ask.x != raise, x, k0, u, rare, pv);
         raise = ask.x;
@@ -1315,6 +1318,7 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
                     a = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], half ? lo[gr] : hi[gr], a, 0, 0, 0);
                 }
         }
+        __builtin_amdgcn_s_setprio(0);
         layer[N].put_k(s_k[N], wave, lane, magic);
         layer[1 - N].put_v(s_v[1 - N], wave, lane, magic);
         layer[N].load_k(kc, k0 + 4 * step, cap, wave, lane);
