@@ -1176,7 +1176,7 @@ struct QLayer {
 // together, each unpacking its part of a block's codes into LDS for all of them.
 //
 // A round of a wave (32 keys, heads of 128) has 34 matrix instructions of 16 cycles or 32
-// and about 150 vector instructions of 4, which run beside them only where they lie
+// and about 165 vector instructions of 4, which run beside them only where they lie
 // between them: the next block's scores are multiplied among this block's exponentials,
 // this block's sums among the unpacking of later codes.  So a round needs the next
 // block's keys and this block's values, both in two buffers, and one barrier; codes are
@@ -1185,9 +1185,9 @@ struct QLayer {
 // other workgroups that unpack or wait, which keeps them apart in their rounds.
 //
 // 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 112 to 125 us
-// with the join, 0.33 to 0.37 PFLOP/s (1.16 for a large fp16 product).  A round's chain
-// of LDS reads, products, exponentials and products bounds it, three waves to a SIMD:
-// vector instructions take 40 % of the cycles, matrix instructions a third, LDS 40 %.
+// with the join, 0.33 to 0.37 PFLOP/s (1.16 for a large fp16 product).  Instructions bound
+// it, at three waves to a SIMD: vector ones take 45 % of the cycles, matrix ones 40 %, LDS
+// 42 %; a wave waits for its turn to issue for 36 % of its time.
 // Eight waves a workgroup took 143 us where four took 138; codes one round ahead 135
 // where this takes 129; 32 rows a wave spilled 22 registers and took 177 where 16 took
 // 136; four sums of scores at a time in place of two, spilled too, 143 where two took
