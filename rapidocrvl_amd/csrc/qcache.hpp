@@ -522,7 +522,10 @@ struct QAttnPlan {
 constexpr int kQBlock = 32;      // keys per step of a wave
 constexpr int kQTop = 9;         // weights times steps stay below 2^(kQTop + kQSlack)
 constexpr int kQSlack = 6;       // a score may pass its row's reference by this before that moves
-constexpr float kQFar = 4194304.0f;  // up to here whole numbers and their differences are exact
+// From here on a reference's exponent stands apart from its whole number: a score's last
+// bit is 1/2 and more, and so a rounded multiply-add would lose the exponent's.  Nor may
+// scores pass such a reference: six of them are one step of fp32 further up.
+constexpr float kQFar = 4194304.0f;
 
 // the query rows of a tile: [first, last] and what they see
 struct QTile {
@@ -822,12 +825,17 @@ struct QScale {
     }
 };
 
-// A row's running sums, in a lane of its tile.
+// A row's running sums, in a lane of its tile.  Weights are 2^(score - m + raise), m a
+// whole number near the row's largest score, raise an exponent: ref is m - raise, and of
+// a row whose m is far from zero -raise, where `shape` takes m from its scores.
 template <int HD>
 struct QSums {
     static constexpr int G = HD / 64, T = HD / 16;
     v4f acc[T];
-    float ref = kLowest, m = kLowest, total = 0.0f, mids[G];
+    float ref = 0.0f, m = kLowest, total = 0.0f, mids[G];
+    bool far = false;  // some row of the wave's
+    // what of m its scores lose beforehand
+    __device__ __forceinline__ static float apart(float m) { return fabsf(m) >= kQFar ? m : 0.0f; }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int k = 0; k < T; ++k) acc[k] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
@@ -870,16 +878,23 @@ struct QSums {
             }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * size;
-        if (__any(moved || top > m + kQSlack)) {
+        if (__any(moved || far || top > m + kQSlack)) {
             top = groups_max(top);
+            const float before = apart(m);
             if (top > m) m = fminf(ceilf(top), 3.0e38f);
-            const float now = fabsf(m) < kQFar ? m - (float)raise : m, by = __builtin_amdgcn_exp2f(ref - now);
+            const float less = apart(m), now = m - less - (float)raise, by = __builtin_amdgcn_exp2f((before - less) + (ref - now));
             ref = now;
+            far = __any(fabsf(m) >= kQFar && m > kLowest);
             total *= by;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) mids[gr] *= by;
 #pragma unroll
             for (int k = 0; k < T; ++k) acc[k] *= by;
+            if (far) {  // `split` multiplies by size again: a power of two
+                const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(size));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = less != 0.0f ? fmaf(x[j], size, -less) * inverse : x[j];
+            }
         }
     }
     // scores → weights times V's steps, as halves
@@ -915,6 +930,13 @@ struct QSums {
             mids[gr] = groups_sum(mids[gr]);
 #pragma unroll
             for (int k = 4 * gr; k < 4 * gr + 4; ++k) acc[k] = acc[k] * (QCodes<HD, BITS>::v_upper(k) ? 0.0625f : 1.0f) + mids[gr];
+        }
+        if (far && apart(m) != 0.0f) {  // the exponent into the sums
+            const float by = __builtin_amdgcn_exp2f(ref);
+            ref = m;
+            total *= by;
+#pragma unroll
+            for (int k = 0; k < T; ++k) acc[k] *= by;
         }
         if (total == 0.0f) ref = kLowest;
     }
@@ -1290,7 +1312,10 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         constexpr int N = decltype(number)::value;
         __syncthreads();
         put_par(std::integral_constant<int, 1 - N>{}, k0 + step);
-        const int2 ask = s_raise[N];
+        // scalar registers: with a cap or slopes at once, which spares three registers that
+        // would spill (a chunk 163 us for 167), else where they are used (112 for 114)
+        int2 ask = s_raise[N];
+        if (SHAPED) ask = make_int2(__builtin_amdgcn_readfirstlane(ask.x), __builtin_amdgcn_readfirstlane(ask.y));
         float x[8];  // row i, keys 16 · kt + 4u + k
         v8h pv[2][G];
 #pragma unroll
@@ -1299,9 +1324,10 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
             Params::get(s_vpar[N], kt, u, pv[kt]);
         }
         __builtin_amdgcn_s_setprio(1);
+        const int asked = __builtin_amdgcn_readfirstlane(ask.x);
         const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
-        sums.template shape<SHAPED>(p, query, ask.x, ask.x != raise, x, k0, u, rare, pv);
-        raise = ask.x;
+        sums.template shape<SHAPED>(p, query, asked, asked != raise, x, k0, u, rare, pv);
+        raise = asked;
         v8h hi[G], lo[G];
         multiply(s_k[1 - N]);
         sums.template split<SHAPED>(query, x, pv, hi, lo);

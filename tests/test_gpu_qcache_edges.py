@@ -1,0 +1,101 @@
+"""The attention over caches in 4 or 8 bits at the ends of the ranges that its
+header states.  Definitions and bounds: qcache_f64.py."""
+import cache_ops_f64 as base
+import numpy as np
+import pytest
+import qcache_f64 as ref
+from test_gpu_qcache import F32, U, Attend
+
+pytestmark = pytest.mark.gpu
+
+
+def heads_of(a, s=0):
+    """Head, its query rows, its keys' and values' (step * code, mid), and what each token sees."""
+    _, n, rows, heads, kvh, hd = a.shape
+    dist = (int(a.lens[s]) - n + np.arange(n))[:, None] - np.arange(rows)
+    seen = (dist >= 0) & (dist < (a.window or rows))
+    for h in range(heads):
+        g = h // (heads // kvh)
+        yield h, a.q[s, :, h * hd:(h + 1) * hd].astype(np.float64), *([x[i][s, g] for i in (0, 1)] for x in (a.k, a.v)), seen
+
+
+def weigh(s, seen, v):
+    """Scores that the device has exactly → out, lse and the bounds of their errors, as
+    qcache_f64.attention without an error of the scores."""
+    va, vb = v
+    s = np.where(seen, s, -np.inf)
+    m = s.max(1, keepdims=True)
+    e = np.exp(s - m)
+    total = e.sum(1, keepdims=True)
+    p, lse = e / total, m[:, 0] + np.log(total[:, 0])
+    steps = (seen.sum(1) / 16 + 32) * U
+    d = np.where(seen, (m - np.where(seen, s, m)) * 2 * U + 2 * U, 0.0)
+    rows = (p * d).sum(1) + steps
+    size = np.abs(va) + np.abs(vb)
+    out_err = (p * (d + rows[:, None])) @ size + (p @ size) * (2.0 ** -21 + steps[:, None] + 2 * U) + 1e-38
+    out_err += (np.where(seen, size.max(1), 0.0).max(1) * seen.sum(1))[:, None] * 2.0 ** -32
+    return p @ (va + vb), lse, out_err, rows + np.abs(lse) * 4 * U + 2 * U
+
+
+VALUES = {"one": lambda rng, *shape: rng.standard_normal(shape), "large": lambda rng, *shape: rng.uniform(-6e4, 6e4, shape),
+          "small": lambda rng, *shape: rng.standard_normal(shape) * 1e-5}
+
+
+@pytest.mark.parametrize("values", VALUES)
+@pytest.mark.parametrize("far", [21, 22, 23, 25, 26, -22, -23, -25, 40])
+@pytest.mark.parametrize("n", [1, 40], ids=["few", "many"])
+@pytest.mark.parametrize("hd,bits,bias", [(128, 4, False), (128, 8, False), (64, 4, True), (128, 4, True)])
+def test_scores_that_differ_little_far_from_zero(ctx, rng, hd, bits, bias, n, far, values):
+    """Scores of 2^far + unit * (16 + t) to the base 2, t from -8 on and up to 5 in later
+    blocks, unit a step of fp32 there and 1 or more.  They are exact on the device: the scale
+    times log2(e) is 1; a key row's group has the midpoint 16 and the step 1; the sum of the
+    query row is the large part, and only its small element meets codes other than zero.  So
+    weights are 2^(unit * t), whatever the values' size."""
+    with base.Hip() as hip:
+        rows, half = 400, 1 << (bits - 1)
+        unit = 2.0 ** max(0, abs(far) - 23)
+        t = np.where(np.arange(rows) < 200, rng.integers(-8, 1, rows), rng.integers(-8, 6, rows))
+        k = np.full((1, 1, rows, hd), 16.0, F32)
+        k[0, 0, :, 1] += t
+        k[..., 3], k[..., 4] = 16 - half, 16 + half - 1
+        q = np.zeros((1, n, 2, hd), F32)
+        q[..., 1], q[..., 2] = unit, np.sign(far) * 2.0 ** (abs(far) - 4)
+        v = VALUES[values](rng, 1, 1, rows, hd).astype(F32)
+        a = Attend(hip, rng, 1, n, rows, 2, 1, hd, bits, q=q.reshape(1, n, -1), k=k, v=v, scale=F32(np.log(2)),
+                   slopes=np.zeros(2, F32) if bias else None)
+        assert np.array_equal(a.k[1][0, 0, :, :64], np.full((rows, 64), 16.0)) and np.array_equal(a.k[0][0, 0, :, 1], t)
+        out, lse = a.run(ctx).got()
+        for h, x, (ka, kb), v, seen in heads_of(a):
+            o, e, ob, eb = weigh(x @ (ka + kb).T * a.scale, seen, v)
+            base.close(out[0, :, h * hd:(h + 1) * hd], o, ob, f"out of head {h}")
+            base.close(lse[0, :, h], e, eb, f"lse of head {h}")
+
+
+@pytest.mark.parametrize("values", VALUES)
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 24, 2.0 ** 40, 2.0 ** 80])
+@pytest.mark.parametrize("n,hd,bits", [(1, 128, 4), (20, 128, 4), (70, 128, 8), (20, 64, 8), (70, 64, 4)])
+def test_the_one_key_of_far_scores(ctx, rng, n, hd, bits, size, values):
+    """Where the largest score stands above the next by more than both errors and 90 (a
+    weight of e^-90), out is that key's value row, and lse its score."""
+    with base.Hip() as hip:
+        rows = 300
+        q = (rng.standard_normal((1, n, 2 * hd)) * size).astype(F32)
+        v = VALUES[values](rng, 1, 1, rows, hd).astype(F32)
+        a = Attend(hip, rng, 1, n, rows, 2, 1, hd, bits, q=q, v=v)
+        out, lse = a.run(ctx).got()
+        clear = 0
+        for h, x, (ka, kb), (va, vb), seen in heads_of(a):
+            s = x @ (ka + kb).T * a.scale
+            key = np.abs(ka) + np.abs(kb)
+            err = np.abs(x) @ key.T * a.scale * (17 * U + 2.0 ** -21) + np.abs(s) * 4 * U
+            err = (err + a.scale * 2.0 ** -32 * np.abs(x).max(1)[:, None] * key.sum(1)).max(1)
+            s = np.where(seen, s, -np.inf)
+            at, two = s.argmax(1), np.sort(s, 1)[:, -2:]
+            one = two[:, 1] - two[:, 0] > 2 * err + 90
+            clear += one.sum()
+            o, w = out[0, :, h * hd:(h + 1) * hd], (va + vb)[at]
+            bound = (np.abs(va) + np.abs(vb))[at] * (2.0 ** -21 + 40 * U) + (np.abs(va) + np.abs(vb)).max() * 2.0 ** -32
+            assert np.isfinite(o).all() and np.isfinite(lse).all()
+            assert np.all((np.abs(o - w) <= bound)[one])
+            assert np.all(np.abs(lse[0, :, h] - two[:, 1]) <= err + np.abs(two[:, 1]) * 4 * U + 2 * U + np.log(rows))
+        assert clear >= n
