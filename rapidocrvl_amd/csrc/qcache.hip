@@ -406,6 +406,8 @@ extern "C" int pocr_qcache_attention(pocr_ctx *ctx, const pocr_qattention_args *
     p.window = window_of(a);
     p.scale = default_scale(a->scale, c->head_dim);
     p.cap = a->cap;
+    p.cap_inverse = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
+    p.cap_log2 = a->cap * kLog2e;
     hipStream_t s = (hipStream_t)stream;
     if (c->head_dim == 128)
         return c->bits == 4 ? launch_qattn_t<128, 4>(s, p, shape, a->workspace, c->seqs) : launch_qattn_t<128, 8>(s, p, shape, a->workspace, c->seqs);

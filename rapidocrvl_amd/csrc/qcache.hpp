@@ -504,7 +504,7 @@ struct QAttnCall {
     QRows cache;
     int n, heads, group, max_rows, window;
     uint32_t group_inv;  // 2^32 / group, rounded up (group 1: 0)
-    float scale, cap;
+    float scale, cap, cap_inverse, cap_log2;  // 1 / cap, cap · log2(e)
     // the token of query row r < 2^24: the quotient, at most one too large before its correction
     __device__ __forceinline__ int token(int r) const {
         const uint32_t q = group == 1 ? (uint32_t)r : __umulhi((uint32_t)r, group_inv);
@@ -532,6 +532,8 @@ struct QTile {
     int count, len;
     int lo, hi;          // keys some row sees
     int all_lo, all_hi;  // keys all rows see
+    __device__ __forceinline__ bool partly(int k0) const { return k0 < all_lo || k0 + kQBlock > all_hi; }  // some row, of the block from k0 on
+    __device__ __forceinline__ bool mixed() const { return lo != all_lo || hi != all_hi; }
 };
 __device__ __forceinline__ QTile q_tile(const QAttnCall &p, int s, int first, int rows) {
     QTile t;
@@ -674,7 +676,7 @@ struct QQuery {
     float sum;      // of the row's elements of group u, in lane 16u + i (zero where there is none)
     float size;     // a power of two: score = size · product
     float slope;
-    int from, pos;  // the keys it sees: [from, pos]
+    int pos;        // the last key it sees
 };
 
 // A lane's share of query row r (token, head of the KV head's group), elements 32c +
@@ -699,7 +701,6 @@ __device__ __forceinline__ void q_query(const QAttnCall &p, const QTile &t, int 
     const bool live = r < t.count * p.group;
     const int tok = p.token(live ? r : 0), head = g * p.group + (live ? r - tok * p.group : 0);
     q.pos = live ? t.len - t.count + tok : -1;
-    q.from = p.window ? max(0, q.pos - p.window + 1) : 0;
     const float scale = SHAPED && p.cap > 0.0f ? p.scale : p.scale * kLog2e;  // a cap takes scores as they are
     float x[C][8];
     uint32_t top = 0;
@@ -781,24 +782,30 @@ __device__ __forceinline__ void q_scores(float sum, const uint8_t *par, int kt, 
     }
 }
 
-// V's largest step so far, the exponent that brings it below 2^kQTop, and whether
-// the present block has parameters that are no numbers.
+// The exponent that brings V's step of these bits below 2^kQTop: step < 2^(exponent - 14),
+// subnormal ones < 2^-14.
+__device__ __forceinline__ int q_raise(uint32_t step) { return kQTop + 14 - (int)(step >> 10); }
+
+// V's largest step so far in blocks of which all rows see the same, its exponent, and whether the
+// present block has parameters that are no numbers.
 constexpr uint16_t kQBad = 0x8000;  // in place of such a group's step: no step is a negative zero
 struct QScale {
     uint32_t top = 0;  // its bits
-    int raise = kQTop + 14;
+    int raise = q_raise(0);
     bool moved = false, bad = false;
     // `v`: a lane's word of V's parameters.  What is no number stays out of products,
-    // where it would meet the zero weights of rows that do not see it.
+    // where it would meet the zero weights of rows that do not see it.  alone: rows see
+    // different keys of the block, and each looks for itself (QSums::shape).
     template <int HD>
-    __device__ __forceinline__ void look(uint32_t &v, int lane) {
+    __device__ __forceinline__ void look(uint32_t &v, int lane, bool alone) {
+        const uint32_t most_seen = alone ? 0x7bffu : top;
         const bool mine = HD == 128 || lane < 32, steps = HD == 64 || !(lane & 1);
         const uint32_t low = v & 0x7fffu, high = v >> 16 & 0x7fffu, none = 0x7bffu;  // none: the largest number
         moved = bad = false;
         if constexpr (HD == 128) {
-            if (!__any(max(low, high) > (steps ? top : none))) return;
+            if (!__any(max(low, high) > (steps ? most_seen : none))) return;
         } else {
-            if (!__any(mine && (low > top || high > none))) return;
+            if (!__any(mine && (low > most_seen || high > none))) return;
         }
         bool b0 = low > none, b1 = high > none;
         bad = __any(mine && (b0 || b1));
@@ -814,28 +821,39 @@ struct QScale {
                 if (b0 || b1) v = kQBad;
             }
         }
+        if (alone) return;
         uint32_t most = groups_umax(steps ? max(v & 0x7fffu, HD == 128 ? v >> 16 & 0x7fffu : 0u) : 0u);
 #pragma unroll
         for (int o = 8; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+        most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
         if (most <= top) return;
         top = most;
-        const int now = kQTop + 14 - (int)(most >> 10);  // step < 2^(exponent - 14), subnormal ones < 2^-14
+        const int now = q_raise(most);
         moved = now != raise;
         raise = now;
     }
 };
 
 // A row's running sums, in a lane of its tile.  Weights are 2^(score - m + raise), m a
-// whole number near the row's largest score, raise an exponent: ref is m - raise, and of
-// a row whose m is far from zero -raise, where `shape` takes m from its scores.
+// whole number near the row's largest score, raise the exponent of the largest step of V
+// that it has seen: ref is m - raise, and of a row whose m is far from zero -raise, where
+// `shape` takes m from its scores.
 template <int HD>
 struct QSums {
     static constexpr int G = HD / 64, T = HD / 16;
     v4f acc[T];
-    float ref = 0.0f, m = kLowest, total = 0.0f, mids[G];
+    float ref = -(kQTop + 14), m = kLowest, total = 0.0f, mids[G];
     bool far = false;  // some row of the wave's
     // what of m its scores lose beforehand
     __device__ __forceinline__ static float apart(float m) { return fabsf(m) >= kQFar ? m : 0.0f; }
+    __device__ __forceinline__ float down() const { return ref - (m - apart(m)); }  // -raise
+    __device__ __forceinline__ void rescale(float by) {
+        total *= by;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) mids[gr] *= by;
+#pragma unroll
+        for (int k = 0; k < T; ++k) acc[k] *= by;
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int k = 0; k < T; ++k) acc[k] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
@@ -843,53 +861,67 @@ struct QSums {
         for (int gr = 0; gr < G; ++gr) mids[gr] = 0.0f;
     }
     // products x of a block from key k0 on (lane: keys 16 (j / 4) + 4u + j % 4) → scores,
-    // but for q.size, and the row's reference.  rare: some row does not see all keys, or
-    // some of V's parameters are no numbers.
+    // but for q.size, and the row's reference.  masked: some row does not see all keys;
+    // alone: nor do all see the same, or some of V's parameters are no numbers; raise and
+    // moved: of blocks of which all rows see the same.
     template <bool SHAPED>
-    __device__ __forceinline__ void shape(const QAttnCall &p, const QQuery &q, int raise, bool moved, float (&x)[8], int k0, int u, bool rare,
-                                          const v8h (&v)[2][G]) {
+    __device__ __forceinline__ void shape(const QAttnCall &p, const QQuery &q, int raise, bool moved, float (&x)[8], int k0, int u, bool masked,
+                                          bool alone, const v8h (&v)[2][G]) {
         auto key_of = [&](int j) { return k0 + 16 * (j >> 2) + 4 * u + (j & 3); };
         const float size = SHAPED ? 1.0f : q.size;  // exact, so a score may round with its reference
         if (SHAPED) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= q.size;
             if (p.cap > 0.0f) {
-                const float down = 1.0f / p.cap, up = p.cap * kLog2e;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= down;
+                for (int j = 0; j < 8; ++j) x[j] *= p.cap_inverse;
                 tanh_all<8>(x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= up;
+                for (int j = 0; j < 8; ++j) x[j] *= p.cap_log2;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = rounded(fmaf(-q.slope, (float)(q.pos - key_of(j)), x[j]));
         }
-        if (rare) {
+        // of key_of(j), as bits of a vector register: eight lane masks are more than the
+        // scalar ones hold beside the round's own numbers
+        auto sees = [&](int j) {
+            const int from = p.window ? max(0, q.pos - p.window + 1) : 0;
+            uint32_t bits = (uint32_t)(key_of(j) - from) < (uint32_t)max(0, q.pos + 1 - from) ? ~0u : 0u;
+            asm("" : "+v"(bits));
+            return bits;
+        };
+        float least = -(float)raise;  // of -raise
+        if (__builtin_expect(masked || alone, 0)) {
+            if (masked) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = key_of(j);
-                const bool sees = key >= q.from && key <= q.pos;
-                x[j] = sees ? x[j] : -INFINITY;
+                for (int j = 0; j < 8; ++j) x[j] = __uint_as_float((__float_as_uint(x[j]) & sees(j)) | (0xff800000u & ~sees(j)));
+            }
+            if (alone) {
+                uint32_t most = 0, worst[G] = {};
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) {  // NaN for the rows that see one, in its group
-                    const _Float16 step = QParams<HD>::of(v[j >> 2], j & 3, gr, 0);
-                    if (sees && __builtin_bit_cast(uint16_t, step) == kQBad) mids[gr] = __builtin_nanf("");
-                }
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        const uint32_t step = sees(j) & __builtin_bit_cast(uint16_t, QParams<HD>::of(v[j >> 2], j & 3, gr, 0));
+                        worst[gr] = max(worst[gr], step);
+                        most = max(most, step & 0x7fffu);
+                    }
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)  // NaN for the rows that see one, in its group
+                    if (worst[gr] == kQBad) mids[gr] = __builtin_nanf("");
+                least = fmaxf(least, -(float)q_raise(groups_umax(most)));
+                moved = moved || __any(least > down());
             }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * size;
         if (__any(moved || far || top > m + kQSlack)) {
             top = groups_max(top);
-            const float before = apart(m);
+            const float before = apart(m), own = fmaxf(down(), least);
             if (top > m) m = fminf(ceilf(top), 3.0e38f);
-            const float less = apart(m), now = m - less - (float)raise, by = __builtin_amdgcn_exp2f((before - less) + (ref - now));
+            const float less = apart(m), now = m - less + own, by = __builtin_amdgcn_exp2f((before - less) + (ref - now));
             ref = now;
             far = __any(fabsf(m) >= kQFar && m > kLowest);
-            total *= by;
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) mids[gr] *= by;
-#pragma unroll
-            for (int k = 0; k < T; ++k) acc[k] *= by;
+            rescale(by);
             if (far) {  // `split` multiplies by size again: a power of two
                 const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(size));
 #pragma unroll
@@ -964,9 +996,10 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 //   q . k = sum over groups of step (q . c) + mid (sum of q),
 //   out = sum over keys of (p step) . c + sum of p mid.
 // p = 2^(s - ref), ref a whole number near the row's largest score, lowered by the
-// exponent that brings V's largest step so far to 2^kQTop, so that the halves of p
-// step hold the products that count whatever V's size.  All rescales are by powers
-// of two.  A wave's first block and its query rows do not depend on the sequence's
+// exponent that brings the largest step of V that the row has seen so far to 2^kQTop, so
+// that the halves of p step hold the products that count whatever V's size, and a row's
+// precision does not hang on keys that other rows of its tile see.  All rescales are by
+// powers of two.  A wave's first block and its query rows do not depend on the sequence's
 // length, and are requested with it; a later block's codes as soon as the registers
 // of the one before are free.
 //
@@ -1049,12 +1082,12 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
 
     for (; block < end; block += step) {
         const int k0 = block * kQBlock, next0 = k0 + step * kQBlock;
-        const bool more = block + step < end, masked = k0 < t.all_lo || k0 + kQBlock > t.all_hi;
+        const bool more = block + step < end, masked = t.partly(k0), mixed = masked && t.mixed();
         if (masked) {  // parameters of keys outside the tile's are zero
             const int key = k0 + Params::key_of(lane);
             if (key < t.lo || key >= t.hi) par.k = par.v = 0;
         }
-        scale.look<HD>(par.v, lane);
+        scale.look<HD>(par.v, lane, mixed);
         if (HD == 128 || lane < 32) {
             reinterpret_cast<uint32_t *>(kpar)[lane] = par.k;
             reinterpret_cast<uint32_t *>(vpar)[lane] = par.v;
@@ -1085,7 +1118,7 @@ __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_at
         Params::get(vpar, 1, u, pv[1]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            sums[rt].template shape<SHAPED>(p, query[rt], scale.raise, scale.moved, x[rt], k0, u, masked || scale.bad, pv);
+            sums[rt].template shape<SHAPED>(p, query[rt], scale.raise, scale.moved, x[rt], k0, u, masked, mixed || scale.bad, pv);
             sums[rt].template split<SHAPED>(query[rt], x[rt], pv, hi[rt], lo[rt]);
         }
 #pragma unroll
@@ -1210,12 +1243,16 @@ struct QLayer {
 // with the join, 0.33 to 0.37 PFLOP/s (1.16 for a large fp16 product).  Instructions bound
 // it, at three waves to a SIMD: vector ones take 45 % of the cycles, matrix ones 40 %, LDS
 // 42 %; a wave waits for its turn to issue for 36 % of its time.
+// At least and at most so many waves to a SIMD: told the least alone, the compiler spares
+// registers for more than fit, and the 8-bit kernel's vector instructions end up in one
+// piece behind its matrix ones (540 tokens 128 us for 136).
 // Eight waves a workgroup took 143 us where four took 138; codes one round ahead 135
 // where this takes 129; 32 rows a wave spilled 22 registers and took 177 where 16 took
 // 136; four sums of scores at a time in place of two, spilled too, 143 where two took
 // 126; without the priorities 117 where this takes 112.
 template <int HD, int BITS, bool SHAPED>
-__global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
+__global__ void __launch_bounds__(256)
+    __attribute__((amdgpu_waves_per_eu(HD == 128 && BITS == 4 ? 3 : 2, HD == 64 ? 4 : BITS == 8 ? 2 : 3))) k_qcache_attn_rows(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
     using Layer = QLayer<HD, BITS>;
     using Params = QParams<HD>;
@@ -1269,9 +1306,10 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         if (wave < 2) {
             const int key = from + Params::key_of(lane);
             uint32_t w = par[N];
-            if ((from < wt.all_lo || from + kQBlock > wt.all_hi) && (key < wt.lo || key >= wt.hi)) w = 0;
+            const bool masked = wt.partly(from);
+            if (masked && (key < wt.lo || key >= wt.hi)) w = 0;
             if (wave) {
-                scale.look<HD>(w, lane);
+                scale.look<HD>(w, lane, masked);
                 if (lane == 0) s_raise[N] = make_int2(scale.raise, scale.bad);
             }
             if (HD == 128 || lane < 32) reinterpret_cast<uint32_t *>(wave ? s_vpar[N] : s_kpar[N])[lane] = w;
@@ -1306,7 +1344,7 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
     layer[0].put_v(s_v[0], wave, lane, magic);
     layer[1].load_k(kc, k0 + 3 * step, cap, wave, lane);
     layer[0].load_v(vc, k0 + 2 * step, cap, wave, lane);
-    int raise = kQTop + 14;  // as QScale begins
+    int raise = q_raise(0);  // as QScale begins
     // the round of a block of even (N 0) or odd number; k0 moves on
     auto round = [&](auto number) {
         constexpr int N = decltype(number)::value;
@@ -1325,8 +1363,8 @@ __global__ void __launch_bounds__(256, BITS == 8 ? 2 : 3) k_qcache_attn_rows(QAt
         }
         __builtin_amdgcn_s_setprio(1);
         const int asked = __builtin_amdgcn_readfirstlane(ask.x);
-        const bool rare = k0 < wt.all_lo || k0 + kQBlock > wt.all_hi || __builtin_amdgcn_readfirstlane(ask.y);
-        sums.template shape<SHAPED>(p, query, asked, asked != raise, x, k0, u, rare, pv);
+        const bool rare = wt.partly(k0) || __builtin_amdgcn_readfirstlane(ask.y);
+        sums.template shape<SHAPED>(p, query, asked, asked != raise, x, k0, u, rare, rare, pv);
         raise = asked;
         v8h hi[G], lo[G];
         multiply(s_k[1 - N]);

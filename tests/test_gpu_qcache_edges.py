@@ -99,3 +99,19 @@ def test_the_one_key_of_far_scores(ctx, rng, n, hd, bits, size, values):
             assert np.all((np.abs(o - w) <= bound)[one])
             assert np.all(np.abs(lse[0, :, h] - two[:, 1]) <= err + np.abs(two[:, 1]) * 4 * U + 2 * U + np.log(rows))
         assert clear >= n
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("n,heads", [(8, 2), (15, 2), (40, 2), (24, 8)])
+@pytest.mark.parametrize("hd,bits", [(128, 4), (128, 8), (64, 4)])
+def test_values_that_a_row_does_not_see_cost_it_nothing(ctx, rng, hd, bits, n, heads, window, cap):
+    """Values of about 1e-3, and one row of up to 65504 in the block of the last tokens' own
+    rows (no window), or in one that the window of most has left: the other tokens keep
+    their precision."""
+    with base.Hip() as hip:
+        rows = 200
+        v = (rng.standard_normal((1, 1, rows, hd)) * 1e-3).astype(F32)
+        first = rows - n
+        v[0, 0, first - window + 4 if window else rows - 3, 7::64] = 65504.0
+        Attend(hip, rng, 1, n, rows, heads, 1, hd, bits, window=window, cap=cap, v=v).run(ctx).check()
