@@ -115,3 +115,60 @@ def test_values_that_a_row_does_not_see_cost_it_nothing(ctx, rng, hd, bits, n, h
         first = rows - n
         v[0, 0, first - window + 4 if window else rows - 3, 7::64] = 65504.0
         Attend(hip, rng, 1, n, rows, heads, 1, hd, bits, window=window, cap=cap, v=v).run(ctx).check()
+
+
+def shares(a):
+    """Key shares of a call, from its workspace: [tiles of so many rows][share][sums, reference, denominator]."""
+    seqs, n, _, heads, kvh, hd = a.shape
+    rows = n * (heads // kvh)
+    tile = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    tiles = -(-rows // tile) * kvh * seqs
+    assert a.args.workspace_bytes % (tiles * tile * (hd + 2) * 4) == 0
+    return a.args.workspace_bytes // (tiles * tile * (hd + 2) * 4)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n,heads,kvh,hd,rows", [
+    (1, 4, 2, 64, 1100), (1, 4, 2, 64, 3000), (12, 4, 2, 64, 1100), (12, 8, 8, 64, 3000), (70, 4, 2, 64, 1100), (70, 8, 8, 64, 3000),
+    (1, 16, 2, 128, 640), (2, 16, 2, 128, 900), (3, 16, 2, 128, 300), (3, 16, 2, 128, 700), (4, 16, 2, 128, 700),
+    (4, 16, 2, 128, 5000), (3, 16, 2, 128, 5000), (6, 16, 2, 128, 200), (20, 4, 1, 128, 1500)])
+def test_shares_of_ragged_sequences(ctx, rng, bits, n, heads, kvh, hd, rows):
+    """Keys in shares and their join, in every kind of tile; sequences that end before their first or last share."""
+    with base.Hip() as hip:
+        lens = [rows, rows // 2 + 1, 40, rows - 33, 0]
+        a = Attend(hip, rng, 5, n, rows, heads, kvh, hd, bits, lens=lens, counts=[n, n, n, max(1, n - 1), n], pad=4, capacity=rows + 7)
+        assert shares(a) > 1
+        a.run(ctx).check(np.unique([0, n // 2, n - 2, n - 1])[-4:] % n, [0, heads - 1])
+
+
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (30.0, True)], ids=["plain", "cap-bias"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n,heads,kvh,hd,window", [(1, 16, 2, 128, 700), (1, 4, 2, 64, 2000), (4, 16, 2, 128, 700), (4, 16, 2, 128, 2001),
+                                                   (3, 8, 1, 64, 1033), (33, 4, 2, 128, 700)])
+def test_shares_of_windows(ctx, rng, bits, n, heads, kvh, hd, window, cap, bias):
+    """The first share begins where the window of the tile's first token does, in the middle of a block."""
+    with base.Hip() as hip:
+        slopes = np.array([2.0 ** (-0.7 * (h + 3)) for h in range(heads)], F32) if bias else None
+        a = Attend(hip, rng, 3, n, 5000, heads, kvh, hd, bits, lens=[5000, 4011, 600], window=window, cap=cap, slopes=slopes)
+        assert shares(a) > 1
+        a.run(ctx).check(np.unique([0, n - 1]), [0, heads - 1])
+
+
+@pytest.mark.parametrize("seqs,rows,most", [(1, 600, 5), (8, 1100, 9), (40, 1100, 6), (80, 900, 3), (120, 1500, 2)])
+def test_few_shares_of_few_rows(ctx, rng, seqs, rows, most):
+    """Two to nine shares, the fewer the more sequences there are: joined two or eight at a time."""
+    with base.Hip() as hip:
+        a = Attend(hip, rng, seqs, 1, rows, 4, 2, 128, 4, lens=rows - 7 * np.arange(seqs))
+        assert 1 < shares(a) <= most
+        a.run(ctx).check(heads_at=[0, 3])
+
+
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("seqs,kvh,hd,bits", [(130, 2, 64, 4), (33, 8, 128, 4), (33, 8, 128, 8)])
+def test_long_caches_of_many_sequences(ctx, rng, seqs, kvh, hd, bits, n):
+    """So many (sequence, KV head) pairs that each takes one workgroup, whatever its length."""
+    with base.Hip() as hip:
+        rows = 1300
+        a = Attend(hip, rng, seqs, n, rows, 4 * kvh, kvh, hd, bits, lens=rows - 9 * np.arange(seqs))
+        assert shares(a) == 0
+        a.run(ctx).check(np.array([0, n - 1]), [0, 4 * kvh - 1])
