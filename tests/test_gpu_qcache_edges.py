@@ -1,10 +1,13 @@
 """The attention over caches in 4 or 8 bits at the ends of the ranges that its
 header states.  Definitions and bounds: qcache_f64.py."""
+import threading
+
 import cache_ops_f64 as base
 import numpy as np
 import pytest
-import qcache_f64 as ref
-from test_gpu_qcache import F32, U, Attend
+from test_gpu_qcache import F32, SENTINEL, U, Attend
+
+from rapidocrvl_amd import lib
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +175,66 @@ def test_long_caches_of_many_sequences(ctx, rng, seqs, kvh, hd, bits, n):
         a = Attend(hip, rng, seqs, n, rows, 4 * kvh, kvh, hd, bits, lens=rows - 9 * np.arange(seqs))
         assert shares(a) == 0
         a.run(ctx).check(np.array([0, n - 1]), [0, 4 * kvh - 1])
+
+
+FORMS = [(2, 1, 300), (2, 1, 2500), (2, 3, 200), (2, 3, 600), (1, 70, 100), (2, 70, 900)]  # each tile, in one launch and in shares
+
+
+def fresh(a):
+    """The same call into buffers that hold nothing but the sentinel."""
+    seqs, n, _, heads, _, hd = a.shape
+    args = lib.QAttentionArgs.from_buffer_copy(a.args)
+    args.out, args.lse = a.hip.up(np.full((seqs, n, heads * hd), SENTINEL, F32)), a.hip.up(np.full((seqs, n, heads), SENTINEL, F32))
+    return args
+
+
+@pytest.mark.parametrize("seqs,n,rows", FORMS)
+def test_a_call_without_lse_writes_its_rows_and_no_lse(ctx, rng, seqs, n, rows):
+    with base.Hip() as hip:
+        a = Attend(hip, rng, seqs, n, rows, 16, 2, 128, 4).run(ctx)
+        args = fresh(a)
+        lse, args.lse = args.lse, None
+        ctx.qcache_attention(args, a.cache.args)
+        assert np.all(hip.down(lse, (seqs, n, 16)) == SENTINEL)
+        a.args.out = args.out
+        a.check(heads_at=[0, 15])
+
+
+@pytest.mark.parametrize("seqs,n,rows", FORMS)
+def test_each_call_writes_the_same(ctx, rng, seqs, n, rows):
+    """The same call several times, each into buffers of its own: equal to the last bit."""
+    with base.Hip() as hip:
+        a = Attend(hip, rng, seqs, n, rows, 16, 2, 128, 4).run(ctx).check(heads_at=[0, 15])
+        out, lse = a.got()
+        for _ in range(4):
+            args = fresh(a)
+            ctx.qcache_attention(args, a.cache.args)
+            assert np.array_equal(hip.down(args.out, out.shape), out) and np.array_equal(hip.down(args.lse, lse.shape), lse)
+
+
+def test_threads_write_each_their_own(ctx, rng):
+    """Calls from four threads on streams of their own, workspaces of their own, each call
+    into buffers of its own: all as when alone."""
+    with base.Hip() as hip:
+        work = [Attend(hip, rng, 2, n, rows, 16, 2, 128, 4).run(ctx) for n, rows in ((1, 700), (5, 400), (40, 300), (1, 2500))]
+        calls = [[fresh(a) for _ in range(8)] for a in work]
+        streams = [hip.stream() for _ in work]
+        fails = []
+
+        def run(a, args, stream):
+            try:
+                for x in args:
+                    ctx.qcache_attention(x, a.cache.args, stream)
+            except Exception as e:  # noqa: BLE001
+                fails.append(e)
+
+        threads = [threading.Thread(target=run, args=x) for x in zip(work, calls, streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not fails
+        for a, args in zip(work, calls):
+            out, lse = a.check(heads_at=[0, 15]).got()
+            for x in args:
+                assert np.array_equal(hip.down(x.out, out.shape), out) and np.array_equal(hip.down(x.lse, lse.shape), lse)
