@@ -225,6 +225,7 @@ struct QShape {
     bool many;   // k_qcache_attn_rows
     int rt;      // else: row tiles of 16 a workgroup
     int rows;    // of a workgroup
+    bool brief;  // one launch, however few its workgroups
     int tiles, splits;
     int64_t slots, bytes;
 };
@@ -239,6 +240,12 @@ struct QShape {
 // 11.4 : 10.7; 48 rows 128 keys 10.1 : 10.5, 160 keys 11.3 : 10.9.  Heads of 64: 16 rows
 // 1,024 keys 8.8 : 9.0, 1,280 keys 9.9 : 9.0; 32 rows 512 keys 9.5 : 9.3; 48 rows 192 keys
 // 8.8 : 9.8, 256 keys 10.2 : 9.1.
+// Eight waves a workgroup, up to 16 rows: for short caches (8 tokens of 4 heads of 64 behind
+// 700 rows 7.9 us, four waves 9.6), and for heads of 64 where there are so many workgroups
+// that long ones have one share too (64 sequences of 8 KV heads, 2,048 and 8,192 rows, 22.7
+// and 71 us, four waves 25.3 and 91).  Long ones of heads of 128 then take four: 38.4 and
+// 127.5 us, eight 42.7 and 133; 160 sequences of 2 KV heads in 8 bits 41 and 137, eight 46
+// and 152.
 // Shares: few rows 512 workgroups (16 sequences of 8 rows, 8,192 keys, in 256, 512 and
 // 768: 19.7, 18.3, 18.9) of 4 blocks or more, one for each wave (8 rows, 8,192 keys, 2, 4
 // and 8: 10.4, 9.3, 10.0).  Many rows: one workgroup a CU first, of 2 blocks or more (64
@@ -261,7 +268,8 @@ QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     // so many shares that at most `wgs` workgroups result, of `least` blocks or more
     auto shares = [&](int64_t wgs, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>(wgs / work, round_up_div(blocks, least))); };
     const int64_t most = q.many ? std::max(shares(256, 2), shares(768, 6)) : shares(512, 4);
-    q.splits = blocks <= whole ? 1 : (int)std::min<int64_t>(most, 128);
+    q.brief = blocks <= whole;
+    q.splits = q.brief ? 1 : (int)std::min<int64_t>(most, 128);
     q.slots = q.splits > 1 ? work * q.splits : 0;
     q.bytes = q.slots * q.rows * (c->head_dim + 2) * 4;
     return q;
@@ -279,7 +287,7 @@ int launch_qattn(hipStream_t s, const QAttnCall &p, const QShape &q, void *work,
     if constexpr (ROWS == 64) {
         RC(launch(s, grid, 256, shaped ? k_qcache_attn_rows<HD, BITS, true> : k_qcache_attn_rows<HD, BITS, false>, p, pl));
     } else {
-        if (ROWS == 16 && q.splits == 1) return launch(s, grid, 512, shaped ? k_qcache_attn<HD, BITS, 1, 8, true> : k_qcache_attn<HD, BITS, 1, 8, false>, p, pl);
+        if (ROWS == 16 && q.splits == 1 && (HD == 64 || q.brief)) return launch(s, grid, 512, shaped ? k_qcache_attn<HD, BITS, 1, 8, true> : k_qcache_attn<HD, BITS, 1, 8, false>, p, pl);
         RC(launch(s, grid, 256, shaped ? k_qcache_attn<HD, BITS, ROWS / 16, 4, true> : k_qcache_attn<HD, BITS, ROWS / 16, 4, false>, p, pl));
     }
     if (q.splits == 1) return POCR_OK;

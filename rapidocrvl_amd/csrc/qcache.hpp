@@ -1008,8 +1008,7 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 // 4 bits behind 1,609 rows 9.3 us with the join (two launches alone are 6.2 for the host);
 // 16 of them behind up to 8,192 rows (33 MB) 17.1, of which loads without arithmetic
 // 12.8.  Two blocks of a wave on their way: 18.0, registers for two workgroups a CU in
-// place of three; two blocks a round: one token 10.7.  Eight waves where one launch
-// does it all: 8 tokens of 4 heads of 64 behind 700 rows 7.9 us, with four 9.6.
+// place of three; two blocks a round: one token 10.7.
 template <int HD, int BITS, int RT, int W, bool SHAPED>
 __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;
