@@ -249,9 +249,13 @@ struct QShape {
 // Shares: few rows 512 workgroups (16 sequences of 8 rows, 8,192 keys, in 256, 512 and
 // 768: 19.7, 18.3, 18.9) of 4 blocks or more, one for each wave (8 rows, 8,192 keys, 2, 4
 // and 8: 10.4, 9.3, 10.0).  Many rows: one workgroup a CU first, of 2 blocks or more (64
-// rows, 2,048 keys, 2, 3 and 6: 12.0, 13.2, 15.7), then three, of 6 or more (64 rows of 16
-// sequences, 2,048 keys, 2, 3 and 6: 27.5, 27.2, 24.4; 4,800 rows, 8,192 keys, 3 and 5
-// shares: 169, 136).
+// rows, 2,048 keys, 2, 3 and 6: 12.0, 13.2, 15.7), then as many as a CU holds, of 6 or more
+// (64 rows of 16 sequences, 2,048 keys, 2, 3 and 6: 27.5, 27.2, 24.4).  Those are three of
+// heads of 128 in 4 bits (600 tokens behind 8,192 rows in 512, 768 and 1,024 workgroups:
+// 130, 106, 130), and three of heads of 64 too, of which a CU holds four (88, 70, 73).  In
+// 8 bits they are two (122, 142, 127; 16 sequences of 40: 120, 160, 126), or two after one
+// another where that leaves 8 blocks less in a row: 540 tokens 119, 126, 112; 700: 168,
+// 155, 145.
 QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     QShape q;
     const int64_t rows = (int64_t)a->n * (a->heads / c->kv_heads), groups = (int64_t)c->kv_heads * c->seqs;
@@ -267,7 +271,13 @@ QShape qattn_shape(const pocr_qattention_args *a, const pocr_qcache *c) {
     const int whole = q.many ? (small ? 6 : 4) : (q.rt == 2 ? 8 : 16) * (small ? 2 : 1);
     // so many shares that at most `wgs` workgroups result, of `least` blocks or more
     auto shares = [&](int64_t wgs, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>(wgs / work, round_up_div(blocks, least))); };
-    const int64_t most = q.many ? std::max(shares(256, 2), shares(768, 6)) : shares(512, 4);
+    int64_t most = shares(512, 4);
+    if (q.many && !small && c->bits == 8) {
+        const int64_t once = std::max(shares(256, 2), shares(512, 6)), twice = shares(1024, 6);
+        most = 2 * round_up_div(blocks, twice) + 8 < round_up_div(blocks, once) ? twice : once;
+    } else if (q.many) {
+        most = std::max(shares(256, 2), shares(768, 6));
+    }
     q.brief = blocks <= whole;
     q.splits = q.brief ? 1 : (int)std::min<int64_t>(most, 128);
     q.slots = q.splits > 1 ? work * q.splits : 0;
