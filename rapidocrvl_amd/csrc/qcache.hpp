@@ -282,13 +282,15 @@ __device__ __forceinline__ double xchg(double v) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// 1 / sqrt(x): the instruction's estimate, then a step of third and one of second order
+// 1 / sqrt(x): the instruction's estimate, then a step of third and one of second order;
+// 0 of an infinity, where the steps would multiply it by its estimate
 __device__ __forceinline__ double inverse_root(double x) {
-    double r = __builtin_amdgcn_rsq(x);
-    double e = fma(-x * r, r, 1.0);
-    r = fma(r * e, fma(e, 0.375, 0.5), r);
+    const double first = __builtin_amdgcn_rsq(x);
+    double e = fma(-x * first, first, 1.0);
+    double r = fma(first * e, fma(e, 0.375, 0.5), first);
     e = fma(-x * r, r, 1.0);
-    return fma(r * e, 0.5, r);
+    r = fma(r * e, 0.5, r);
+    return first == 0.0 ? 0.0 : r;
 }
 
 // how a head's pairs lie: (i, H + i) over the whole of it, (2i, 2i + 1), or over part of it by halves

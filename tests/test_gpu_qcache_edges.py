@@ -5,7 +5,7 @@ import threading
 import cache_ops_f64 as base
 import numpy as np
 import pytest
-from test_gpu_qcache import F32, SENTINEL, U, Attend
+from test_gpu_qcache import F32, SENTINEL, U, Attend, Rows
 
 from rapidocrvl_amd import lib
 
@@ -238,3 +238,22 @@ def test_threads_write_each_their_own(ctx, rng):
             out, lse = a.check(heads_at=[0, 15]).got()
             for x in args:
                 assert np.array_equal(hip.down(x.out, out.shape), out) and np.array_equal(hip.down(x.lse, lse.shape), lse)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("hd,rotary,adjacent", [(128, 0, 0), (128, 64, 0), (64, 32, 1)])
+def test_norm_of_an_infinite_element(ctx, rng, hd, rotary, adjacent, sign):
+    """x / sqrt(mean(x^2) + eps) of a head with an infinity: zeros, and NaN in its own place
+    and that of the other element of its pair."""
+    with base.Hip() as hip:
+        q = rng.standard_normal((1, 3, 2 * hd)).astype(F32)
+        q[0, 1, 5] = sign * np.inf
+        r = Rows(hip, rng, 1, 3, 2, 1, hd, rotary, 1, norms=True, q=q, adjacent=adjacent)
+        ctx.rotate_rows(r.args)
+        got = r.got("q")[0]
+        bad = np.zeros(hd, bool)
+        bad[5] = True
+        if rotary:
+            bad[4 if adjacent else 5 + rotary // 2] = True
+        assert np.array_equal(np.isnan(got[1, :hd]), bad) and np.all(got[1, :hd][~bad] == 0.0)
+        assert np.isfinite(np.delete(got.reshape(3, 2, hd).reshape(6, hd), 2, 0)).all()
