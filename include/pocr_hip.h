@@ -443,7 +443,8 @@ int pocr_cache_keep(pocr_ctx *ctx, const pocr_keep_args *args, void *stream);
  * workspaces, numbers that live on the device.  Strides are at most 2^40. */
 
 /* Rows of seqs sequences of up to n tokens each, of q, k and v, on their way to
- * where attention reads them.  Each may be left out (null, with its destination).
+ * where attention reads them.  Each may be left out (null, with its destination),
+ * in pocr_qcache_write q alone.
  *  - Every head x of q (k) becomes x * q_norm / sqrt(mean(x^2) + eps) where q_norm
  *    (k_norm) is given;
  *  - where positions are given (rotary_dim > 0), pair i < rotary_dim / 2 of its
@@ -512,8 +513,8 @@ typedef struct {
     int32_t bits;                  /* 4 or 8 */
 } pocr_qcache;
 
-/* rows into a cache: K and V rows of args as above, into rows first[s] + t, in
- * place of k_out and v_out (null here).  K rows are held as pocr_rotate_rows gives
+/* rows into a cache: K and V rows of args as above, both given, into rows
+ * first[s] + t, in place of k_out and v_out (null here).  K rows are held as pocr_rotate_rows gives
  * them; q rows, where given, go to q_out in the same pass.  seqs, kv_heads and
  * head_dim are the cache's, n is at most its capacity.  No other row changes. */
 int pocr_qcache_write(pocr_ctx *ctx, const pocr_rows_args *args, const pocr_qcache *cache, void *stream);

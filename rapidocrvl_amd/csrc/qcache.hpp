@@ -304,7 +304,7 @@ enum : int { kPairsWhole = 0, kPairsAdjacent = 1, kPairsPart = 2 };
 //
 // Memory bounds it: 8,192 normed tokens of 16 + 2 + 2 heads of 128 rotated 37 us (168 MB,
 // 4.5 TB/s), with K and V into 4 bits 37 too (151 MB: the quantising shows), 18 layers of
-// 1,345 K and V rows of 2 heads into 8 bits 18.4 (62 MB).  1,345 tokens of 16 + 2 heads
+// 1,345 K and V rows of 2 heads into 8 bits 17.7 to 20 (62 MB).  1,345 tokens of 16 + 2 heads
 // take 8.5 us (27 MB), where the launch and the first loads' way count.  The simplest
 // form, a lane with eight neighbouring elements and a wave a head, took 118 us for the
 // first: its loads and stores were halves of lines, and a rotation fetched its other
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) k_rows(RowsCall p) {
     constexpr int L = HD / 8, U = 64 / L, H = HD / 2;
     __shared__ double2 s_turn[4][H];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y, i = lane % L;
-    const uint32_t job = blockIdx.x * 4 + wave;  // at most 2^22 tokens, 2^9 chunks
+    const uint32_t job = blockIdx.x * 4 + wave;  // at most 2^22 tokens, and 768 chunks below 2,048 of them
     const int step = job / (uint32_t)p.chunks, chunk = job - step * p.chunks;
     const int count = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
     int tok = step * p.tokens;
@@ -461,7 +461,7 @@ struct QReadCall {
 // HD / 8 lanes a row of a head, K and V one after the other: mid + step * code, a
 // multiply-add.  Stores bound it: 18 caches of 1,609 rows of 2 heads of 128 in 4 bits
 // (60 MB) 11.4 to 12.3 us, 4.8 to 5.2 TB/s; 2,048 listed rows of each in 8 bits (84 MB)
-// 19.7, 4.3 TB/s.  Loads of codes and parameters are short pieces of lines, which the
+// 19.3, 4.4 TB/s.  Loads of codes and parameters are short pieces of lines, which the
 // neighbours' loads find in the cache.
 template <int HD, int BITS>
 __global__ void __launch_bounds__(256) k_qcache_read(QReadCall p) {
@@ -1007,9 +1007,9 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 //
 // Few rows are bound by the chain of one wave: launch, lengths and first codes (5 us),
 // then 0.7 us a block, sums joined in LDS.  One token of 16 heads on 2 KV heads of 128 in
-// 4 bits behind 1,609 rows 9.3 us with the join (two launches alone are 6.2 for the host);
-// 16 of them behind up to 8,192 rows (33 MB) 17.1, of which loads without arithmetic
-// 12.8.  Two blocks of a wave on their way: 18.0, registers for two workgroups a CU in
+// 4 bits behind 1,609 rows 9.0 to 9.7 us with the join (two launches over 17 blocks of keys
+// 8.9, one over a single block 6.5), in 8 bits 8.9 to 9.8; 16 of them behind up to 8,192
+// rows (33 MB) 17.1, without arithmetic 12.8, the join's 3 in both.  Two blocks of a wave on their way: 18.0, registers for two workgroups a CU in
 // place of three; two blocks a round: one token 10.7.
 template <int HD, int BITS, int RT, int W, bool SHAPED>
 __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
@@ -1232,7 +1232,7 @@ struct QLayer {
 // together, each unpacking its part of a block's codes into LDS for all of them.
 //
 // A round of a wave (32 keys, heads of 128) has 34 matrix instructions of 16 cycles or 32
-// and about 165 vector instructions of 4, which run beside them only where they lie
+// and about 169 vector instructions of 4, which run beside them only where they lie
 // between them: the next block's scores are multiplied among this block's exponentials,
 // this block's sums among the unpacking of later codes.  So a round needs the next
 // block's keys and this block's values, both in two buffers, and one barrier; codes are
@@ -1241,9 +1241,11 @@ struct QLayer {
 // other workgroups that unpack or wait, which keeps them apart in their rounds.
 //
 // 600 tokens of 16 heads on 2 KV heads of 128 in 4 bits behind 8,192 rows: 112 to 125 us
-// with the join, 0.33 to 0.37 PFLOP/s (1.16 for a large fp16 product).  Instructions bound
-// it, at three waves to a SIMD: vector ones take 45 % of the cycles, matrix ones 40 %, LDS
-// 42 %; a wave waits for its turn to issue for 36 % of its time.
+// with the join, 0.31 to 0.35 PFLOP/s and, with two halves each, 0.66 to 0.74 of products
+// (1.16 for a large fp16 product); with cap and slopes 162, in 8 bits 122.  Instructions
+// bound it, at three waves to a SIMD: vector ones take 46 % of the cycles, matrix ones 39 %,
+// LDS 41 %; a wave waits for its turn to issue for 36 % of its time.  With cap or slopes, in
+// 4 bits, seven registers spill.
 // At least and at most so many waves to a SIMD: told the least alone, the compiler spares
 // registers for more than fit, and the 8-bit kernel's vector instructions end up in one
 // piece behind its matrix ones (540 tokens 128 us for 136).
@@ -1351,10 +1353,7 @@ __global__ void __launch_bounds__(256)
         constexpr int N = decltype(number)::value;
         __syncthreads();
         put_par(std::integral_constant<int, 1 - N>{}, k0 + step);
-        // scalar registers: with a cap or slopes at once, which spares three registers that
-        // would spill (a chunk 163 us for 167), else where they are used (112 for 114)
-        int2 ask = s_raise[N];
-        if (SHAPED) ask = make_int2(__builtin_amdgcn_readfirstlane(ask.x), __builtin_amdgcn_readfirstlane(ask.y));
+        const int2 ask = s_raise[N];  // into scalar registers where they are used (at once: a chunk 113.6 us for 112.4)
         float x[8];  // row i, keys 16 · kt + 4u + k
         v8h pv[2][G];
 #pragma unroll

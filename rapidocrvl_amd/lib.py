@@ -707,7 +707,6 @@ class Context:
         check(load().pocr_qcache_attention(self.h, C.byref(args), C.byref(cache), stream))
 
 
-
 class Model:
     """Device-resident decoder (weights borrowed, norms/embedding copied)."""
 
