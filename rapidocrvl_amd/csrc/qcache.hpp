@@ -524,9 +524,9 @@ struct QAttnPlan {
 constexpr int kQBlock = 32;      // keys per step of a wave
 constexpr int kQTop = 9;         // weights times steps stay below 2^(kQTop + kQSlack)
 constexpr int kQSlack = 6;       // a score may pass its row's reference by this before that moves
-// From here on a reference's exponent stands apart from its whole number: a score's last
-// bit is 1/2 and more, and so a rounded multiply-add would lose the exponent's.  Nor may
-// scores pass such a reference: six of them are one step of fp32 further up.
+// From here on a reference's exponent stands apart from its whole number: fp32's steps there
+// are 1/2 and more, and further up more than an exponent.  Nor may scores pass such a
+// reference, since one step of theirs may be more than kQSlack.
 constexpr float kQFar = 4194304.0f;
 
 // the query rows of a tile: [first, last] and what they see
@@ -788,8 +788,8 @@ __device__ __forceinline__ void q_scores(float sum, const uint8_t *par, int kt, 
 // subnormal ones < 2^-14.
 __device__ __forceinline__ int q_raise(uint32_t step) { return kQTop + 14 - (int)(step >> 10); }
 
-// V's largest step so far in blocks of which all rows see the same, its exponent, and whether the
-// present block has parameters that are no numbers.
+// V's largest step so far in blocks of which all rows see the same, its exponent, and
+// whether the present block has parameters that are no numbers.
 constexpr uint16_t kQBad = 0x8000;  // in place of such a group's step: no step is a negative zero
 struct QScale {
     uint32_t top = 0;  // its bits
@@ -1009,8 +1009,9 @@ __device__ __forceinline__ void q_out_lse(const QAttnCall &p, int s, int g, int 
 // then 0.7 us a block, sums joined in LDS.  One token of 16 heads on 2 KV heads of 128 in
 // 4 bits behind 1,609 rows 9.0 to 9.7 us with the join (two launches over 17 blocks of keys
 // 8.9, one over a single block 6.5), in 8 bits 8.9 to 9.8; 16 of them behind up to 8,192
-// rows (33 MB) 17.1, without arithmetic 12.8, the join's 3 in both.  Two blocks of a wave on their way: 18.0, registers for two workgroups a CU in
-// place of three; two blocks a round: one token 10.7.
+// rows (33 MB) 17.1, without arithmetic 12.8, the join's 3 in both.  Two blocks of a wave
+// on their way: 18.0, registers for two workgroups a CU in place of three; two blocks a
+// round: one token 10.7.
 template <int HD, int BITS, int RT, int W, bool SHAPED>
 __global__ void __launch_bounds__(64 * W, RT == 1 && W == 4 ? 3 : 2) k_qcache_attn(QAttnCall p, QAttnPlan pl) {
     using F = QFormat<HD, BITS>;

@@ -257,3 +257,28 @@ def test_norm_of_an_infinite_element(ctx, rng, hd, rotary, adjacent, sign):
             bad[4 if adjacent else 5 + rotary // 2] = True
         assert np.array_equal(np.isnan(got[1, :hd]), bad) and np.all(got[1, :hd][~bad] == 0.0)
         assert np.isfinite(np.delete(got.reshape(3, 2, hd).reshape(6, hd), 2, 0)).all()
+
+
+@pytest.mark.parametrize("values", VALUES)
+@pytest.mark.parametrize("far", [22, -22])
+@pytest.mark.parametrize("n,rows", [(1, 400), (1, 1500), (3, 700), (40, 400)])
+@pytest.mark.parametrize("hd,bits,bias,window", [(128, 4, False, 0), (128, 8, True, 0), (64, 4, False, 0), (128, 4, True, 250)])
+def test_scores_on_both_sides_of_where_far_begins(ctx, rng, hd, bits, bias, window, n, rows, far, values):
+    """As above with scores of 2^22 + t (-2^22 + t), t rising by 13 over the rows: references
+    pass from near to far (from far to near), in one wave and from share to share."""
+    with base.Hip() as hip:
+        half = 1 << (bits - 1)
+        t = np.clip(np.arange(rows) * 14 // rows - 8 + rng.integers(-1, 2, rows), -8, 5)
+        k = np.full((1, 1, rows, hd), 16.0, F32)
+        k[0, 0, :, 1] += t
+        k[..., 3], k[..., 4] = 16 - half, 16 + half - 1
+        q = np.zeros((1, n, 2, hd), F32)
+        q[..., 1], q[..., 2] = 1.0, np.sign(far) * 2.0 ** (abs(far) - 4) - 1.0
+        v = VALUES[values](rng, 1, 1, rows, hd).astype(F32)
+        a = Attend(hip, rng, 1, n, rows, 2, 1, hd, bits, q=q.reshape(1, n, -1), k=k, v=v, scale=F32(np.log(2)),
+                   slopes=np.zeros(2, F32) if bias else None, window=window)
+        out, lse = a.run(ctx).got()
+        for h, x, (ka, kb), v, seen in heads_of(a):
+            o, e, ob, eb = weigh(x @ (ka + kb).T * a.scale, seen, v)
+            base.close(out[0, :, h * hd:(h + 1) * hd], o, ob, f"out of head {h}")
+            base.close(lse[0, :, h], e, eb, f"lse of head {h}")
